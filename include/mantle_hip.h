@@ -274,6 +274,36 @@ int mh_cross_entropy_fwd(float* loss, const float* x, const float* target, int64
 int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* target, const float* ug, int64_t rows,
                                int64_t classes);
 
+/* ---- losses of a language model (no reference counterpart) ----
+ * Class ids are int32 in device memory. The gradients of these calls are added to grad with
+ * accumulate != 0 and written over it with accumulate == 0, which saves zeroing and reading a
+ * gradient as large as a vocabulary's logits. Masked entries count as nothing: a logit of minus
+ * infinity has probability 0. No tensor may overlap a result. */
+
+/* Softmax cross entropy of a vocabulary head: the logits are z = x w^T of x [rows, dim] and
+ * w [classes, dim], which are never held as a tensor (CrossEntropyLoss, loss.mojo:45-61, with class
+ * ids for the one-hot target, after the head's product). A row whose label is negative is left out
+ * whatever it holds: its row_lse and row_loss are 0, its grad_x is left alone (accumulate == 0:
+ * zero), and it counts in no sum. With n kept rows:
+ *   row_lse = log sum_v exp z_v,  row_loss = row_lse - z_label,  loss = sum row_loss / n
+ * (0 without kept rows). A label of classes or more makes the row's loss, the loss and the gradients
+ * NaN; so does a kept row or a class that holds a NaN or an infinity. row_loss and row_lse may be null.
+ * x and w are each held with 22 bits relative to every element down to 2^-29 of the tensor's largest
+ * (of the kept rows for x), which a product needs to be as exact as one of fp32 operands; sums are fp32. */
+int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,
+                                const int32_t* labels, int64_t rows, int64_t dim, int64_t classes);
+/* The gradients from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
+ *   G = (exp(z - row_lse) - onehot(label)) ug / n,  grad_x = G w,  grad_w = G^T x.
+ * Either gradient may be null. An element of G is exact to 2^-22 of itself or 2^-40 ug / n. */
+int mh_linear_cross_entropy_bwd(float* grad_x, float* grad_w, const float* x, const float* w, const int32_t* labels,
+                                const float* row_lse, const float* ug, int64_t rows, int64_t dim, int64_t classes,
+                                int accumulate);
+/* Both at once, for a training step whose ug is known before: the logits' product is made once.
+ * row_lse and either gradient may be null. */
+int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, float* grad_w, const float* x,
+                                 const float* w, const int32_t* labels, const float* ug, int64_t rows, int64_t dim,
+                                 int64_t classes, int accumulate);
+
 /* ---- graph and model: Graph (mantle/autograd/graph.mojo:33-217), Model
  * (mantle/nn/model.mojo:55-340) and its Collections (mantle/autograd/collection.mojo:24-224)
  * in device memory ---- */

@@ -6,7 +6,7 @@ a mirror of Mantle's op structs and forward_op / backward_op. Nothing here falls
 the CPU: if the library is missing or the device is absent, calls raise.
 """
 from ._lib import MantleHipError, lib  # noqa: F401
-from .tensor import Tensor, TensorShape, init, sync  # noqa: F401
+from .tensor import IndexTensor, Tensor, TensorShape, init, sync  # noqa: F401
 from .optim import Adam  # noqa: F401
 from .graph import Graph, Symbol  # noqa: F401
 from .model import Collection, Model, Parameters  # noqa: F401
@@ -20,7 +20,7 @@ from .ops import (  # noqa: F401
     elwise_transform, elwise_pow, elwise_op, accumulate_grad, tsum, tmean, tmax, tstd, static_result_shape,
     bias_relu_forward, bias_relu_backward, softmax_log_mul_mean_forward, softmax_log_mul_mean_backward,
     softmax_forward, softmax_backward, logsoftmax_forward, logsoftmax_backward, cross_entropy_forward,
-    cross_entropy_backward,
+    cross_entropy_backward, linear_cross_entropy_forward, linear_cross_entropy_backward, linear_cross_entropy_step,
 )
 
 __all__ = [
@@ -29,6 +29,7 @@ __all__ = [
     "elwise_pow", "elwise_op", "accumulate_grad", "tsum", "tmean", "tmax", "tstd", "static_result_shape", "bias_relu_forward",
     "bias_relu_backward", "softmax_log_mul_mean_forward", "softmax_log_mul_mean_backward", "softmax_forward",
     "softmax_backward", "logsoftmax_forward", "logsoftmax_backward", "cross_entropy_forward",
-    "cross_entropy_backward", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
+    "cross_entropy_backward", "IndexTensor", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
+    "linear_cross_entropy_step", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
     "load_checkpoint", "load_checkpoint_with_optim",
 ]

@@ -124,6 +124,9 @@ SIGNATURES = {
     "mh_logsoftmax_bwd_accum": [_VP, _VP, _VP, _I64, _I64],
     "mh_cross_entropy_fwd": [_VP, _VP, _VP, _I64, _I64],
     "mh_cross_entropy_bwd_accum": [_VP, _VP, _VP, _VP, _I64, _I64],
+    "mh_linear_cross_entropy_fwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64],
+    "mh_linear_cross_entropy_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
+    "mh_linear_cross_entropy_step": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
     "mh_fma_fwd": [_VP, _VP, _VP, _VP, _I64],
     "mh_fma_bwd_accum": [_I, _VP, _VP, _VP, _VP, _I64],
     "mh_leakyrelu_fwd": [_VP, _VP, _I64, _F],

@@ -1,0 +1,816 @@
+// mh_head.hip -- softmax cross entropy of a vocabulary head, x [rows, dim] against w [classes, dim],
+// without the logits as a tensor, and both gradients.
+//
+//   z = x w^T;  lse_n = log sum_v exp z_nv;  loss = mean over the kept rows of lse_n - z_n,label
+//   G = (exp(z - lse) - onehot) ug / n;  grad_x = G w;  grad_w = G^T x
+//
+// Three products of 2 rows classes dim operations carry the time. The matrix instructions take fp32
+// operands at a sixteenth of the fp16 rate, so every fp32 operand is held as two halves (hi, lo):
+// v 2^e = hi + lo + r, |r| <= 2^-23 |v 2^e|, with one power of two e for the whole tensor that puts its
+// largest element into [2^14, 2^15). A product is hi hi + hi lo + lo hi, each exact in the fp32
+// accumulator; what is dropped, lo lo, is below 2^-22 of |a b|. That is the error of fp32 operands within
+// a factor of 4 for one term and below the rounding of an fp32 sum from some tens of terms on, at three
+// fp16 instructions a product. Elements below 2^-29 of the tensor's largest lose bits to the halves' least
+// exponent: the absolute error stays below 2^-39 of the largest. G is held the same way with e = 15 (|G| <= 1
+// before the factor ug / n, which the store applies).
+//
+// Operands lie in panels, the order the matrix instruction wants them: blocks of 32 rows x 16 of the
+// contracted axis, hi then lo, 1 KB each, lane l's 16 bytes being 8 elements of row l % 32 from
+// 8 (l / 32). A wavefront moves a block with one 16-byte load a lane, from memory straight to LDS, and
+// reads it from there without bank conflicts. Panels are padded with zeros to whole tiles, so the loop
+// over the contracted axis tests nothing.
+#include "mh_internal.h"
+#include "mh_math.h"
+
+namespace mh {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kBlk = 2048;       // bytes of a panel block: 32 x 16 elements, hi and lo
+constexpr int kGExp = 15;        // the power of two G is held with
+constexpr int kAmaxBlocks = 256;  // workgroups of k_amax for each of x and w
+
+// What the kernels of one call share, in device memory.
+struct HeadInfo {
+    int32_t ex, ew;  // powers of two of x and w
+    int32_t kept;    // rows with a label
+    int32_t pad;
+};
+struct HeadPart {  // k_amax's partials
+    float ax[kAmaxBlocks], aw[kAmaxBlocks];
+    int32_t kept[kAmaxBlocks];
+};
+
+__host__ __device__ inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+// e^x to about an ulp for x <= 0: the rounding of x log2(e) is carried into the result. mexp stops at
+// e^-88.4, as the reference does; here what a mask leaves is 0.
+__device__ __forceinline__ float exp_neg(float x) {
+    x = x < -1.0e4f ? -1.0e4f : x;  // keeps NaN, and infinity out of the fma
+    const float t = x * 1.44269504088896341f;
+    const float r = __builtin_fmaf(x, 1.925963033500e-8f, __builtin_fmaf(x, 1.44269504088896341f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, r * 0.693147180559945f, e);
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = __builtin_fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.0f;  // NaN and infinity do not set the scale
+}
+
+// The largest finite magnitude of x's kept rows and of w, and the kept rows' count, as partials.
+__global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, const float* w, const int32_t* labels,
+                                              int64_t rows, int64_t dim, int64_t nw) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float red[4];
+    __shared__ int32_t cnt[4];
+    float a = 0.0f;
+    int32_t kept = 0;
+    const bool isx = blockIdx.x < kAmaxBlocks;
+    const int b = isx ? blockIdx.x : blockIdx.x - kAmaxBlocks;
+    if (isx) {
+        for (int64_t r = (int64_t)b * 4 + wave; r < rows; r += kAmaxBlocks * 4) {
+            if (labels[r] < 0) continue;  // a row left out may hold anything
+            ++kept;
+            for (int64_t k = lane; k < dim; k += 64) a = __builtin_fmaxf(a, finite_abs(x[r * dim + k]));
+        }
+    } else {
+        const int64_t nq = nw >> 2;
+        for (int64_t q = (int64_t)b * 256 + threadIdx.x; q < nq; q += kAmaxBlocks * 256) {
+            const vf4 v = *reinterpret_cast<const vf4u*>(w + 4 * q);
+            a = __builtin_fmaxf(a, __builtin_fmaxf(__builtin_fmaxf(finite_abs(v.x), finite_abs(v.y)),
+                                                   __builtin_fmaxf(finite_abs(v.z), finite_abs(v.w))));
+        }
+        if (b == 0 && threadIdx.x < (nw & 3)) a = __builtin_fmaxf(a, finite_abs(w[4 * nq + threadIdx.x]));
+    }
+    a = wave_max(a);
+    if (lane == 0) {
+        red[wave] = a;
+        cnt[wave] = kept;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a = __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3]));
+        if (isx) {
+            part->ax[b] = a;
+            part->kept[b] = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+        } else {
+            part->aw[b] = a;
+        }
+    }
+}
+
+// The power of two that puts a into [2^14, 2^15).
+__device__ __forceinline__ int scale_exp(float a) {
+    if (!(a > 0.0f)) return 0;
+    int e;
+    __builtin_frexpf(a, &e);  // a = f 2^e, f in [1/2, 1)
+    return 15 - e;
+}
+
+__device__ __forceinline__ void split8(const float* v, half8* hi, half8* lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const _Float16 h = (_Float16)v[j];
+        (*hi)[j] = h;
+        (*lo)[j] = (_Float16)(v[j] - (float)h);
+    }
+}
+
+constexpr int kSplitTile = 64;
+
+// A [nr, nc] matrix into its row panels (contracted over columns) and, with colp, its column panels
+// (contracted over rows), zero-padded: one 64 x 64 tile a workgroup. x's tiles come first, then w's.
+struct SplitOne {
+    const float* src;
+    int64_t nr, nc;      // the matrix
+    char* rowp;          // [tiles_r * 2][rkb] blocks; column blocks at or past rkb are not stored
+    char* colp;          // [tiles_c * 2][ckb] blocks
+    int64_t rkb, ckb;
+    int64_t tiles_r, tiles_c;
+    int64_t rb_end, cb_end;  // row blocks of rowp, of colp
+};
+__global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const HeadPart* part, HeadInfo* info,
+                                               const int32_t* labels) {
+    __shared__ float t[kSplitTile][kSplitTile + 1];
+    __shared__ float red[4];
+    __shared__ int32_t cnt[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t ntx = sx.tiles_r * sx.tiles_c;
+    const bool isx = (int64_t)blockIdx.x < ntx;
+    const SplitOne s = isx ? sx : sw;
+    const int64_t tile = isx ? blockIdx.x : blockIdx.x - ntx;
+    const int64_t r0 = tile / s.tiles_c * kSplitTile, c0 = tile % s.tiles_c * kSplitTile;
+    float a = isx ? part->ax[tid] : part->aw[tid];
+    a = wave_max(a);
+    if (lane == 0) red[wave] = a;
+    // the tile's rows, a wavefront a row
+    for (int i = 0; i < kSplitTile / 4; ++i) {
+        const int64_t r = r0 + i * 4 + wave, c = c0 + lane;
+        const bool in = r < s.nr && c < s.nc && !(isx && labels[r < s.nr ? r : 0] < 0);
+        t[i * 4 + wave][lane] = in ? s.src[r * s.nc + c] : 0.0f;
+    }
+    __syncthreads();
+    const int e = scale_exp(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
+    const int r = lane & 31, k8 = (lane >> 5) * 8;
+    // 2 row blocks x 4 blocks of the contracted axis each way: 8 blocks, two a wavefront
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int rb = i, kb = wave;
+        float v[8];
+        half8 hi, lo;
+        if (r0 / 32 + rb < s.rb_end && c0 / 16 + kb < s.rkb) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[rb * 32 + r][kb * 16 + k8 + j], e);
+            split8(v, &hi, &lo);
+            half8* p = reinterpret_cast<half8*>(s.rowp + ((r0 / 32 + rb) * s.rkb + c0 / 16 + kb) * kBlk);
+            p[lane] = hi;
+            p[64 + lane] = lo;
+        }
+        if (s.colp && c0 / 32 + rb < s.cb_end && r0 / 16 + kb < s.ckb) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[kb * 16 + k8 + j][rb * 32 + r], e);
+            split8(v, &hi, &lo);
+            half8* p = reinterpret_cast<half8*>(s.colp + ((c0 / 32 + rb) * s.ckb + r0 / 16 + kb) * kBlk);
+            p[lane] = hi;
+            p[64 + lane] = lo;
+        }
+    }
+    if (blockIdx.x == 0) {  // the scales and the count, for the kernels behind
+        float b = wave_max(part->aw[tid]);
+        int32_t kept = part->kept[tid];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o);
+        __syncthreads();
+        if (lane == 0) {
+            red[wave] = b;
+            cnt[wave] = kept;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            info->ex = e;
+            info->ew = scale_exp(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
+            info->kept = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// the product of two panels
+// ---------------------------------------------------------------------------------------
+enum HeadEpi { EPI_LOGITS = 0, EPI_GRAD = 1 };
+
+struct GemmArg {
+    const char *a, *b;       // panels: M operand, N operand
+    int64_t akb, bkb;        // blocks along the contracted axis that a row block of each panel holds
+    int64_t kb;              // blocks contracted here, of one split: a multiple of 2
+    int64_t kb_all;          // blocks contracted by all splits
+    int32_t tiles_m, tiles_n;
+    const HeadInfo* info;
+    // EPI_LOGITS: M is classes, N rows
+    const int32_t* labels;   // at the first row of the panel; EPI_GRAD: rows to leave alone, or null
+    int64_t rows, classes;   // of the operands; rows counted from the panel's first
+    float* stat;             // [class groups of a wavefront][2][stat_ld]: maximum, sum of exponentials
+    int64_t stat_ld;
+    float* target;           // [rows] the label's logit
+    char* z;                 // the logits, in the blocks of G's row panels, or null
+    int64_t zkb;
+    // EPI_GRAD: out [m, n] += or = ug / kept * acc
+    float* out;
+    int64_t m, n;
+    const float* ug;
+    float* part;             // split sums [splits][tiles_m * TM][tiles_n * TN], or null
+    int32_t exp_b;           // 0: x's power of two, 1: w's
+    int32_t accumulate;
+};
+
+// ug / kept and the exponent that undoes the panels' scales, applied to one sum.
+__device__ __forceinline__ float grad_value(float acc, float c, int e) { return c * __builtin_ldexpf(acc, e); }
+
+template <int TM, int TN, int WM, int WN, int EPI>
+__global__ __launch_bounds__(WM* WN * 64) void k_gemm(GemmArg g) {
+    constexpr int kWaves = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32;
+    constexpr int kRowB = 2 * kBlk;                       // bytes a row block adds to a stage: 32 of the axis
+    constexpr int kStage = (TM + TN) / 32 * kRowB;
+    constexpr int kLoads = (TM + TN) / 32 / kWaves;       // row blocks a wavefront brings a stage
+    static_assert((TM + TN) / 32 % kWaves == 0, "loads");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 tile rows,
+    // so that its L2 holds what its workgroups share.
+    const int64_t T = (int64_t)g.tiles_m * g.tiles_n;
+    const int64_t per = (T + 7) / 8;
+    const int64_t id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= per || id >= T) return;
+    const int64_t gsz = (int64_t)8 * g.tiles_n, grp = id / gsz;
+    const int gm = (int)(g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8);
+    const int64_t tm = grp * 8 + (id - grp * gsz) % gm, tn = (id - grp * gsz) / gm;
+
+    const int64_t k0 = (int64_t)blockIdx.y * g.kb;
+    int64_t kb = g.kb_all - k0;
+    if (kb > g.kb) kb = g.kb;
+    const int S = (int)(kb / 2);
+
+    const char* src[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int rb = wave * kLoads + i;
+        src[i] = (rb < TM / 32 ? g.a + ((tm * (TM / 32) + rb) * g.akb + k0) * kBlk
+                               : g.b + ((tn * (TN / 32) + rb - TM / 32) * g.bkb + k0) * kBlk) + lane * 16;
+    }
+    auto load = [&](int s, int buf) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            char* to = lds + buf * kStage + (wave * kLoads + i) * kRowB;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)(src[i] + (int64_t)s * kRowB + j * 1024),
+                    (__attribute__((address_space(3))) void*)(to + j * 1024), 16, 0, 0);
+        }
+    };
+
+    f32x16 acc[MI][NI] = {};
+    if (S > 0) load(0, 0);
+    __syncthreads();
+    for (int s = 0; s < S; ++s) {
+        if (s + 1 < S) load(s + 1, (s + 1) & 1);
+        const char* la = lds + (s & 1) * kStage + wm * MI * kRowB + lane * 16;
+        const char* lb = lds + (s & 1) * kStage + (TM / 32 + wn * NI) * kRowB + lane * 16;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            half8 b[NI][2];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                b[j][0] = *reinterpret_cast<const half8*>(lb + j * kRowB + kk * kBlk);
+                b[j][1] = *reinterpret_cast<const half8*>(lb + j * kRowB + kk * kBlk + 1024);
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const half8 hi = *reinterpret_cast<const half8*>(la + i * kRowB + kk * kBlk);
+                const half8 lo = *reinterpret_cast<const half8*>(la + i * kRowB + kk * kBlk + 1024);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, b[j][1], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, b[j][0], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, b[j][0], acc[i][j], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+
+    // acc[i][j][r]: row (of M) 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4, column (of N) 32 j + lane % 32
+    const int half = lane >> 5, col = lane & 31;
+    if constexpr (EPI == EPI_LOGITS) {
+        const int e = -(g.info->ex + g.info->ew);
+        const int64_t v0 = tm * TM + wm * MI * 32;  // the wavefront's first class
+        const int64_t grp_v = tm * WM + wm;         // its group of MI * 32 classes
+        // register r of tile i holds class v0 + 4 half + cls_of(i, r): compared with the label and the
+        // last class relative to the first two terms
+        const int64_t left = g.classes - v0 - 4 * half;
+        const int last = left < 0 ? 0 : left < MI * 32 ? (int)left : MI * 32;
+        auto cls_of = [](int i, int r) { return i * 32 + 8 * (r >> 2) + (r & 3); };
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int64_t n = tn * TN + (wn * NI + j) * 32 + col;
+            const int64_t want = (n < g.rows ? (int64_t)g.labels[n] : -1) - v0 - 4 * half;
+            const int label = want < 0 || want >= MI * 32 ? -1 : (int)want;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], e);
+            if (g.stat) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float z = acc[i][j][r];
+                        if (cls_of(i, r) == label) g.target[n] = z;
+                        if (cls_of(i, r) < last) top = z > top || z != z ? z : top;
+                    }
+                const float other = __shfl_xor(top, 32);
+                top = other > top || other != other ? other : top;
+                float sum = 0.0f;
+                const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (cls_of(i, r) < last) sum += exp_neg(acc[i][j][r] - base);
+                sum += __shfl_xor(sum, 32);
+                if (half == 0) {
+                    g.stat[grp_v * 2 * g.stat_ld + n] = top;
+                    g.stat[(grp_v * 2 + 1) * g.stat_ld + n] = sum;
+                }
+            }
+            if (g.z) {  // 4 consecutive classes a lane: 16 bytes of the block of (n / 32, v / 16)
+                char* zb = g.z + (n >> 5) * g.zkb * kBlk;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int64_t vb = (v0 >> 4) + i * 2 + (q >> 1);
+                        vf4 o = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                        *reinterpret_cast<vf4*>(zb + vb * kBlk + (col + 32 * (q & 1)) * 32 + half * 16) = o;
+                    }
+            }
+        }
+    } else {
+        if (g.part) {
+            const int64_t ld = (int64_t)g.tiles_n * TN;
+            float* p = g.part + (int64_t)blockIdx.y * g.tiles_m * TM * ld;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t m = tm * TM + (wm * MI + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+                        p[m * ld + tn * TN + (wn * NI + j) * 32 + col] = acc[i][j][r];
+                    }
+            return;
+        }
+        const int e = -(kGExp + (g.exp_b ? g.info->ew : g.info->ex));
+        const float c = g.ug[0] / (float)(g.info->kept > 0 ? g.info->kept : 1);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t m = tm * TM + (wm * MI + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+                if (m >= g.m) continue;
+                const bool out = g.labels && g.labels[m] < 0;  // a row left out: as it was, or zero
+                if (out && g.accumulate) continue;
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    const int64_t n = tn * TN + (wn * NI + j) * 32 + col;
+                    if (n >= g.n) continue;
+                    float* o = g.out + m * g.n + n;
+                    const float v = out ? 0.0f : grad_value(acc[i][j][r], c, e);
+                    *o = g.accumulate ? *o + v : v;
+                }
+            }
+    }
+}
+
+// Joins the splits of a gradient product, in their order.
+__global__ __launch_bounds__(256) void k_join(GemmArg g, int32_t splits, int64_t ld, int64_t plane) {
+    const int e = -(kGExp + (g.exp_b ? g.info->ew : g.info->ex));
+    const float c = g.ug[0] / (float)(g.info->kept > 0 ? g.info->kept : 1);
+    const int64_t total = g.m * g.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / g.n, n = i - m * g.n;
+        const bool out = g.labels && g.labels[m] < 0;
+        if (out && g.accumulate) continue;
+        float v = 0.0f;
+        if (!out) {
+            for (int s = 0; s < splits; ++s) v += g.part[s * plane + m * ld + n];
+            v = grad_value(v, c, e);
+        }
+        g.out[i] = g.accumulate ? g.out[i] + v : v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// rows' statistics, the loss, and G's panels
+// ---------------------------------------------------------------------------------------
+// Each row's log-sum-exp from its class groups' statistics: 32 rows x 8 threads a workgroup.
+__global__ __launch_bounds__(256) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
+                                                  const float* target, const int32_t* labels, int64_t rows,
+                                                  int64_t classes, float* row_lse, float* row_loss) {
+    __shared__ float sm[8][32], ss[8][32];
+    const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + r;
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (int64_t gr = p; gr < groups; gr += 8) {
+        const float m = stat[gr * 2 * stat_ld + n], s = stat[(gr * 2 + 1) * stat_ld + n];
+        if (m != m) top = m;
+        if (m > top) {
+            sum = sum * exp_neg(top - m) + s;
+            top = m;
+        } else if (m > -__builtin_inff()) {
+            sum += s * exp_neg(m - top);
+        }
+    }
+    sm[p][r] = top;
+    ss[p][r] = sum;
+    __syncthreads();
+    if (p != 0 || n >= rows) return;
+    float t = -__builtin_inff(), s = 0.0f;
+    for (int i = 0; i < 8; ++i) t = sm[i][r] > t || sm[i][r] != sm[i][r] ? sm[i][r] : t;
+    for (int i = 0; i < 8; ++i)
+        if (sm[i][r] > -__builtin_inff() || sm[i][r] != sm[i][r]) s += ss[i][r] * exp_neg(sm[i][r] - t);
+    const int32_t label = labels[n];
+    float lse = t + mlog(s);
+    if (label >= classes) lse = __builtin_nanf("");  // no such class: shown in the loss and the gradients
+    if (label < 0) lse = 0.0f;
+    row_lse[n] = lse;
+    row_loss[n] = label < 0 ? 0.0f : (label >= classes ? lse : lse - target[n]);
+}
+
+// loss = sum of the rows' losses / kept, in one workgroup and a fixed order.
+__global__ __launch_bounds__(1024) void k_rows_loss(const float* row_loss, int64_t rows, const HeadInfo* info,
+                                                    float* loss) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t n = threadIdx.x; n < rows; n += 1024) s += (double)row_loss[n];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        for (int i = 0; i < 16; ++i) s += red[i];
+        loss[0] = (float)(s / (double)(info->kept > 0 ? info->kept : 1));
+    }
+}
+
+// Logits to G's panels: a wavefront takes 32 rows x 32 classes (two blocks of logits, which become two
+// blocks of the row panel in place) and writes the same elements to the column panel through LDS.
+__global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, int64_t gtkb, const float* lse,
+                                              const int32_t* labels, int64_t rows, int64_t classes, int64_t tiles_v) {
+    __shared__ __attribute__((aligned(16))) _Float16 t[4][2][32][40];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t nb = id / tiles_v, vt = id % tiles_v;  // the grid covers whole workgroups of tiles
+    const int64_t n = nb * 32 + (lane & 31);
+    const int32_t label = n < rows ? labels[n] : -1;
+    const float l = n < rows ? lse[n] : 0.0f;
+    const int k8 = (lane >> 5) * 8;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        char* blk = z + (nb * zkb + vt * 2 + b) * kBlk;
+        const vf4 q0 = reinterpret_cast<const vf4*>(blk)[lane * 2], q1 = reinterpret_cast<const vf4*>(blk)[lane * 2 + 1];
+        float v[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t cls = vt * 32 + b * 16 + k8 + j;
+            const float p = exp_neg(v[j] - l) - (cls == label ? 1.0f : 0.0f);
+            v[j] = label < 0 || cls >= classes ? 0.0f : p * (float)(1 << kGExp);
+        }
+        half8 hi, lo;
+        split8(v, &hi, &lo);
+        // every lane of the wavefront has its logits before the block is written over
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        reinterpret_cast<half8*>(blk)[lane] = hi;
+        reinterpret_cast<half8*>(blk)[64 + lane] = lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            t[wave][0][b * 16 + k8 + j][lane & 31] = hi[j];
+            t[wave][1][b * 16 + k8 + j][lane & 31] = lo[j];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {  // rows n of 16 b .. 16 b + 15 as the contracted axis
+        char* blk = gt + (vt * gtkb + nb * 2 + b) * kBlk;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            reinterpret_cast<half8*>(blk)[64 * p + lane] =
+                *reinterpret_cast<const half8*>(&t[wave][p][lane & 31][b * 16 + k8]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------
+// The logits of one chunk of rows and G's column panel take 8 bytes an element; a chunk's rows keep them
+// within this, 256 rows at least.
+constexpr int64_t kChunkBytes = (int64_t)4 << 30;
+constexpr int64_t kMaxChunk = 32768;
+
+struct Carve {
+    size_t at = 0;
+    size_t take(int64_t bytes) {
+        const size_t o = at;
+        at += (size_t)up(bytes, 1024);
+        return o;
+    }
+};
+
+template <int T, int EPI>
+void launch_gemm(const GemmArg& g, int64_t tiles, int splits) {
+    const dim3 grid((unsigned)(8 * ((tiles + 7) / 8)), (unsigned)splits);
+    if constexpr (T == 256)
+        hipLaunchKernelGGL((k_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, ctx().stream, g);
+    else
+        hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, g);
+}
+
+// The tile of a product: 256 x 256 where that fills the chip.
+int tile_of(int64_t m, int64_t n, int64_t splits) {
+    return up(m, 256) / 256 * (up(n, 256) / 256) * splits >= ctx().num_cus ? 256 : 128;
+}
+
+// Splits of a gradient product over its contracted axis of kb blocks: as many as fill the chip, each of
+// 16 blocks at least.
+int splits_of(int64_t m, int64_t n, int64_t kb) {
+    const int64_t tiles = up(m, 128) / 128 * (up(n, 128) / 128);
+    int64_t s = 2 * ctx().num_cus / tiles;
+    if (s > kb / 16) s = kb / 16;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+struct HeadCall {
+    const char* what;
+    float *loss, *row_loss, *row_lse_out;
+    const float* row_lse_in;
+    float *gx, *gw;
+    const float *x, *w;
+    const int32_t* labels;
+    const float* ug;
+    int64_t rows, dim, classes;
+    bool train, accumulate;
+};
+
+// grad [m, n] from panels a (rows of m) and b (rows of n), contracted over kb blocks.
+int grad_product(GemmArg g, int64_t m, int64_t n, int64_t kb, float* part) {
+    const int splits = splits_of(m, n, kb);
+    const int T = splits > 1 ? 128 : tile_of(m, n, 1);
+    g.m = m;
+    g.n = n;
+    g.tiles_m = (int32_t)(up(m, T) / T);
+    g.tiles_n = (int32_t)(up(n, T) / T);
+    g.kb_all = kb;
+    g.kb = up((kb + splits - 1) / splits, 2);
+    const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+    g.part = splits > 1 ? part : nullptr;
+    if (T == 256) launch_gemm<256, EPI_GRAD>(g, tiles, splits);
+    else launch_gemm<128, EPI_GRAD>(g, tiles, splits);
+    if (splits > 1) {
+        const int64_t ld = (int64_t)g.tiles_n * T, plane = (int64_t)g.tiles_m * T * ld;
+        int64_t nb = grid_blocks(m * n, 256);
+        if (nb > 4096) nb = 4096;
+        hipLaunchKernelGGL(k_join, dim3((unsigned)nb), dim3(256), 0, ctx().stream, g, splits, ld, plane);
+    }
+    return MH_OK;
+}
+
+size_t part_bytes(int64_t m, int64_t n, int64_t kb) {
+    const int s = splits_of(m, n, kb);
+    return s > 1 ? (size_t)s * up(m, 128) * up(n, 128) * sizeof(float) : 0;
+}
+
+int head_run(const HeadCall& h) {
+    const int64_t rows = h.rows, dim = h.dim, classes = h.classes;
+    const int64_t rowsP = up(rows, 256), dimP = up(dim, 256), clsP = up(classes, 256);
+    const int64_t dkb = up(dim, 32) / 16;
+    int64_t chunk = kMaxChunk;
+    if (h.train) {
+        chunk = kChunkBytes / (clsP * 8) / 256 * 256;
+        chunk = chunk < 256 ? 256 : chunk > kMaxChunk ? kMaxChunk : chunk;
+    }
+    if (chunk > rowsP) chunk = rowsP;
+    const int64_t groups = clsP / 64;  // of the smaller tile's wavefronts
+
+    Carve cv;
+    const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
+    const size_t o_xr = cv.take(rowsP / 32 * dkb * kBlk), o_wr = cv.take(clsP / 32 * dkb * kBlk);
+    const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * (rowsP / 16) * kBlk) : 0;
+    const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * (clsP / 16) * kBlk) : 0;
+    const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
+    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP * 4);
+    size_t o_z = 0, o_gt = 0, o_sp = 0;
+    if (h.train) {
+        o_z = cv.take(chunk / 32 * (clsP / 16) * kBlk);
+        o_gt = cv.take(clsP / 32 * (chunk / 16) * kBlk);
+        // every chunk has this many rows but the last
+        size_t sp = 0;
+        for (const int64_t nr : {rows < chunk ? rows : chunk, rows - (rows - 1) / chunk * chunk}) {
+            const size_t a = h.gx ? part_bytes(nr, dim, clsP / 16) : 0;
+            const size_t b = h.gw ? part_bytes(classes, dim, up(nr, 256) / 16) : 0;
+            sp = a > sp ? a : sp;
+            sp = b > sp ? b : sp;
+        }
+        o_sp = cv.take((int64_t)sp);
+    }
+    char* base = nullptr;
+    MH_TRY(scratch(cv.at, reinterpret_cast<void**>(&base)));
+    hipStream_t st = ctx().stream;
+    HeadInfo* info = reinterpret_cast<HeadInfo*>(base + o_info);
+    HeadPart* part = reinterpret_cast<HeadPart*>(base + o_part);
+    float* lse = h.row_lse_out ? h.row_lse_out : reinterpret_cast<float*>(base + o_lse);
+    float* row_loss = h.row_loss ? h.row_loss : reinterpret_cast<float*>(base + o_rl);
+    float* target = reinterpret_cast<float*>(base + o_tgt);
+
+    hipLaunchKernelGGL(k_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, st, part, h.x, h.w, h.labels, rows, dim,
+                       classes * dim);
+    SplitOne sx = {h.x, rows, dim, base + o_xr, h.train && h.gw ? base + o_xt : nullptr, dkb, rowsP / 16,
+                   rowsP / 64, up(dim, 64) / 64, rowsP / 32, dimP / 32};
+    SplitOne sw = {h.w, classes, dim, base + o_wr, h.train && h.gx ? base + o_wt : nullptr, dkb, clsP / 16,
+                   clsP / 64, up(dim, 64) / 64, clsP / 32, dimP / 32};
+    if (sx.colp) sx.tiles_c = dimP / 64;
+    if (sw.colp) sw.tiles_c = dimP / 64;
+    const int64_t nsplit = sx.tiles_r * sx.tiles_c + sw.tiles_r * sw.tiles_c;
+    hipLaunchKernelGGL(k_split, dim3((unsigned)nsplit), dim3(256), 0, st, sx, sw, part, info, h.labels);
+
+    for (int64_t r0 = 0; r0 < rows; r0 += chunk) {
+        const int64_t nr = rows - r0 < chunk ? rows - r0 : chunk, nrP = up(nr, 256);
+        GemmArg g = {};
+        g.a = base + o_wr;
+        g.b = base + o_xr + r0 / 32 * dkb * kBlk;
+        g.akb = g.bkb = g.kb = g.kb_all = dkb;
+        g.info = info;
+        g.labels = h.labels + r0;
+        g.rows = nr;
+        g.classes = classes;
+        g.stat = h.row_lse_in ? nullptr : reinterpret_cast<float*>(base + o_stat);
+        g.stat_ld = chunk;
+        g.target = target;
+        g.z = h.train ? base + o_z : nullptr;
+        g.zkb = clsP / 16;
+        // every row and class of the padded chunk gets its logits: the panels behind have no gaps
+        const int T = tile_of(classes, nr, 1);
+        g.tiles_m = (int32_t)(clsP / T);
+        g.tiles_n = (int32_t)(nrP / T);
+        const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+        if (T == 256) launch_gemm<256, EPI_LOGITS>(g, tiles, 1);
+        else launch_gemm<128, EPI_LOGITS>(g, tiles, 1);
+        if (!h.row_lse_in)
+            hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)(nrP / 32)), dim3(256), 0, st, g.stat, clsP / (T / 2),
+                               g.stat_ld, target, h.labels + r0, nr, classes, lse + r0, row_loss + r0);
+        if (!h.train) continue;
+        const int64_t tiles_v = clsP / 32;
+        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(nrP / 32 * tiles_v / 4)), dim3(256), 0, st, base + o_z, clsP / 16,
+                           base + o_gt, nrP / 16, (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr, classes,
+                           tiles_v);
+        GemmArg d = {};
+        d.info = info;
+        d.ug = h.ug;
+        if (h.gx) {
+            d.a = base + o_z;
+            d.akb = clsP / 16;
+            d.b = base + o_wt;
+            d.bkb = clsP / 16;
+            d.exp_b = 1;
+            d.labels = h.labels + r0;
+            d.out = h.gx + r0 * dim;
+            d.accumulate = h.accumulate;
+            MH_TRY(grad_product(d, nr, dim, clsP / 16, reinterpret_cast<float*>(base + o_sp)));
+        }
+        if (h.gw) {
+            d.a = base + o_gt;
+            d.akb = nrP / 16;
+            d.b = base + o_xt + r0 / 16 * kBlk;
+            d.bkb = rowsP / 16;
+            d.exp_b = 0;
+            d.labels = nullptr;
+            d.out = h.gw;
+            d.accumulate = h.accumulate || r0 > 0;
+            MH_TRY(grad_product(d, classes, dim, nrP / 16, reinterpret_cast<float*>(base + o_sp)));
+        }
+    }
+    if (!h.row_lse_in)
+        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(1024), 0, st, row_loss, rows, info, h.loss);
+    return finish(h.what);
+}
+
+int head_check(const HeadCall& h) {
+    if (h.rows < 0 || h.dim < 1 || h.classes < 1)
+        return fail(MH_ERR_INVALID, "%s: needs rows >= 0, dim >= 1, classes >= 1 (%lld, %lld, %lld)", h.what,
+                    (long long)h.rows, (long long)h.dim, (long long)h.classes);
+    if (h.classes > 0x7fffffff || h.dim > (1 << 24) || h.rows > 0x7fffffff)
+        return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 rows or classes, or 2^24 dims", h.what);
+    // one workgroup a 64 x 64 tile of x and of w
+    if ((up(h.rows, 256) / 64 + up(h.classes, 256) / 64) * (up(h.dim, 256) / 64) > max_grid_blocks(256))
+        return fail(MH_ERR_OVERFLOW, "%s: operands of more than 2^36 elements", h.what);
+    return MH_OK;
+}
+
+}  // namespace
+}  // namespace mh
+
+using namespace mh;
+
+extern "C" {
+
+int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,
+                                const int32_t* labels, int64_t rows, int64_t dim, int64_t classes) {
+    MH_TRACE("mh_linear_cross_entropy_fwd");
+    HeadCall h = {};
+    h.what = "mh_linear_cross_entropy_fwd";
+    h.loss = loss;
+    h.row_loss = row_loss;
+    h.row_lse_out = row_lse;
+    h.x = x;
+    h.w = w;
+    h.labels = labels;
+    h.rows = rows;
+    h.dim = dim;
+    h.classes = classes;
+    MH_TRY(head_check(h));
+    if (!loss || !w || (rows > 0 && (!x || !labels))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
+    MH_TRY(require_init());
+    if (rows == 0) return mh_fill(loss, 0.0f, 1);
+    return head_run(h);
+}
+
+int mh_linear_cross_entropy_bwd(float* grad_x, float* grad_w, const float* x, const float* w, const int32_t* labels,
+                                const float* row_lse, const float* ug, int64_t rows, int64_t dim, int64_t classes,
+                                int accumulate) {
+    MH_TRACE("mh_linear_cross_entropy_bwd");
+    HeadCall h = {};
+    h.what = "mh_linear_cross_entropy_bwd";
+    h.gx = grad_x;
+    h.gw = grad_w;
+    h.row_lse_in = row_lse;
+    h.x = x;
+    h.w = w;
+    h.labels = labels;
+    h.ug = ug;
+    h.rows = rows;
+    h.dim = dim;
+    h.classes = classes;
+    h.train = true;
+    h.accumulate = accumulate != 0;
+    MH_TRY(head_check(h));
+    if (!grad_x && !grad_w) return MH_OK;
+    if (!w || !ug || (rows > 0 && (!x || !labels || !row_lse))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
+    MH_TRY(require_init());
+    if (rows == 0) return grad_w && !accumulate ? mh_zero(grad_w, classes * dim) : MH_OK;
+    return head_run(h);
+}
+
+int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, float* grad_w, const float* x,
+                                 const float* w, const int32_t* labels, const float* ug, int64_t rows, int64_t dim,
+                                 int64_t classes, int accumulate) {
+    MH_TRACE("mh_linear_cross_entropy_step");
+    HeadCall h = {};
+    h.what = "mh_linear_cross_entropy_step";
+    h.loss = loss;
+    h.row_lse_out = row_lse;
+    h.gx = grad_x;
+    h.gw = grad_w;
+    h.x = x;
+    h.w = w;
+    h.labels = labels;
+    h.ug = ug;
+    h.rows = rows;
+    h.dim = dim;
+    h.classes = classes;
+    h.train = grad_x || grad_w;
+    h.accumulate = accumulate != 0;
+    MH_TRY(head_check(h));
+    if (!loss || !w || (h.train && !ug) || (rows > 0 && (!x || !labels))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
+    MH_TRY(require_init());
+    if (rows == 0) {
+        if (grad_w && !accumulate) MH_TRY(mh_zero(grad_w, classes * dim));
+        return mh_fill(loss, 0.0f, 1);
+    }
+    return head_run(h);
+}
+
+}  // extern "C"

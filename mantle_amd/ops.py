@@ -19,7 +19,7 @@ from __future__ import annotations
 from typing import Optional
 
 from . import _lib
-from .tensor import Tensor, TensorShape, as_shape
+from .tensor import IndexTensor, Tensor, TensorShape, as_shape
 
 
 class OP:
@@ -486,3 +486,61 @@ def cross_entropy_backward(grad_x: Tensor, x: Tensor, target: Tensor, ug: Tensor
     """grad_x += d loss / dx of CrossEntropyLoss from the loss grad ug (one element)."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("target", target)), scalar=(("ug", ug),))
     _lib.call("mh_cross_entropy_bwd_accum", grad_x.ptr, x.ptr, target.ptr, ug.ptr, r, k)
+
+
+# ---------------------------------------------------------------------------------------
+# losses of a language model (no reference counterpart)
+# ---------------------------------------------------------------------------------------
+def _want(name: str, t, shape, index: bool = False, optional: bool = False) -> Optional[int]:
+    """The address of t after checking that it is there, of the right kind and of `shape`."""
+    if t is None and optional:
+        return None
+    if not isinstance(t, Tensor) or isinstance(t, IndexTensor) != index:
+        kind = "an IndexTensor" if index else "a Tensor"
+        raise _lib.MantleHipError(_lib.ERR_INVALID, f"{name} must be {kind}, not {type(t).__name__}")
+    if t.shape() != TensorShape(shape):
+        raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{name} has shape {t.shape()}, not {TensorShape(shape)}")
+    return t.ptr
+
+
+def _matrix(name: str, t):
+    if not isinstance(t, Tensor) or t.rank() != 2:
+        raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{name} must be a tensor of two dimensions")
+    return t.shape().dims
+
+
+def linear_cross_entropy_forward(loss: Tensor, row_lse: Optional[Tensor], x: Tensor, w: Tensor, labels: IndexTensor,
+                                 row_loss: Optional[Tensor] = None) -> None:
+    """Softmax cross entropy of a vocabulary head, CrossEntropyLoss (loss.mojo:45-61) of the logits
+    x [rows, dim] . w [classes, dim]^T against class ids, without the logits as a tensor. A row with a
+    negative label is left out. loss (1) is the mean over the kept rows; row_lse and row_loss (rows) are
+    each row's log-sum-exp, which the backward takes, and loss."""
+    (rows, dim), (classes, _) = _matrix("x", x), _matrix("w", w)
+    _lib.call("mh_linear_cross_entropy_fwd", _want("loss", loss, (1,)),
+              _want("row_loss", row_loss, (rows,), optional=True), _want("row_lse", row_lse, (rows,), optional=True),
+              _want("x", x, (rows, dim)), _want("w", w, (classes, dim)), _want("labels", labels, (rows,), index=True),
+              rows, dim, classes)
+
+
+def linear_cross_entropy_backward(grad_x: Optional[Tensor], grad_w: Optional[Tensor], x: Tensor, w: Tensor,
+                                  labels: IndexTensor, row_lse: Tensor, ug: Tensor, accumulate: bool = True) -> None:
+    """grad_x and grad_w += (accumulate=False: =) the gradients of linear_cross_entropy_forward's loss
+    from ug, the loss's (shape (1)), and the forward's row_lse. Either may be None."""
+    (rows, dim), (classes, _) = _matrix("x", x), _matrix("w", w)
+    _lib.call("mh_linear_cross_entropy_bwd", _want("grad_x", grad_x, (rows, dim), optional=True),
+              _want("grad_w", grad_w, (classes, dim), optional=True), _want("x", x, (rows, dim)),
+              _want("w", w, (classes, dim)), _want("labels", labels, (rows,), index=True),
+              _want("row_lse", row_lse, (rows,)), _want("ug", ug, (1,)), rows, dim, classes, int(bool(accumulate)))
+
+
+def linear_cross_entropy_step(loss: Tensor, grad_x: Optional[Tensor], grad_w: Optional[Tensor], x: Tensor, w: Tensor,
+                              labels: IndexTensor, ug: Tensor, row_lse: Optional[Tensor] = None,
+                              accumulate: bool = True) -> None:
+    """linear_cross_entropy_forward and _backward in one call, for a training step: the logits'
+    product is made once."""
+    (rows, dim), (classes, _) = _matrix("x", x), _matrix("w", w)
+    _lib.call("mh_linear_cross_entropy_step", _want("loss", loss, (1,)),
+              _want("row_lse", row_lse, (rows,), optional=True), _want("grad_x", grad_x, (rows, dim), optional=True),
+              _want("grad_w", grad_w, (classes, dim), optional=True), _want("x", x, (rows, dim)),
+              _want("w", w, (classes, dim)), _want("labels", labels, (rows,), index=True), _want("ug", ug, (1,)),
+              rows, dim, classes, int(bool(accumulate)))

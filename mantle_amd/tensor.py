@@ -135,6 +135,12 @@ class Tensor:
                 pass
             self._ptr = None
 
+    @staticmethod
+    def over(ptr: int, shape, owner=None) -> "Tensor":
+        """A tensor over device memory that another allocator holds, `owner` kept alive with it. What
+        wrote that memory has to be done: the library works on a stream of its own."""
+        return Tensor(as_shape(shape), _ptr=int(ptr), _owner=owner if owner is not None else int(ptr))
+
     # ---- properties ----
     def shape(self) -> TensorShape:
         return self._shape
@@ -190,3 +196,51 @@ class Tensor:
 
     def __repr__(self) -> str:
         return f"Tensor({self._shape})"
+
+
+class IndexTensor(Tensor):
+    """int32 tensor in device memory: class labels, chosen ids and counts. The reference holds these
+    as one-hot float tensors (loss.mojo:45-61), which a large vocabulary rules out."""
+
+    __slots__ = ()
+
+    @staticmethod
+    def from_numpy(a) -> "IndexTensor":
+        a = np.asarray(a)
+        if a.dtype.kind not in "iub" or (a.size and (a.max() > 0x7fffffff or a.min() < -0x80000000)):
+            raise ValueError(f"ids are whole numbers of 32 bits, not {a.dtype}")
+        a = np.ascontiguousarray(a, dtype=np.int32)
+        t = IndexTensor(TensorShape(a.shape if a.ndim else (1,)))
+        if a.size:
+            _lib.call("mh_memcpy_h2d", t._ptr, a.ctypes.data, a.size * 4)
+        return t
+
+    @staticmethod
+    def over(ptr: int, shape, owner=None) -> "IndexTensor":
+        return IndexTensor(as_shape(shape), _ptr=int(ptr), _owner=owner if owner is not None else int(ptr))
+
+    def to_numpy(self) -> np.ndarray:
+        out = np.empty(self._shape.dims, dtype=np.int32)
+        if out.size:
+            _lib.call("mh_memcpy_d2h", out.ctypes.data, self._ptr, out.size * 4)
+        return out
+
+    def copy(self) -> "IndexTensor":
+        t = IndexTensor(self._shape)
+        _lib.call("mh_memcpy_d2d", t._ptr, self._ptr, self.num_elements() * 4)
+        return t
+
+    def share(self) -> "IndexTensor":
+        return IndexTensor(self._shape, _ptr=self._ptr, _owner=self)
+
+    def __getitem__(self, i: int) -> int:
+        v = np.empty(1, dtype=np.int32)
+        _lib.call("mh_memcpy_d2h", v.ctypes.data, self._ptr + 4 * int(i), 4)
+        return int(v[0])
+
+    def __setitem__(self, i: int, val: int) -> None:
+        v = np.array([val], dtype=np.int32)
+        _lib.call("mh_memcpy_h2d", self._ptr + 4 * int(i), v.ctypes.data, 4)
+
+    def __repr__(self) -> str:
+        return f"IndexTensor({self._shape})"

@@ -1,0 +1,300 @@
+"""The vocabulary head's cross entropy (linear_cross_entropy_*) against the formulas in 64 bits.
+
+Tolerances, from the arithmetic: an operand is held with 22 bits (2^-23 of itself off, and the product of
+two remainders, below 2^-22, is dropped), so a product is off by 2^-21 of |x w| at most. A sum over K
+elements takes 3 K / 16 additions into an fp32 accumulator, each off by at most 2^-23 of the sum so far
+(a truncating adder; a rounding one has half). From these: Z, the bound of a logit; then a log-sum-exp is
+off by Z, the sums' roundings and the log's; an element of G by p (Z + L + 2^-21) and 2^-22 of itself or
+2^-40; a gradient by the sum of |dG| |operand| and its own product's bound."""
+import numpy as np
+import pytest
+import torch
+
+from util import GpuEngine
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def m_():
+    return GpuEngine().m
+
+
+def reference(x, w, labels, ug=1.0, device="cpu"):
+    """loss, row_loss, row_lse, grad_x, grad_w and the bounds of their errors."""
+    x, w = (torch.from_numpy(a).to(device).double() for a in (x, w))
+    labels = torch.from_numpy(labels).to(device).long()
+    keep = labels >= 0
+    x = torch.where(keep[:, None], x, 0.0)
+    n = max(1, int(keep.sum()))
+    rows, dim = x.shape
+    classes = w.shape[0]
+    z = x @ w.t()
+    lse = torch.logsumexp(z, 1)
+    at = labels.clamp(min=0)
+    picked = z[torch.arange(rows, device=device), at]
+    row = torch.where(keep, lse - picked, 0.0)
+    p = torch.exp(z - lse[:, None])
+    g = p.clone()
+    g[torch.arange(rows, device=device), at] -= 1.0
+    g *= keep[:, None]
+    c = ug / n
+
+    def product(k):
+        return 2.0 ** -21 + (3 * k / 16 + 8) * 2 * U
+
+    bz = (x.abs() @ w.abs().t()) * product(dim)
+    # 64 or 128 terms a lane, then the groups' statistics
+    bl = bz.amax(1) + (128 + classes / 512 + 40) * U + 4 * U * lse.abs()
+    brow = bl + bz[torch.arange(rows, device=device), at] + 4 * U * (lse.abs() + picked.abs())
+    dg = p * (bz + bl[:, None] + 2.0 ** -21 + 8 * U * (z.abs() + lse.abs()[:, None])) + 2.0 ** -22 * g.abs() + 2.0 ** -40
+    dg *= keep[:, None]
+    bgx = abs(c) * (dg @ w.abs() + (g.abs() @ w.abs()) * product(classes + 256))
+    bgw = abs(c) * (dg.t() @ x.abs() + (g.abs().t() @ x.abs()) * product(rows + 256))
+    out = {"loss": row.sum() / n, "row_loss": row, "row_lse": torch.where(keep, lse, 0.0), "grad_x": c * (g @ w),
+           "grad_w": c * (g.t() @ x)}
+    bound = {"loss": (brow * keep).sum() / n + 4 * U * out["loss"].abs(), "row_loss": brow * keep,
+             "row_lse": bl * keep, "grad_x": bgx + 4 * U * out["grad_x"].abs(), "grad_w": bgw + 4 * U * out["grad_w"].abs()}
+    return ({k: v.cpu().numpy() for k, v in out.items()}, {k: v.cpu().numpy() for k, v in bound.items()})
+
+
+def inputs(rows, dim, classes, seed, left_out=0.1, std=2.0):
+    r = np.random.RandomState(seed)
+    x = r.standard_normal((rows, dim)).astype(np.float32)
+    w = (r.standard_normal((classes, dim)) * std / np.sqrt(dim)).astype(np.float32)
+    labels = r.randint(0, classes, rows).astype(np.int32)
+    labels[r.uniform(size=rows) < left_out] = -100
+    return x, w, labels
+
+
+def run(m, x, w, labels, ug=1.0, how="step", grads=None):
+    """The results by name. `grads`: (grad_x, grad_w) that the gradients are added to."""
+    rows, dim = x.shape
+    classes = w.shape[0]
+    tx, tw, tl, tu = m.Tensor.from_numpy(x), m.Tensor.from_numpy(w), m.IndexTensor.from_numpy(labels), m.Tensor.from_numpy(np.float32([ug]))
+    loss, lse, rl = m.Tensor(1), m.Tensor(rows), m.Tensor(rows)
+    add = grads is not None
+    fill = np.full  # what accumulate=False has to write over
+    gx = m.Tensor.from_numpy(grads[0] if add else fill((rows, dim), 7.0, np.float32))
+    gw = m.Tensor.from_numpy(grads[1] if add else fill((classes, dim), 7.0, np.float32))
+    if how == "step":
+        m.linear_cross_entropy_step(loss, gx, gw, tx, tw, tl, tu, row_lse=lse, accumulate=add)
+    else:
+        m.linear_cross_entropy_forward(loss, lse, tx, tw, tl, row_loss=rl)
+        m.linear_cross_entropy_backward(gx, gw, tx, tw, tl, lse, tu, accumulate=add)
+    out = {"loss": loss.to_numpy()[0], "row_lse": lse.to_numpy(), "grad_x": gx.to_numpy(), "grad_w": gw.to_numpy()}
+    if how != "step":
+        out["row_loss"] = rl.to_numpy()
+    return out
+
+
+def check(got, want, bound, what=""):
+    for k, v in got.items():
+        off = np.abs(v.astype(np.float64) - want[k])
+        assert np.isfinite(v).all(), f"{what} {k}: not finite"
+        over = off > bound[k] + 1e-42
+        assert not over.any(), f"{what} {k}: {over.sum()} of {over.size} beyond the bound, worst {off.max():.3g} of {np.max(bound[k]):.3g}"
+        # the roundings are as good as random: their sum is far below the bound of the worst case
+        norm = np.linalg.norm(want[k])
+        if norm > 0 and k.startswith("grad"):
+            assert np.linalg.norm(off) <= 1e-5 * norm, f"{what} {k}: {np.linalg.norm(off) / norm:.3g} off in the norm"
+
+
+SIZES = [(1, 1, 1), (1, 1, 2), (2, 3, 5), (1, 70, 300), (16, 64, 1000), (31, 33, 63), (33, 100, 257), (64, 128, 256),
+         (257, 31, 2049), (300, 129, 5003), (130, 513, 999), (1024, 40, 130), (255, 16, 256), (256, 32, 8191)]
+
+
+@pytest.mark.parametrize("how", ["step", "two calls"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_sizes(size, how):
+    print(f"\n[head] {size} {how}", flush=True)
+    x, w, labels = inputs(*size, seed=sum(size))
+    want, bound = reference(x, w, labels, ug=0.75)
+    check(run(m_(), x, w, labels, ug=0.75, how=how), want, bound, str(size))
+
+
+def test_larger_tiles_and_splits():
+    """Products of whole 256 x 256 tiles, and gradients whose long axis is split."""
+    m = m_()
+    for size in ((4096, 96, 5000), (2048, 300, 9001), (300, 2500, 4000)):
+        print(f"\n[head] {size}", flush=True)
+        x, w, labels = inputs(*size, seed=3)
+        want, bound = reference(x, w, labels, device="cuda")
+        check(run(m, x, w, labels), want, bound, str(size))
+
+
+def test_rows_in_chunks():
+    """2^21 classes: the logits of 256 rows at a time, the last chunk shorter, grad_w over all of them."""
+    x, w, labels = inputs(600, 4, 1 << 21, seed=5)
+    print("\n[head] chunks", flush=True)
+    got = run(m_(), x, w, labels)
+    two = run(m_(), x, w, labels, how="two calls")
+    for k in got:
+        assert np.array_equal(got[k], two[k]), k
+    # the formulas 100 rows at a time (the loss's mean is over all 600), with reference()'s bounds, which
+    # grow with a logit's size: four elements of x and w make logits beyond +-30 here, whose fp32 step
+    # alone is 2^-20 of e^z
+    n = int((labels >= 0).sum())
+    loss, gw, bw = 0.0, 0.0, 0.0
+    for r in range(0, 600, 100):
+        part = labels[r:r + 100]
+        share = int((part >= 0).sum()) / n
+        want, bound = reference(x[r:r + 100], w, part, device="cuda")
+        loss += want["loss"] * share
+        gw, bw = gw + want["grad_w"] * share, bw + bound["grad_w"] * share
+        check({"row_lse": got["row_lse"][r:r + 100], "grad_x": got["grad_x"][r:r + 100]},
+              {"row_lse": want["row_lse"], "grad_x": want["grad_x"] * share},
+              {"row_lse": bound["row_lse"], "grad_x": bound["grad_x"] * share}, f"rows {r}")
+    check({"loss": np.float32(got["loss"]), "grad_w": got["grad_w"]}, {"loss": loss, "grad_w": gw},
+          {"loss": 1e-6 * abs(loss), "grad_w": bw}, "chunks")
+
+
+def test_accumulates():
+    m = m_()
+    x, w, labels = inputs(70, 50, 600, seed=9)
+    r = np.random.RandomState(1)
+    g0 = r.standard_normal((70, 50)).astype(np.float32), r.standard_normal((600, 50)).astype(np.float32)
+    plain = run(m, x, w, labels)
+    for how in ("step", "two calls"):
+        got = run(m, x, w, labels, how=how, grads=g0)
+        assert np.array_equal(got["grad_x"], g0[0] + plain["grad_x"])
+        assert np.array_equal(got["grad_w"], g0[1] + plain["grad_w"])
+
+
+def test_same_bits_again_and_in_both_forms():
+    m = m_()
+    x, w, labels = inputs(300, 200, 3001, seed=10)
+    one, two, three = run(m, x, w, labels), run(m, x, w, labels), run(m, x, w, labels, how="two calls")
+    for k in one:
+        assert np.array_equal(one[k], two[k]) and np.array_equal(one[k], three[k]), k
+
+
+def test_rows_left_out_may_hold_anything():
+    m = m_()
+    x, w, labels = inputs(90, 65, 500, seed=11, left_out=0.3)
+    want, bound = reference(x, w, labels)
+    out = np.flatnonzero(labels < 0)
+    bad = x.copy()
+    bad[out[0]], bad[out[1]], bad[out[2]], bad[out[3:]] = np.nan, np.inf, 3e38, -3.4028234663852886e38
+    labels[out[0]] = -1
+    labels[out[1]] = -2147483648
+    check(run(m, bad, w, labels), want, bound, "left out")
+    g0 = np.full((90, 65), -0.0, np.float32), np.zeros((500, 65), np.float32)
+    got = run(m, bad, w, labels, grads=g0)
+    assert (got["grad_x"][out].view(np.uint32) == 0x80000000).all()  # left as they were
+
+
+def test_no_row_kept():
+    m = m_()
+    x, w, labels = inputs(40, 20, 100, seed=12)
+    labels[:] = -1
+    x[:] = np.nan
+    for how in ("step", "two calls"):
+        got = run(m, x, w, labels, how=how)
+        assert got["loss"] == 0 and not got["row_lse"].any() and not got["grad_x"].any() and not got["grad_w"].any()
+
+
+def test_no_rows():
+    m = m_()
+    x, w, labels = np.zeros((0, 20), np.float32), np.ones((30, 20), np.float32), np.zeros(0, np.int32)
+    for how in ("step", "two calls"):
+        got = run(m, x, w, labels, how=how)
+        assert got["loss"] == 0 and not got["grad_w"].any()
+        assert (run(m, x, w, labels, how=how, grads=(x, w))["grad_w"] == 1).all()
+
+
+def test_label_past_the_classes_shows():
+    m = m_()
+    for label in (100, 2147483647):
+        x, w, labels = inputs(40, 20, 100, seed=13)
+        labels[:] = np.arange(40)
+        labels[7] = label
+        got = run(m, x, w, labels)
+        assert np.isnan(got["loss"]) and np.isnan(got["row_lse"][7]) and np.isfinite(np.delete(got["row_lse"], 7)).all()
+        assert np.isnan(got["grad_x"][7]).all() and np.isfinite(np.delete(got["grad_x"], 7, 0)).all()
+        assert np.isnan(got["grad_w"]).all()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_not_finite_shows(value):
+    m = m_()
+    x, w, labels = inputs(40, 20, 100, seed=14, left_out=0)
+    x[3, 5] = value
+    got = run(m, x, w, labels)
+    assert np.isnan(got["loss"]) and np.isnan(got["row_lse"][3]) and np.isfinite(np.delete(got["row_lse"], 3)).all()
+    x, w, labels = inputs(40, 20, 100, seed=14, left_out=0)
+    w[99, 19] = value
+    assert np.isnan(run(m, x, w, labels)["loss"])
+
+
+@pytest.mark.parametrize("sx, sw", [(1e4, 1e-6), (1e-20, 1e20), (1e-30, 1e15), (1e18, 1e-18), (0.0, 1.0), (1.0, 0.0), (1.0, 40.0)])
+def test_scales(sx, sw):
+    """Operands of any scale: the powers of two follow the largest element. The last: logits to +-300."""
+    m = m_()
+    x, w, labels = inputs(65, 40, 333, seed=15)
+    x, w = (x * np.float32(sx)).astype(np.float32), (w * np.float32(sw)).astype(np.float32)
+    want, bound = reference(x, w, labels)
+    got = run(m, x, w, labels)
+    for k in got:
+        off = np.abs(got[k].astype(np.float64) - want[k])
+        # results below the least normal number round to a step of 2^-149
+        assert (off <= bound[k] + 2.0 ** -148).all(), (k, off.max())
+
+
+def test_one_gradient_only():
+    m = m_()
+    x, w, labels = inputs(70, 50, 600, seed=16)
+    both = run(m, x, w, labels)
+    tx, tw, tl, tu = m.Tensor.from_numpy(x), m.Tensor.from_numpy(w), m.IndexTensor.from_numpy(labels), m.Tensor.from_numpy(np.float32([1]))
+    loss, gx, gw = m.Tensor(1), m.Tensor(70, 50), m.Tensor(600, 50)
+    m.linear_cross_entropy_step(loss, gx, None, tx, tw, tl, tu)
+    assert np.array_equal(gx.to_numpy(), both["grad_x"])
+    m.linear_cross_entropy_step(loss, None, gw, tx, tw, tl, tu)
+    assert np.array_equal(gw.to_numpy(), both["grad_w"])
+    m.linear_cross_entropy_step(loss, None, None, tx, tw, tl, tu)
+    assert loss.to_numpy()[0] == both["loss"]
+
+
+def test_gradients_against_differences():
+    """<grad, d> against (loss(+h d) - loss(-h d)) / 2 h. The loss is off by up to 2^-22 of its size, so the
+    quotient by 2^-22 loss / h; the third derivative of a row's log-sum-exp along d is at most 2 (max |z'|)^3,
+    the loss is the rows' mean, and the quotient's error a sixth of its third derivative times h^2."""
+    m = m_()
+    x, w, labels = inputs(24, 12, 50, seed=17)
+    g = run(m, x, w, labels)
+    r = np.random.RandomState(2)
+    for which in ("x", "w"):
+        a = x if which == "x" else w
+        d = r.standard_normal(a.shape).astype(np.float32)
+        h = 2.0 ** -6
+        loss, slope = [], 0.0
+        for s in (h, -h):
+            a2 = (a + np.float32(s) * d).astype(np.float32)
+            xx, ww = (a2, w) if which == "x" else (x, a2)
+            loss.append(float(run(m, xx, ww, labels)["loss"]))
+        row = np.abs(d @ w.T if which == "x" else x @ d.T).max(1).astype(np.float64)
+        slope, cubed = row.max(), (row ** 3).mean()
+        quotient, inner = (loss[0] - loss[1]) / (2 * h), float((g["grad_" + which].astype(np.float64) * d).sum())
+        tol = 2.0 ** -22 * loss[0] / h + cubed * h * h / 3 + 2.0 ** -23 * np.abs(a).max() * slope / h
+        assert abs(quotient - inner) <= tol, (which, quotient, inner, tol)
+        assert tol < abs(inner) or abs(inner) < 0.05
+
+
+def test_memory_of_another_allocator():
+    m = m_()
+    x, w, labels = inputs(70, 51, 601, seed=18)
+    want = run(m, x, w, labels)
+    # odd addresses: views that start one element into an allocation
+    hold = [torch.zeros(a.size + 1, device="cuda", dtype=torch.float32 if a.dtype == np.float32 else torch.int32) for a in (x, w, labels)]
+    for t, a in zip(hold, (x, w, labels)):
+        t[1:] = torch.from_numpy(a.reshape(-1)).cuda()
+    gx, gw = torch.zeros(x.size + 1, device="cuda"), torch.zeros(w.size + 1, device="cuda")
+    torch.cuda.synchronize()
+    tx, tw = (m.Tensor.over(t.data_ptr() + 4, a.shape, t) for t, a in zip(hold, (x, w)))
+    tl = m.IndexTensor.over(hold[2].data_ptr() + 4, labels.shape, hold[2])
+    loss, tu = m.Tensor(1), m.Tensor.from_numpy(np.float32([1]))
+    m.linear_cross_entropy_step(loss, m.Tensor.over(gx.data_ptr() + 4, x.shape), m.Tensor.over(gw.data_ptr() + 4, w.shape),
+                                tx, tw, tl, tu)
+    m.sync()
+    assert np.array_equal(gx[1:].cpu().numpy().reshape(x.shape), want["grad_x"]) and gx[0] == 0
+    assert np.array_equal(gw[1:].cpu().numpy().reshape(w.shape), want["grad_w"]) and gw[0] == 0
