@@ -31,7 +31,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kBlk = 2048;       // bytes of a panel block: 32 x 16 elements, hi and lo
 constexpr int kGExp = 15;        // the power of two G is held with
-constexpr int kAmaxBlocks = 256;  // workgroups of k_amax for each of x and w
+constexpr int kAmaxBlocks = 1024;  // workgroups of k_amax for each of x and w
 
 // What the kernels of one call share, in device memory.
 struct HeadInfo {
@@ -39,7 +39,8 @@ struct HeadInfo {
     int32_t kept;    // rows with a label
     int32_t pad;
 };
-struct HeadPart {  // k_amax's partials
+static_assert(kAmaxBlocks == 4 * 256, "a workgroup of k_split reads four partials a thread");
+struct alignas(16) HeadPart {  // k_amax's partials
     float ax[kAmaxBlocks], aw[kAmaxBlocks];
     int32_t kept[kAmaxBlocks];
 };
@@ -68,6 +69,10 @@ __device__ __forceinline__ float finite_abs(float v) {
 }
 
 // The largest finite magnitude of x's kept rows and of w, and the kept rows' count, as partials.
+__device__ __forceinline__ float amax4(float a, vf4 v) {
+    return __builtin_fmaxf(__builtin_fmaxf(a, __builtin_fmaxf(finite_abs(v.x), finite_abs(v.y))),
+                           __builtin_fmaxf(finite_abs(v.z), finite_abs(v.w)));
+}
 __global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, const float* w, const int32_t* labels,
                                               int64_t rows, int64_t dim, int64_t nw) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -81,15 +86,22 @@ __global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, co
         for (int64_t r = (int64_t)b * 4 + wave; r < rows; r += kAmaxBlocks * 4) {
             if (labels[r] < 0) continue;  // a row left out may hold anything
             ++kept;
-            for (int64_t k = lane; k < dim; k += 64) a = __builtin_fmaxf(a, finite_abs(x[r * dim + k]));
+            const float* row = x + r * dim;
+#pragma unroll 4
+            for (int64_t k = lane * 4; k + 3 < dim; k += 256) a = amax4(a, *reinterpret_cast<const vf4u*>(row + k));
+            if (lane < (dim & 3)) a = __builtin_fmaxf(a, finite_abs(row[(dim & ~(int64_t)3) + lane]));
         }
     } else {
-        const int64_t nq = nw >> 2;
-        for (int64_t q = (int64_t)b * 256 + threadIdx.x; q < nq; q += kAmaxBlocks * 256) {
-            const vf4 v = *reinterpret_cast<const vf4u*>(w + 4 * q);
-            a = __builtin_fmaxf(a, __builtin_fmaxf(__builtin_fmaxf(finite_abs(v.x), finite_abs(v.y)),
-                                                   __builtin_fmaxf(finite_abs(v.z), finite_abs(v.w))));
+        const int64_t nq = nw >> 2, step = kAmaxBlocks * 256;
+        int64_t q = (int64_t)b * 256 + threadIdx.x;
+        for (; q + 7 * step < nq; q += 8 * step) {  // eight loads in flight: 0.52 -> 0.2 ms a GB
+            vf4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = ld_ntu(w + 4 * (q + u * step));
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a = amax4(a, v[u]);
         }
+        for (; q < nq; q += step) a = amax4(a, ld_ntu(w + 4 * q));
         if (b == 0 && threadIdx.x < (nw & 3)) a = __builtin_fmaxf(a, finite_abs(w[4 * nq + threadIdx.x]));
     }
     a = wave_max(a);
@@ -150,7 +162,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
     const SplitOne s = isx ? sx : sw;
     const int64_t tile = isx ? blockIdx.x : blockIdx.x - ntx;
     const int64_t r0 = tile / s.tiles_c * kSplitTile, c0 = tile % s.tiles_c * kSplitTile;
-    float a = isx ? part->ax[tid] : part->aw[tid];
+    float a = amax4(0.0f, reinterpret_cast<const vf4*>(isx ? part->ax : part->aw)[tid]);
     a = wave_max(a);
     if (lane == 0) red[wave] = a;
     // the tile's rows, a wavefront a row
@@ -186,8 +198,8 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
         }
     }
     if (blockIdx.x == 0) {  // the scales and the count, for the kernels behind
-        float b = wave_max(part->aw[tid]);
-        int32_t kept = part->kept[tid];
+        float b = wave_max(amax4(0.0f, reinterpret_cast<const vf4*>(part->aw)[tid]));
+        int32_t kept = part->kept[tid] + part->kept[tid + 256] + part->kept[tid + 512] + part->kept[tid + 768];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o);
         __syncthreads();
@@ -219,7 +231,7 @@ struct GemmArg {
     // EPI_LOGITS: M is classes, N rows
     const int32_t* labels;   // at the first row of the panel; EPI_GRAD: rows to leave alone, or null
     int64_t rows, classes;   // of the operands; rows counted from the panel's first
-    float* stat;             // [class groups of a wavefront][2][stat_ld]: maximum, sum of exponentials
+    float* stat;             // [64-class groups][2][stat_ld]: maximum, sum of exponentials
     int64_t stat_ld;
     float* target;           // [rows] the label's logit
     char* z;                 // the logits, in the blocks of G's row panels, or null
@@ -236,14 +248,30 @@ struct GemmArg {
 // ug / kept and the exponent that undoes the panels' scales, applied to one sum.
 __device__ __forceinline__ float grad_value(float acc, float c, int e) { return c * __builtin_ldexpf(acc, e); }
 
+// Waits until at most N of this wavefront's loads are under way and its LDS reads are done, then for the
+// workgroup's other wavefronts. The compiler moves nothing across.
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x70 | N);  // vmcnt N (below 16), lgkmcnt 0, expcnt as it is
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// Four stages of 16 of the contracted axis circle through LDS. In step s a wavefront waits for its loads of
+// stage s + 1, meets the others, starts reading stage s + 1 into registers and loading stage s + 3 into
+// LDS (over stage s - 1, whose last reads ended before the barrier), and multiplies stage s, which is in
+// registers already: neither the loads' latency nor LDS's stands before a matrix instruction.
 template <int TM, int TN, int WM, int WN, int EPI>
-__global__ __launch_bounds__(WM* WN * 64) void k_gemm(GemmArg g) {
+__global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
     constexpr int kWaves = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32;
-    constexpr int kRowB = 2 * kBlk;                       // bytes a row block adds to a stage: 32 of the axis
-    constexpr int kStage = (TM + TN) / 32 * kRowB;
-    constexpr int kLoads = (TM + TN) / 32 / kWaves;       // row blocks a wavefront brings a stage
-    static_assert((TM + TN) / 32 % kWaves == 0, "loads");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    constexpr int kRows = (TM + TN) / 32;        // row blocks of a stage
+    constexpr int kStage = kRows * kBlk;
+    constexpr int kLoads = kRows * 2 / kWaves;   // 1 KB loads of a wavefront a stage
+    static_assert(kLoads == 4 && kRows % kWaves == 0, "the waits below count 4 loads a stage");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kStage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -258,57 +286,70 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(GemmArg g) {
     const int64_t tm = grp * 8 + (id - grp * gsz) % gm, tn = (id - grp * gsz) / gm;
 
     const int64_t k0 = (int64_t)blockIdx.y * g.kb;
-    int64_t kb = g.kb_all - k0;
-    if (kb > g.kb) kb = g.kb;
-    const int S = (int)(kb / 2);
+    const int64_t kb = g.kb_all - k0 < g.kb ? g.kb_all - k0 : g.kb;
+    const int S = (int)kb;  // even; 0 or less for a split past the end
 
-    const char* src[kLoads];
+    const char* src[2];  // the two row blocks this wavefront brings
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int rb = wave * kLoads + i;
+    for (int i = 0; i < 2; ++i) {
+        const int rb = wave * 2 + i;
         src[i] = (rb < TM / 32 ? g.a + ((tm * (TM / 32) + rb) * g.akb + k0) * kBlk
-                               : g.b + ((tn * (TN / 32) + rb - TM / 32) * g.bkb + k0) * kBlk) + lane * 16;
+                               : g.b + ((tn * (TN / 32) + rb - TM / 32) * g.bkb + k0) * kBlk);
     }
-    auto load = [&](int s, int buf) {
+    const uint32_t lane16 = lane * 16;
+    auto load = [&](int s) {  // past the end: the last stage again, into a buffer that no one reads
+        const int64_t at = (int64_t)(s < S ? s : S - 1) * kBlk;
+        char* to = lds + (s & 3) * kStage + wave * 2 * kBlk;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            char* to = lds + buf * kStage + (wave * kLoads + i) * kRowB;
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(src[i >> 1] + at + (i & 1) * 1024 + lane16),
+                (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+    };
+    auto read = [&](int s, half8(&a)[MI][2], half8(&b)[NI][2]) {
+        const char* la = lds + (s & 3) * kStage + wm * MI * kBlk + lane * 16;
+        const char* lb = lds + (s & 3) * kStage + (TM / 32 + wn * NI) * kBlk + lane * 16;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(src[i] + (int64_t)s * kRowB + j * 1024),
-                    (__attribute__((address_space(3))) void*)(to + j * 1024), 16, 0, 0);
+        for (int j = 0; j < NI; ++j) {
+            b[j][0] = *reinterpret_cast<const half8*>(lb + j * kBlk);
+            b[j][1] = *reinterpret_cast<const half8*>(lb + j * kBlk + 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            a[i][0] = *reinterpret_cast<const half8*>(la + i * kBlk);
+            a[i][1] = *reinterpret_cast<const half8*>(la + i * kBlk + 1024);
         }
     };
 
     f32x16 acc[MI][NI] = {};
-    if (S > 0) load(0, 0);
-    __syncthreads();
-    for (int s = 0; s < S; ++s) {
-        if (s + 1 < S) load(s + 1, (s + 1) & 1);
-        const char* la = lds + (s & 1) * kStage + wm * MI * kRowB + lane * 16;
-        const char* lb = lds + (s & 1) * kStage + (TM / 32 + wn * NI) * kRowB + lane * 16;
+    auto step = [&](int s, half8(&a)[MI][2], half8(&b)[NI][2], half8(&an)[MI][2], half8(&bn)[NI][2]) {
+        wait_and_meet<4>();
+        read(s + 1, an, bn);
+        load(s + 3);
+        __builtin_amdgcn_sched_barrier(0);  // issued before the matrix instructions, not where registers are fewest
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            half8 b[NI][2];
+        for (int i = 0; i < MI; ++i) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                b[j][0] = *reinterpret_cast<const half8*>(lb + j * kRowB + kk * kBlk);
-                b[j][1] = *reinterpret_cast<const half8*>(lb + j * kRowB + kk * kBlk + 1024);
-            }
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                const half8 hi = *reinterpret_cast<const half8*>(la + i * kRowB + kk * kBlk);
-                const half8 lo = *reinterpret_cast<const half8*>(la + i * kRowB + kk * kBlk + 1024);
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0);
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, b[j][1], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, b[j][0], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, b[j][0], acc[i][j], 0, 0, 0);
-            }
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
         }
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (S > 0) {
+        half8 a0[MI][2], b0[NI][2], a1[MI][2], b1[NI][2];
+        load(0);
+        load(1);
+        load(2);
+        wait_and_meet<8>();
+        read(0, a0, b0);
+        for (int s = 0; s < S; s += 2) {
+            step(s, a0, b0, a1, b1);
+            step(s + 1, a1, b1, a0, b0);
+        }
+        wait_and_meet<0>();  // no load into LDS outlives the workgroup
     }
 
     // acc[i][j][r]: row (of M) 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4, column (of N) 32 j + lane % 32
@@ -316,7 +357,6 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(GemmArg g) {
     if constexpr (EPI == EPI_LOGITS) {
         const int e = -(g.info->ex + g.info->ew);
         const int64_t v0 = tm * TM + wm * MI * 32;  // the wavefront's first class
-        const int64_t grp_v = tm * WM + wm;         // its group of MI * 32 classes
         // register r of tile i holds class v0 + 4 half + cls_of(i, r): compared with the label and the
         // last class relative to the first two terms
         const int64_t left = g.classes - v0 - 4 * half;
@@ -325,35 +365,45 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(GemmArg g) {
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             const int64_t n = tn * TN + (wn * NI + j) * 32 + col;
-            const int64_t want = (n < g.rows ? (int64_t)g.labels[n] : -1) - v0 - 4 * half;
-            const int label = want < 0 || want >= MI * 32 ? -1 : (int)want;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], e);
             if (g.stat) {
-                float top = -__builtin_inff();
+                const int64_t want = (n < g.rows ? (int64_t)g.labels[n] : -1) - v0 - 4 * half;
+                if (want >= 0 && want < MI * 32) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                    for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float z = acc[i][j][r];
-                        if (cls_of(i, r) == label) g.target[n] = z;
-                        if (cls_of(i, r) < last) top = z > top || z != z ? z : top;
+                        for (int r = 0; r < 16; ++r)
+                            if (cls_of(i, r) == (int)want) g.target[n] = acc[i][j][r];
+                }
+                // the maximum and the sum of exponentials of each 64 classes, whatever the tile, so that the
+                // sums' order does not depend on it: one multiply-add and one exp2 a logit; only the last
+                // class's wavefront masks what lies past it
+                const bool whole = g.classes - v0 >= MI * 32;
+#pragma unroll
+                for (int h = 0; h < MI / 2; ++h) {
+                    float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+                    for (int i = 2 * h; i < 2 * h + 2; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (whole || cls_of(i, r) < last) top = __builtin_fmaxf(top, acc[i][j][r]);
+                    top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                    const float base = top == -__builtin_inff() ? 0.0f : top * -1.44269504088896341f;
+#pragma unroll
+                    for (int i = 2 * h; i < 2 * h + 2; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (whole || cls_of(i, r) < last)
+                                sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], 1.44269504088896341f, base));
+                    sum += __shfl_xor(sum, 32);  // a NaN among the logits is in the sum, whatever the maximum says
+                    if (half == 0) {
+                        const int64_t at = ((v0 >> 6) + h) * 2 * g.stat_ld + n;
+                        g.stat[at] = top;
+                        g.stat[at + g.stat_ld] = sum;
                     }
-                const float other = __shfl_xor(top, 32);
-                top = other > top || other != other ? other : top;
-                float sum = 0.0f;
-                const float base = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (cls_of(i, r) < last) sum += exp_neg(acc[i][j][r] - base);
-                sum += __shfl_xor(sum, 32);
-                if (half == 0) {
-                    g.stat[grp_v * 2 * g.stat_ld + n] = top;
-                    g.stat[(grp_v * 2 + 1) * g.stat_ld + n] = sum;
                 }
             }
             if (g.z) {  // 4 consecutive classes a lane: 16 bytes of the block of (n / 32, v / 16)
@@ -426,46 +476,64 @@ __global__ __launch_bounds__(256) void k_join(GemmArg g, int32_t splits, int64_t
 // ---------------------------------------------------------------------------------------
 // rows' statistics, the loss, and G's panels
 // ---------------------------------------------------------------------------------------
-// Each row's log-sum-exp from its class groups' statistics: 32 rows x 8 threads a workgroup.
-__global__ __launch_bounds__(256) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
-                                                  const float* target, const int32_t* labels, int64_t rows,
-                                                  int64_t classes, float* row_lse, float* row_loss) {
-    __shared__ float sm[8][32], ss[8][32];
+// Each row's log-sum-exp from its class groups' statistics, and the workgroup's sum of losses: 32 rows x 32
+// threads, whose loads of a group's statistics are 128 bytes each.
+constexpr int kLseParts = 32;
+__global__ __launch_bounds__(1024) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
+                                                   const float* target, const int32_t* labels, int64_t rows,
+                                                   int64_t classes, float* row_lse, float* row_loss, double* block_loss) {
+    __shared__ float sm[kLseParts][32], ss[kLseParts][32];
     const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
     const int64_t n = (int64_t)blockIdx.x * 32 + r;
     float top = -__builtin_inff(), sum = 0.0f;
-    for (int64_t gr = p; gr < groups; gr += 8) {
-        const float m = stat[gr * 2 * stat_ld + n], s = stat[(gr * 2 + 1) * stat_ld + n];
-        if (m != m) top = m;
+    // a sum that is not a number stays so; a group of logits at minus infinity adds nothing
+    auto join = [&](float m, float s) {
         if (m > top) {
             sum = sum * exp_neg(top - m) + s;
             top = m;
-        } else if (m > -__builtin_inff()) {
+        } else if (m > -__builtin_inff() || s != s) {
             sum += s * exp_neg(m - top);
         }
+    };
+    for (int64_t gr = p; gr < groups; gr += 4 * kLseParts) {
+        float m[4], s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t at = gr + u * kLseParts < groups ? gr + u * kLseParts : gr;
+            m[u] = stat[at * 2 * stat_ld + n];
+            s[u] = stat[(at * 2 + 1) * stat_ld + n];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (gr + u * kLseParts < groups) join(m[u], s[u]);
     }
     sm[p][r] = top;
     ss[p][r] = sum;
     __syncthreads();
-    if (p != 0 || n >= rows) return;
-    float t = -__builtin_inff(), s = 0.0f;
-    for (int i = 0; i < 8; ++i) t = sm[i][r] > t || sm[i][r] != sm[i][r] ? sm[i][r] : t;
-    for (int i = 0; i < 8; ++i)
-        if (sm[i][r] > -__builtin_inff() || sm[i][r] != sm[i][r]) s += ss[i][r] * exp_neg(sm[i][r] - t);
-    const int32_t label = labels[n];
-    float lse = t + mlog(s);
-    if (label >= classes) lse = __builtin_nanf("");  // no such class: shown in the loss and the gradients
-    if (label < 0) lse = 0.0f;
-    row_lse[n] = lse;
-    row_loss[n] = label < 0 ? 0.0f : (label >= classes ? lse : lse - target[n]);
+    if (p != 0) return;
+    for (int i = 1; i < kLseParts; ++i) join(sm[i][r], ss[i][r]);
+    float loss = 0.0f;
+    if (n < rows) {
+        const int32_t label = labels[n];
+        float lse = top + mlog(sum);
+        if (label >= classes) lse = __builtin_nanf("");  // no such class: shown in the loss and the gradients
+        if (label < 0) lse = 0.0f;
+        loss = label < 0 ? 0.0f : (label >= classes ? lse : lse - target[n]);
+        row_lse[n] = lse;
+        if (row_loss) row_loss[n] = loss;
+    }
+    double total = loss;  // lanes 0-31 hold the rows
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    if (r == 0) block_loss[blockIdx.x] = total;
 }
 
-// loss = sum of the rows' losses / kept, in one workgroup and a fixed order.
-__global__ __launch_bounds__(1024) void k_rows_loss(const float* row_loss, int64_t rows, const HeadInfo* info,
+// loss = sum of the workgroups' losses / kept, in one workgroup and a fixed order.
+__global__ __launch_bounds__(1024) void k_rows_loss(const double* block_loss, int64_t blocks, const HeadInfo* info,
                                                     float* loss) {
     __shared__ double red[16];
     double s = 0.0;
-    for (int64_t n = threadIdx.x; n < rows; n += 1024) s += (double)row_loss[n];
+    for (int64_t n = threadIdx.x; n < blocks; n += 1024) s += block_loss[n];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -550,18 +618,32 @@ void launch_gemm(const GemmArg& g, int64_t tiles, int splits) {
         hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, g);
 }
 
-// The tile of a product: 256 x 256 where that fills the chip.
-int tile_of(int64_t m, int64_t n, int64_t splits) {
-    return up(m, 256) / 256 * (up(n, 256) / 256) * splits >= ctx().num_cus ? 256 : 128;
-}
-
-// Splits of a gradient product over its contracted axis of kb blocks: as many as fill the chip, each of
-// 16 blocks at least.
-int splits_of(int64_t m, int64_t n, int64_t kb) {
-    const int64_t tiles = up(m, 128) / 128 * (up(n, 128) / 128);
-    int64_t s = 2 * ctx().num_cus / tiles;
-    if (s > kb / 16) s = kb / 16;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// The tile of a product and, with `split`, the splits of its contracted axis of kb blocks: the least time in
+// units of a 128 x 128 tile's block on a whole CU. A 256 x 256 tile takes four on a CU of its own; of the
+// 128 x 128 ones two share a CU, each half as fast, and reread more (1.2 each). A split holds 16 blocks at
+// least, and its partial sums cost a store and a load.
+struct Form {
+    int tile, splits;
+};
+Form form_of(int64_t m, int64_t n, int64_t kb, bool split) {
+    Form best = {128, 1};
+    double least = 0.0;
+    const int64_t cus = ctx().num_cus;
+    for (const int T : {256, 128}) {
+        const int64_t tiles = up(m, T) / T * (up(n, T) / T);
+        for (int s = 1; s <= 64 && (s == 1 || (split && kb / s >= 16)); ++s) {
+            const int64_t wg = tiles * s, per = T == 256 ? cus : 2 * cus;
+            const int64_t rounds = (wg + per - 1) / per;
+            // a round of small tiles on half the CUs' places runs one a CU
+            const double unit = T == 256 ? 4.0 : (wg <= cus ? 1.2 : 2.4);
+            const double cost = (double)rounds * unit * ((double)kb / s + 8) + (s > 1 ? 0.5 * s * (double)tiles * T * T / (128 * 128) / cus + 8 : 0);
+            if (least == 0.0 || cost < least) {
+                least = cost;
+                best = {T, s};
+            }
+        }
+    }
+    return best;
 }
 
 struct HeadCall {
@@ -578,8 +660,8 @@ struct HeadCall {
 
 // grad [m, n] from panels a (rows of m) and b (rows of n), contracted over kb blocks.
 int grad_product(GemmArg g, int64_t m, int64_t n, int64_t kb, float* part) {
-    const int splits = splits_of(m, n, kb);
-    const int T = splits > 1 ? 128 : tile_of(m, n, 1);
+    const Form f = form_of(m, n, kb, true);
+    const int splits = f.splits, T = f.tile;
     g.m = m;
     g.n = n;
     g.tiles_m = (int32_t)(up(m, T) / T);
@@ -600,8 +682,8 @@ int grad_product(GemmArg g, int64_t m, int64_t n, int64_t kb, float* part) {
 }
 
 size_t part_bytes(int64_t m, int64_t n, int64_t kb) {
-    const int s = splits_of(m, n, kb);
-    return s > 1 ? (size_t)s * up(m, 128) * up(n, 128) * sizeof(float) : 0;
+    const Form f = form_of(m, n, kb, true);
+    return f.splits > 1 ? (size_t)f.splits * up(m, f.tile) * up(n, f.tile) * sizeof(float) : 0;
 }
 
 int head_run(const HeadCall& h) {
@@ -614,7 +696,7 @@ int head_run(const HeadCall& h) {
         chunk = chunk < 256 ? 256 : chunk > kMaxChunk ? kMaxChunk : chunk;
     }
     if (chunk > rowsP) chunk = rowsP;
-    const int64_t groups = clsP / 64;  // of the smaller tile's wavefronts
+    const int64_t groups = clsP / 64;
 
     Carve cv;
     const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
@@ -622,7 +704,7 @@ int head_run(const HeadCall& h) {
     const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * (rowsP / 16) * kBlk) : 0;
     const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * (clsP / 16) * kBlk) : 0;
     const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
-    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP * 4);
+    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / 32 * 8);
     size_t o_z = 0, o_gt = 0, o_sp = 0;
     if (h.train) {
         o_z = cv.take(chunk / 32 * (clsP / 16) * kBlk);
@@ -643,7 +725,7 @@ int head_run(const HeadCall& h) {
     HeadInfo* info = reinterpret_cast<HeadInfo*>(base + o_info);
     HeadPart* part = reinterpret_cast<HeadPart*>(base + o_part);
     float* lse = h.row_lse_out ? h.row_lse_out : reinterpret_cast<float*>(base + o_lse);
-    float* row_loss = h.row_loss ? h.row_loss : reinterpret_cast<float*>(base + o_rl);
+    double* block_loss = reinterpret_cast<double*>(base + o_rl);
     float* target = reinterpret_cast<float*>(base + o_tgt);
 
     hipLaunchKernelGGL(k_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, st, part, h.x, h.w, h.labels, rows, dim,
@@ -673,15 +755,16 @@ int head_run(const HeadCall& h) {
         g.z = h.train ? base + o_z : nullptr;
         g.zkb = clsP / 16;
         // every row and class of the padded chunk gets its logits: the panels behind have no gaps
-        const int T = tile_of(classes, nr, 1);
+        const int T = form_of(classes, nr, dkb, false).tile;
         g.tiles_m = (int32_t)(clsP / T);
         g.tiles_n = (int32_t)(nrP / T);
         const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
         if (T == 256) launch_gemm<256, EPI_LOGITS>(g, tiles, 1);
         else launch_gemm<128, EPI_LOGITS>(g, tiles, 1);
         if (!h.row_lse_in)
-            hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)(nrP / 32)), dim3(256), 0, st, g.stat, clsP / (T / 2),
-                               g.stat_ld, target, h.labels + r0, nr, classes, lse + r0, row_loss + r0);
+            hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)((nr + 31) / 32)), dim3(1024), 0, st, g.stat,
+                               groups, g.stat_ld, target, h.labels + r0, nr, classes, lse + r0,
+                               h.row_loss ? h.row_loss + r0 : nullptr, block_loss + r0 / 32);
         if (!h.train) continue;
         const int64_t tiles_v = clsP / 32;
         hipLaunchKernelGGL(k_to_g, dim3((unsigned)(nrP / 32 * tiles_v / 4)), dim3(256), 0, st, base + o_z, clsP / 16,
@@ -714,7 +797,7 @@ int head_run(const HeadCall& h) {
         }
     }
     if (!h.row_lse_in)
-        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(1024), 0, st, row_loss, rows, info, h.loss);
+        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(1024), 0, st, block_loss, (rows + 31) / 32, info, h.loss);
     return finish(h.what);
 }
 
