@@ -304,6 +304,44 @@ int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, flo
                                  const float* w, const int32_t* labels, const float* ug, int64_t rows, int64_t dim,
                                  int64_t classes, int accumulate);
 
+/* Distillation from a teacher's top logits: x [rows, classes] are the student's logits, teacher
+ * [rows, k] the teacher's at the classes ids [rows, k]; an entry with a negative id, or a teacher logit
+ * of minus infinity, is none. With T the temperature (1e-6..1e6) and n the rows that have an entry,
+ *   q = softmax(teacher / T) over the row's entries, p = softmax(x / T) over all classes,
+ *   row_lse = log sum_v exp(x_v / T),  loss = T^2 / n sum_rows sum_k q (log q - log p_id).
+ * A row without entries is left out whatever its logits hold: row_lse 0, its gradient left alone
+ * (accumulate == 0: zero). A class that several entries name gets the sum of their q, in their order. An id of
+ * classes or more makes the row's row_lse and gradient, and the loss, NaN. 1 <= k <= 1024; row_lse
+ * may be null. */
+int mh_distill_fwd(float* loss, float* row_lse, const float* x, const int32_t* ids, const float* teacher, int64_t rows,
+                   int64_t classes, int64_t k, float temperature);
+/* The gradient from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
+ * grad_x = ug T / n (p - q at the entries' classes). */
+int mh_distill_bwd(float* grad_x, const float* x, const int32_t* ids, const float* teacher, const float* row_lse,
+                   const float* ug, int64_t rows, int64_t classes, int64_t k, float temperature, int accumulate);
+/* Both at once, for a training step whose ug is known before: the logits are read once, or while the
+ * caches hold them. row_lse may be null. */
+int mh_distill_step(float* loss, float* row_lse, float* grad_x, const float* x, const int32_t* ids,
+                    const float* teacher, const float* ug, int64_t rows, int64_t classes, int64_t k, float temperature,
+                    int accumulate);
+
+/* A mixture-of-experts router over x [rows, experts]: chosen [rows, k] are each row's k largest logits,
+ * largest first, ties to the lowest index (a NaN after every number); weights [rows, k] their
+ * probabilities p = softmax(x), divided by their sum with normalise != 0; counts [experts] how many rows chose
+ * an expert; and the balance loss
+ *   loss = experts sum_e f_e P_e,  f_e = counts_e / (n k),  P_e = the mean of p_e,
+ * over the n kept rows: those with keep[row] != 0, or all where keep is null. A row that is not kept has
+ * chosen -1 and weights 0 and counts nowhere. 1 <= experts <= 1024, 1 <= k <= min(64, experts). */
+int mh_router_fwd(float* weights, int32_t* chosen, int32_t* counts, float* loss, const float* x, const int32_t* keep,
+                  int64_t rows, int64_t experts, int64_t k, int normalise);
+/* The gradient of the logits from grad_weights [rows, k], the gradient of the weights, and ug, that of the
+ * loss (a device scalar): either may be null. chosen and counts are the forward's (counts carry no
+ * gradient); keep and normalise as given to it. A row that is not kept is left alone (accumulate == 0:
+ * zero). */
+int mh_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int32_t* chosen, const int32_t* counts,
+                  const float* grad_weights, const float* ug, int64_t rows, int64_t experts, int64_t k, int normalise,
+                  int accumulate);
+
 /* ---- graph and model: Graph (mantle/autograd/graph.mojo:33-217), Model
  * (mantle/nn/model.mojo:55-340) and its Collections (mantle/autograd/collection.mojo:24-224)
  * in device memory ---- */

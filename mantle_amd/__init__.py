@@ -21,6 +21,7 @@ from .ops import (  # noqa: F401
     bias_relu_forward, bias_relu_backward, softmax_log_mul_mean_forward, softmax_log_mul_mean_backward,
     softmax_forward, softmax_backward, logsoftmax_forward, logsoftmax_backward, cross_entropy_forward,
     cross_entropy_backward, linear_cross_entropy_forward, linear_cross_entropy_backward, linear_cross_entropy_step,
+    distill_forward, distill_backward, distill_step, router_forward, router_backward,
 )
 
 __all__ = [
@@ -30,6 +31,7 @@ __all__ = [
     "bias_relu_backward", "softmax_log_mul_mean_forward", "softmax_log_mul_mean_backward", "softmax_forward",
     "softmax_backward", "logsoftmax_forward", "logsoftmax_backward", "cross_entropy_forward",
     "cross_entropy_backward", "IndexTensor", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
-    "linear_cross_entropy_step", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
+    "linear_cross_entropy_step", "distill_forward", "distill_backward", "distill_step", "router_forward",
+    "router_backward", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
     "load_checkpoint", "load_checkpoint_with_optim",
 ]

@@ -127,6 +127,11 @@ SIGNATURES = {
     "mh_linear_cross_entropy_fwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64],
     "mh_linear_cross_entropy_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
     "mh_linear_cross_entropy_step": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
+    "mh_distill_fwd": [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _F],
+    "mh_distill_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _F, _I],
+    "mh_distill_step": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _F, _I],
+    "mh_router_fwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
+    "mh_router_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I, _I],
     "mh_fma_fwd": [_VP, _VP, _VP, _VP, _I64],
     "mh_fma_bwd_accum": [_I, _VP, _VP, _VP, _VP, _I64],
     "mh_leakyrelu_fwd": [_VP, _VP, _I64, _F],

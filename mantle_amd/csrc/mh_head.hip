@@ -21,6 +21,7 @@
 // over the contracted axis tests nothing.
 #include "mh_internal.h"
 #include "mh_math.h"
+#include "mh_rows.h"
 
 namespace mh {
 namespace {
@@ -51,16 +52,6 @@ __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o));
     return v;
-}
-
-// e^x to about an ulp for x <= 0: the rounding of x log2(e) is carried into the result. mexp stops at
-// e^-88.4, as the reference does; here what a mask leaves is 0.
-__device__ __forceinline__ float exp_neg(float x) {
-    x = x < -1.0e4f ? -1.0e4f : x;  // keeps NaN, and infinity out of the fma
-    const float t = x * 1.44269504088896341f;
-    const float r = __builtin_fmaf(x, 1.925963033500e-8f, __builtin_fmaf(x, 1.44269504088896341f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e, r * 0.693147180559945f, e);
 }
 
 __device__ __forceinline__ float finite_abs(float v) {
@@ -379,7 +370,7 @@ __global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
                             if (cls_of(i, r) == (int)want) g.target[n] = acc[i][j][r];
                 }
                 // the maximum and the sum of exponentials of each 64 classes, whatever the tile, so that the
-                // sums' order does not depend on it: one multiply-add and one exp2 a logit; only the last
+                // sums' order does not depend on it: a difference, a product and one exp2 a logit; only the last
                 // class's wavefront masks what lies past it
                 const bool whole = g.classes - v0 >= MI * 32;
 #pragma unroll
@@ -391,13 +382,13 @@ __global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
                         for (int r = 0; r < 16; ++r)
                             if (whole || cls_of(i, r) < last) top = __builtin_fmaxf(top, acc[i][j][r]);
                     top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                    const float base = top == -__builtin_inff() ? 0.0f : top * -1.44269504088896341f;
+                    const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
                     for (int i = 2 * h; i < 2 * h + 2; ++i)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             if (whole || cls_of(i, r) < last)
-                                sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], 1.44269504088896341f, base));
+                                sum += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
                     sum += __shfl_xor(sum, 32);  // a NaN among the logits is in the sum, whatever the maximum says
                     if (half == 0) {
                         const int64_t at = ((v0 >> 6) + h) * 2 * g.stat_ld + n;
@@ -565,7 +556,9 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int64_t cls = vt * 32 + b * 16 + k8 + j;
-            const float p = exp_neg(v[j] - l) - (cls == label ? 1.0f : 0.0f);
+            // above 0 only by the log-sum-exp's own rounding, which counts where logits are very large
+            const float d = v[j] - l;
+            const float p = exp_neg(d > 0.0f ? 0.0f : d) - (cls == label ? 1.0f : 0.0f);
             v[j] = label < 0 || cls >= classes ? 0.0f : p * (float)(1 << kGExp);
         }
         half8 hi, lo;

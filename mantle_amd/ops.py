@@ -544,3 +544,60 @@ def linear_cross_entropy_step(loss: Tensor, grad_x: Optional[Tensor], grad_w: Op
               _want("grad_w", grad_w, (classes, dim), optional=True), _want("x", x, (rows, dim)),
               _want("w", w, (classes, dim)), _want("labels", labels, (rows,), index=True), _want("ug", ug, (1,)),
               rows, dim, classes, int(bool(accumulate)))
+
+
+def distill_forward(loss: Tensor, row_lse: Optional[Tensor], x: Tensor, ids: IndexTensor, teacher: Tensor,
+                    temperature: float = 1.0) -> None:
+    """Distillation from a teacher's top logits: the divergence of softmax(x / T), x [rows, classes], from
+    softmax(teacher / T) over the entries teacher [rows, k] at the classes ids [rows, k] (negative: no entry),
+    times T^2, as the mean over the rows that have an entry."""
+    (rows, classes), (_, k) = _matrix("x", x), _matrix("ids", ids)
+    _lib.call("mh_distill_fwd", _want("loss", loss, (1,)), _want("row_lse", row_lse, (rows,), optional=True),
+              _want("x", x, (rows, classes)), _want("ids", ids, (rows, k), index=True),
+              _want("teacher", teacher, (rows, k)), rows, classes, k, float(temperature))
+
+
+def distill_backward(grad_x: Tensor, x: Tensor, ids: IndexTensor, teacher: Tensor, row_lse: Tensor, ug: Tensor,
+                     temperature: float = 1.0, accumulate: bool = True) -> None:
+    """grad_x += (accumulate=False: =) the gradient of distill_forward's loss from ug, the loss's
+    (shape (1)), and the forward's row_lse."""
+    (rows, classes), (_, k) = _matrix("x", x), _matrix("ids", ids)
+    _lib.call("mh_distill_bwd", _want("grad_x", grad_x, (rows, classes)), _want("x", x, (rows, classes)),
+              _want("ids", ids, (rows, k), index=True), _want("teacher", teacher, (rows, k)),
+              _want("row_lse", row_lse, (rows,)), _want("ug", ug, (1,)), rows, classes, k, float(temperature),
+              int(bool(accumulate)))
+
+
+def distill_step(loss: Tensor, grad_x: Tensor, x: Tensor, ids: IndexTensor, teacher: Tensor, ug: Tensor,
+                 temperature: float = 1.0, row_lse: Optional[Tensor] = None, accumulate: bool = True) -> None:
+    """distill_forward and distill_backward in one call, for a training step."""
+    (rows, classes), (_, k) = _matrix("x", x), _matrix("ids", ids)
+    _lib.call("mh_distill_step", _want("loss", loss, (1,)), _want("row_lse", row_lse, (rows,), optional=True),
+              _want("grad_x", grad_x, (rows, classes)), _want("x", x, (rows, classes)),
+              _want("ids", ids, (rows, k), index=True), _want("teacher", teacher, (rows, k)), _want("ug", ug, (1,)),
+              rows, classes, k, float(temperature), int(bool(accumulate)))
+
+
+def router_forward(weights: Tensor, chosen: IndexTensor, counts: IndexTensor, loss: Tensor, x: Tensor,
+                   keep: Optional[IndexTensor] = None, normalise: bool = False) -> None:
+    """A mixture-of-experts router: the k largest logits of each row of x [rows, experts] (chosen, ties to the
+    lowest index), their probabilities (weights, both [rows, k]; normalise: divided by their sum), how
+    often each expert was chosen (counts [experts]) and the balance loss experts * sum_e f_e P_e. Rows with
+    keep 0 are padding: chosen -1, weights 0, counted nowhere."""
+    (rows, experts), (_, k) = _matrix("x", x), _matrix("chosen", chosen)
+    _lib.call("mh_router_fwd", _want("weights", weights, (rows, k)), _want("chosen", chosen, (rows, k), index=True),
+              _want("counts", counts, (experts,), index=True), _want("loss", loss, (1,)),
+              _want("x", x, (rows, experts)), _want("keep", keep, (rows,), index=True, optional=True), rows, experts, k,
+              int(bool(normalise)))
+
+
+def router_backward(grad_x: Tensor, x: Tensor, chosen: IndexTensor, counts: IndexTensor,
+                    grad_weights: Optional[Tensor], ug: Optional[Tensor], keep: Optional[IndexTensor] = None,
+                    normalise: bool = False, accumulate: bool = True) -> None:
+    """grad_x += (accumulate=False: =) the gradient of router_forward from grad_weights, the weights', and
+    ug, the balance loss's (shape (1)); either may be None."""
+    (rows, experts), (_, k) = _matrix("x", x), _matrix("chosen", chosen)
+    _lib.call("mh_router_bwd", _want("grad_x", grad_x, (rows, experts)), _want("x", x, (rows, experts)),
+              _want("keep", keep, (rows,), index=True, optional=True), _want("chosen", chosen, (rows, k), index=True),
+              _want("counts", counts, (experts,), index=True), _want("grad_weights", grad_weights, (rows, k), optional=True),
+              _want("ug", ug, (1,), optional=True), rows, experts, k, int(bool(normalise)), int(bool(accumulate)))
