@@ -495,18 +495,18 @@ def _want(name: str, t, shape, index: bool = False, optional: bool = False) -> O
     """The address of t after checking that it is there, of the right kind and of `shape`."""
     if t is None and optional:
         return None
-    if not isinstance(t, Tensor) or isinstance(t, IndexTensor) != index:
+    if not isinstance(t, IndexTensor if index else Tensor) or (not index and isinstance(t, IndexTensor)):
         kind = "an IndexTensor" if index else "a Tensor"
         raise _lib.MantleHipError(_lib.ERR_INVALID, f"{name} must be {kind}, not {type(t).__name__}")
-    if t.shape() != TensorShape(shape):
+    if t._shape._dims != shape:
         raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{name} has shape {t.shape()}, not {TensorShape(shape)}")
-    return t.ptr
+    return t._ptr
 
 
 def _matrix(name: str, t):
-    if not isinstance(t, Tensor) or t.rank() != 2:
+    if not isinstance(t, Tensor) or len(t._shape._dims) != 2:
         raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{name} must be a tensor of two dimensions")
-    return t.shape().dims
+    return t._shape._dims
 
 
 def linear_cross_entropy_forward(loss: Tensor, row_lse: Optional[Tensor], x: Tensor, w: Tensor, labels: IndexTensor,

@@ -135,11 +135,17 @@ class Tensor:
                 pass
             self._ptr = None
 
-    @staticmethod
-    def over(ptr: int, shape, owner=None) -> "Tensor":
+    @classmethod
+    def over(cls, ptr: int, shape, owner=None) -> "Tensor":
         """A tensor over device memory that another allocator holds, `owner` kept alive with it. What
         wrote that memory has to be done: the library works on a stream of its own."""
-        return Tensor(as_shape(shape), _ptr=int(ptr), _owner=owner if owner is not None else int(ptr))
+        if not _initialized:
+            init(0)
+        t = cls.__new__(cls)
+        t._shape = shape if isinstance(shape, TensorShape) else TensorShape(shape)
+        t._ptr = int(ptr)
+        t._owner = t._ptr if owner is None else owner  # anything but None: not freed here
+        return t
 
     # ---- properties ----
     def shape(self) -> TensorShape:
@@ -214,10 +220,6 @@ class IndexTensor(Tensor):
         if a.size:
             _lib.call("mh_memcpy_h2d", t._ptr, a.ctypes.data, a.size * 4)
         return t
-
-    @staticmethod
-    def over(ptr: int, shape, owner=None) -> "IndexTensor":
-        return IndexTensor(as_shape(shape), _ptr=int(ptr), _owner=owner if owner is not None else int(ptr))
 
     def to_numpy(self) -> np.ndarray:
         out = np.empty(self._shape.dims, dtype=np.int32)
