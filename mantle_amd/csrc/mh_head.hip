@@ -288,54 +288,44 @@ __global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
                                : g.b + ((tn * (TN / 32) + rb - TM / 32) * g.bkb + k0) * kBlk);
     }
     const uint32_t lane16 = lane * 16;
-    auto load = [&](int s) {  // past the end: the last stage again, into a buffer that no one reads
+    // Part i of 4 of a stage's loads. Past the end: the last stage again, into a buffer that no one reads.
+    auto load = [&](int s, int i) {
         const int64_t at = (int64_t)(s < S ? s : S - 1) * kBlk;
         char* to = lds + (s & 3) * kStage + wave * 2 * kBlk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(src[i >> 1] + at + (i & 1) * 1024 + lane16),
-                (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(src[i >> 1] + at + (i & 1) * 1024 + lane16),
+            (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
     };
-    auto read = [&](int s, half8(&a)[MI][2], half8(&b)[NI][2]) {
-        const char* la = lds + (s & 3) * kStage + wm * MI * kBlk + lane * 16;
-        const char* lb = lds + (s & 3) * kStage + (TM / 32 + wn * NI) * kBlk + lane * 16;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            b[j][0] = *reinterpret_cast<const half8*>(lb + j * kBlk);
-            b[j][1] = *reinterpret_cast<const half8*>(lb + j * kBlk + 1024);
-        }
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            a[i][0] = *reinterpret_cast<const half8*>(la + i * kBlk);
-            a[i][1] = *reinterpret_cast<const half8*>(la + i * kBlk + 1024);
-        }
+    // Part i of kReads of a stage's operands: N's first, both halves of each.
+    constexpr int kReads = 2 * (MI + NI), kProducts = 3 * MI * NI;
+    auto read = [&](int s, int i, half8(&a)[MI][2], half8(&b)[NI][2]) {
+        const char* at = lds + (s & 3) * kStage + lane16;
+        if (i < 2 * NI) b[i >> 1][i & 1] = *reinterpret_cast<const half8*>(at + (TM / 32 + wn * NI) * kBlk + i * 1024);
+        else a[(i - 2 * NI) >> 1][i & 1] = *reinterpret_cast<const half8*>(at + wm * MI * kBlk + (i - 2 * NI) * 1024);
     };
 
     f32x16 acc[MI][NI] = {};
+    // The next stage's reads and loads go between the matrix instructions, one at a time: issued together at
+    // the step's start they fill LDS's queue, and the wavefronts stand before it.
     auto step = [&](int s, half8(&a)[MI][2], half8(&b)[NI][2], half8(&an)[MI][2], half8(&bn)[NI][2]) {
         wait_and_meet<4>();
-        read(s + 1, an, bn);
-        load(s + 3);
-        __builtin_amdgcn_sched_barrier(0);  // issued before the matrix instructions, not where registers are fewest
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
+        for (int t = 0; t < kProducts; ++t) {
+            constexpr int kEvery = kProducts / kReads;  // 2 in the large tile, 1 in the small one
+            if (t % kEvery == 0 && t / kEvery < kReads) read(s + 1, t / kEvery, an, bn);
+            if (t % (kProducts / 4) == kProducts / 8) load(s + 3, t / (kProducts / 4));
+            const int u = t / (MI * NI), i = t % (MI * NI) / NI, j = t % NI;  // the small terms first
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][u == 1], b[j][u == 0], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0x6);  // but address arithmetic
         }
-        __builtin_amdgcn_sched_barrier(0);
     };
     if (S > 0) {
         half8 a0[MI][2], b0[NI][2], a1[MI][2], b1[NI][2];
-        load(0);
-        load(1);
-        load(2);
+#pragma unroll
+        for (int i = 0; i < 12; ++i) load(i / 4, i % 4);
         wait_and_meet<8>();
-        read(0, a0, b0);
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) read(0, i, a0, b0);
         for (int s = 0; s < S; s += 2) {
             step(s, a0, b0, a1, b1);
             step(s + 1, a1, b1, a0, b0);

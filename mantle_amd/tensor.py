@@ -8,6 +8,7 @@ tensor.mojo:250-302). Here the storage is HBM on the initialised gfx950 device
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Iterable, Optional, Tuple, Union
 
 import numpy as np
@@ -41,16 +42,13 @@ class TensorShape:
     __slots__ = ("_dims", "_n", "_cs")
 
     def __init__(self, *dims: Union[int, Iterable[int]]):
-        if len(dims) == 1 and not isinstance(dims[0], (int, np.integer)):
+        if len(dims) == 1 and type(dims[0]) is not int and not isinstance(dims[0], (int, np.integer)):
             dims = tuple(dims[0])
-        d = tuple(int(x) for x in dims)
+        d = tuple(map(int, dims))
         if not 1 <= len(d) <= MAX_RANK:
             raise ValueError(f"rank {len(d)} outside 1..{MAX_RANK}")
         self._dims = d
-        n = 1
-        for x in d:
-            n *= x
-        self._n = n
+        self._n = math.prod(d)
         self._cs = None
 
     def __getstate__(self):
