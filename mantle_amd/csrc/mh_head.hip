@@ -46,6 +46,10 @@ struct alignas(16) HeadPart {  // k_amax's partials
     int32_t kept[kAmaxBlocks];
 };
 
+// Blocks from one row block of a panel to the next, of kb in use: odd, so that the row blocks that workgroups
+// read at the same time lie in different memory channels: 17.2 -> 16.5 ms a step over [4096, 2048] x
+// [131072, 2048], 489 -> 450 us over [32768, 512] x [1000, 512], where powers of two were apart.
+__host__ __device__ inline int64_t stride_of(int64_t kb) { return kb | 1; }
 __host__ __device__ inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -136,8 +140,8 @@ constexpr int kSplitTile = 64;
 struct SplitOne {
     const float* src;
     int64_t nr, nc;      // the matrix
-    char* rowp;          // [tiles_r * 2][rkb] blocks; column blocks at or past rkb are not stored
-    char* colp;          // [tiles_c * 2][ckb] blocks
+    char* rowp;          // row blocks of rkb blocks, stride_of(rkb) apart; blocks at or past rkb are not stored
+    char* colp;          // the same of ckb
     int64_t rkb, ckb;
     int64_t tiles_r, tiles_c;
     int64_t rb_end, cb_end;  // row blocks of rowp, of colp
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[rb * 32 + r][kb * 16 + k8 + j], e);
             split8(v, &hi, &lo);
-            half8* p = reinterpret_cast<half8*>(s.rowp + ((r0 / 32 + rb) * s.rkb + c0 / 16 + kb) * kBlk);
+            half8* p = reinterpret_cast<half8*>(s.rowp + ((r0 / 32 + rb) * stride_of(s.rkb) + c0 / 16 + kb) * kBlk);
             p[lane] = hi;
             p[64 + lane] = lo;
         }
@@ -183,7 +187,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[kb * 16 + k8 + j][rb * 32 + r], e);
             split8(v, &hi, &lo);
-            half8* p = reinterpret_cast<half8*>(s.colp + ((c0 / 32 + rb) * s.ckb + r0 / 16 + kb) * kBlk);
+            half8* p = reinterpret_cast<half8*>(s.colp + ((c0 / 32 + rb) * stride_of(s.ckb) + r0 / 16 + kb) * kBlk);
             p[lane] = hi;
             p[64 + lane] = lo;
         }
@@ -214,10 +218,10 @@ enum HeadEpi { EPI_LOGITS = 0, EPI_GRAD = 1 };
 
 struct GemmArg {
     const char *a, *b;       // panels: M operand, N operand
-    int64_t akb, bkb;        // blocks along the contracted axis that a row block of each panel holds
+    int64_t akb, bkb;        // blocks from one row block of each panel to the next
     int64_t kb;              // blocks contracted here, of one split: a multiple of 2
     int64_t kb_all;          // blocks contracted by all splits
-    int32_t tiles_m, tiles_n;
+    int32_t tiles_m, tiles_n, splits;
     const HeadInfo* info;
     // EPI_LOGITS: M is classes, N rows
     const int32_t* labels;   // at the first row of the panel; EPI_GRAD: rows to leave alone, or null
@@ -251,79 +255,82 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("" ::: "memory");
 }
 
-// Four stages of 16 of the contracted axis circle through LDS. In step s a wavefront waits for its loads of
-// stage s + 1, meets the others, starts reading stage s + 1 into registers and loading stage s + 3 into
-// LDS (over stage s - 1, whose last reads ended before the barrier), and multiplies stage s, which is in
-// registers already: neither the loads' latency nor LDS's stands before a matrix instruction.
+// Three stages of 16 of the contracted axis circle through LDS. In step s a wavefront waits for its loads of
+// stage s + 1 and its reads of stage s, meets the others, and then, between the matrix instructions of
+// stage s, which is in registers, reads stage s + 1 and loads stage s + 3 over stage s: neither the loads'
+// latency nor LDS's stands before a matrix instruction.
 template <int TM, int TN, int WM, int WN, int EPI>
-__global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmArg g) {
     constexpr int kWaves = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32;
     constexpr int kRows = (TM + TN) / 32;        // row blocks of a stage
     constexpr int kStage = kRows * kBlk;
     constexpr int kLoads = kRows * 2 / kWaves;   // 1 KB loads of a wavefront a stage
-    static_assert(kLoads == 4 && kRows % kWaves == 0, "the waits below count 4 loads a stage");
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kStage];
+    static_assert(kRows % kWaves == 0 && 2 * kLoads < 16, "the waits' counts");
+    __shared__ __attribute__((aligned(1024))) char lds[3 * kStage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    // Workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 tile rows,
-    // so that its L2 holds what its workgroups share.
-    const int64_t T = (int64_t)g.tiles_m * g.tiles_n;
-    const int64_t per = (T + 7) / 8;
-    const int64_t id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int64_t)(blockIdx.x >> 3) >= per || id >= T) return;
+    // Workgroup b runs on XCD b % 8: each XCD takes a contiguous run of a split's tiles, in groups of 8 tile
+    // rows, so that its L2 holds what its workgroups share, and as many as the others.
+    const int64_t T = (int64_t)g.tiles_m * g.tiles_n, all = T * g.splits;
+    const int64_t item = (int64_t)(blockIdx.x & 7) * ((all + 7) / 8) + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= (all + 7) / 8 || item >= all) return;
+    const int64_t split = item / T, id = item - split * T;
     const int64_t gsz = (int64_t)8 * g.tiles_n, grp = id / gsz;
     const int gm = (int)(g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8);
     const int64_t tm = grp * 8 + (id - grp * gsz) % gm, tn = (id - grp * gsz) / gm;
 
-    const int64_t k0 = (int64_t)blockIdx.y * g.kb;
+    const int64_t k0 = split * g.kb;
     const int64_t kb = g.kb_all - k0 < g.kb ? g.kb_all - k0 : g.kb;
     const int S = (int)kb;  // even; 0 or less for a split past the end
 
-    const char* src[2];  // the two row blocks this wavefront brings
+    const char* src[kLoads / 2];  // the row blocks this wavefront brings
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int rb = wave * 2 + i;
+    for (int i = 0; i < kLoads / 2; ++i) {
+        const int rb = wave * (kLoads / 2) + i;
         src[i] = (rb < TM / 32 ? g.a + ((tm * (TM / 32) + rb) * g.akb + k0) * kBlk
                                : g.b + ((tn * (TN / 32) + rb - TM / 32) * g.bkb + k0) * kBlk);
     }
     const uint32_t lane16 = lane * 16;
-    // Part i of 4 of a stage's loads. Past the end: the last stage again, into a buffer that no one reads.
-    auto load = [&](int s, int i) {
+    // Part i of kLoads of a stage's loads, into the stage at `to`. Past the end: the last stage again, which no
+    // one reads.
+    auto load = [&](int s, int to, int i) {
         const int64_t at = (int64_t)(s < S ? s : S - 1) * kBlk;
-        char* to = lds + (s & 3) * kStage + wave * 2 * kBlk;
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(src[i >> 1] + at + (i & 1) * 1024 + lane16),
-            (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+            (__attribute__((address_space(3))) void*)(lds + to + wave * (kLoads / 2) * kBlk + i * 1024), 16, 0, 0);
     };
-    // Part i of kReads of a stage's operands: N's first, both halves of each.
+    // Part i of kReads of the operands of the stage at `from`: N's first, both halves of each.
     constexpr int kReads = 2 * (MI + NI), kProducts = 3 * MI * NI;
-    auto read = [&](int s, int i, half8(&a)[MI][2], half8(&b)[NI][2]) {
-        const char* at = lds + (s & 3) * kStage + lane16;
+    auto read = [&](int from, int i, half8(&a)[MI][2], half8(&b)[NI][2]) {
+        const char* at = lds + from + lane16;
         if (i < 2 * NI) b[i >> 1][i & 1] = *reinterpret_cast<const half8*>(at + (TM / 32 + wn * NI) * kBlk + i * 1024);
         else a[(i - 2 * NI) >> 1][i & 1] = *reinterpret_cast<const half8*>(at + wm * MI * kBlk + (i - 2 * NI) * 1024);
     };
 
     f32x16 acc[MI][NI] = {};
+    int here = 0;  // the stage in registers
     // The next stage's reads and loads go between the matrix instructions, one at a time: issued together at
     // the step's start they fill LDS's queue, and the wavefronts stand before it.
     auto step = [&](int s, half8(&a)[MI][2], half8(&b)[NI][2], half8(&an)[MI][2], half8(&bn)[NI][2]) {
-        wait_and_meet<4>();
+        wait_and_meet<kLoads>();
+        const int next = here == 2 * kStage ? 0 : here + kStage;
 #pragma unroll
         for (int t = 0; t < kProducts; ++t) {
-            constexpr int kEvery = kProducts / kReads;  // 2 in the large tile, 1 in the small one
-            if (t % kEvery == 0 && t / kEvery < kReads) read(s + 1, t / kEvery, an, bn);
-            if (t % (kProducts / 4) == kProducts / 8) load(s + 3, t / (kProducts / 4));
+            constexpr int kEvery = kProducts / kReads;  // 2 in the large tiles, 1 in the small one
+            if (t % kEvery == 0 && t / kEvery < kReads) read(next, t / kEvery, an, bn);
+            if (t % (kProducts / kLoads) == kProducts / kLoads / 2) load(s + 3, here, t / (kProducts / kLoads));
             const int u = t / (MI * NI), i = t % (MI * NI) / NI, j = t % NI;  // the small terms first
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][u == 1], b[j][u == 0], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0x6);  // but address arithmetic
         }
+        here = next;
     };
     if (S > 0) {
         half8 a0[MI][2], b0[NI][2], a1[MI][2], b1[NI][2];
 #pragma unroll
-        for (int i = 0; i < 12; ++i) load(i / 4, i % 4);
-        wait_and_meet<8>();
+        for (int i = 0; i < 3 * kLoads; ++i) load(i / kLoads, i / kLoads * kStage, i % kLoads);
+        wait_and_meet<2 * kLoads>();
 #pragma unroll
         for (int i = 0; i < kReads; ++i) read(0, i, a0, b0);
         for (int s = 0; s < S; s += 2) {
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(WM* WN * 64, WM * WN / 4) void k_gemm(GemmArg g) {
     } else {
         if (g.part) {
             const int64_t ld = (int64_t)g.tiles_n * TN;
-            float* p = g.part + (int64_t)blockIdx.y * g.tiles_m * TM * ld;
+            float* p = g.part + split * g.tiles_m * TM * ld;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -592,41 +599,58 @@ struct Carve {
     }
 };
 
-template <int T, int EPI>
-void launch_gemm(const GemmArg& g, int64_t tiles, int splits) {
-    const dim3 grid((unsigned)(8 * ((tiles + 7) / 8)), (unsigned)splits);
-    if constexpr (T == 256)
-        hipLaunchKernelGGL((k_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, ctx().stream, g);
-    else
-        hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, g);
-}
-
-// The tile of a product and, with `split`, the splits of its contracted axis of kb blocks: the least time in
-// units of a 128 x 128 tile's block on a whole CU. A 256 x 256 tile takes four on a CU of its own; of the
-// 128 x 128 ones two share a CU, each half as fast, and reread more (1.2 each). A split holds 16 blocks at
-// least, and its partial sums cost a store and a load.
+// A product's tile and the splits of its contracted axis.
 struct Form {
     int tile, splits;
 };
+
+// The least time, in units of one 128 x 128 x 16 block on a whole CU (0.23 us). A 256 x 256 tile takes four a
+// block on a CU of its own and 24 blocks' time around them (its 256 KB store stands alone); of the 128 x 128
+// ones up to three share a CU, which then works at 0.5, 0.78 or 0.82 of the large tile's rate, with 10 around
+// them. Measured on either side: [4096, 1024] x [32000, 1024]'s logits take 625 us in large tiles and 670 in
+// small ones; [1023, 30011] x [30011, 513]'s gradient 85 us in 12 splits of small tiles, 140 in 20 of large
+// ones. A split writes and reads its sums and costs one more launch. Sums run over at most 65536 elements
+// each: the matrix unit's fp32 sums drift by 4e-11 of themselves an element (8e-5 over 2^21 of them unsplit).
+constexpr int64_t kMaxSplit = 64, kLongest = 4096;
 Form form_of(int64_t m, int64_t n, int64_t kb, bool split) {
-    Form best = {128, 1};
-    double least = 0.0;
-    const int64_t cus = ctx().num_cus;
+    static const double rate[4] = {1.0, 0.5, 0.78, 0.82};
+    const int64_t cus = ctx().num_cus, least = split ? (kb + kLongest - 1) / kLongest : 1;
+    Form best = {0, 0};
+    double time = 0.0;
     for (const int T : {256, 128}) {
         const int64_t tiles = up(m, T) / T * (up(n, T) / T);
-        for (int s = 1; s <= 64 && (s == 1 || (split && kb / s >= 16)); ++s) {
-            const int64_t wg = tiles * s, per = T == 256 ? cus : 2 * cus;
-            const int64_t rounds = (wg + per - 1) / per;
-            // a round of small tiles on half the CUs' places runs one a CU
-            const double unit = T == 256 ? 4.0 : (wg <= cus ? 1.2 : 2.4);
-            const double cost = (double)rounds * unit * ((double)kb / s + 8) + (s > 1 ? 0.5 * s * (double)tiles * T * T / (128 * 128) / cus + 8 : 0);
-            if (least == 0.0 || cost < least) {
-                least = cost;
-                best = {T, s};
+        for (int64_t s = least < kMaxSplit ? least : kMaxSplit; s <= kMaxSplit; ++s) {
+            const int64_t wg = tiles * s, steps = (kb + s - 1) / s;
+            double t;
+            if (T == 256) {
+                t = (double)((wg + cus - 1) / cus) * 4.0 * (double)(steps + 24);
+            } else {
+                const int64_t w = (wg + cus - 1) / cus < 3 ? (wg + cus - 1) / cus : 3;
+                const double rounds = (double)wg / (double)(cus * w) + 0.3;
+                t = (rounds > 1.0 ? rounds : 1.0) * (double)w / rate[w] * (double)(steps + 10);
             }
+            if (s > 1) t += (double)(s * m * n) * 8.0 / 5.0e6 / 0.23 + 20.0;
+            if (best.tile == 0 || t < time) {
+                time = t;
+                best = {T, (int)s};
+            }
+            if (!split || steps <= 16) break;
         }
     }
     return best;
+}
+
+template <int EPI>
+void launch_gemm(GemmArg g, int64_t m, int64_t n, const Form& f) {
+    g.tiles_m = (int32_t)(up(m, f.tile) / f.tile);
+    g.tiles_n = (int32_t)(up(n, f.tile) / f.tile);
+    g.kb = up((g.kb_all + f.splits - 1) / f.splits, 2);
+    g.splits = f.splits;
+    const dim3 grid((unsigned)(8 * (((int64_t)g.tiles_m * g.tiles_n * f.splits + 7) / 8)));
+    if (f.tile == 256)
+        hipLaunchKernelGGL((k_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, ctx().stream, g);
+    else
+        hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, g);
 }
 
 struct HeadCall {
@@ -644,22 +668,16 @@ struct HeadCall {
 // grad [m, n] from panels a (rows of m) and b (rows of n), contracted over kb blocks.
 int grad_product(GemmArg g, int64_t m, int64_t n, int64_t kb, float* part) {
     const Form f = form_of(m, n, kb, true);
-    const int splits = f.splits, T = f.tile;
     g.m = m;
     g.n = n;
-    g.tiles_m = (int32_t)(up(m, T) / T);
-    g.tiles_n = (int32_t)(up(n, T) / T);
     g.kb_all = kb;
-    g.kb = up((kb + splits - 1) / splits, 2);
-    const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
-    g.part = splits > 1 ? part : nullptr;
-    if (T == 256) launch_gemm<256, EPI_GRAD>(g, tiles, splits);
-    else launch_gemm<128, EPI_GRAD>(g, tiles, splits);
-    if (splits > 1) {
-        const int64_t ld = (int64_t)g.tiles_n * T, plane = (int64_t)g.tiles_m * T * ld;
+    g.part = f.splits > 1 ? part : nullptr;
+    launch_gemm<EPI_GRAD>(g, m, n, f);
+    if (f.splits > 1) {
+        const int64_t ld = up(n, f.tile), plane = up(m, f.tile) * ld;
         int64_t nb = grid_blocks(m * n, 256);
         if (nb > 4096) nb = 4096;
-        hipLaunchKernelGGL(k_join, dim3((unsigned)nb), dim3(256), 0, ctx().stream, g, splits, ld, plane);
+        hipLaunchKernelGGL(k_join, dim3((unsigned)nb), dim3(256), 0, ctx().stream, g, f.splits, ld, plane);
     }
     return MH_OK;
 }
@@ -683,15 +701,16 @@ int head_run(const HeadCall& h) {
 
     Carve cv;
     const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
-    const size_t o_xr = cv.take(rowsP / 32 * dkb * kBlk), o_wr = cv.take(clsP / 32 * dkb * kBlk);
-    const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * (rowsP / 16) * kBlk) : 0;
-    const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * (clsP / 16) * kBlk) : 0;
+    const size_t o_xr = cv.take(rowsP / 32 * stride_of(dkb) * kBlk),
+                 o_wr = cv.take(clsP / 32 * stride_of(dkb) * kBlk);
+    const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
+    const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
     const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
     const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / 32 * 8);
     size_t o_z = 0, o_gt = 0, o_sp = 0;
     if (h.train) {
-        o_z = cv.take(chunk / 32 * (clsP / 16) * kBlk);
-        o_gt = cv.take(clsP / 32 * (chunk / 16) * kBlk);
+        o_z = cv.take(chunk / 32 * stride_of(clsP / 16) * kBlk);
+        o_gt = cv.take(clsP / 32 * stride_of(chunk / 16) * kBlk);
         // every chunk has this many rows but the last
         size_t sp = 0;
         for (const int64_t nr : {rows < chunk ? rows : chunk, rows - (rows - 1) / chunk * chunk}) {
@@ -726,8 +745,9 @@ int head_run(const HeadCall& h) {
         const int64_t nr = rows - r0 < chunk ? rows - r0 : chunk, nrP = up(nr, 256);
         GemmArg g = {};
         g.a = base + o_wr;
-        g.b = base + o_xr + r0 / 32 * dkb * kBlk;
-        g.akb = g.bkb = g.kb = g.kb_all = dkb;
+        g.b = base + o_xr + r0 / 32 * stride_of(dkb) * kBlk;
+        g.akb = g.bkb = stride_of(dkb);
+        g.kb_all = dkb;
         g.info = info;
         g.labels = h.labels + r0;
         g.rows = nr;
@@ -736,31 +756,26 @@ int head_run(const HeadCall& h) {
         g.stat_ld = chunk;
         g.target = target;
         g.z = h.train ? base + o_z : nullptr;
-        g.zkb = clsP / 16;
+        g.zkb = stride_of(clsP / 16);
         // every row and class of the padded chunk gets its logits: the panels behind have no gaps
-        const int T = form_of(classes, nr, dkb, false).tile;
-        g.tiles_m = (int32_t)(clsP / T);
-        g.tiles_n = (int32_t)(nrP / T);
-        const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
-        if (T == 256) launch_gemm<256, EPI_LOGITS>(g, tiles, 1);
-        else launch_gemm<128, EPI_LOGITS>(g, tiles, 1);
+        launch_gemm<EPI_LOGITS>(g, clsP, nrP, form_of(clsP, nrP, dkb, false));
         if (!h.row_lse_in)
             hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)((nr + 31) / 32)), dim3(1024), 0, st, g.stat,
                                groups, g.stat_ld, target, h.labels + r0, nr, classes, lse + r0,
                                h.row_loss ? h.row_loss + r0 : nullptr, block_loss + r0 / 32);
         if (!h.train) continue;
         const int64_t tiles_v = clsP / 32;
-        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(nrP / 32 * tiles_v / 4)), dim3(256), 0, st, base + o_z, clsP / 16,
-                           base + o_gt, nrP / 16, (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr, classes,
+        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(nrP / 32 * tiles_v / 4)), dim3(256), 0, st, base + o_z, g.zkb,
+                           base + o_gt, stride_of(nrP / 16), (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr, classes,
                            tiles_v);
         GemmArg d = {};
         d.info = info;
         d.ug = h.ug;
         if (h.gx) {
             d.a = base + o_z;
-            d.akb = clsP / 16;
+            d.akb = stride_of(clsP / 16);
             d.b = base + o_wt;
-            d.bkb = clsP / 16;
+            d.bkb = stride_of(clsP / 16);
             d.exp_b = 1;
             d.labels = h.labels + r0;
             d.out = h.gx + r0 * dim;
@@ -769,9 +784,9 @@ int head_run(const HeadCall& h) {
         }
         if (h.gw) {
             d.a = base + o_gt;
-            d.akb = nrP / 16;
+            d.akb = stride_of(nrP / 16);
             d.b = base + o_xt + r0 / 16 * kBlk;
-            d.bkb = rowsP / 16;
+            d.bkb = stride_of(rowsP / 16);
             d.exp_b = 0;
             d.labels = nullptr;
             d.out = h.gw;
