@@ -4,11 +4,14 @@
 //   q = softmax(teacher / T) over a row's entries;  p = softmax(x / T);  lse = log sum_v exp(x_v / T)
 //   loss = T^2 / n sum_rows sum_k q_k (log q_k - x_id / T + lse);  grad_v = ug T / n (p_v - sum_{id_k = v} q_k)
 //
-// The logits are all that is large: the floor is one read of x and one write of its gradient. One workgroup
-// takes a row, holds a row of up to 32768 classes in registers between its statistics and its gradient, and
-// reads a longer one twice, the second time from its end, where the caches still hold it. Where rows are
-// fewer than CUs, a row is shared by several workgroups: their statistics, then the gradient.
-// An exponential is a difference, a product with log2(e) / T and one instruction; sums are fp32 over at most C / 1024 elements a thread, then a tree.
+// The logits are all that is large: the floor is one read of x and one write of its gradient. A first kernel
+// takes the entries, a wavefront a row: q, the logit at each id, entries of one class joined. A chain of loads
+// that depend on each other, it would stand in the way of the stream (75 -> 58 us over [1025, 30011], 50
+// entries). Then a workgroup takes a row: of up to 32768 classes it holds it in registers and reads it
+// once; a longer one it reads twice, the second time from its end, where the caches still hold it. Where
+// rows are fewer than CUs, several workgroups share a row: their statistics, then the gradient.
+// An exponential is a difference, a product with log2(e) / T and one instruction; sums are fp32 over at
+// most C / 1024 elements a thread, then a tree.
 #include "mh_internal.h"
 #include "mh_math.h"
 #include "mh_rows.h"
@@ -16,8 +19,9 @@
 namespace mh {
 namespace {
 
-constexpr int kMaxK = 1024;      // entries of a row: LDS holds their ids and weights
-constexpr int kCountBlocks = 256;
+constexpr int kMaxK = 1024;       // entries of a row
+constexpr int kEntryBlocks = 512;  // workgroups of k_distill_entries at most: partial counts of rows
+constexpr int64_t kInRegs = 32768;
 
 struct DistillArg {
     const float* x;
@@ -26,116 +30,146 @@ struct DistillArg {
     const float* ug;
     const float* lse_in;  // rows' log-sum-exp of the forward, or null
     float* grad;
-    float* row_lse;   // or null
-    float* row_loss;  // scratch
-    const int32_t* kept;  // [kCountBlocks] partial counts of rows with an entry
-    float* stat;      // [rows][splits][2] or null
+    float* row_lse;  // or null
+    // of k_distill_entries
+    int32_t* kept;    // [parts] rows with an entry
+    int32_t* flag;    // [rows] 0: no entry, 1, 2: an id past the classes
+    float* term;      // [rows] sum of q (log q - x / T)
+    int32_t* ent_id;  // [rows][k] the class of its first entry, -1 at the others
+    float* ent_q;     // the class's q
+    float* ent_x;     // its logit
+    float* row_loss;  // [rows]
+    float* stat;      // [rows][splits][2]
     int64_t rows, classes;
-    int32_t k, splits;
+    int32_t k, splits, parts, slots;
     int64_t span;     // classes of a split, a multiple of 4
     float inv_t, temperature;
 };
 
-__device__ __forceinline__ bool entry(int32_t id, float t) { return id >= 0 && t != -__builtin_inff(); }
-
-// Rows with an entry, as partial counts: a wavefront a row.
-__global__ __launch_bounds__(256) void k_distill_count(int32_t* part, const int32_t* ids, const float* teacher,
-                                                       int64_t rows, int32_t k) {
-    __shared__ int32_t red[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int32_t n = 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += kCountBlocks * 4) {
-        bool any = false;
-        for (int32_t i = lane; i < k; i += 64) any = any || entry(ids[r * k + i], teacher[r * k + i]);
-        n += __any(any) ? 1 : 0;
-    }
-    if (lane == 0) red[wave] = n;
-    __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
-}
-
-// A row's entries in LDS: ids (-1: none) and q.
-struct Entries {
-    int32_t id[kMaxK];
-    float q[kMaxK];
-    float u[kMaxK];  // log q
-};
-
-// Fills e for row r. Returns 0 where the row has no entry, 2 where an id is past the classes, else 1.
-template <int W>
-__device__ int load_entries(const DistillArg& a, int64_t r, Entries& e, float* red) {
-    const int tid = threadIdx.x;
-    float best = -__builtin_inff();
-    bool any = false, bad = false;
-    for (int i = tid; i < a.k; i += W * 64) {
-        const int32_t id = a.ids[r * a.k + i];
-        const float t = a.teacher[r * a.k + i];
-        const bool in = entry(id, t);
-        any = any || in;
-        bad = bad || (in && id >= a.classes);
-        e.id[i] = in ? id : -1;
-        e.u[i] = in ? t * a.inv_t : -__builtin_inff();
-        if (in) best = __builtin_fmaxf(best, t * a.inv_t);
-    }
-    const int what = (__syncthreads_or(any) ? 1 : 0) | (__syncthreads_or(bad) ? 2 : 0);
-    if (what != 1) return what ? 2 : 0;
-    best = block_max<W>(best, red);
-    float mass = 0.0f;
-    for (int i = tid; i < a.k; i += W * 64) {
-        const float v = e.id[i] >= 0 ? exp_neg(e.u[i] - best) : 0.0f;
-        e.q[i] = v;
-        mass += v;
-    }
-    mass = block_sum<W>(mass, red);
-    const float lm = mlog(mass);
-    for (int i = tid; i < a.k; i += W * 64) {
-        e.q[i] = e.q[i] / mass;
-        e.u[i] = e.u[i] - best - lm;
-    }
-    __syncthreads();
-    return 1;
-}
-
-// The row's loss before T^2 / n from its entries and log-sum-exp.
-template <int W>
-__device__ float row_loss_of(const DistillArg& a, int64_t r, const Entries& e, float lse, float* red) {
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < a.k; i += W * 64)
-        if (e.id[i] >= 0 && e.q[i] != 0.0f) s += e.q[i] * (e.u[i] - (a.x[r * a.classes + e.id[i]] * a.inv_t - lse));
-    return block_sum<W>(s, red);
-}
-
-// The entries' elements of the gradient, c0..c1 of row r: written after the dense part, each by the first
-// entry of its class, which adds up those of the same class in their order.
-template <int W, bool ACC>
-__device__ __forceinline__ float entry_old(const DistillArg& a, int64_t at) { return ACC ? a.grad[at] : 0.0f; }
-
-template <int W>
-__device__ __forceinline__ bool entry_first(const DistillArg& a, const Entries& e, int i, int64_t c0, int64_t c1,
-                                            float* q) {
-    const int32_t id = e.id[i];
-    if (id < c0 || id >= c1) return false;
-    float s = 0.0f;
-    for (int j = 0; j < a.k; ++j)
-        if (e.id[j] == id) {
-            if (j < i) return false;
-            s += e.q[j];
-        }
-    *q = s;
-    return true;
-}
-
-__device__ __forceinline__ int32_t kept_rows(const int32_t* part) {
-    const int lane = threadIdx.x & 63;
-    int32_t n = 0;
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < kCountBlocks / 64; ++i) n += part[lane + 64 * i];
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The rows' entries, a wavefront a row. Entries of one class meet in a hash table in LDS, of twice as many slots
+// as entries at least: the first of them, by its place, takes the sum of their q in their order.
+__global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
+    extern __shared__ int32_t lds[];
+    __shared__ int32_t red[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int32_t* key = lds + (size_t)wave * (3 * a.slots + 2 * a.k);  // a slot's class
+    int32_t* first = key + a.slots;                                // its first entry
+    int32_t* many = first + a.slots;                               // its entries
+    int32_t* id = many + a.slots;
+    float* q = reinterpret_cast<float*>(id + a.k);
+    const float ninf = -__builtin_inff();
+    int32_t kept = 0;
+    for (int64_t r = (int64_t)blockIdx.x * waves + wave; r < a.rows; r += (int64_t)gridDim.x * waves) {
+        const int64_t at = r * a.k;
+        float best = ninf;
+        bool any = false, bad = false;
+        wave_sync();
+        for (int i = lane; i < a.k; i += 64) {
+            const int32_t c = a.ids[at + i];
+            const float t = a.teacher[at + i];
+            const bool in = c >= 0 && t != ninf;
+            any = any || in;
+            bad = bad || (in && c >= a.classes);
+            id[i] = in ? c : -1;
+            q[i] = in ? t * a.inv_t : ninf;
+            if (in) best = __builtin_fmaxf(best, t * a.inv_t);
+        }
+        any = __any(any);
+        bad = __any(bad);
+        kept += any;
+        if (lane == 0) a.flag[r] = bad ? 2 : any ? 1 : 0;
+        if (!any || bad) {
+            for (int i = lane; i < a.k; i += 64) a.ent_id[at + i] = -1;
+            if (lane == 0) a.term[r] = 0.0f;
+            continue;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
+        for (int s = lane; s < a.slots; s += 64) {
+            key[s] = -1;
+            first[s] = 0x7fffffff;
+            many[s] = 0;
+        }
+        float mass = 0.0f;
+        for (int i = lane; i < a.k; i += 64) mass += id[i] >= 0 ? exp_neg(q[i] - best) : 0.0f;
+        mass = wave_sum(mass);
+        const float lm = mlog(mass), inv = 1.0f / mass;
+        wave_sync();
+        float term = 0.0f;
+        for (int i = lane; i < a.k; i += 64) {
+            const int32_t c = id[i];
+            if (c < 0) {
+                q[i] = 0.0f;
+                continue;
+            }
+            const float x = a.x[r * a.classes + c], u = q[i] - best;
+            const float v = exp_neg(u) * inv;
+            a.ent_x[at + i] = x;
+            q[i] = v;
+            if (v != 0.0f) term += v * (u - lm - x * a.inv_t);  // 0 log 0 = 0
+            uint32_t s = ((uint32_t)c * 2654435761u) & (uint32_t)(a.slots - 1);
+            for (;;) {  // ends: slots are more than entries
+                const int32_t old = atomicCAS(&key[s], -1, c);
+                if (old == -1 || old == c) break;
+                s = (s + 1) & (uint32_t)(a.slots - 1);
+            }
+            atomicMin(&first[s], i);
+            atomicAdd(&many[s], 1);
+            a.ent_q[at + i] = __int_as_float((int)s);  // for the pass below
+        }
+        wave_sync();
+        for (int i = lane; i < a.k; i += 64) {
+            const int32_t c = id[i];
+            bool mine = c >= 0;
+            float v = q[i];
+            if (mine) {
+                const int s = __float_as_int(a.ent_q[at + i]);
+                mine = first[s] == i;
+                if (mine && many[s] > 1)
+                    for (int j = i + 1; j < a.k; ++j) v += id[j] == c ? q[j] : 0.0f;
+            }
+            a.ent_id[at + i] = mine ? c : -1;
+            a.ent_q[at + i] = v;
+        }
+        term = wave_sum(term);
+        if (lane == 0) a.term[r] = term;
+    }
+    if (lane == 0) red[wave] = kept;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int32_t n = 0;
+        for (int i = 0; i < waves; ++i) n += red[i];
+        a.kept[blockIdx.x] = n;
+    }
+}
+
+// Rows with an entry, 1 at least; every lane of a wavefront gets them.
+__device__ __forceinline__ int32_t kept_rows(const DistillArg& a) {
+    int32_t n = 0;
+    for (int i = threadIdx.x & 63; i < a.parts; i += 64) n += a.kept[i];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     return n > 0 ? n : 1;
 }
+// ug T / n: by the first wavefront, to every thread; `out` is LDS, read after a barrier.
+__device__ __forceinline__ void factor_to(const DistillArg& a, float* out) {
+    if (threadIdx.x < 64) {
+        const float c = a.ug[0] * a.temperature / (float)kept_rows(a);
+        if (threadIdx.x == 0) *out = c;
+    }
+}
 
-// Running maximum and sum of exponentials, in base 2: t = x log2(e) / T.
+// Running maximum and sum of exponentials, in base 2.
 struct Run {
     float top, sum;
 };
@@ -149,6 +183,26 @@ __device__ __forceinline__ void run_add(Run& r, vf4 v, float kf) {
     const float b = r.top == -__builtin_inff() ? 0.0f : r.top;
     r.sum += (__builtin_amdgcn_exp2f((v.x - b) * kf) + __builtin_amdgcn_exp2f((v.y - b) * kf)) +
              (__builtin_amdgcn_exp2f((v.z - b) * kf) + __builtin_amdgcn_exp2f((v.w - b) * kf));
+}
+// Adds classes c0..c1 of a row, four loads in flight a thread.
+template <int W>
+__device__ __forceinline__ void run_row(Run& run, const float* x, int64_t c0, int64_t c1, float kf) {
+    constexpr int64_t step = W * 64;
+    const int64_t nq = (c1 - c0) >> 2;
+    const float* p = x + c0;
+    int64_t q = threadIdx.x;
+    for (; q + 3 * step < nq; q += 4 * step) {
+        vf4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const vf4u*>(p + 4 * (q + u * step));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) run_add(run, v[u], kf);
+    }
+    for (; q < nq; q += step) run_add(run, *reinterpret_cast<const vf4u*>(p + 4 * q), kf);
+    if ((int64_t)threadIdx.x < (c1 - c0) - 4 * nq) {
+        const float ninf = -__builtin_inff();
+        run_add(run, vf4{p[4 * nq + threadIdx.x], ninf, ninf, ninf}, kf);
+    }
 }
 template <int W>
 __device__ __forceinline__ Run run_join(Run r, float kf, float* red) {
@@ -175,6 +229,14 @@ template <bool LSE>
 __device__ __forceinline__ vf4 grad4(const Scale<LSE>& s, vf4 v, float c) {
     return {prob(s, v.x) * c, prob(s, v.y) * c, prob(s, v.z) * c, prob(s, v.w) * c};
 }
+template <bool ACC>
+__device__ __forceinline__ void grad_put(float* o, vf4 v) {
+    if (ACC) {
+        const vf4 old = ld_ntu(o);
+        v = {old.x + v.x, old.y + v.y, old.z + v.z, old.w + v.w};
+    }
+    st_ntu(o, v);
+}
 
 // A row left out: its gradient is left alone, or zero.
 template <int W, bool ACC>
@@ -187,92 +249,154 @@ __device__ void row_zero(const DistillArg& a, int64_t r, int64_t c0, int64_t c1)
     if ((int64_t)threadIdx.x < c1 - q1) g[q1 + threadIdx.x] = 0.0f;
 }
 
-// Classes c0..c1 of row r's gradient.
-template <int W, bool ACC, bool LSE>
-__device__ void row_grad(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, const Entries& e, const Scale<LSE>& s,
-                         float c) {
-    const float* x = a.x + r * a.classes;
-    float* g = a.grad + r * a.classes;
-    const int tid = threadIdx.x;
-    // each thread's entries before the dense part writes over them; kMaxK / (W * 64) at most
-    constexpr int NE = (kMaxK + W * 64 - 1) / (W * 64);
-    float mine[NE];
-    int32_t at[NE];
+// A row's loss before T^2 / n, its log-sum-exp, and the marks of a row without entries or with a bad id.
+__device__ __forceinline__ void row_out(const DistillArg& a, int64_t r, int flag, float lse) {
+    if (threadIdx.x != 0) return;
+    a.row_loss[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : a.term[r] + lse;  // the q sum to 1
+    if (a.row_lse) a.row_lse[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : lse;
+}
+
+// A thread's entries of classes c0..c1: with ACC what the gradient held there is read before the dense part
+// writes over it; all are stored after it.
+template <int W>
+struct Mine {
+    static constexpr int N = (kMaxK + W * 64 - 1) / (W * 64);
+    int32_t at[N];
+    float old[N];
+};
+template <int W, bool ACC>
+__device__ __forceinline__ void entries_take(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, Mine<W>& mine) {
 #pragma unroll
-    for (int u = 0; u < NE; ++u) {
-        const int i = tid + u * W * 64;
-        float q = 0.0f;
-        at[u] = -1;
-        if (i < a.k && entry_first<W>(a, e, i, c0, c1, &q)) {
-            at[u] = e.id[i];
-            mine[u] = (prob(s, x[at[u]]) - q) * c;
-            if (ACC) mine[u] = g[at[u]] + mine[u];
-        }
+    for (int u = 0; u < Mine<W>::N; ++u) {
+        const int i = threadIdx.x + u * W * 64;
+        int32_t c = i < a.k ? a.ent_id[r * a.k + i] : -1;
+        if (c < c0 || c >= c1) c = -1;
+        mine.at[u] = c;
+        mine.old[u] = ACC && c >= 0 ? a.grad[r * a.classes + c] : 0.0f;
     }
+    if (ACC) __syncthreads();
+}
+template <int W, bool ACC, bool LSE>
+__device__ __forceinline__ void entries_put(const DistillArg& a, int64_t r, const Scale<LSE>& s, float c, const Mine<W>& mine) {
     __syncthreads();
-    const int64_t nq = (c1 - c0) >> 2;
-    const int tail = (int)((c1 - c0) & 3);
-    for (int64_t q = nq - 1 - tid; q >= 0; q -= W * 64) {  // from the end, which was read last
-        float* o = g + c0 + 4 * q;
-        vf4 v = grad4(s, ld_ntu(x + c0 + 4 * q), c);
-        if (ACC) {
-            const vf4 old = ld_ntu(o);
-            v = {old.x + v.x, old.y + v.y, old.z + v.z, old.w + v.w};
-        }
-        st_ntu(o, v);
+#pragma unroll
+    for (int u = 0; u < Mine<W>::N; ++u) {
+        if (mine.at[u] < 0) continue;
+        const int64_t i = r * a.k + threadIdx.x + u * W * 64;
+        const float v = (prob(s, a.ent_x[i]) - a.ent_q[i]) * c;
+        a.grad[r * a.classes + mine.at[u]] = ACC ? mine.old[u] + v : v;
     }
-    if (tid < tail) {
-        const int64_t p = c0 + 4 * nq + tid;
+}
+
+// Classes c0..c1 of row r's gradient, from the end, which was read last; four loads in flight a thread.
+template <int W, bool ACC, bool LSE>
+__device__ void row_grad(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, const Scale<LSE>& s, float c) {
+    constexpr int64_t step = W * 64;
+    const float* x = a.x + r * a.classes + c0;
+    float* g = a.grad + r * a.classes + c0;
+    const int tid = threadIdx.x;
+    Mine<W> mine;
+    entries_take<W, ACC>(a, r, c0, c1, mine);
+    const int64_t nq = (c1 - c0) >> 2;
+    int64_t q = nq - 1 - tid;
+    for (; q - 3 * step >= 0; q -= 4 * step) {
+        vf4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = ld_ntu(x + 4 * (q - u * step));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) grad_put<ACC>(g + 4 * (q - u * step), grad4(s, v[u], c));
+    }
+    for (; q >= 0; q -= step) grad_put<ACC>(g + 4 * q, grad4(s, ld_ntu(x + 4 * q), c));
+    if (tid < (int)((c1 - c0) & 3)) {
+        const int64_t p = 4 * nq + tid;
         const float v = prob(s, x[p]) * c;
         g[p] = ACC ? g[p] + v : v;
     }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < NE; ++u)
-        if (at[u] >= 0) g[at[u]] = mine[u];
+    entries_put<W, ACC>(a, r, s, c, mine);
 }
 
 // A whole row a workgroup: statistics, loss and, with GRAD, the gradient.
 template <int W, bool GRAD, bool ACC>
 __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
-    __shared__ Entries e;
-    __shared__ float red[W];
+    __shared__ float red[W], factor;
     const int64_t r = blockIdx.x;
-    const int what = load_entries<W>(a, r, e, red);
-    if (what == 0) {
-        if (threadIdx.x == 0) {
-            a.row_loss[r] = 0.0f;
-            if (a.row_lse) a.row_lse[r] = 0.0f;
-        }
+    const int flag = a.flag[r];
+    if (flag == 0) {
+        row_out(a, r, 0, 0.0f);
         if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
         return;
     }
+    if (GRAD) factor_to(a, &factor);
     const float kf = a.inv_t * kLog2e;
-    const float* x = a.x + r * a.classes;
     Run run = {-__builtin_inff(), 0.0f};
-    const int64_t nq = a.classes >> 2;
-    for (int64_t q = threadIdx.x; q < nq; q += W * 64) run_add(run, *reinterpret_cast<const vf4u*>(x + 4 * q), kf);
-    const int tail = (int)(a.classes & 3);
-    if ((int)threadIdx.x < tail) {
-        const float ninf = -__builtin_inff();
-        run_add(run, vf4{x[4 * nq + threadIdx.x], ninf, ninf, ninf}, kf);
-    }
+    run_row<W>(run, a.x + r * a.classes, 0, a.classes, kf);
     run = run_join<W>(run, kf, red);
-    float lse = run.top * a.inv_t + mlog(run.sum);
-    if (what == 2) lse = __builtin_nanf("");  // an id past the classes: shown in the loss and the gradient
-    const float loss = what == 2 ? lse : row_loss_of<W>(a, r, e, lse, red);
-    if (threadIdx.x == 0) {
-        a.row_loss[r] = loss;
-        if (a.row_lse) a.row_lse[r] = lse;
+    row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
+    if (GRAD) {  // an id past the classes: NaN all over the row
+        const Scale<false> s = {kf, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
+        row_grad<W, ACC>(a, r, 0, a.classes, s, factor);
     }
+}
+
+// The same with the row in registers, NQ quads a thread, read once; a row's exponentials are taken once too.
+// Two workgroups of 16 wavefronts share a CU at 64 registers, one loading while the other stores; at the 78
+// that the compiler took unbounded one workgroup ran alone (91 us against 69 over [1025, 30011]).
+template <int W, int NQ, bool GRAD, bool ACC>
+__global__ __launch_bounds__(W * 64, 8) void k_distill_regs(DistillArg a) {
+    __shared__ float red[W], factor;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const float ninf = -__builtin_inff();
+    const float* x = a.x + r * a.classes;
+    const int nq = (int)(a.classes >> 2), tail = (int)(a.classes & 3);
+    const int flag = a.flag[r];
+    if (flag == 0) {
+        row_out(a, r, 0, 0.0f);
+        if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
+        return;
+    }
+    vf4 v[NQ];
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
+        const int q = tid + u * W * 64;
+        v[u] = q < nq ? ld_ntu(x + 4 * q) : vf4{ninf, ninf, ninf, ninf};
+    }
+    float last = tid < tail ? x[4 * nq + tid] : ninf;
+    if (GRAD) factor_to(a, &factor);
+    const float kf = a.inv_t * kLog2e;
+    float top = last;
+#pragma unroll
+    for (int u = 0; u < NQ; ++u)
+        top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(v[u].x, v[u].y), __builtin_fmaxf(v[u].z, v[u].w)));
+    top = block_max<W>(top, red);
+    const float base = top == ninf ? 0.0f : top;
+    const Scale<false> raw = {kf, base, 1.0f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
+        v[u] = grad4(raw, v[u], 1.0f);
+        sum += (v[u].x + v[u].y) + (v[u].z + v[u].w);
+    }
+    last = prob(raw, last);
+    sum = block_sum<W>(sum + last, red);
+    row_out(a, r, flag, top * a.inv_t + mlog(sum));
     if (GRAD) {
-        const float c = a.ug[0] * a.temperature / (float)kept_rows(a.kept);
-        if (what == 2) {  // NaN all over the row, entries or not
-            for (int i = threadIdx.x; i < a.k; i += W * 64) e.id[i] = -1;
-            __syncthreads();
+        const float c = factor;
+        const Scale<false> s = {kf, base, flag == 2 ? __builtin_nanf("") : 1.0f / sum};
+        Mine<W> mine;
+        entries_take<W, ACC>(a, r, 0, a.classes, mine);
+        float* g = a.grad + r * a.classes;
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            const int q = tid + u * W * 64;
+            const vf4 o = {v[u].x * s.inv * c, v[u].y * s.inv * c, v[u].z * s.inv * c, v[u].w * s.inv * c};
+            if (q < nq) grad_put<ACC>(g + 4 * q, o);
         }
-        const Scale<false> s = {kf, run.top, 1.0f / (what == 2 ? lse : run.sum)};
-        row_grad<W, ACC>(a, r, 0, a.classes, e, s, c);
+        if (tid < tail) {
+            const float o = last * s.inv * c;
+            g[4 * nq + tid] = ACC ? g[4 * nq + tid] + o : o;
+        }
+        entries_put<W, ACC>(a, r, s, c, mine);
     }
 }
 
@@ -281,17 +405,11 @@ template <int W>
 __global__ __launch_bounds__(W * 64) void k_distill_stat(DistillArg a) {
     __shared__ float red[W];
     const int64_t r = blockIdx.x / a.splits, sp = blockIdx.x % a.splits;
+    if (a.flag[r] == 0) return;
     const int64_t c0 = sp * a.span, c1 = c0 + a.span < a.classes ? c0 + a.span : a.classes;
     const float kf = a.inv_t * kLog2e;
-    const float* x = a.x + r * a.classes;
     Run run = {-__builtin_inff(), 0.0f};
-    const int64_t nq = (c1 - c0) >> 2;
-    for (int64_t q = threadIdx.x; q < nq; q += W * 64) run_add(run, *reinterpret_cast<const vf4u*>(x + c0 + 4 * q), kf);
-    const int tail = (int)((c1 - c0) & 3);
-    if ((int)threadIdx.x < tail) {
-        const float ninf = -__builtin_inff();
-        run_add(run, vf4{x[c0 + 4 * nq + threadIdx.x], ninf, ninf, ninf}, kf);
-    }
+    run_row<W>(run, a.x + r * a.classes, c0, c1, kf);
     run = run_join<W>(run, kf, red);
     if (threadIdx.x == 0) {
         a.stat[blockIdx.x * 2] = run.top;
@@ -310,67 +428,48 @@ __device__ __forceinline__ Run join_splits(const DistillArg& a, int64_t r) {
     return {top, sum};
 }
 
-// A split of a row's gradient, from the forward's log-sum-exp or the splits' statistics; with LOSS the first
-// split writes the row's loss. GRAD off: the loss alone, a workgroup a row.
+// A split of a row's gradient, from the forward's log-sum-exp (LOSS off) or the splits' statistics, of which the
+// first split also writes the row's loss. GRAD off: the loss alone, a workgroup a row.
 template <int W, bool LOSS, bool GRAD, bool ACC>
 __global__ __launch_bounds__(W * 64) void k_distill_split(DistillArg a) {
-    __shared__ Entries e;
-    __shared__ float red[W];
+    __shared__ float factor;
     const int32_t per = GRAD ? a.splits : 1;
     const int64_t r = blockIdx.x / per, sp = blockIdx.x % per;
     const int64_t c0 = sp * a.span, c1 = c0 + a.span < a.classes ? c0 + a.span : a.classes;
-    const int what = load_entries<W>(a, r, e, red);
-    if (what == 0) {
-        if (LOSS && sp == 0 && threadIdx.x == 0) {
-            a.row_loss[r] = 0.0f;
-            if (a.row_lse) a.row_lse[r] = 0.0f;
-        }
+    const int flag = a.flag[r];
+    if (flag == 0) {
+        if (LOSS && sp == 0) row_out(a, r, 0, 0.0f);
         if (GRAD) row_zero<W, ACC>(a, r, c0, c1);
         return;
     }
-    float lse;
+    if (GRAD) {
+        factor_to(a, &factor);
+        __syncthreads();
+    }
     if (LOSS) {
         const Run run = join_splits(a, r);
-        lse = run.top * a.inv_t + mlog(run.sum);
+        if (sp == 0) row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
+        if (GRAD) {
+            const Scale<false> s = {a.inv_t * kLog2e, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
+            row_grad<W, ACC>(a, r, c0, c1, s, factor);
+        }
     } else {
-        lse = a.lse_in[r];
-    }
-    if (what == 2) lse = __builtin_nanf("");
-    if (LOSS && sp == 0) {
-        const float loss = what == 2 ? lse : row_loss_of<W>(a, r, e, lse, red);
-        if (threadIdx.x == 0) {
-            a.row_loss[r] = loss;
-            if (a.row_lse) a.row_lse[r] = lse;
-        }
-    }
-    if (GRAD) {
-        const float c = a.ug[0] * a.temperature / (float)kept_rows(a.kept);
-        if (what == 2) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < a.k; i += W * 64) e.id[i] = -1;
-            __syncthreads();
-        }
-        if (LOSS) {  // the splits' statistics are there
-            const Run run = join_splits(a, r);
-            const Scale<false> s = {a.inv_t * kLog2e, run.top, 1.0f / (what == 2 ? lse : run.sum)};
-            row_grad<W, ACC>(a, r, c0, c1, e, s, c);
-        } else {
-            const Scale<true> s = {a.inv_t, lse, 1.0f};
-            row_grad<W, ACC>(a, r, c0, c1, e, s, c);
-        }
+        const Scale<true> s = {a.inv_t, flag == 2 ? __builtin_nanf("") : a.lse_in[r], 1.0f};
+        row_grad<W, ACC>(a, r, c0, c1, s, factor);
     }
 }
 
 // loss = T^2 / n sum of the rows' losses, in a fixed order.
-__global__ __launch_bounds__(1024) void k_distill_loss(const float* row_loss, int64_t rows, const int32_t* kept,
-                                                       float temperature, float* loss) {
+__global__ __launch_bounds__(1024) void k_distill_loss(DistillArg a, float* loss) {
     __shared__ double red[16];
     double s = 0.0;
 #pragma unroll 4
-    for (int64_t n = threadIdx.x; n < rows; n += 1024) s += (double)row_loss[n];
+    for (int64_t n = threadIdx.x; n < a.rows; n += 1024) s += (double)a.row_loss[n];
     s = block_sum<16>(s, red);
-    const double n = kept_rows(kept);
-    if (threadIdx.x == 0) loss[0] = (float)(s * ((double)temperature * temperature) / n);
+    if (threadIdx.x < 64) {
+        const double n = kept_rows(a);
+        if (threadIdx.x == 0) loss[0] = (float)(s * ((double)a.temperature * a.temperature) / n);
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -425,22 +524,52 @@ int distill_run(const DistillCall& d) {
     a.splits = row_splits(d.rows, d.classes);
     a.span = ((d.classes + a.splits - 1) / a.splits + 3) & ~(int64_t)3;
     a.splits = (int32_t)((d.classes + a.span - 1) / a.span);
-    const size_t n_kept = kCountBlocks * sizeof(int32_t);
-    const size_t n_loss = ((size_t)d.rows * sizeof(float) + 255) & ~(size_t)255;
+    a.slots = 64;
+    while (a.slots < 2 * a.k) a.slots *= 2;
+    // wavefronts of a workgroup of k_distill_entries by what LDS holds: 16 up to 128 entries a row, 2 at 1024
+    const size_t row_lds = (3 * (size_t)a.slots + 2 * (size_t)a.k) * sizeof(int32_t);
+    int waves = 16;
+    while (waves > 1 && waves * row_lds > 65536) waves /= 2;
+    while (waves > 4 && d.rows < (int64_t)waves * ctx().num_cus) waves /= 2;
+    const int64_t blocks = (d.rows + waves - 1) / waves;
+    a.parts = (int32_t)(blocks < kEntryBlocks ? blocks : kEntryBlocks);
+    const size_t rows_b = ((size_t)d.rows * 4 + 255) & ~(size_t)255, ent_b = ((size_t)d.rows * a.k * 4 + 255) & ~(size_t)255;
     char* base = nullptr;
-    MH_TRY(scratch(n_kept + n_loss + (size_t)d.rows * a.splits * 2 * sizeof(float), reinterpret_cast<void**>(&base)));
-    int32_t* kept = reinterpret_cast<int32_t*>(base);
-    a.kept = kept;
-    a.row_loss = reinterpret_cast<float*>(base + n_kept);
-    a.stat = reinterpret_cast<float*>(base + n_kept + n_loss);
+    MH_TRY(scratch(kEntryBlocks * 4 + 3 * rows_b + 3 * ent_b + (size_t)d.rows * a.splits * 8, reinterpret_cast<void**>(&base)));
+    auto take = [&base](size_t bytes) {
+        char* p = base;
+        base += bytes;
+        return p;
+    };
+    a.kept = reinterpret_cast<int32_t*>(take(kEntryBlocks * 4));
+    a.flag = reinterpret_cast<int32_t*>(take(rows_b));
+    a.term = reinterpret_cast<float*>(take(rows_b));
+    a.row_loss = reinterpret_cast<float*>(take(rows_b));
+    a.ent_id = reinterpret_cast<int32_t*>(take(ent_b));
+    a.ent_q = reinterpret_cast<float*>(take(ent_b));
+    a.ent_x = reinterpret_cast<float*>(take(ent_b));
+    a.stat = reinterpret_cast<float*>(base);
     hipStream_t st = ctx().stream;
-    hipLaunchKernelGGL(k_distill_count, dim3(kCountBlocks), dim3(256), 0, st, kept, d.ids, d.teacher, d.rows, a.k);
+    hipLaunchKernelGGL(k_distill_entries, dim3((unsigned)a.parts), dim3(waves * 64), waves * row_lds, st, a);
     constexpr int W = 16;
     const dim3 rows((unsigned)d.rows), all((unsigned)(d.rows * a.splits)), t(W * 64);
     const bool grad = d.grad != nullptr;
     if (d.lse_in) {
         if (d.accumulate) hipLaunchKernelGGL((k_distill_split<W, false, true, true>), all, t, 0, st, a);
         else hipLaunchKernelGGL((k_distill_split<W, false, true, false>), all, t, 0, st, a);
+    } else if (a.splits == 1 && a.classes <= kInRegs) {
+#define MH_REGS(WW, NQ)                                                                                                \
+    do {                                                                                                              \
+        const dim3 tt(WW * 64);                                                                                       \
+        if (!grad) hipLaunchKernelGGL((k_distill_regs<WW, NQ, false, false>), rows, tt, 0, st, a);                    \
+        else if (d.accumulate) hipLaunchKernelGGL((k_distill_regs<WW, NQ, true, true>), rows, tt, 0, st, a);          \
+        else hipLaunchKernelGGL((k_distill_regs<WW, NQ, true, false>), rows, tt, 0, st, a);                           \
+    } while (0)
+        if (a.classes <= 4096) MH_REGS(4, 4);
+        else if (a.classes <= 8192) MH_REGS(4, 8);
+        else if (a.classes <= 16384) MH_REGS(8, 8);
+        else MH_REGS(16, 8);
+#undef MH_REGS
     } else if (a.splits == 1) {
         if (!grad) hipLaunchKernelGGL((k_distill_row<W, false, false>), rows, t, 0, st, a);
         else if (d.accumulate) hipLaunchKernelGGL((k_distill_row<W, true, true>), rows, t, 0, st, a);
@@ -452,7 +581,7 @@ int distill_run(const DistillCall& d) {
         else hipLaunchKernelGGL((k_distill_split<W, true, true, false>), all, t, 0, st, a);
     }
     if (d.loss)
-        hipLaunchKernelGGL(k_distill_loss, dim3(1), dim3(1024), 0, st, a.row_loss, d.rows, kept, d.temperature, d.loss);
+        hipLaunchKernelGGL(k_distill_loss, dim3(1), dim3(1024), 0, st, a, d.loss);
     return finish(d.what);
 }
 
