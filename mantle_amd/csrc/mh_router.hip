@@ -10,7 +10,8 @@
 // Bound by the logits' read and the gradient's write over long batches, by launches over short ones. L lanes
 // hold a row in registers, V elements a lane in quads (element 4 (i L + lane) + c), so that the columns of a lane
 // are the same for all its rows: the sums P_e and the loss's f_e stay in registers over the rows of a workgroup.
-// Selection takes k rounds of a maximum of sortable integers over the lane's elements, then over the row's lanes.
+// Up to 8 choices come from sorted lists, more from rounds of a maximum over the lane's elements, then the row's
+// lanes.
 // Sums over rows are fp32 per workgroup and in a fixed order; counts are whole numbers.
 #include "mh_internal.h"
 #include "mh_rows.h"
@@ -128,9 +129,10 @@ __device__ __forceinline__ void get_row(const float* row, int l, float* v) {
     }
 }
 
-// v to e^(v - max); returns their sum. Past the experts 0.
+// v to e^(v - max); returns their sum and the maximum. Past the experts 0.
+__device__ __forceinline__ float exp_diff(float v, float m) { return __builtin_amdgcn_exp2f((v - m) * kLog2e); }
 template <int L, int V>
-__device__ __forceinline__ float row_exp(float* v) {
+__device__ __forceinline__ float row_exp(float* v, float* top) {
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) m = __builtin_fmaxf(m, v[i]);
@@ -138,10 +140,107 @@ __device__ __forceinline__ float row_exp(float* v) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        v[i] = exp_neg(v[i] - m);
+        v[i] = exp_diff(v[i], m);
         s += v[i];
     }
+    *top = m;
     return group_sum<L>(s);
+}
+
+// Up to 8 choices: sorted lists. A logit's order and its index become the mantissa of a double in [1, 2), which
+// the maximum and minimum of doubles sort, one instruction each and at full rate; a larger index is smaller.
+// Each lane sorts its elements and keeps 8; neighbours' lists merge, and in the end each lane has the row's 8.
+// [131072, 256], 8 of them: 84 us by rounds of a maximum, 58 by lists.
+constexpr int kList = 8;
+__device__ __forceinline__ double list_key(int key, int index) {
+    const uint32_t u = (uint32_t)key ^ 0x80000000u;
+    return __hiloint2double((int)(0x3ff00000u | (u >> 22)), (int)(u << 10 | (uint32_t)(kMaxExperts - 1 - index)));
+}
+__device__ __forceinline__ int list_index(double d) { return kMaxExperts - 1 - (__double2loint(d) & (kMaxExperts - 1)); }
+__device__ __forceinline__ int list_value(double d) {
+    return (int)((((uint32_t)__double2hiint(d) << 22) | ((uint32_t)__double2loint(d) >> 10)) ^ 0x80000000u);
+}
+__device__ __forceinline__ double max_d(double a, double b) {
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double min_d(double a, double b) {
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ void order(double& a, double& b) {
+    const double hi = max_d(a, b), lo = min_d(a, b);
+    a = hi;
+    b = lo;
+}
+__device__ __forceinline__ void sort4(double* d) {
+    order(d[0], d[1]);
+    order(d[2], d[3]);
+    order(d[0], d[2]);
+    order(d[1], d[3]);
+    order(d[1], d[2]);
+}
+__device__ __forceinline__ void merge8(double* d) {  // 8 that rise and fall
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(i & s)) order(d[i], d[i + s]);
+}
+__device__ __forceinline__ void sort8(double* d) {
+    sort4(d);
+    sort4(d + 4);
+    double t = d[4];
+    d[4] = d[7];
+    d[7] = t;
+    t = d[5];
+    d[5] = d[6];
+    d[6] = t;
+    merge8(d);
+}
+__device__ __forceinline__ void join8(double* d, const double* o) {  // the 8 largest of two sorted lists
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = max_d(d[i], o[7 - i]);
+    merge8(d);
+}
+template <int STEP>
+__device__ __forceinline__ int other_lane(int v) {
+    return STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(v) : STEP == 8 ? dpp<0x140>(v)
+                                                                                                  : __shfl_xor(v, STEP);
+}
+template <int STEP, int L>
+__device__ __forceinline__ void join_lanes(double* d) {
+    if constexpr (STEP < L) {
+        double o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = __hiloint2double(other_lane<STEP>(__double2hiint(d[i])), other_lane<STEP>(__double2loint(d[i])));
+        join8(d, o);
+        join_lanes<2 * STEP, L>(d);
+    }
+}
+template <int L, int V>
+__device__ __forceinline__ void row_list(const float* v, int E, int l, double* list) {
+    double d[V < 8 ? 8 : V];
+#pragma unroll
+    for (int i = 0; i < (V < 8 ? 8 : V); ++i) {
+        const int e = 4 * ((i / 4) * L + l) + (i & 3);
+        d[i] = i < V && e < E ? list_key(sort_key(v[i < V ? i : 0]), e) : 1.0;
+    }
+    if constexpr (V == 4) {
+        sort4(d);
+    } else {
+        sort8(d);
+        if constexpr (V == 16) {
+            sort8(d + 8);
+            join8(d, d + 8);
+        }
+    }
+    join_lanes<1, L>(d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) list[i] = d[i];
 }
 
 // The counts, the mean probabilities and the loss from the workgroups' partials: one workgroup, over a few
@@ -166,12 +265,12 @@ __device__ void router_total(const RouterArg& a, float* red) {
     if (threadIdx.x == 0) a.loss[0] = (float)a.experts * (s / nk / nk / (float)a.k);
 }
 
-template <int L, int V>
+template <int L, int V, bool LIST>
 __global__ __launch_bounds__(kRThreads) void k_router_fwd(RouterArg a) {
     constexpr int G = kRThreads / L;  // rows in flight in a workgroup
+    constexpr int K = LIST ? kList : L * V < kMaxChosen ? L * V : kMaxChosen;
     __shared__ float red[kRThreads / 64];
     __shared__ int32_t cnt[L * V];
-    constexpr int K = L * V < kMaxChosen ? L * V : kMaxChosen;
     __shared__ float pick[G][K];
     __shared__ int32_t pick_id[G][K];
     __shared__ float sum_p[(G > 1 ? G : 2) / 2 * L * V];
@@ -188,60 +287,64 @@ __global__ __launch_bounds__(kRThreads) void k_router_fwd(RouterArg a) {
         const int64_t r = r0 + g;
         const bool in = r < a.rows;
         const bool keep = in && (!a.keep || a.keep[r] != 0);
-        float v[V];
-        int key[V];
+        float v[V], m;
         load_row<L, V>(a.x + (in ? r : r0) * a.experts, a.experts, l, v);
+        if constexpr (LIST) {
+            double list[kList];
+            row_list<L, V>(v, a.experts, l, list);
+            wave_sync();
+            if (l == 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts ? sort_key(v[i]) : kTaken;
-        float m = v[0];
+                for (int t = 0; t < kList; ++t) {
+                    pick[g][t] = key_value(list_value(list[t]));
+                    pick_id[g][t] = list_index(list[t]);
+                }
+            }
+        } else {
+            int key[V];
 #pragma unroll
-        for (int i = 1; i < V; ++i) m = __builtin_fmaxf(m, v[i]);
-        m = group_max<L>(m);
-        float s = 0.0f;
+            for (int i = 0; i < V; ++i) key[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts ? sort_key(v[i]) : kTaken;
+            wave_sync();
+            for (int t = 0; t < a.k; ++t) {
+                int best = key[0];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            v[i] = exp_neg(v[i] - m);
-            s += v[i];
+                for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
+                best = group_red<L>(best, [](int p, int q) { return p > q ? p : q; });
+                int at = 0x7fffffff;  // the lowest index that holds it
+#pragma unroll
+                for (int i = V - 1; i >= 0; --i) at = key[i] == best ? 4 * (i / 4) * L + (i & 3) : at;
+                at = at == 0x7fffffff ? at : at + 4 * l;
+                at = group_red<L>(at, [](int p, int q) { return p < q ? p : q; });
+                const int mine = at - 4 * l;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (mine == 4 * (i / 4) * L + (i & 3)) key[i] = kTaken;
+                if (l == 0) {
+                    pick[g][t] = key_value(best);
+                    pick_id[g][t] = at;
+                }
+            }
         }
-        s = group_sum<L>(s);
-        const float inv = 1.0f / s;
+        const float inv = 1.0f / row_exp<L, V>(v, &m);
         if (keep) {
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] += v[i] * inv;
             kept += l == 0;
         }
-        float all = 0.0f;  // of the chosen's exponentials
-        for (int t = 0; t < a.k; ++t) {
-            int best = key[0];
-#pragma unroll
-            for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
-            best = group_red<L>(best, [](int p, int q) { return p > q ? p : q; });
-            int at = 0x7fffffff;  // the lowest index that holds it
-#pragma unroll
-            for (int i = V - 1; i >= 0; --i) at = key[i] == best ? 4 * (i / 4) * L + (i & 3) : at;
-            at = at == 0x7fffffff ? at : at + 4 * l;
-            at = group_red<L>(at, [](int p, int q) { return p < q ? p : q; });
-            const int mine = at - 4 * l;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (mine == 4 * (i / 4) * L + (i & 3)) key[i] = kTaken;
-            const float e = exp_neg(key_value(best) - m);
-            all += e;
-            if (l == 0) {
-                pick[g][t] = e;
-                pick_id[g][t] = at;
-            }
-        }
         wave_sync();
-        const float scale = a.normalise ? 1.0f / all : inv;
+        float scale = inv;
+        if (a.normalise) {
+            float all = 0.0f;  // of the chosen's exponentials
+            for (int t = l; t < a.k; t += L) all += exp_diff(pick[g][t], m);
+            scale = 1.0f / group_sum<L>(all);
+        }
         if (in)
             for (int t = l; t < a.k; t += L) {
                 const int32_t id = pick_id[g][t];
                 a.chosen[r * a.k + t] = keep ? id : -1;
-                a.weights[r * a.k + t] = keep ? pick[g][t] * scale : 0.0f;
+                a.weights[r * a.k + t] = keep ? exp_diff(pick[g][t], m) * scale : 0.0f;
                 if (keep) atomicAdd(&cnt[id], 1);
             }
-        wave_sync();
     }
     // the workgroup's sums over its rows: halves of the groups added in turn
     kept = block_sum<kRThreads / 64>(kept, reinterpret_cast<int32_t*>(red));
@@ -335,7 +438,8 @@ __global__ __launch_bounds__(kRThreads) void k_router_bwd(RouterArg a) {
         const int64_t row = (in ? r : r0) * a.experts;
         float v[V], t[V];
         load_row<L, V>(a.x + row, a.experts, l, v);
-        const float inv = 1.0f / row_exp<L, V>(v);
+        float top;
+        const float inv = 1.0f / row_exp<L, V>(v, &top);
         // normalised weights w = e / sum of the chosen's e: their softmax's gradient first, from the row's
         // exponentials in LDS
         float w = 0.0f, mean = 0.0f;
@@ -481,7 +585,11 @@ int mh_router_fwd(float* weights, int32_t* chosen, int32_t* counts, float* loss,
     a.part_c = reinterpret_cast<int32_t*>(base + n);
     a.part_n = reinterpret_cast<int32_t*>(base + 2 * n);
     hipStream_t st = ctx().stream;
-#define MH_CALL(L, V) hipLaunchKernelGGL((k_router_fwd<L, V>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a)
+#define MH_CALL(L, V)                                                                                               \
+    do {                                                                                                           \
+        if (a.k <= kList) hipLaunchKernelGGL((k_router_fwd<L, V, true>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a); \
+        else hipLaunchKernelGGL((k_router_fwd<L, V, false>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a);   \
+    } while (0)
     MH_ROUTER(MH_CALL);
 #undef MH_CALL
     if (blocks > 1) {
