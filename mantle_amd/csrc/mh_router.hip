@@ -243,26 +243,48 @@ __device__ __forceinline__ void row_list(const float* v, int E, int l, double* l
     for (int i = 0; i < 8; ++i) list[i] = d[i];
 }
 
-// The counts, the mean probabilities and the loss from the workgroups' partials: one workgroup, over a few
-// partials.
-__device__ void router_total(const RouterArg& a, float* red) {
-    float s = 0.0f;
+// The counts and the loss from the workgroups' partials, by one workgroup of N threads: threads of 64 columns or
+// as many as there are experts, the others along the partials. `red` and `buf` are LDS of N each.
+template <int N>
+__device__ void router_total(const RouterArg& a, float* red, float* buf) {
     int32_t n = 0;
-    for (int b = threadIdx.x; b < a.blocks; b += kRThreads) n += a.part_n[b];
-    n = block_sum<kRThreads / 64>(n, reinterpret_cast<int32_t*>(red));
-    for (int e = threadIdx.x; e < a.experts; e += kRThreads) {
+    for (int b = threadIdx.x; b < a.blocks; b += N) n += a.part_n[b];
+    n = block_sum<N / 64>(n, reinterpret_cast<int32_t*>(red));
+    int32_t* buf_c = reinterpret_cast<int32_t*>(buf + N);
+    int cols = 8;
+    while (cols < 64 && cols < a.experts) cols *= 2;
+    const int col = threadIdx.x % cols, part = threadIdx.x / cols, parts = N / cols;
+    float s = 0.0f;
+    for (int e0 = 0; e0 < a.experts; e0 += cols) {
+        const int e = e0 + col;
         float p = 0.0f;
         int32_t c = 0;
-        for (int b = 0; b < a.blocks; ++b) {
-            p += a.part_p[(int64_t)b * a.experts + e];
-            c += a.part_c[(int64_t)b * a.experts + e];
+        if (e < a.experts)
+#pragma unroll 4
+            for (int b = part; b < a.blocks; b += parts) {
+                p += a.part_p[(int64_t)b * a.experts + e];
+                c += a.part_c[(int64_t)b * a.experts + e];
+            }
+        __syncthreads();
+        buf[threadIdx.x] = p;
+        buf_c[threadIdx.x] = c;
+        __syncthreads();
+        if (part == 0 && e < a.experts) {
+            for (int i = 1; i < parts; ++i) {
+                p += buf[i * cols + col];
+                c += buf_c[i * cols + col];
+            }
+            a.counts[e] = c;
+            s += (float)c * p;
         }
-        a.counts[e] = c;
-        s += (float)c * p;
     }
-    s = block_sum<kRThreads / 64>(s, red);
+    s = block_sum<N / 64>(s, red);
     const float nk = n > 0 ? (float)n : 1.0f;
     if (threadIdx.x == 0) a.loss[0] = (float)a.experts * (s / nk / nk / (float)a.k);
+}
+__global__ __launch_bounds__(1024) void k_router_total(RouterArg a) {
+    __shared__ float red[16], buf[2 * 1024];
+    router_total<1024>(a, red, buf);
 }
 
 template <int L, int V, bool LIST>
@@ -273,7 +295,8 @@ __global__ __launch_bounds__(kRThreads) void k_router_fwd(RouterArg a) {
     __shared__ int32_t cnt[L * V];
     __shared__ float pick[G][K];
     __shared__ int32_t pick_id[G][K];
-    __shared__ float sum_p[(G > 1 ? G : 2) / 2 * L * V];
+    constexpr int kSums = (G > 1 ? G : 2) / 2 * L * V;
+    __shared__ float sum_p[kSums > 2 * kRThreads ? kSums : 2 * kRThreads];  // for router_total at the end too
     const int tid = threadIdx.x, l = tid % L, g = tid / L;
     for (int e = tid; e < L * V; e += kRThreads) cnt[e] = 0;
     __syncthreads();
@@ -376,7 +399,7 @@ __global__ __launch_bounds__(kRThreads) void k_router_fwd(RouterArg a) {
     if (a.blocks == 1) {  // a short batch ends here
         __threadfence_block();
         __syncthreads();
-        router_total(a, red);
+        router_total<kRThreads>(a, red, sum_p);
     }
 }
 
@@ -592,7 +615,10 @@ int mh_router_fwd(float* weights, int32_t* chosen, int32_t* counts, float* loss,
     } while (0)
     MH_ROUTER(MH_CALL);
 #undef MH_CALL
-    if (blocks > 1) {
+    // few partials: one workgroup adds them up in the time of a launch; else a workgroup an expert, and the loss
+    if (blocks > 1 && blocks * experts <= 16384) {
+        hipLaunchKernelGGL(k_router_total, dim3(1), dim3(1024), 0, st, a);
+    } else if (blocks > 1) {
         hipLaunchKernelGGL(k_router_join, dim3((unsigned)experts), dim3(kRThreads), 0, st, a);
         hipLaunchKernelGGL(k_router_loss, dim3(1), dim3(kRThreads), 0, st, a);
     }

@@ -42,9 +42,13 @@ class TensorShape:
     __slots__ = ("_dims", "_n", "_cs")
 
     def __init__(self, *dims: Union[int, Iterable[int]]):
-        if len(dims) == 1 and type(dims[0]) is not int and not isinstance(dims[0], (int, np.integer)):
+        if len(dims) == 1 and not isinstance(dims[0], (int, np.integer)):
             dims = tuple(dims[0])
-        d = tuple(map(int, dims))
+        d = dims
+        for x in dims:  # plain ints, as nearly always, are taken as they are
+            if type(x) is not int:
+                d = tuple(map(int, dims))
+                break
         if not 1 <= len(d) <= MAX_RANK:
             raise ValueError(f"rank {len(d)} outside 1..{MAX_RANK}")
         self._dims = d
