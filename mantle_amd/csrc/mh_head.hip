@@ -124,13 +124,10 @@ __device__ __forceinline__ int scale_exp(float a) {
     return 15 - e;
 }
 
-__device__ __forceinline__ void split8(const float* v, half8* hi, half8* lo) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const _Float16 h = (_Float16)v[j];
-        (*hi)[j] = h;
-        (*lo)[j] = (_Float16)(v[j] - (float)h);
-    }
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void split8(f32x8 v, half8* hi, half8* lo) {
+    *hi = __builtin_convertvector(v, half8);
+    *lo = __builtin_convertvector(v - __builtin_convertvector(*hi, f32x8), half8);
 }
 
 constexpr int kSplitTile = 64;
@@ -148,7 +145,8 @@ struct SplitOne {
 };
 __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const HeadPart* part, HeadInfo* info,
                                                const int32_t* labels) {
-    __shared__ float t[kSplitTile][kSplitTile + 1];
+    // 68 floats a row: 16-byte accesses along a row and 4-byte ones along a column without bank conflicts
+    __shared__ __attribute__((aligned(16))) float t[kSplitTile][kSplitTile + 4];
     __shared__ float red[4];
     __shared__ int32_t cnt[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -160,12 +158,25 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
     float a = amax4(0.0f, reinterpret_cast<const vf4*>(isx ? part->ax : part->aw)[tid]);
     a = wave_max(a);
     if (lane == 0) red[wave] = a;
-    // the tile's rows, a wavefront a row
-    for (int i = 0; i < kSplitTile / 4; ++i) {
-        const int64_t r = r0 + i * 4 + wave, c = c0 + lane;
-        const bool in = r < s.nr && c < s.nc && !(isx && labels[r < s.nr ? r : 0] < 0);
-        t[i * 4 + wave][lane] = in ? s.src[r * s.nc + c] : 0.0f;
+    // 16 threads a row, a quad each
+    vf4 in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + i * 16 + (tid >> 4), c = c0 + (tid & 15) * 4;
+        in[i] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < s.nr && !(isx && labels[r] < 0)) {  // a row left out: zeros, whatever it holds
+            const float* p = s.src + r * s.nc + c;
+            if (c + 3 < s.nc) {
+                in[i] = ld_ntu(p);
+            } else {
+                if (c < s.nc) in[i].x = p[0];
+                if (c + 1 < s.nc) in[i].y = p[1];
+                if (c + 2 < s.nc) in[i].z = p[2];
+            }
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<vf4*>(&t[i * 16 + (tid >> 4)][(tid & 15) * 4]) = in[i];
     __syncthreads();
     const int e = scale_exp(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
     const int r = lane & 31, k8 = (lane >> 5) * 8;
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int rb = i, kb = wave;
-        float v[8];
+        f32x8 v;
         half8 hi, lo;
         if (r0 / 32 + rb < s.rb_end && c0 / 16 + kb < s.rkb) {
 #pragma unroll
@@ -240,6 +251,12 @@ struct GemmArg {
     int32_t accumulate;
 };
 
+// One or two products in a launch: the second starts with workgroup `first`, a multiple of 8.
+struct GemmPair {
+    GemmArg g[2];
+    uint32_t first;
+};
+
 // ug / kept and the exponent that undoes the panels' scales, applied to one sum.
 __device__ __forceinline__ float grad_value(float acc, float c, int e) { return c * __builtin_ldexpf(acc, e); }
 
@@ -260,7 +277,10 @@ __device__ __forceinline__ void wait_and_meet() {
 // stage s, which is in registers, reads stage s + 1 and loads stage s + 3 over stage s: neither the loads'
 // latency nor LDS's stands before a matrix instruction.
 template <int TM, int TN, int WM, int WN, int EPI>
-__global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmArg g) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmPair pair) {
+    const bool second = blockIdx.x >= pair.first;
+    const GemmArg& g = pair.g[second];
+    const uint32_t block = blockIdx.x - (second ? pair.first : 0);
     constexpr int kWaves = WM * WN, MI = TM / WM / 32, NI = TN / WN / 32;
     constexpr int kRows = (TM + TN) / 32;        // row blocks of a stage
     constexpr int kStage = kRows * kBlk;
@@ -273,8 +293,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmArg g) {
     // Workgroup b runs on XCD b % 8: each XCD takes a contiguous run of a split's tiles, in groups of 8 tile
     // rows, so that its L2 holds what its workgroups share, and as many as the others.
     const int64_t T = (int64_t)g.tiles_m * g.tiles_n, all = T * g.splits;
-    const int64_t item = (int64_t)(blockIdx.x & 7) * ((all + 7) / 8) + (blockIdx.x >> 3);
-    if ((int64_t)(blockIdx.x >> 3) >= (all + 7) / 8 || item >= all) return;
+    const int64_t item = (int64_t)(block & 7) * ((all + 7) / 8) + (block >> 3);
+    if ((int64_t)(block >> 3) >= (all + 7) / 8 || item >= all) return;
     const int64_t split = item / T, id = item - split * T;
     const int64_t gsz = (int64_t)8 * g.tiles_n, grp = id / gsz;
     const int gm = (int)(g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8);
@@ -443,18 +463,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmArg g) {
     }
 }
 
-// Joins the splits of a gradient product, in their order.
-__global__ __launch_bounds__(256) void k_join(GemmArg g, int32_t splits, int64_t ld, int64_t plane) {
+// Joins the splits of the gradient products that have them, in their order. A product's rows of sums are
+// tiles_n tiles of `tile` wide.
+__global__ __launch_bounds__(256) void k_join(GemmPair pair, int32_t tile) {
+    const bool second = blockIdx.x >= pair.first;
+    const GemmArg& g = pair.g[second];
+    const int64_t block = blockIdx.x - (second ? pair.first : 0), blocks = second ? gridDim.x - pair.first : pair.first;
+    const int64_t ld = (int64_t)g.tiles_n * tile, plane = (int64_t)g.tiles_m * tile * ld;
     const int e = -(kGExp + (g.exp_b ? g.info->ew : g.info->ex));
     const float c = g.ug[0] / (float)(g.info->kept > 0 ? g.info->kept : 1);
     const int64_t total = g.m * g.n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = block * 256 + threadIdx.x; i < total; i += blocks * 256) {
         const int64_t m = i / g.n, n = i - m * g.n;
         const bool out = g.labels && g.labels[m] < 0;
         if (out && g.accumulate) continue;
         float v = 0.0f;
         if (!out) {
-            for (int s = 0; s < splits; ++s) v += g.part[s * plane + m * ld + n];
+            for (int s = 0; s < g.splits; ++s) v += g.part[s * plane + m * ld + n];
             v = grad_value(v, c, e);
         }
         g.out[i] = g.accumulate ? g.out[i] + v : v;
@@ -516,28 +541,33 @@ __global__ __launch_bounds__(1024) void k_rows_lse(const float* stat, int64_t gr
     if (r == 0) block_loss[blockIdx.x] = total;
 }
 
-// loss = sum of the workgroups' losses / kept, in one workgroup and a fixed order.
-__global__ __launch_bounds__(1024) void k_rows_loss(const double* block_loss, int64_t blocks, const HeadInfo* info,
-                                                    float* loss) {
-    __shared__ double red[16];
+// loss = sum of the workgroups' losses / kept, by one workgroup of 256 threads and in a fixed order.
+__device__ void rows_loss(const double* block_loss, int64_t blocks, const HeadInfo* info, float* loss, double* red) {
     double s = 0.0;
-    for (int64_t n = threadIdx.x; n < blocks; n += 1024) s += block_loss[n];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s = 0.0;
-        for (int i = 0; i < 16; ++i) s += red[i];
-        loss[0] = (float)(s / (double)(info->kept > 0 ? info->kept : 1));
-    }
+#pragma unroll 4
+    for (int64_t n = threadIdx.x; n < blocks; n += 256) s += block_loss[n];
+    s = block_sum<4>(s, red);
+    if (threadIdx.x == 0) loss[0] = (float)(s / (double)(info->kept > 0 ? info->kept : 1));
+}
+__global__ __launch_bounds__(256) void k_rows_loss(const double* block_loss, int64_t blocks, const HeadInfo* info,
+                                                   float* loss) {
+    __shared__ double red[4];
+    rows_loss(block_loss, blocks, info, loss, red);
 }
 
 // Logits to G's panels: a wavefront takes 32 rows x 32 classes (two blocks of logits, which become two
-// blocks of the row panel in place) and writes the same elements to the column panel through LDS.
-__global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, int64_t gtkb, const float* lse,
-                                              const int32_t* labels, int64_t rows, int64_t classes, int64_t tiles_v) {
+// blocks of the row panel in place) and writes the same elements to the column panel through LDS. With `loss`,
+// `tiles` workgroups do that and one more adds up the loss.
+__global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, int64_t gtkb, int64_t gt_blocks, const float* lse,
+                                              const int32_t* labels, int64_t rows, int64_t classes, int64_t tiles_v,
+                                              int64_t tiles, const double* block_loss, int64_t loss_blocks,
+                                              const HeadInfo* info, float* loss) {
     __shared__ __attribute__((aligned(16))) _Float16 t[4][2][32][40];
+    __shared__ double red[4];
+    if (blockIdx.x >= tiles) {  // one workgroup more, behind the last chunk's: the loss
+        rows_loss(block_loss, loss_blocks, info, loss, red);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t id = (int64_t)blockIdx.x * 4 + wave;
     const int64_t nb = id / tiles_v, vt = id % tiles_v;  // the grid covers whole workgroups of tiles
@@ -549,7 +579,7 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
     for (int b = 0; b < 2; ++b) {
         char* blk = z + (nb * zkb + vt * 2 + b) * kBlk;
         const vf4 q0 = reinterpret_cast<const vf4*>(blk)[lane * 2], q1 = reinterpret_cast<const vf4*>(blk)[lane * 2 + 1];
-        float v[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+        f32x8 v = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int64_t cls = vt * 32 + b * 16 + k8 + j;
@@ -572,6 +602,7 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
         }
     }
     __syncthreads();
+    if (nb >= gt_blocks) return;  // rows that grad_w's product does not reach
 #pragma unroll
     for (int b = 0; b < 2; ++b) {  // rows n of 16 b .. 16 b + 15 as the contracted axis
         char* blk = gt + (vt * gtkb + nb * 2 + b) * kBlk;
@@ -640,17 +671,24 @@ Form form_of(int64_t m, int64_t n, int64_t kb, bool split) {
     return best;
 }
 
-template <int EPI>
-void launch_gemm(GemmArg g, int64_t m, int64_t n, const Form& f) {
+void set_form(GemmArg& g, int64_t m, int64_t n, const Form& f) {
+    g.m = m;
+    g.n = n;
     g.tiles_m = (int32_t)(up(m, f.tile) / f.tile);
     g.tiles_n = (int32_t)(up(n, f.tile) / f.tile);
-    g.kb = up((g.kb_all + f.splits - 1) / f.splits, 2);
     g.splits = f.splits;
-    const dim3 grid((unsigned)(8 * (((int64_t)g.tiles_m * g.tiles_n * f.splits + 7) / 8)));
-    if (f.tile == 256)
-        hipLaunchKernelGGL((k_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, ctx().stream, g);
-    else
-        hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, g);
+    g.kb = up((g.kb_all + f.splits - 1) / f.splits, 2);
+}
+uint32_t gemm_blocks(const GemmArg& g) {
+    return (uint32_t)(8 * (((int64_t)g.tiles_m * g.tiles_n * g.splits + 7) / 8));
+}
+// `n` products of one tile in a launch.
+template <int EPI>
+void launch_gemm(const GemmArg* g, int n, int tile) {
+    GemmPair p = {{g[0], g[n - 1]}, gemm_blocks(g[0])};
+    const dim3 grid(p.first + (n > 1 ? gemm_blocks(g[1]) : 0));
+    if (tile == 256) hipLaunchKernelGGL((k_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, ctx().stream, p);
+    else hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, ctx().stream, p);
 }
 
 struct HeadCall {
@@ -665,26 +703,51 @@ struct HeadCall {
     bool train, accumulate;
 };
 
-// grad [m, n] from panels a (rows of m) and b (rows of n), contracted over kb blocks.
-int grad_product(GemmArg g, int64_t m, int64_t n, int64_t kb, float* part) {
-    const Form f = form_of(m, n, kb, true);
-    g.m = m;
-    g.n = n;
-    g.kb_all = kb;
-    g.part = f.splits > 1 ? part : nullptr;
-    launch_gemm<EPI_GRAD>(g, m, n, f);
-    if (f.splits > 1) {
-        const int64_t ld = up(n, f.tile), plane = up(m, f.tile) * ld;
-        int64_t nb = grid_blocks(m * n, 256);
-        if (nb > 4096) nb = 4096;
-        hipLaunchKernelGGL(k_join, dim3((unsigned)nb), dim3(256), 0, ctx().stream, g, f.splits, ld, plane);
+// The gradient products, both in one launch where they take the same tile, and the joins of their splits.
+void grad_products(GemmArg* g, const Form* f, int n) {
+    if (n == 2 && f[0].tile != f[1].tile) {
+        grad_products(g, f, 1);
+        grad_products(g + 1, f + 1, 1);
+        return;
     }
-    return MH_OK;
+    launch_gemm<EPI_GRAD>(g, n, f[0].tile);
+    GemmArg j[2];
+    int nj = 0;
+    uint32_t blocks[2] = {0, 0};
+    for (int i = 0; i < n; ++i)
+        if (g[i].splits > 1) {
+            const int64_t b = grid_blocks(g[i].m * g[i].n, 256);
+            blocks[nj] = (uint32_t)(b > 4096 ? 4096 : b);
+            j[nj++] = g[i];
+        }
+    if (nj == 0) return;
+    const GemmPair p = {{j[0], j[nj - 1]}, blocks[0]};
+    hipLaunchKernelGGL(k_join, dim3(blocks[0] + blocks[1]), dim3(256), 0, ctx().stream, p, f[0].tile);
 }
 
-size_t part_bytes(int64_t m, int64_t n, int64_t kb) {
-    const Form f = form_of(m, n, kb, true);
+size_t part_bytes(int64_t m, int64_t n, const Form& f) {
     return f.splits > 1 ? (size_t)f.splits * up(m, f.tile) * up(n, f.tile) * sizeof(float) : 0;
+}
+
+// The forms of a chunk of nr rows. The contracted axes end at whole pairs of blocks; the rows behind nr and the
+// classes behind the last are zeros in the panels.
+struct Forms {
+    Form logits, grad[2];  // of x, of w
+    int64_t rows;          // padded to the tiles that read them
+    size_t part[2];
+};
+Forms forms_of(const HeadCall& h, int64_t nr, int64_t dkb) {
+    Forms f = {};
+    f.logits = form_of(h.classes, nr, dkb, false);
+    f.rows = up(nr, f.logits.tile);
+    if (h.train) {
+        f.grad[0] = form_of(nr, h.dim, up(h.classes, 32) / 16, true);
+        f.grad[1] = form_of(h.classes, h.dim, up(nr, 32) / 16, true);
+        if (h.gx && up(nr, f.grad[0].tile) > f.rows) f.rows = up(nr, f.grad[0].tile);
+        f.part[0] = h.gx ? part_bytes(nr, h.dim, f.grad[0]) : 0;
+        f.part[1] = h.gw ? part_bytes(h.classes, h.dim, f.grad[1]) : 0;
+    }
+    return f;
 }
 
 int head_run(const HeadCall& h) {
@@ -714,10 +777,8 @@ int head_run(const HeadCall& h) {
         // every chunk has this many rows but the last
         size_t sp = 0;
         for (const int64_t nr : {rows < chunk ? rows : chunk, rows - (rows - 1) / chunk * chunk}) {
-            const size_t a = h.gx ? part_bytes(nr, dim, clsP / 16) : 0;
-            const size_t b = h.gw ? part_bytes(classes, dim, up(nr, 256) / 16) : 0;
-            sp = a > sp ? a : sp;
-            sp = b > sp ? b : sp;
+            const Forms f = forms_of(h, nr, dkb);
+            if (f.part[0] + f.part[1] > sp) sp = f.part[0] + f.part[1];
         }
         o_sp = cv.take((int64_t)sp);
     }
@@ -742,7 +803,9 @@ int head_run(const HeadCall& h) {
     hipLaunchKernelGGL(k_split, dim3((unsigned)nsplit), dim3(256), 0, st, sx, sw, part, info, h.labels);
 
     for (int64_t r0 = 0; r0 < rows; r0 += chunk) {
-        const int64_t nr = rows - r0 < chunk ? rows - r0 : chunk, nrP = up(nr, 256);
+        const int64_t nr = rows - r0 < chunk ? rows - r0 : chunk;
+        const Forms f = forms_of(h, nr, dkb);
+        const int64_t nrP = f.rows, zkb = stride_of(clsP / 16), gtkb = stride_of(up(nr, 32) / 16);
         GemmArg g = {};
         g.a = base + o_wr;
         g.b = base + o_xr + r0 / 32 * stride_of(dkb) * kBlk;
@@ -756,46 +819,60 @@ int head_run(const HeadCall& h) {
         g.stat_ld = chunk;
         g.target = target;
         g.z = h.train ? base + o_z : nullptr;
-        g.zkb = stride_of(clsP / 16);
-        // every row and class of the padded chunk gets its logits: the panels behind have no gaps
-        launch_gemm<EPI_LOGITS>(g, clsP, nrP, form_of(clsP, nrP, dkb, false));
+        g.zkb = zkb;
+        // every row and class that a gradient's tiles read gets its logits: the panels behind have no gaps
+        set_form(g, clsP, nrP, f.logits);
+        launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
         if (!h.row_lse_in)
             hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)((nr + 31) / 32)), dim3(1024), 0, st, g.stat,
                                groups, g.stat_ld, target, h.labels + r0, nr, classes, lse + r0,
                                h.row_loss ? h.row_loss + r0 : nullptr, block_loss + r0 / 32);
         if (!h.train) continue;
-        const int64_t tiles_v = clsP / 32;
-        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(nrP / 32 * tiles_v / 4)), dim3(256), 0, st, base + o_z, g.zkb,
-                           base + o_gt, stride_of(nrP / 16), (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr, classes,
-                           tiles_v);
-        GemmArg d = {};
-        d.info = info;
-        d.ug = h.ug;
+        const int64_t tiles_v = clsP / 32, tiles = nrP / 32 * tiles_v / 4;
+        const bool with_loss = !h.row_lse_in && r0 + chunk >= rows;
+        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(tiles + with_loss)), dim3(256), 0, st, base + o_z, zkb,
+                           base + o_gt, gtkb, up(nr, 32) / 32, (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr,
+                           classes, tiles_v, tiles, block_loss, (rows + 31) / 32, info, h.loss);
+        GemmArg d[2] = {};
+        Form df[2];
+        int nd = 0;
+        float* sp = reinterpret_cast<float*>(base + o_sp);
         if (h.gx) {
-            d.a = base + o_z;
-            d.akb = stride_of(clsP / 16);
-            d.b = base + o_wt;
-            d.bkb = stride_of(clsP / 16);
-            d.exp_b = 1;
-            d.labels = h.labels + r0;
-            d.out = h.gx + r0 * dim;
-            d.accumulate = h.accumulate;
-            MH_TRY(grad_product(d, nr, dim, clsP / 16, reinterpret_cast<float*>(base + o_sp)));
+            GemmArg& p = d[nd];
+            p.a = base + o_z;
+            p.akb = zkb;
+            p.b = base + o_wt;
+            p.bkb = stride_of(clsP / 16);
+            p.kb_all = up(classes, 32) / 16;
+            p.exp_b = 1;
+            p.labels = h.labels + r0;
+            p.out = h.gx + r0 * dim;
+            p.accumulate = h.accumulate;
+            p.part = f.grad[0].splits > 1 ? sp : nullptr;
+            set_form(p, nr, dim, f.grad[0]);
+            df[nd++] = f.grad[0];
         }
         if (h.gw) {
-            d.a = base + o_gt;
-            d.akb = stride_of(nrP / 16);
-            d.b = base + o_xt + r0 / 16 * kBlk;
-            d.bkb = stride_of(rowsP / 16);
-            d.exp_b = 0;
-            d.labels = nullptr;
-            d.out = h.gw;
-            d.accumulate = h.accumulate || r0 > 0;
-            MH_TRY(grad_product(d, classes, dim, nrP / 16, reinterpret_cast<float*>(base + o_sp)));
+            GemmArg& p = d[nd];
+            p.a = base + o_gt;
+            p.akb = gtkb;
+            p.b = base + o_xt + r0 / 16 * kBlk;
+            p.bkb = stride_of(rowsP / 16);
+            p.kb_all = up(nr, 32) / 16;
+            p.out = h.gw;
+            p.accumulate = h.accumulate || r0 > 0;
+            p.part = f.grad[1].splits > 1 ? sp + f.part[0] / sizeof(float) : nullptr;
+            set_form(p, classes, dim, f.grad[1]);
+            df[nd++] = f.grad[1];
         }
+        for (int i = 0; i < nd; ++i) {
+            d[i].info = info;
+            d[i].ug = h.ug;
+        }
+        grad_products(d, df, nd);
     }
-    if (!h.row_lse_in)
-        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(1024), 0, st, block_loss, (rows + 31) / 32, info, h.loss);
+    if (!h.train)
+        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(256), 0, st, block_loss, (rows + 31) / 32, info, h.loss);
     return finish(h.what);
 }
 
