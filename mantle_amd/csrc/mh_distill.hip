@@ -6,8 +6,8 @@
 //
 // The logits are all that is large: the floor is one read of x and one write of its gradient. A first kernel
 // takes the entries, a wavefront a row: q, the logit at each id, entries of one class joined. A chain of loads
-// that depend on each other, it would stand in the way of the stream (75 -> 58 us over [1025, 30011], 50
-// entries). Then a workgroup takes a row: of up to 32768 classes it holds it in registers and reads it
+// that depend on each other, it would stand in the way of the stream (70 -> 64 us over [1025, 30011], 50
+// entries). Then a workgroup takes a row: of up to 65536 classes it holds it in registers and reads it
 // once; a longer one it reads twice, the second time from its end, where the caches still hold it. Where
 // rows are fewer than CUs, several workgroups share a row: their statistics, then the gradient.
 // An exponential is a difference, a product with log2(e) / T and one instruction; sums are fp32 over at
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kMaxK = 1024;       // entries of a row
 constexpr int kEntryBlocks = 512;  // workgroups of k_distill_entries at most: partial counts of rows
-constexpr int64_t kInRegs = 32768;
+constexpr int64_t kHeld = 65536;  // classes of a row that a CU holds
 
 struct DistillArg {
     const float* x;
@@ -45,6 +45,8 @@ struct DistillArg {
     int64_t span;     // classes of a split, a multiple of 4
     float inv_t, temperature;
 };
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -338,36 +340,49 @@ __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
     }
 }
 
-// The same with the row in registers, NQ quads a thread, read once; a row's exponentials are taken once too.
-// Two workgroups of 16 wavefronts share a CU at 64 registers, one loading while the other stores; at the 78
-// that the compiler took unbounded one workgroup ran alone (91 us against 69 over [1025, 30011]).
+// The same with the row in registers, NQ quads a thread, and read once; a row's exponentials are taken once too.
+// Up to 32768 classes two workgroups of 16 wavefronts share a CU at 64 registers, one loading while the other
+// stores; at the 78 that the compiler took unbounded one workgroup ran alone (91 us against 69 over [1025,
+// 30011]). Rows of up to 65536 have a CU to themselves: a workgroup ends with its stores under way and the next
+// one's loads follow ([8192, 65536]: 787 us, 5.5 TB/s, against 846 read twice). Longer ones do not fit: 92
+// registers of data leave too few of 128, and what spills costs more than reading twice (945 against 916 us
+// over [4096, 131072]).
 template <int W, int NQ, bool GRAD, bool ACC>
-__global__ __launch_bounds__(W * 64, 8) void k_distill_regs(DistillArg a) {
+__global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(DistillArg a) {
     __shared__ float red[W], factor;
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const float ninf = -__builtin_inff();
-    const float* x = a.x + r * a.classes;
-    const int nq = (int)(a.classes >> 2), tail = (int)(a.classes & 3);
     const int flag = a.flag[r];
     if (flag == 0) {
         row_out(a, r, 0, 0.0f);
         if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
         return;
     }
+    const float* x = a.x + r * a.classes;
+    const int nq = (int)(a.classes >> 2), tail = (int)(a.classes & 3);
     vf4 v[NQ];
+    float top = ninf;
+    auto max4 = [](vf4 q) { return __builtin_fmaxf(__builtin_fmaxf(q.x, q.y), __builtin_fmaxf(q.z, q.w)); };
+    // Quad u of the thread: the row's address and u's in scalar registers, one offset in a vector register for
+    // all of them (an address each is what spills). Bit 1 is the non-temporal path.
+    const uint32_t off = (uint32_t)tid * 16;
+    const auto row_of = [&](const float* p) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, nq * 16, 0x00020000);
+    };
+    const auto load = [&](__amdgpu_buffer_rsrc_t row, int u) {
+        return __builtin_bit_cast(vf4, __builtin_amdgcn_raw_buffer_load_b128(row, off, u * W * 1024, 2));
+    };
+    const auto in_row = row_of(x);
+    auto get = [&](int u) { return tid < nq - u * W * 64 ? load(in_row, u) : vf4{ninf, ninf, ninf, ninf}; };
 #pragma unroll
-    for (int u = 0; u < NQ; ++u) {
-        const int q = tid + u * W * 64;
-        v[u] = q < nq ? ld_ntu(x + 4 * q) : vf4{ninf, ninf, ninf, ninf};
-    }
+    for (int u = 0; u < NQ; ++u) v[u] = get(u);
     float last = tid < tail ? x[4 * nq + tid] : ninf;
     if (GRAD) factor_to(a, &factor);
     const float kf = a.inv_t * kLog2e;
-    float top = last;
+    top = __builtin_fmaxf(top, last);
 #pragma unroll
-    for (int u = 0; u < NQ; ++u)
-        top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(v[u].x, v[u].y), __builtin_fmaxf(v[u].z, v[u].w)));
+    for (int u = 0; u < NQ; ++u) top = __builtin_fmaxf(top, max4(v[u]));
     top = block_max<W>(top, red);
     const float base = top == ninf ? 0.0f : top;
     const Scale<false> raw = {kf, base, 1.0f};
@@ -386,12 +401,18 @@ __global__ __launch_bounds__(W * 64, 8) void k_distill_regs(DistillArg a) {
         Mine<W> mine;
         entries_take<W, ACC>(a, r, 0, a.classes, mine);
         float* g = a.grad + r * a.classes;
+        const auto out_row = row_of(g);
+        auto put = [&](int u, vf4 e) {
+            if (tid >= nq - u * W * 64) return;
+            vf4 o = {e.x * s.inv * c, e.y * s.inv * c, e.z * s.inv * c, e.w * s.inv * c};
+            if (ACC) {
+                const vf4 old = load(out_row, u);
+                o = {old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w};
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), out_row, off, u * W * 1024, 2);
+        };
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            const int q = tid + u * W * 64;
-            const vf4 o = {v[u].x * s.inv * c, v[u].y * s.inv * c, v[u].z * s.inv * c, v[u].w * s.inv * c};
-            if (q < nq) grad_put<ACC>(g + 4 * q, o);
-        }
+        for (int u = 0; u < NQ; ++u) put(u, v[u]);
         if (tid < tail) {
             const float o = last * s.inv * c;
             g[4 * nq + tid] = ACC ? g[4 * nq + tid] + o : o;
@@ -557,7 +578,7 @@ int distill_run(const DistillCall& d) {
     if (d.lse_in) {
         if (d.accumulate) hipLaunchKernelGGL((k_distill_split<W, false, true, true>), all, t, 0, st, a);
         else hipLaunchKernelGGL((k_distill_split<W, false, true, false>), all, t, 0, st, a);
-    } else if (a.splits == 1 && a.classes <= kInRegs) {
+    } else if (a.splits == 1 && a.classes <= kHeld && (grad || a.classes <= 32768)) {
 #define MH_REGS(WW, NQ)                                                                                                \
     do {                                                                                                              \
         const dim3 tt(WW * 64);                                                                                       \
@@ -568,7 +589,8 @@ int distill_run(const DistillCall& d) {
         if (a.classes <= 4096) MH_REGS(4, 4);
         else if (a.classes <= 8192) MH_REGS(4, 8);
         else if (a.classes <= 16384) MH_REGS(8, 8);
-        else MH_REGS(16, 8);
+        else if (a.classes <= 32768) MH_REGS(16, 8);
+        else MH_REGS(16, 16);
 #undef MH_REGS
     } else if (a.splits == 1) {
         if (!grad) hipLaunchKernelGGL((k_distill_row<W, false, false>), rows, t, 0, st, a);

@@ -78,13 +78,25 @@ __global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, co
     const bool isx = blockIdx.x < kAmaxBlocks;
     const int b = isx ? blockIdx.x : blockIdx.x - kAmaxBlocks;
     if (isx) {
-        for (int64_t r = (int64_t)b * 4 + wave; r < rows; r += kAmaxBlocks * 4) {
-            if (labels[r] < 0) continue;  // a row left out may hold anything
-            ++kept;
-            const float* row = x + r * dim;
-#pragma unroll 4
-            for (int64_t k = lane * 4; k + 3 < dim; k += 256) a = amax4(a, *reinterpret_cast<const vf4u*>(row + k));
-            if (lane < (dim & 3)) a = __builtin_fmaxf(a, finite_abs(row[(dim & ~(int64_t)3) + lane]));
+        // four rows at a time, so that their labels and their elements are under way together
+        for (int64_t r0 = ((int64_t)b * 4 + wave) * 4; r0 < rows; r0 += kAmaxBlocks * 16) {
+            bool in[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) in[u] = r0 + u < rows && labels[r0 + u < rows ? r0 + u : r0] >= 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) kept += in[u];  // a row left out may hold anything
+            const float* row = x + r0 * dim;
+            for (int64_t k = lane * 4; k + 3 < dim; k += 256) {
+                vf4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = in[u] ? *reinterpret_cast<const vf4u*>(row + u * dim + k) : vf4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) a = amax4(a, v[u]);
+            }
+            if (lane < (dim & 3))
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (in[u]) a = __builtin_fmaxf(a, finite_abs(row[u * dim + (dim & ~(int64_t)3) + lane]));
         }
     } else {
         const int64_t nq = nw >> 2, step = kAmaxBlocks * 256;
@@ -489,55 +501,70 @@ __global__ __launch_bounds__(256) void k_join(GemmPair pair, int32_t tile) {
 // ---------------------------------------------------------------------------------------
 // rows' statistics, the loss, and G's panels
 // ---------------------------------------------------------------------------------------
-// Each row's log-sum-exp from its class groups' statistics, and the workgroup's sum of losses: 32 rows x 32
-// threads, whose loads of a group's statistics are 128 bytes each.
-constexpr int kLseParts = 32;
-__global__ __launch_bounds__(1024) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
+// Each row's log-sum-exp from its class groups' statistics, and the workgroup's sum of losses: 16 rows x 4 W
+// threads, whose loads of a group's statistics are 64 bytes each. W = 16 wavefronts a workgroup, or 4 where the
+// groups are few ([32768, 512] x [1000, 512]'s 16 groups: 17 and 9 us).
+constexpr int kLseRows = 16;
+struct Lse {
+    float top, sum;
+};
+// A sum that is not a number stays so; a group of logits at minus infinity adds nothing.
+__device__ __forceinline__ void lse_join(Lse& a, float m, float s) {
+    const float d = m > a.top ? a.top - m : m - a.top;
+    const float e = __builtin_amdgcn_exp2f(d * kLog2e);
+    if (m > a.top) {
+        a.sum = a.sum * e + s;
+        a.top = m;
+    } else if (m > -__builtin_inff() || s != s) {
+        a.sum += s * e;
+    }
+}
+template <int W>
+__global__ __launch_bounds__(W * 64) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
                                                    const float* target, const int32_t* labels, int64_t rows,
                                                    int64_t classes, float* row_lse, float* row_loss, double* block_loss) {
-    __shared__ float sm[kLseParts][32], ss[kLseParts][32];
-    const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 32 + r;
-    float top = -__builtin_inff(), sum = 0.0f;
-    // a sum that is not a number stays so; a group of logits at minus infinity adds nothing
-    auto join = [&](float m, float s) {
-        if (m > top) {
-            sum = sum * exp_neg(top - m) + s;
-            top = m;
-        } else if (m > -__builtin_inff() || s != s) {
-            sum += s * exp_neg(m - top);
-        }
-    };
-    for (int64_t gr = p; gr < groups; gr += 4 * kLseParts) {
+    __shared__ float sm[W][kLseRows], ss[W][kLseRows];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, p = wave * 4 + (lane >> 4);
+    const int64_t n = (int64_t)blockIdx.x * kLseRows + r;
+    Lse a = {-__builtin_inff(), 0.0f};
+    for (int64_t gr = p; gr < groups; gr += 16 * W) {
         float m[4], s[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int64_t at = gr + u * kLseParts < groups ? gr + u * kLseParts : gr;
+            const int64_t at = gr + u * 4 * W < groups ? gr + u * 4 * W : gr;
             m[u] = stat[at * 2 * stat_ld + n];
             s[u] = stat[(at * 2 + 1) * stat_ld + n];
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (gr + u * kLseParts < groups) join(m[u], s[u]);
+            if (gr + u * 4 * W < groups) lse_join(a, m[u], s[u]);
     }
-    sm[p][r] = top;
-    ss[p][r] = sum;
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) {
+        const float m = __shfl_xor(a.top, o), s = __shfl_xor(a.sum, o);
+        lse_join(a, m, s);
+    }
+    if (lane < kLseRows) {
+        sm[wave][r] = a.top;
+        ss[wave][r] = a.sum;
+    }
     __syncthreads();
-    if (p != 0) return;
-    for (int i = 1; i < kLseParts; ++i) join(sm[i][r], ss[i][r]);
+    if (threadIdx.x >= kLseRows) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) lse_join(a, sm[i][r], ss[i][r]);
     float loss = 0.0f;
     if (n < rows) {
         const int32_t label = labels[n];
-        float lse = top + mlog(sum);
+        float lse = a.top + mlog(a.sum);
         if (label >= classes) lse = __builtin_nanf("");  // no such class: shown in the loss and the gradients
         if (label < 0) lse = 0.0f;
         loss = label < 0 ? 0.0f : (label >= classes ? lse : lse - target[n]);
         row_lse[n] = lse;
         if (row_loss) row_loss[n] = loss;
     }
-    double total = loss;  // lanes 0-31 hold the rows
+    double total = loss;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    for (int o = 8; o > 0; o >>= 1) total += __shfl_xor(total, o);
     if (r == 0) block_loss[blockIdx.x] = total;
 }
 
@@ -769,7 +796,7 @@ int head_run(const HeadCall& h) {
     const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
     const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
     const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
-    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / 32 * 8);
+    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / kLseRows * 8);
     size_t o_z = 0, o_gt = 0, o_sp = 0;
     if (h.train) {
         o_z = cv.take(chunk / 32 * stride_of(clsP / 16) * kBlk);
@@ -823,16 +850,23 @@ int head_run(const HeadCall& h) {
         // every row and class that a gradient's tiles read gets its logits: the panels behind have no gaps
         set_form(g, clsP, nrP, f.logits);
         launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
-        if (!h.row_lse_in)
-            hipLaunchKernelGGL(k_rows_lse, dim3((unsigned)((nr + 31) / 32)), dim3(1024), 0, st, g.stat,
-                               groups, g.stat_ld, target, h.labels + r0, nr, classes, lse + r0,
-                               h.row_loss ? h.row_loss + r0 : nullptr, block_loss + r0 / 32);
+        if (!h.row_lse_in) {
+            const dim3 grid((unsigned)((nr + kLseRows - 1) / kLseRows));
+            float* rl = h.row_loss ? h.row_loss + r0 : nullptr;
+            double* bl = block_loss + r0 / kLseRows;
+            if (groups <= 32)
+                hipLaunchKernelGGL((k_rows_lse<4>), grid, dim3(256), 0, st, g.stat, groups, g.stat_ld, target,
+                                   h.labels + r0, nr, classes, lse + r0, rl, bl);
+            else
+                hipLaunchKernelGGL((k_rows_lse<16>), grid, dim3(1024), 0, st, g.stat, groups, g.stat_ld, target,
+                                   h.labels + r0, nr, classes, lse + r0, rl, bl);
+        }
         if (!h.train) continue;
         const int64_t tiles_v = clsP / 32, tiles = nrP / 32 * tiles_v / 4;
         const bool with_loss = !h.row_lse_in && r0 + chunk >= rows;
         hipLaunchKernelGGL(k_to_g, dim3((unsigned)(tiles + with_loss)), dim3(256), 0, st, base + o_z, zkb,
                            base + o_gt, gtkb, up(nr, 32) / 32, (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr,
-                           classes, tiles_v, tiles, block_loss, (rows + 31) / 32, info, h.loss);
+                           classes, tiles_v, tiles, block_loss, (rows + kLseRows - 1) / kLseRows, info, h.loss);
         GemmArg d[2] = {};
         Form df[2];
         int nd = 0;
@@ -872,7 +906,7 @@ int head_run(const HeadCall& h) {
         grad_products(d, df, nd);
     }
     if (!h.train)
-        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(256), 0, st, block_loss, (rows + 31) / 32, info, h.loss);
+        hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(256), 0, st, block_loss, (rows + kLseRows - 1) / kLseRows, info, h.loss);
     return finish(h.what);
 }
 
