@@ -8,7 +8,6 @@ off by Z, the sums' roundings and the log's; an element of G by p (Z + L + 2^-21
 2^-40; a gradient by the sum of |dG| |operand| and its own product's bound."""
 import numpy as np
 import pytest
-import torch
 
 from util import GpuEngine
 
@@ -20,42 +19,42 @@ def m_():
     return GpuEngine().m
 
 
-def reference(x, w, labels, ug=1.0, device="cpu"):
+def reference(x, w, labels, ug=1.0):
     """loss, row_loss, row_lse, grad_x, grad_w and the bounds of their errors."""
-    x, w = (torch.from_numpy(a).to(device).double() for a in (x, w))
-    labels = torch.from_numpy(labels).to(device).long()
+    labels = labels.astype(np.int64)
     keep = labels >= 0
-    x = torch.where(keep[:, None], x, 0.0)
+    x, w = np.where(keep[:, None], x, 0.0).astype(np.float64), w.astype(np.float64)
     n = max(1, int(keep.sum()))
     rows, dim = x.shape
     classes = w.shape[0]
-    z = x @ w.t()
-    lse = torch.logsumexp(z, 1)
-    at = labels.clamp(min=0)
-    picked = z[torch.arange(rows, device=device), at]
-    row = torch.where(keep, lse - picked, 0.0)
-    p = torch.exp(z - lse[:, None])
-    g = p.clone()
-    g[torch.arange(rows, device=device), at] -= 1.0
+    z = x @ w.T
+    top = z.max(1, keepdims=True)
+    lse = top[:, 0] + np.log(np.exp(z - top).sum(1))
+    at = np.arange(rows), np.maximum(labels, 0)
+    picked = z[at]
+    row = np.where(keep, lse - picked, 0.0)
+    p = np.exp(z - lse[:, None])
+    g = p.copy()
+    g[at] -= 1.0
     g *= keep[:, None]
     c = ug / n
 
     def product(k):
         return 2.0 ** -21 + (3 * k / 16 + 8) * 2 * U
 
-    bz = (x.abs() @ w.abs().t()) * product(dim)
+    ax, aw, ag = np.abs(x), np.abs(w), np.abs(g)
+    bz = (ax @ aw.T) * product(dim)
     # 64 or 128 terms a lane, then the groups' statistics
-    bl = bz.amax(1) + (128 + classes / 512 + 40) * U + 4 * U * lse.abs()
-    brow = bl + bz[torch.arange(rows, device=device), at] + 4 * U * (lse.abs() + picked.abs())
-    dg = p * (bz + bl[:, None] + 2.0 ** -21 + 8 * U * (z.abs() + lse.abs()[:, None])) + 2.0 ** -22 * g.abs() + 2.0 ** -40
+    bl = bz.max(1) + (128 + classes / 512 + 40) * U + 4 * U * np.abs(lse)
+    brow = bl + bz[at] + 4 * U * (np.abs(lse) + np.abs(picked))
+    dg = p * (bz + bl[:, None] + 2.0 ** -21 + 8 * U * (np.abs(z) + np.abs(lse)[:, None])) + 2.0 ** -22 * ag + 2.0 ** -40
     dg *= keep[:, None]
-    bgx = abs(c) * (dg @ w.abs() + (g.abs() @ w.abs()) * product(classes + 256))
-    bgw = abs(c) * (dg.t() @ x.abs() + (g.abs().t() @ x.abs()) * product(rows + 256))
-    out = {"loss": row.sum() / n, "row_loss": row, "row_lse": torch.where(keep, lse, 0.0), "grad_x": c * (g @ w),
-           "grad_w": c * (g.t() @ x)}
-    bound = {"loss": (brow * keep).sum() / n + 4 * U * out["loss"].abs(), "row_loss": brow * keep,
-             "row_lse": bl * keep, "grad_x": bgx + 4 * U * out["grad_x"].abs(), "grad_w": bgw + 4 * U * out["grad_w"].abs()}
-    return ({k: v.cpu().numpy() for k, v in out.items()}, {k: v.cpu().numpy() for k, v in bound.items()})
+    bgx = abs(c) * (dg @ aw + (ag @ aw) * product(classes + 256))
+    bgw = abs(c) * (dg.T @ ax + (ag.T @ ax) * product(rows + 256))
+    out = {"loss": row.sum() / n, "row_loss": row, "row_lse": np.where(keep, lse, 0.0), "grad_x": c * (g @ w), "grad_w": c * (g.T @ x)}
+    bound = {"loss": (brow * keep).sum() / n + 4 * U * abs(out["loss"]), "row_loss": brow * keep, "row_lse": bl * keep,
+             "grad_x": bgx + 4 * U * np.abs(out["grad_x"]), "grad_w": bgw + 4 * U * np.abs(out["grad_w"])}
+    return out, bound
 
 
 def inputs(rows, dim, classes, seed, left_out=0.1, std=2.0):
@@ -119,34 +118,48 @@ def test_larger_tiles_and_splits():
     for size in ((4096, 96, 5000), (2048, 300, 9001), (300, 2500, 4000)):
         print(f"\n[head] {size}", flush=True)
         x, w, labels = inputs(*size, seed=3)
-        want, bound = reference(x, w, labels, device="cuda")
+        want, bound = reference(x, w, labels)
         check(run(m, x, w, labels), want, bound, str(size))
 
 
 def test_rows_in_chunks():
-    """2^21 classes: the logits of 256 rows at a time, the last chunk shorter, grad_w over all of them."""
-    x, w, labels = inputs(600, 4, 1 << 21, seed=5)
+    """2^20 classes: the logits of 512 rows at a time, the last chunk shorter, grad_w over both."""
+    rows, classes = 600, 1 << 20
+    x, w, labels = inputs(rows, 4, classes, seed=5)
     print("\n[head] chunks", flush=True)
     got = run(m_(), x, w, labels)
     two = run(m_(), x, w, labels, how="two calls")
     for k in got:
         assert np.array_equal(got[k], two[k]), k
-    # the formulas 100 rows at a time (the loss's mean is over all 600), with reference()'s bounds, which
-    # grow with a logit's size: four elements of x and w make logits beyond +-30 here, whose fp32 step
-    # alone is 2^-20 of e^z
-    n = int((labels >= 0).sum())
-    loss, gw, bw = 0.0, 0.0, 0.0
-    for r in range(0, 600, 100):
-        part = labels[r:r + 100]
-        share = int((part >= 0).sum()) / n
-        want, bound = reference(x[r:r + 100], w, part, device="cuda")
-        loss += want["loss"] * share
-        gw, bw = gw + want["grad_w"] * share, bw + bound["grad_w"] * share
-        check({"row_lse": got["row_lse"][r:r + 100], "grad_x": got["grad_x"][r:r + 100]},
-              {"row_lse": want["row_lse"], "grad_x": want["grad_x"] * share},
-              {"row_lse": bound["row_lse"], "grad_x": bound["grad_x"] * share}, f"rows {r}")
-    check({"loss": np.float32(got["loss"]), "grad_w": got["grad_w"]}, {"loss": loss, "grad_w": gw},
-          {"loss": 1e-6 * abs(loss), "grad_w": bw}, "chunks")
+    # every row's log-sum-exp and loss, 40 rows at a time; the gradients of some rows and some classes, with
+    # reference()'s bounds, which grow with a logit's size (four elements make logits beyond +-30, whose fp32
+    # step alone is 2^-20 of e^z)
+    keep, n = labels >= 0, int((labels >= 0).sum())
+    some = np.concatenate([np.arange(3), np.arange(508, 516), np.arange(597, 600)])
+    part = np.sort(np.concatenate([np.random.RandomState(1).choice(classes, 300, replace=False), labels[keep][:200]]))
+    xd, wd = np.where(keep[:, None], x, 0.0).astype(np.float64), w.astype(np.float64)
+    lse, loss = np.zeros(rows), 0.0
+    for r in range(0, rows, 40):
+        z = xd[r:r + 40] @ wd.T
+        top = z.max(1, keepdims=True)
+        picked = z[np.arange(len(z)), np.maximum(labels[r:r + 40], 0)]
+        np.subtract(z, top, out=z)
+        lse[r:r + 40] = top[:, 0] + np.log(np.exp(z, out=z).sum(1))
+        loss += ((lse[r:r + 40] - picked) * keep[r:r + 40]).sum() / n
+    one, bound = reference(x[some], w, labels[some])
+    share = int(keep[some].sum()) / n
+    check({"row_lse": got["row_lse"][some], "grad_x": got["grad_x"][some]}, {"row_lse": one["row_lse"], "grad_x": one["grad_x"] * share},
+          {"row_lse": bound["row_lse"], "grad_x": bound["grad_x"] * share}, "some rows")
+    assert np.allclose(got["row_lse"][keep], lse[keep], rtol=2e-6) and abs(got["loss"] - loss) <= 2e-6 * loss
+    z = xd @ wd[part].T
+    p = np.exp(z - lse[:, None])
+    g = p - (part[None, :] == labels[:, None])
+    g *= keep[:, None]
+    bz = (np.abs(xd) @ np.abs(wd[part]).T) * 2.0 ** -20
+    dg = p * (bz + 2.0 ** -14 + 8 * U * (np.abs(z) + lse[:, None])) + 2.0 ** -22 * np.abs(g) + 2.0 ** -40
+    # 2^-14: the log-sum-exp's own bound there is (128 + 2^20 / 512) U and the largest logit's
+    bw = ((dg * keep[:, None]).T @ np.abs(xd) + (np.abs(g).T @ np.abs(xd)) * (2.0 ** -21 + 150 * U)) / n
+    check({"grad_w": got["grad_w"][part]}, {"grad_w": g.T @ xd / n}, {"grad_w": bw}, "some classes")
 
 
 def test_accumulates():
@@ -285,16 +298,12 @@ def test_memory_of_another_allocator():
     x, w, labels = inputs(70, 51, 601, seed=18)
     want = run(m, x, w, labels)
     # odd addresses: views that start one element into an allocation
-    hold = [torch.zeros(a.size + 1, device="cuda", dtype=torch.float32 if a.dtype == np.float32 else torch.int32) for a in (x, w, labels)]
-    for t, a in zip(hold, (x, w, labels)):
-        t[1:] = torch.from_numpy(a.reshape(-1)).cuda()
-    gx, gw = torch.zeros(x.size + 1, device="cuda"), torch.zeros(w.size + 1, device="cuda")
-    torch.cuda.synchronize()
-    tx, tw = (m.Tensor.over(t.data_ptr() + 4, a.shape, t) for t, a in zip(hold, (x, w)))
-    tl = m.IndexTensor.over(hold[2].data_ptr() + 4, labels.shape, hold[2])
+    hold = [(m.IndexTensor if a.dtype == np.int32 else m.Tensor).from_numpy(np.concatenate([[0], a.reshape(-1)]).astype(a.dtype)) for a in (x, w, labels)]
+    gx, gw = m.Tensor(x.size + 2), m.Tensor(w.size + 2)
+    tx, tw = (m.Tensor.over(t.ptr + 4, a.shape, t) for t, a in zip(hold, (x, w)))
+    tl = m.IndexTensor.over(hold[2].ptr + 4, labels.shape, hold[2])
     loss, tu = m.Tensor(1), m.Tensor.from_numpy(np.float32([1]))
-    m.linear_cross_entropy_step(loss, m.Tensor.over(gx.data_ptr() + 4, x.shape), m.Tensor.over(gw.data_ptr() + 4, w.shape),
+    m.linear_cross_entropy_step(loss, m.Tensor.over(gx.ptr + 4, x.shape), m.Tensor.over(gw.ptr + 4, w.shape),
                                 tx, tw, tl, tu)
-    m.sync()
-    assert np.array_equal(gx[1:].cpu().numpy().reshape(x.shape), want["grad_x"]) and gx[0] == 0
-    assert np.array_equal(gw[1:].cpu().numpy().reshape(w.shape), want["grad_w"]) and gw[0] == 0
+    for name, t, shape in (("grad_x", gx.to_numpy(), x.shape), ("grad_w", gw.to_numpy(), w.shape)):
+        assert np.array_equal(t[1:-1].reshape(shape), want[name]) and t[0] == 0 and t[-1] == 0

@@ -5,7 +5,6 @@ lane, the rest a tree), so a probability by R = (|x - max| + 40) U; sums over ro
 counts are whole. A gradient p (A - sum A p) is off by p (|A| + sum |A| p) times twice R and 40 U."""
 import numpy as np
 import pytest
-import torch
 
 from util import GpuEngine
 
@@ -19,39 +18,40 @@ def m_():
 
 def reference(x, k, keep=None, normalise=False, gw=None, ug=None):
     rows, experts = x.shape
-    order = torch.sort(torch.from_numpy(x) + 0.0, dim=1, descending=True, stable=True)[1][:, :k]
-    kept = torch.ones(rows, dtype=torch.bool) if keep is None else torch.from_numpy(keep) != 0
-    xd = torch.where(kept[:, None], torch.from_numpy(x).double(), 0.0).requires_grad_(True)
+    order = np.argsort(-(x + np.float32(0.0)), axis=1, kind="stable")[:, :k]
+    kept = np.ones(rows, bool) if keep is None else keep != 0
+    xd = np.where(kept[:, None], x, 0.0).astype(np.float64)
     n = max(1, int(kept.sum()))
-    p = torch.softmax(xd, 1)
-    counts = torch.bincount(order[kept].reshape(-1), minlength=experts)
-    picked = p.gather(1, order)
-    weights = picked / picked.sum(1, keepdim=True) if normalise else picked
-    weights = weights * kept[:, None]
-    f = counts.double() / (n * k)
+    top = xd.max(1, keepdims=True)
+    p = np.exp(xd - top)
+    p /= p.sum(1, keepdims=True)
+    counts = np.bincount(order[kept].reshape(-1), minlength=experts)
+    r = np.arange(rows)[:, None]
+    picked = p[r, order]
+    mass = picked.sum(1, keepdims=True)
+    weights = picked / mass if normalise else picked
+    weights = np.where(kept[:, None], weights, 0.0)
+    f = counts / (n * k)
     loss = experts * (f * (p * kept[:, None]).sum(0)).sum() / n
-    total = xd.sum() * 0.0
-    s = 0.0
-    if ug is not None:
-        total = total + loss * ug
-        s = abs(ug) * experts / n
-    g = torch.zeros(rows, experts, dtype=torch.float64)
+    s = 0.0 if ug is None else ug * experts / n
+    grad = s * p * (f - (f * p).sum(1, keepdims=True))
+    g = np.zeros((rows, experts))
     if gw is not None:
-        total = total + (weights * torch.from_numpy(gw).double()).sum()
-        g.scatter_(1, order, torch.from_numpy(gw).double().abs())
-        if normalise:  # the weights' own softmax: w (g - mean), with w at most 1 / (sum of the chosen's p) times p
-            g = g / picked.detach().sum(1, keepdim=True)
-    total.backward()
-    pd = p.detach()
-    rel = ((xd.detach().amax(1, keepdim=True) - xd.detach()).clamp(max=1e4) + 40) * U
-    A = g + s * f
-    bg = pd * (A + (A * pd).sum(1, keepdim=True) + (g * pd).sum(1, keepdim=True) / picked.detach().sum(1, keepdim=True)) * (2 * rel + 40 * U)
-    bw = weights.detach() * (rel.gather(1, order) + rel.gather(1, order).amax(1, keepdim=True) + 80 * U)
-    bl = experts * (f * (pd * rel * kept[:, None]).sum(0)).sum() / n + (rows / 1024 + 40 + experts / 64) * U * loss.detach()
-    out = {"weights": weights.detach(), "loss": loss.detach(), "grad_x": xd.grad * kept[:, None]}
+        gd = np.where(kept[:, None], gw, 0.0).astype(np.float64)
+        if normalise:
+            grad[r, order] += picked / mass * (gd - (gd * picked / mass).sum(1, keepdims=True))
+        else:
+            grad -= p * (gd * picked).sum(1, keepdims=True)
+            grad[r, order] += picked * gd
+        g[r, order] = np.abs(gd) / (mass if normalise else 1.0)  # the weights' own softmax: w is p / mass
+    rel = (np.minimum(top - xd, 1e4) + 40) * U
+    A = g + abs(s) * f
+    bg = p * (A + (A * p).sum(1, keepdims=True) + (g * p).sum(1, keepdims=True) / mass) * (2 * rel + 40 * U)
+    bw = weights * (rel[r, order] + rel[r, order].max(1, keepdims=True) + 80 * U)
+    bl = experts * (f * (p * rel * kept[:, None]).sum(0)).sum() / n + (rows / 1024 + 40 + experts / 64) * U * loss
+    out = {"weights": weights, "loss": loss, "grad_x": grad * kept[:, None]}
     bound = {"weights": bw, "loss": bl, "grad_x": bg * kept[:, None]}
-    whole = {"chosen": torch.where(kept[:, None], order, -1).numpy(), "counts": counts.numpy()}
-    return {a: v.numpy() for a, v in out.items()}, {a: v.numpy() for a, v in bound.items()}, whole
+    return out, bound, {"chosen": np.where(kept[:, None], order, -1), "counts": counts}
 
 
 def run(m, x, k, keep=None, normalise=False, gw=None, ug=None, grad=None):
@@ -200,19 +200,17 @@ def test_unaligned_memory():
     m = m_()
     x, keep, gw = inputs(50, 37, 5, seed=12)
     want = run(m, x, 5, keep, True, gw, 1.0)
-    tx = torch.zeros(x.size + 1, device="cuda")
-    tx[1:] = torch.from_numpy(x.reshape(-1)).cuda()
-    gx = torch.zeros(x.size + 2, device="cuda")
-    torch.cuda.synchronize()
-    X = m.Tensor.over(tx.data_ptr() + 4, x.shape, tx)
+    tx = m.Tensor.from_numpy(np.concatenate([[0], x.reshape(-1)]).astype(np.float32))
+    gx = m.Tensor(x.size + 2)
+    X = m.Tensor.over(tx.ptr + 4, x.shape, tx)
     K = m.IndexTensor.from_numpy(keep)
     weights, chosen, counts, loss = m.Tensor(50, 5), m.IndexTensor(50, 5), m.IndexTensor(37), m.Tensor(1)
     m.router_forward(weights, chosen, counts, loss, X, keep=K, normalise=True)
-    m.router_backward(m.Tensor.over(gx.data_ptr() + 4, x.shape), X, chosen, counts, m.Tensor.from_numpy(gw),
+    m.router_backward(m.Tensor.over(gx.ptr + 4, x.shape), X, chosen, counts, m.Tensor.from_numpy(gw),
                       m.Tensor.from_numpy(np.float32([1])), keep=K, normalise=True, accumulate=False)
-    m.sync()
+    got = gx.to_numpy()
     assert np.array_equal(weights.to_numpy(), want["weights"])
-    assert np.array_equal(gx[1:-1].cpu().numpy().reshape(x.shape), want["grad_x"]) and gx[0] == 0 and gx[-1] == 0
+    assert np.array_equal(got[1:-1].reshape(x.shape), want["grad_x"]) and got[0] == 0 and got[-1] == 0
 
 
 def test_ids_of_other_origin_stay_in_bounds():
