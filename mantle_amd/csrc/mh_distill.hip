@@ -20,7 +20,8 @@ namespace mh {
 namespace {
 
 constexpr int kMaxK = 1024;       // entries of a row
-constexpr int kEntryBlocks = 512;  // workgroups of k_distill_entries at most: partial counts of rows
+constexpr int kEntryBlocks = 1024;  // workgroups of k_distill_entries at most
+constexpr int kTicketStride = 32;   // counters in use lie in 128-byte lines of their own
 constexpr int64_t kHeld = 65536;  // classes of a row that a CU holds
 
 struct DistillArg {
@@ -32,7 +33,8 @@ struct DistillArg {
     float* grad;
     float* row_lse;  // or null
     // of k_distill_entries
-    int32_t* kept;    // [parts] rows with an entry
+    int32_t* kept;    // rows with an entry
+    uint32_t* tickets;  // their sum so far and the workgroups' arrivals: zero before and after
     int32_t* flag;    // [rows] 0: no entry, 1, 2: an id past the classes
     float* term;      // [rows] sum of q (log q - x / T)
     int32_t* ent_id;  // [rows][k] the class of its first entry, -1 at the others
@@ -41,7 +43,7 @@ struct DistillArg {
     float* row_loss;  // [rows]
     float* stat;      // [rows][splits][2]
     int64_t rows, classes;
-    int32_t k, splits, parts, slots;
+    int32_t k, splits, slots;
     int64_t span;     // classes of a split, a multiple of 4
     float inv_t, temperature;
 };
@@ -148,27 +150,25 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
     }
     if (lane == 0) red[wave] = kept;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int32_t n = 0;
-        for (int i = 0; i < waves; ++i) n += red[i];
-        a.kept[blockIdx.x] = n;
+    if (threadIdx.x == 0) {  // the last workgroup to arrive has the whole count
+        uint32_t n = 0;
+        for (int i = 0; i < waves; ++i) n += (uint32_t)red[i];
+        uint32_t *sum = a.tickets, *arrived = a.tickets + kTicketStride;
+        // the sum's answer is waited for before the arrival: an order for these two counters alone, where a
+        // release would write the L2 back, once a workgroup
+        const uint32_t before = __hip_atomic_fetch_add(sum, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" ::"v"(before) : "memory");
+        if (__hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+            a.kept[0] = (int32_t)__hip_atomic_load(sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(sum, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
 }
 
-// Rows with an entry, 1 at least; every lane of a wavefront gets them.
-__device__ __forceinline__ int32_t kept_rows(const DistillArg& a) {
-    int32_t n = 0;
-    for (int i = threadIdx.x & 63; i < a.parts; i += 64) n += a.kept[i];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-    return n > 0 ? n : 1;
-}
-// ug T / n: by the first wavefront, to every thread; `out` is LDS, read after a barrier.
-__device__ __forceinline__ void factor_to(const DistillArg& a, float* out) {
-    if (threadIdx.x < 64) {
-        const float c = a.ug[0] * a.temperature / (float)kept_rows(a);
-        if (threadIdx.x == 0) *out = c;
-    }
+// ug T / n over the n rows with an entry.
+__device__ __forceinline__ float factor_of(const DistillArg& a) {
+    return a.ug[0] * a.temperature / (float)(a.kept[0] > 0 ? a.kept[0] : 1);
 }
 
 // Running maximum and sum of exponentials, in base 2.
@@ -186,19 +186,20 @@ __device__ __forceinline__ void run_add(Run& r, vf4 v, float kf) {
     r.sum += (__builtin_amdgcn_exp2f((v.x - b) * kf) + __builtin_amdgcn_exp2f((v.y - b) * kf)) +
              (__builtin_amdgcn_exp2f((v.z - b) * kf) + __builtin_amdgcn_exp2f((v.w - b) * kf));
 }
-// Adds classes c0..c1 of a row, four loads in flight a thread.
+// Adds classes c0..c1 of a row, N loads in flight a thread.
 template <int W>
 __device__ __forceinline__ void run_row(Run& run, const float* x, int64_t c0, int64_t c1, float kf) {
+    constexpr int N = 4;
     constexpr int64_t step = W * 64;
     const int64_t nq = (c1 - c0) >> 2;
     const float* p = x + c0;
     int64_t q = threadIdx.x;
-    for (; q + 3 * step < nq; q += 4 * step) {
-        vf4 v[4];
+    for (; q + (N - 1) * step < nq; q += N * step) {
+        vf4 v[N];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const vf4u*>(p + 4 * (q + u * step));
+        for (int u = 0; u < N; ++u) v[u] = *reinterpret_cast<const vf4u*>(p + 4 * (q + u * step));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) run_add(run, v[u], kf);
+        for (int u = 0; u < N; ++u) run_add(run, v[u], kf);
     }
     for (; q < nq; q += step) run_add(run, *reinterpret_cast<const vf4u*>(p + 4 * q), kf);
     if ((int64_t)threadIdx.x < (c1 - c0) - 4 * nq) {
@@ -260,16 +261,16 @@ __device__ __forceinline__ void row_out(const DistillArg& a, int64_t r, int flag
 
 // A thread's entries of classes c0..c1: with ACC what the gradient held there is read before the dense part
 // writes over it; all are stored after it.
-template <int W>
+constexpr int entries_of(int W) { return kMaxK / (W * 64); }
+template <int W, int N = entries_of(W)>
 struct Mine {
-    static constexpr int N = (kMaxK + W * 64 - 1) / (W * 64);
     int32_t at[N];
     float old[N];
 };
-template <int W, bool ACC>
-__device__ __forceinline__ void entries_take(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, Mine<W>& mine) {
+template <int W, bool ACC, int N>
+__device__ __forceinline__ void entries_take(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, Mine<W, N>& mine) {
 #pragma unroll
-    for (int u = 0; u < Mine<W>::N; ++u) {
+    for (int u = 0; u < N; ++u) {
         const int i = threadIdx.x + u * W * 64;
         int32_t c = i < a.k ? a.ent_id[r * a.k + i] : -1;
         if (c < c0 || c >= c1) c = -1;
@@ -278,11 +279,12 @@ __device__ __forceinline__ void entries_take(const DistillArg& a, int64_t r, int
     }
     if (ACC) __syncthreads();
 }
-template <int W, bool ACC, bool LSE>
-__device__ __forceinline__ void entries_put(const DistillArg& a, int64_t r, const Scale<LSE>& s, float c, const Mine<W>& mine) {
+template <int W, bool ACC, bool LSE, int N>
+__device__ __forceinline__ void entries_put(const DistillArg& a, int64_t r, const Scale<LSE>& s, float c,
+                                            const Mine<W, N>& mine) {
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < Mine<W>::N; ++u) {
+    for (int u = 0; u < N; ++u) {
         if (mine.at[u] < 0) continue;
         const int64_t i = r * a.k + threadIdx.x + u * W * 64;
         const float v = (prob(s, a.ent_x[i]) - a.ent_q[i]) * c;
@@ -290,25 +292,32 @@ __device__ __forceinline__ void entries_put(const DistillArg& a, int64_t r, cons
     }
 }
 
-// Classes c0..c1 of row r's gradient, from the end, which was read last; four loads in flight a thread.
+// nq quads of a row's gradient, from the end, which was read last; N loads in flight a thread.
+template <int W, bool ACC, bool LSE>
+__device__ __forceinline__ void dense_grad(const float* x, float* g, int64_t nq, const Scale<LSE>& s, float c) {
+    constexpr int N = 4;  // 8: 900 us where 4 take 871 over [4096, 131072]
+    constexpr int64_t step = W * 64;
+    int64_t q = nq - 1 - threadIdx.x;
+    for (; q - (N - 1) * step >= 0; q -= N * step) {
+        vf4 v[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] = ld_ntu(x + 4 * (q - u * step));
+#pragma unroll
+        for (int u = 0; u < N; ++u) grad_put<ACC>(g + 4 * (q - u * step), grad4(s, v[u], c));
+    }
+    for (; q >= 0; q -= step) grad_put<ACC>(g + 4 * q, grad4(s, ld_ntu(x + 4 * q), c));
+}
+
+// Classes c0..c1 of row r's gradient.
 template <int W, bool ACC, bool LSE>
 __device__ void row_grad(const DistillArg& a, int64_t r, int64_t c0, int64_t c1, const Scale<LSE>& s, float c) {
-    constexpr int64_t step = W * 64;
     const float* x = a.x + r * a.classes + c0;
     float* g = a.grad + r * a.classes + c0;
     const int tid = threadIdx.x;
     Mine<W> mine;
     entries_take<W, ACC>(a, r, c0, c1, mine);
     const int64_t nq = (c1 - c0) >> 2;
-    int64_t q = nq - 1 - tid;
-    for (; q - 3 * step >= 0; q -= 4 * step) {
-        vf4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = ld_ntu(x + 4 * (q - u * step));
-#pragma unroll
-        for (int u = 0; u < 4; ++u) grad_put<ACC>(g + 4 * (q - u * step), grad4(s, v[u], c));
-    }
-    for (; q >= 0; q -= step) grad_put<ACC>(g + 4 * q, grad4(s, ld_ntu(x + 4 * q), c));
+    dense_grad<W, ACC>(x, g, nq, s, c);
     if (tid < (int)((c1 - c0) & 3)) {
         const int64_t p = 4 * nq + tid;
         const float v = prob(s, x[p]) * c;
@@ -317,26 +326,58 @@ __device__ void row_grad(const DistillArg& a, int64_t r, int64_t c0, int64_t c1,
     entries_put<W, ACC>(a, r, s, c, mine);
 }
 
-// A whole row a workgroup: statistics, loss and, with GRAD, the gradient.
+// A whole row a workgroup, of any length: statistics, loss and, with GRAD, the gradient, for which the row is read
+// again but for its last 32768 classes, which wait in LDS. That LDS also keeps a second workgroup off the CU:
+// two rows a CU, 268 MB of [*, 131072] in use at a time, are more than the last cache holds.
 template <int W, bool GRAD, bool ACC>
 __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
-    __shared__ float red[W], factor;
+    constexpr int NH = GRAD ? 8 : 1, step = W * 64;
+    __shared__ float red[W];
+    __shared__ vf4 held[GRAD ? NH * step : 1];
     const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
     const int flag = a.flag[r];
     if (flag == 0) {
         row_out(a, r, 0, 0.0f);
         if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
         return;
     }
-    if (GRAD) factor_to(a, &factor);
     const float kf = a.inv_t * kLog2e;
     Run run = {-__builtin_inff(), 0.0f};
-    run_row<W>(run, a.x + r * a.classes, 0, a.classes, kf);
+    const float* x = a.x + r * a.classes;
+    const int64_t nq = a.classes >> 2, c_held = GRAD ? (nq - NH * step) * 4 : a.classes;
+    run_row<W>(run, x, 0, c_held, kf);
+    if (GRAD) {  // rows here are longer than what is held
+        vf4 v[NH];
+#pragma unroll
+        for (int u = 0; u < NH; ++u) v[u] = ld_ntu(x + c_held + 4 * (u * step + tid));
+#pragma unroll
+        for (int u = 0; u < NH; ++u) {
+            held[u * step + tid] = v[u];
+            run_add(run, v[u], kf);
+        }
+        if (tid < (int)(a.classes & 3)) {
+            const float ninf = -__builtin_inff();
+            run_add(run, vf4{x[4 * nq + tid], ninf, ninf, ninf}, kf);
+        }
+    }
     run = run_join<W>(run, kf, red);
     row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
     if (GRAD) {  // an id past the classes: NaN all over the row
         const Scale<false> s = {kf, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
-        row_grad<W, ACC>(a, r, 0, a.classes, s, factor);
+        const float c = factor_of(a);
+        float* g = a.grad + r * a.classes;
+        Mine<W> mine;
+        entries_take<W, ACC>(a, r, 0, a.classes, mine);
+        if (tid < (int)(a.classes & 3)) {
+            const int64_t p = 4 * nq + tid;
+            const float v = prob(s, x[p]) * c;
+            g[p] = ACC ? g[p] + v : v;
+        }
+#pragma unroll
+        for (int u = 0; u < NH; ++u) grad_put<ACC>(g + c_held + 4 * (u * step + tid), grad4(s, held[u * step + tid], c));
+        dense_grad<W, ACC>(x, g, c_held >> 2, s, c);
+        entries_put<W, ACC>(a, r, s, c, mine);
     }
 }
 
@@ -347,9 +388,9 @@ __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
 // one's loads follow ([8192, 65536]: 787 us, 5.5 TB/s, against 846 read twice). Longer ones do not fit: 92
 // registers of data leave too few of 128, and what spills costs more than reading twice (945 against 916 us
 // over [4096, 131072]).
-template <int W, int NQ, bool GRAD, bool ACC>
+template <int W, int NQ, int NE, bool GRAD, bool ACC>
 __global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(DistillArg a) {
-    __shared__ float red[W], factor;
+    __shared__ float red[W];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const float ninf = -__builtin_inff();
@@ -378,7 +419,6 @@ __global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(Distill
 #pragma unroll
     for (int u = 0; u < NQ; ++u) v[u] = get(u);
     float last = tid < tail ? x[4 * nq + tid] : ninf;
-    if (GRAD) factor_to(a, &factor);
     const float kf = a.inv_t * kLog2e;
     top = __builtin_fmaxf(top, last);
 #pragma unroll
@@ -396,9 +436,9 @@ __global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(Distill
     sum = block_sum<W>(sum + last, red);
     row_out(a, r, flag, top * a.inv_t + mlog(sum));
     if (GRAD) {
-        const float c = factor;
+        const float c = factor_of(a);
         const Scale<false> s = {kf, base, flag == 2 ? __builtin_nanf("") : 1.0f / sum};
-        Mine<W> mine;
+        Mine<W, NE> mine;
         entries_take<W, ACC>(a, r, 0, a.classes, mine);
         float* g = a.grad + r * a.classes;
         const auto out_row = row_of(g);
@@ -453,7 +493,6 @@ __device__ __forceinline__ Run join_splits(const DistillArg& a, int64_t r) {
 // first split also writes the row's loss. GRAD off: the loss alone, a workgroup a row.
 template <int W, bool LOSS, bool GRAD, bool ACC>
 __global__ __launch_bounds__(W * 64) void k_distill_split(DistillArg a) {
-    __shared__ float factor;
     const int32_t per = GRAD ? a.splits : 1;
     const int64_t r = blockIdx.x / per, sp = blockIdx.x % per;
     const int64_t c0 = sp * a.span, c1 = c0 + a.span < a.classes ? c0 + a.span : a.classes;
@@ -463,20 +502,16 @@ __global__ __launch_bounds__(W * 64) void k_distill_split(DistillArg a) {
         if (GRAD) row_zero<W, ACC>(a, r, c0, c1);
         return;
     }
-    if (GRAD) {
-        factor_to(a, &factor);
-        __syncthreads();
-    }
     if (LOSS) {
         const Run run = join_splits(a, r);
         if (sp == 0) row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
         if (GRAD) {
             const Scale<false> s = {a.inv_t * kLog2e, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
-            row_grad<W, ACC>(a, r, c0, c1, s, factor);
+            row_grad<W, ACC>(a, r, c0, c1, s, factor_of(a));
         }
     } else {
         const Scale<true> s = {a.inv_t, flag == 2 ? __builtin_nanf("") : a.lse_in[r], 1.0f};
-        row_grad<W, ACC>(a, r, c0, c1, s, factor);
+        row_grad<W, ACC>(a, r, c0, c1, s, factor_of(a));
     }
 }
 
@@ -487,10 +522,8 @@ __global__ __launch_bounds__(1024) void k_distill_loss(DistillArg a, float* loss
 #pragma unroll 4
     for (int64_t n = threadIdx.x; n < a.rows; n += 1024) s += (double)a.row_loss[n];
     s = block_sum<16>(s, red);
-    if (threadIdx.x < 64) {
-        const double n = kept_rows(a);
-        if (threadIdx.x == 0) loss[0] = (float)(s * ((double)a.temperature * a.temperature) / n);
-    }
+    const double n = a.kept[0] > 0 ? a.kept[0] : 1;
+    if (threadIdx.x == 0) loss[0] = (float)(s * ((double)a.temperature * a.temperature) / n);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -553,16 +586,17 @@ int distill_run(const DistillCall& d) {
     while (waves > 1 && waves * row_lds > 65536) waves /= 2;
     while (waves > 4 && d.rows < (int64_t)waves * ctx().num_cus) waves /= 2;
     const int64_t blocks = (d.rows + waves - 1) / waves;
-    a.parts = (int32_t)(blocks < kEntryBlocks ? blocks : kEntryBlocks);
+    const int64_t parts = blocks < kEntryBlocks ? blocks : kEntryBlocks;
     const size_t rows_b = ((size_t)d.rows * 4 + 255) & ~(size_t)255, ent_b = ((size_t)d.rows * a.k * 4 + 255) & ~(size_t)255;
     char* base = nullptr;
-    MH_TRY(scratch(kEntryBlocks * 4 + 3 * rows_b + 3 * ent_b + (size_t)d.rows * a.splits * 8, reinterpret_cast<void**>(&base)));
+    MH_TRY(tickets(2 * kTicketStride, &a.tickets));
+    MH_TRY(scratch(256 + 3 * rows_b + 3 * ent_b + (size_t)d.rows * a.splits * 8, reinterpret_cast<void**>(&base)));
     auto take = [&base](size_t bytes) {
         char* p = base;
         base += bytes;
         return p;
     };
-    a.kept = reinterpret_cast<int32_t*>(take(kEntryBlocks * 4));
+    a.kept = reinterpret_cast<int32_t*>(take(256));
     a.flag = reinterpret_cast<int32_t*>(take(rows_b));
     a.term = reinterpret_cast<float*>(take(rows_b));
     a.row_loss = reinterpret_cast<float*>(take(rows_b));
@@ -571,7 +605,7 @@ int distill_run(const DistillCall& d) {
     a.ent_x = reinterpret_cast<float*>(take(ent_b));
     a.stat = reinterpret_cast<float*>(base);
     hipStream_t st = ctx().stream;
-    hipLaunchKernelGGL(k_distill_entries, dim3((unsigned)a.parts), dim3(waves * 64), waves * row_lds, st, a);
+    hipLaunchKernelGGL(k_distill_entries, dim3((unsigned)parts), dim3(waves * 64), waves * row_lds, st, a);
     constexpr int W = 16;
     const dim3 rows((unsigned)d.rows), all((unsigned)(d.rows * a.splits)), t(W * 64);
     const bool grad = d.grad != nullptr;
@@ -579,18 +613,21 @@ int distill_run(const DistillCall& d) {
         if (d.accumulate) hipLaunchKernelGGL((k_distill_split<W, false, true, true>), all, t, 0, st, a);
         else hipLaunchKernelGGL((k_distill_split<W, false, true, false>), all, t, 0, st, a);
     } else if (a.splits == 1 && a.classes <= kHeld && (grad || a.classes <= 32768)) {
-#define MH_REGS(WW, NQ)                                                                                                \
+#define MH_REGS(WW, NQ, NE)                                                                                                \
     do {                                                                                                              \
         const dim3 tt(WW * 64);                                                                                       \
-        if (!grad) hipLaunchKernelGGL((k_distill_regs<WW, NQ, false, false>), rows, tt, 0, st, a);                    \
-        else if (d.accumulate) hipLaunchKernelGGL((k_distill_regs<WW, NQ, true, true>), rows, tt, 0, st, a);          \
-        else hipLaunchKernelGGL((k_distill_regs<WW, NQ, true, false>), rows, tt, 0, st, a);                           \
+        if (!grad) hipLaunchKernelGGL((k_distill_regs<WW, NQ, NE, false, false>), rows, tt, 0, st, a);                    \
+        else if (d.accumulate) hipLaunchKernelGGL((k_distill_regs<WW, NQ, NE, true, true>), rows, tt, 0, st, a);          \
+        else hipLaunchKernelGGL((k_distill_regs<WW, NQ, NE, true, false>), rows, tt, 0, st, a);                           \
     } while (0)
-        if (a.classes <= 4096) MH_REGS(4, 4);
-        else if (a.classes <= 8192) MH_REGS(4, 8);
-        else if (a.classes <= 16384) MH_REGS(8, 8);
-        else if (a.classes <= 32768) MH_REGS(16, 8);
-        else MH_REGS(16, 16);
+        // short rows with few entries: a wavefront each, with no barrier
+        if (a.classes <= 1024 && a.k <= 128) MH_REGS(1, 4, 2);
+        else if (a.classes <= 2048) MH_REGS(4, 2, 4);
+        else if (a.classes <= 4096) MH_REGS(4, 4, 4);
+        else if (a.classes <= 8192) MH_REGS(4, 8, 4);
+        else if (a.classes <= 16384) MH_REGS(8, 8, 2);
+        else if (a.classes <= 32768) MH_REGS(16, 8, 1);
+        else MH_REGS(16, 16, 1);
 #undef MH_REGS
     } else if (a.splits == 1) {
         if (!grad) hipLaunchKernelGGL((k_distill_row<W, false, false>), rows, t, 0, st, a);

@@ -99,7 +99,7 @@ def check(got, want, bound, what=""):
 
 
 SIZES = [(1, 1, 1), (3, 2, 1), (1, 3, 3), (5, 7, 2), (16, 1000, 8), (33, 257, 64), (7, 4096, 100), (9, 4099, 65),
-         (300, 1023, 5), (2, 32768, 17), (3, 32771, 128), (520, 33001, 3), (4, 70001, 256), (1, 131072, 1024), (513, 8191, 12)]
+         (300, 1023, 5), (2, 32768, 17), (3, 32771, 128), (520, 33001, 3), (4, 70001, 256), (1, 131072, 1024), (513, 8191, 12), (300, 70003, 9)]
 
 
 @pytest.mark.parametrize("how", ["step", "two calls"])
@@ -122,7 +122,7 @@ def test_same_class_many_times(size, how):
 
 
 @pytest.mark.parametrize("how", ["step", "two calls"])
-@pytest.mark.parametrize("size", [(70, 999, 20), (300, 33000, 9), (3, 70001, 30)], ids=str)
+@pytest.mark.parametrize("size", [(70, 999, 20), (300, 33000, 9), (3, 70001, 30), (258, 65541, 4)], ids=str)
 def test_accumulates(size, how):
     a = inputs(*size, seed=2)
     g = np.random.RandomState(0).standard_normal(a[0].shape).astype(np.float32)
