@@ -150,7 +150,8 @@ __device__ __forceinline__ float row_exp(float* v, float* top) {
 // Up to 8 choices: sorted lists. A logit's order and its index become the mantissa of a double in [1, 2), which
 // the maximum and minimum of doubles sort, one instruction each and at full rate; a larger index is smaller.
 // Each lane sorts its elements and keeps 8; neighbours' lists merge, and in the end each lane has the row's 8.
-// [131072, 256], 8 of them: 84 us by rounds of a maximum, 58 by lists.
+// [131072, 256], 8 of them: 84 us by rounds of a maximum, 60 by lists, which the sorting bounds (the read alone
+// takes 24; loading a round ahead changed nothing).
 constexpr int kList = 8;
 __device__ __forceinline__ double list_key(int key, int index) {
     const uint32_t u = (uint32_t)key ^ 0x80000000u;
@@ -542,8 +543,9 @@ __global__ __launch_bounds__(kRThreads) void k_router_bwd(RouterArg a) {
 // ---------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------
-// Lanes and elements of a lane by the experts: 16 elements a lane at most, which is where a round of the
-// selection costs least a row (a lane's scan is plain arithmetic, the lanes' is a chain).
+// Lanes and elements of a lane by the experts, 16 elements a lane at most: 32 would make the lanes' part of the
+// selection shorter, but take 152 and 174 registers a thread (over [131072, 256] 65 and 78 us forward and
+// backward, against 60 and 56 with 16).
 #define MH_ROUTER(CALL)                      \
     do {                                     \
         if (a.experts <= 8) CALL(2, 4);      \
