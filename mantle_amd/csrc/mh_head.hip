@@ -259,7 +259,7 @@ struct GemmArg {
     int64_t m, n;
     const float* ug;
     float* part;             // split sums [splits][tiles_m * TM][tiles_n * TN], or null
-    int32_t exp_b;           // 0: x's power of two, 1: w's
+    int32_t exp_b;           // 0: x's power of two, 1: w's, 2: none
     int32_t accumulate;
 };
 
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmPair pair) {
                     }
             return;
         }
-        const int e = -(kGExp + (g.exp_b ? g.info->ew : g.info->ex));
+        const int e = -(kGExp + (g.exp_b == 2 ? 0 : g.exp_b ? g.info->ew : g.info->ex));
         const float c = g.ug[0] / (float)(g.info->kept > 0 ? g.info->kept : 1);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(256) void k_join(GemmPair pair, int32_t tile) {
     const GemmArg& g = pair.g[second];
     const int64_t block = blockIdx.x - (second ? pair.first : 0), blocks = second ? gridDim.x - pair.first : pair.first;
     const int64_t ld = (int64_t)g.tiles_n * tile, plane = (int64_t)g.tiles_m * tile * ld;
-    const int e = -(kGExp + (g.exp_b ? g.info->ew : g.info->ex));
+    const int e = -(kGExp + (g.exp_b == 2 ? 0 : g.exp_b ? g.info->ew : g.info->ex));
     const float c = g.ug[0] / (float)(g.info->kept > 0 ? g.info->kept : 1);
     const int64_t total = g.m * g.n;
     for (int64_t i = block * 256 + threadIdx.x; i < total; i += blocks * 256) {
@@ -641,12 +641,201 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
 }
 
 // ---------------------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------------------
+// Up to 64 rows against a large w, whose bytes bound both products that read it: w goes to the matrix unit from
+// memory, as it lies, split in registers. A power of two for all of it would take a pass of its own, so each
+// element becomes three bf16 (hi, mid, lo: 24 bits at fp32's own exponents), and a product six instructions:
+// all but mid lo, lo mid and lo lo, below 2^-24. [16, 4096] x [32000, 4096]: 433 -> 175 us forward,
+// 859 -> 497 with both gradients; torch's fp32 operations take 178 and 623.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+constexpr int kFewRows = 64, kFewBlk = 3072;  // bytes of a block of x: three planes of 32 rows x 16
+
+struct Tri {
+    bf16x8 h, m, l;
+};
+__device__ __forceinline__ Tri split3(f32x8 v) {
+    Tri t;
+    t.h = __builtin_convertvector(v, bf16x8);
+    v -= __builtin_convertvector(t.h, f32x8);
+    t.m = __builtin_convertvector(v, bf16x8);
+    v -= __builtin_convertvector(t.m, f32x8);
+    t.l = __builtin_convertvector(v, bf16x8);
+    return t;
+}
+__device__ __forceinline__ f32x16 mul3(const Tri& a, const Tri& b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.l, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.m, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.m, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.h, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.h, c, 0, 0, 0);
+}
+
+struct FewArg {
+    const float *x, *w;
+    const int32_t* labels;
+    int64_t rows, dim, classes, dkb;
+    char* xp;        // x's blocks, [row blocks][dkb]
+    float* stat;     // [32-class groups][2][stat_ld]
+    int64_t stat_ld;
+    float* target;
+    char* z;         // as GemmArg's, or null; G's panel for k_few_dx
+    int64_t zkb;
+    float* part;     // [splits][rows of blocks][dim_p]
+    int64_t dim_p, ckb, per;  // padded dims; 16-class blocks in all and of a split
+};
+
+// x to its three planes, a wavefront a block; a row left out becomes zeros, whatever it holds.
+__global__ __launch_bounds__(64) void k_few_x(FewArg f) {
+    const int lane = threadIdx.x;
+    const int64_t r = blockIdx.x / f.dkb * 32 + (lane & 31), c = blockIdx.x % f.dkb * 16 + (lane >> 5) * 8;
+    const bool in = r < f.rows && f.labels[r] >= 0;
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = in && c + j < f.dim ? f.x[r * f.dim + c + j] : 0.0f;
+    const Tri t = split3(v);
+    bf16x8* p = reinterpret_cast<bf16x8*>(f.xp + (int64_t)blockIdx.x * kFewBlk);
+    p[lane] = t.h;
+    p[64 + lane] = t.m;
+    p[128 + lane] = t.l;
+}
+
+// Logits of 32 classes by all rows a workgroup: eight wavefronts take an eighth of the dims each, four 2 KB blocks of
+// w under way a wavefront, and add up in LDS.
+template <int NT>
+__global__ __launch_bounds__(512) void k_few_logits(FewArg f) {
+    __shared__ float sums[8][NT][16 * 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int64_t v0 = (int64_t)blockIdx.x * 32, v = v0 + col;
+    const int64_t per = (f.dkb + 7) / 8;
+    const int64_t k1 = (wave + 1) * per < f.dkb ? (wave + 1) * per : f.dkb;
+    const float* row = f.w + (v < f.classes ? v : 0) * f.dim;
+    // a class past the last reads the first one's: its logits count nowhere
+    auto whole = [&](int64_t kb) {
+        const float* p = row + kb * 16 + half * 8;
+        const vf4 a = *reinterpret_cast<const vf4u*>(p), b = *reinterpret_cast<const vf4u*>(p + 4);
+        return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    };
+    auto edge = [&](int64_t kb) {
+        f32x8 o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t c = kb * 16 + half * 8 + j;
+            o[j] = c < f.dim ? row[c] : 0.0f;
+        }
+        return o;
+    };
+    f32x16 acc[NT] = {};
+    for (int64_t k = wave * per; k < k1; k += 4) {
+        f32x8 in[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) in[u] = (k + 4) * 16 <= f.dim ? whole(k + u) : edge(k + u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (k + u >= k1) break;
+            const Tri a = split3(in[u]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8* p = reinterpret_cast<const bf16x8*>(f.xp + (t * f.dkb + k + u) * kFewBlk);
+                acc[t] = mul3(a, Tri{p[lane], p[64 + lane], p[128 + lane]}, acc[t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[wave][t][r * 64 + lane] = acc[t][r];
+    __syncthreads();
+    if (wave >= NT) return;
+    float z[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        z[r] = sums[0][wave][r * 64 + lane];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) z[r] += sums[i][wave][r * 64 + lane];
+    }
+    // register r: class v0 + 8 (r / 4) + 4 half + r % 4 of row n, as in k_gemm
+    const int64_t n = wave * 32 + col;
+    if (f.stat) {
+        const int64_t left = f.classes - v0 - 4 * half;
+        const int64_t want = (n < f.rows ? (int64_t)f.labels[n] : -1) - v0 - 4 * half;
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int c = 8 * (r >> 2) + (r & 3);
+            if (c == want && c < left) f.target[n] = z[r];
+            if (c < left) top = __builtin_fmaxf(top, z[r]);
+        }
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) < left) sum += __builtin_amdgcn_exp2f((z[r] - base) * kLog2e);
+        sum += __shfl_xor(sum, 32);
+        if (half == 0) {
+            f.stat[(int64_t)blockIdx.x * 2 * f.stat_ld + n] = top;
+            f.stat[((int64_t)blockIdx.x * 2 + 1) * f.stat_ld + n] = sum;
+        }
+    }
+    if (f.z) {
+        char* zb = f.z + wave * f.zkb * kBlk;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<vf4*>(zb + ((v0 >> 4) + (q >> 1)) * kBlk + (col + 32 * (q & 1)) * 32 + half * 16) =
+                vf4{z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]};
+    }
+}
+
+// G w over a split of the classes, 32 dims by all rows a wavefront: its loads of w are 128 bytes of a class, 512 of
+// four wavefronts, and four blocks' are under way.
+template <int NT>
+__global__ __launch_bounds__(256) void k_few_dx(FewArg f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int64_t d = ((int64_t)blockIdx.x * 4 + wave) * 32 + col;
+    const int64_t k0 = blockIdx.y * f.per, k1 = k0 + f.per < f.ckb ? k0 + f.per : f.ckb;
+    const float* wd = f.w + (d < f.dim ? d : 0);  // a dim past the last reads the first one's, for sums that no one reads
+    f32x16 acc[NT] = {};
+    for (int64_t k = k0; k < k1; k += 4) {
+        f32x8 in[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t v = (k + u) * 16 + half * 8;
+            if ((k + 4) * 16 <= f.classes) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) in[u][j] = wd[(v + j) * f.dim];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) in[u][j] = v + j < f.classes ? wd[(v + j) * f.dim] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (k + u >= k1) break;
+            const Tri b = split3(in[u]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const half8* p = reinterpret_cast<const half8*>(f.z + (t * f.zkb + k + u) * kBlk);
+                const f32x8 g = __builtin_convertvector(p[lane], f32x8) + __builtin_convertvector(p[64 + lane], f32x8);
+                acc[t] = mul3(split3(g), b, acc[t]);
+            }
+        }
+    }
+    float* o = f.part + blockIdx.y * (NT * 32) * f.dim_p;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[(t * 32 + 8 * (r >> 2) + 4 * half + (r & 3)) * f.dim_p + d] = acc[t][r];
+}
+
+// ---------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------
 // The logits of one chunk of rows and G's column panel take 8 bytes an element; a chunk's rows keep them
 // within this, 256 rows at least.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 constexpr int64_t kMaxChunk = 32768;
+constexpr int64_t kFewElements = (int64_t)1 << 22;  // of w, from which its bytes and not launches count
 
 struct Carve {
     size_t at = 0;
@@ -787,14 +976,23 @@ int head_run(const HeadCall& h) {
         chunk = chunk < 256 ? 256 : chunk > kMaxChunk ? kMaxChunk : chunk;
     }
     if (chunk > rowsP) chunk = rowsP;
-    const int64_t groups = clsP / 64;
+    // w straight from memory where rows are few and w is large enough to bound the products, in rows long enough
+    // for eight wavefronts each ([32, 64] x [100000, 64]: 178 us so, 146 by panels)
+    const bool few = rows <= kFewRows && dim >= 256 && classes * dim >= kFewElements;
+    const int nt = rows > 32 ? 2 : 1;
+    const int64_t groups = few ? clsP / 32 : clsP / 64;
+    const int64_t fdim = up(dim, 128), fkb = up(classes, 16) / 16;
+    // splits of the classes that give every CU eight wavefronts or so, of 16 blocks at least
+    int64_t fsplits = few ? (2 * ctx().num_cus + fdim / 128 - 1) / (fdim / 128) : 1;
+    if (fsplits > fkb / 16) fsplits = fkb / 16;
+    fsplits = fsplits < 1 ? 1 : fsplits > kMaxSplit ? kMaxSplit : fsplits;
 
     Carve cv;
     const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
     const size_t o_xr = cv.take(rowsP / 32 * stride_of(dkb) * kBlk),
-                 o_wr = cv.take(clsP / 32 * stride_of(dkb) * kBlk);
+                 o_wr = few ? 0 : cv.take(clsP / 32 * stride_of(dkb) * kBlk);
     const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
-    const size_t o_wt = h.train && h.gx ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
+    const size_t o_wt = h.train && h.gx && !few ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
     const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
     const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / kLseRows * 8);
     size_t o_z = 0, o_gt = 0, o_sp = 0;
@@ -802,13 +1000,14 @@ int head_run(const HeadCall& h) {
         o_z = cv.take(chunk / 32 * stride_of(clsP / 16) * kBlk);
         o_gt = cv.take(clsP / 32 * stride_of(chunk / 16) * kBlk);
         // every chunk has this many rows but the last
-        size_t sp = 0;
+        size_t sp = few ? (size_t)(fsplits * nt * 32 * fdim) * sizeof(float) : 0;
         for (const int64_t nr : {rows < chunk ? rows : chunk, rows - (rows - 1) / chunk * chunk}) {
             const Forms f = forms_of(h, nr, dkb);
             if (f.part[0] + f.part[1] > sp) sp = f.part[0] + f.part[1];
         }
         o_sp = cv.take((int64_t)sp);
     }
+    const size_t o_fx = few ? cv.take(nt * dkb * kFewBlk) : 0;
     char* base = nullptr;
     MH_TRY(scratch(cv.at, reinterpret_cast<void**>(&base)));
     hipStream_t st = ctx().stream;
@@ -818,7 +1017,7 @@ int head_run(const HeadCall& h) {
     double* block_loss = reinterpret_cast<double*>(base + o_rl);
     float* target = reinterpret_cast<float*>(base + o_tgt);
 
-    hipLaunchKernelGGL(k_amax, dim3(2 * kAmaxBlocks), dim3(256), 0, st, part, h.x, h.w, h.labels, rows, dim,
+    hipLaunchKernelGGL(k_amax, dim3(few ? kAmaxBlocks : 2 * kAmaxBlocks), dim3(256), 0, st, part, h.x, h.w, h.labels, rows, dim,
                        classes * dim);
     SplitOne sx = {h.x, rows, dim, base + o_xr, h.train && h.gw ? base + o_xt : nullptr, dkb, rowsP / 16,
                    rowsP / 64, up(dim, 64) / 64, rowsP / 32, dimP / 32};
@@ -826,7 +1025,7 @@ int head_run(const HeadCall& h) {
                    clsP / 64, up(dim, 64) / 64, clsP / 32, dimP / 32};
     if (sx.colp) sx.tiles_c = dimP / 64;
     if (sw.colp) sw.tiles_c = dimP / 64;
-    const int64_t nsplit = sx.tiles_r * sx.tiles_c + sw.tiles_r * sw.tiles_c;
+    const int64_t nsplit = sx.tiles_r * sx.tiles_c + (few ? 0 : sw.tiles_r * sw.tiles_c);
     hipLaunchKernelGGL(k_split, dim3((unsigned)nsplit), dim3(256), 0, st, sx, sw, part, info, h.labels);
 
     for (int64_t r0 = 0; r0 < rows; r0 += chunk) {
@@ -849,7 +1048,16 @@ int head_run(const HeadCall& h) {
         g.zkb = zkb;
         // every row and class that a gradient's tiles read gets its logits: the panels behind have no gaps
         set_form(g, clsP, nrP, f.logits);
-        launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
+        FewArg fa = {h.x, h.w, h.labels, rows, dim, classes, dkb, base + o_fx, g.stat, g.stat_ld, target, g.z, zkb,
+                     reinterpret_cast<float*>(base + o_sp), fdim, fkb, (fkb + fsplits - 1) / fsplits};
+        if (few) {
+            hipLaunchKernelGGL(k_few_x, dim3((unsigned)(nt * dkb)), dim3(64), 0, st, fa);
+            const dim3 grid((unsigned)(clsP / 32));
+            if (nt == 1) hipLaunchKernelGGL((k_few_logits<1>), grid, dim3(512), 0, st, fa);
+            else hipLaunchKernelGGL((k_few_logits<2>), grid, dim3(512), 0, st, fa);
+        } else {
+            launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
+        }
         if (!h.row_lse_in) {
             const dim3 grid((unsigned)((nr + kLseRows - 1) / kLseRows));
             float* rl = h.row_loss ? h.row_loss + r0 : nullptr;
@@ -885,6 +1093,21 @@ int head_run(const HeadCall& h) {
             p.part = f.grad[0].splits > 1 ? sp : nullptr;
             set_form(p, nr, dim, f.grad[0]);
             df[nd++] = f.grad[0];
+            if (few) {
+                const dim3 grid((unsigned)(fdim / 128), (unsigned)fsplits);
+                if (nt == 1) hipLaunchKernelGGL((k_few_dx<1>), grid, dim3(256), 0, st, fa);
+                else hipLaunchKernelGGL((k_few_dx<2>), grid, dim3(256), 0, st, fa);
+                p.info = info;
+                p.ug = h.ug;
+                p.exp_b = 2;
+                p.part = fa.part;
+                p.splits = (int32_t)fsplits;
+                p.tiles_m = nt;
+                p.tiles_n = (int32_t)(fdim / 32);
+                const uint32_t blocks = (uint32_t)((rows * dim + 255) / 256);
+                hipLaunchKernelGGL(k_join, dim3(blocks), dim3(256), 0, st, (GemmPair{{p, p}, blocks}), 32);
+                d[--nd] = GemmArg{};
+            }
         }
         if (h.gw) {
             GemmArg& p = d[nd];
@@ -895,7 +1118,8 @@ int head_run(const HeadCall& h) {
             p.kb_all = up(nr, 32) / 16;
             p.out = h.gw;
             p.accumulate = h.accumulate || r0 > 0;
-            p.part = f.grad[1].splits > 1 ? sp + f.part[0] / sizeof(float) : nullptr;
+            // behind grad_x's sums; those of few rows are joined by then
+            p.part = f.grad[1].splits > 1 ? sp + (few ? 0 : f.part[0] / sizeof(float)) : nullptr;
             set_form(p, classes, dim, f.grad[1]);
             df[nd++] = f.grad[1];
         }
@@ -903,7 +1127,7 @@ int head_run(const HeadCall& h) {
             d[i].info = info;
             d[i].ug = h.ug;
         }
-        grad_products(d, df, nd);
+        if (nd) grad_products(d, df, nd);
     }
     if (!h.train)
         hipLaunchKernelGGL(k_rows_loss, dim3(1), dim3(256), 0, st, block_loss, (rows + kLseRows - 1) / kLseRows, info, h.loss);

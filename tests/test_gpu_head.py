@@ -122,6 +122,30 @@ def test_larger_tiles_and_splits():
         check(run(m, x, w, labels), want, bound, str(size))
 
 
+@pytest.mark.parametrize("size", [(1, 513, 9001), (16, 4097, 1031), (32, 1024, 4100), (33, 700, 6007), (64, 2050, 2049), (9, 257, 16390), (9, 48, 100003)], ids=str)
+def test_few_rows_against_a_large_head(size):
+    """Up to 64 rows: w read as it lies, three bf16 an element, whose products are off by 2^-22 at most."""
+    m = m_()
+    x, w, labels = inputs(*size, seed=21)
+    labels[0] = 3
+    want, bound = reference(x, w, labels)
+    for how in ("step", "two calls"):
+        check(run(m, x, w, labels, how=how), want, bound, how)
+    r = np.random.RandomState(1)
+    g0 = r.standard_normal(x.shape).astype(np.float32), r.standard_normal(w.shape).astype(np.float32)
+    plain, got = run(m, x, w, labels), run(m, x, w, labels, grads=g0)
+    assert np.array_equal(got["grad_w"], g0[1] + plain["grad_w"]) and np.array_equal(got["grad_x"], g0[0] + plain["grad_x"])
+    if size[0] > 4:  # rows left out, classes that do not exist, infinities
+        labels[1], x[1] = -5, np.nan
+        labels[2] = size[2]
+        got = run(m, x, w, labels)
+        assert np.isnan(got["row_lse"][2]) and got["row_lse"][1] == 0 and not got["grad_x"][1].any()
+        assert np.isfinite(np.delete(got["grad_x"], 2, 0)).all() and np.isnan(got["grad_x"][2]).all()
+        labels[2] = 0
+        w[5, 7] = np.inf
+        assert np.isnan(run(m, x, w, labels)["loss"])
+
+
 def test_rows_in_chunks():
     """2^20 classes: the logits of 512 rows at a time, the last chunk shorter, grad_w over both."""
     rows, classes = 600, 1 << 20
