@@ -21,7 +21,9 @@
  *     negative dim or a null tensor pointer returns an error and launches nothing.
  *   - One context per process, one HIP stream (default priority). Calls are complete when
  *     they return unless mh_init was given MH_INIT_ASYNC; then mh_sync() waits.
- *   - Backward entry points ACCUMULATE into grad (grad = grad + op gradient), fusing the
+ *   - Class ids, where the losses of a language model take them, are int32.
+ *   - Backward entry points ACCUMULATE into grad (grad = grad + op gradient; the losses of a
+ *     language model take an argument that says so), fusing the
  *     op struct's backward with accumulate_grad exactly as backward_op does
  *     (ops.mojo:355-463). Pass a zeroed grad to get the plain gradient.
  *   - Not re-entrant across host threads (the reference calls ops from one thread).
@@ -289,7 +291,10 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
  * (0 without kept rows). A label of classes or more makes the row's loss, the loss and the gradients
  * NaN; so does a kept row or a class that holds a NaN or an infinity. row_loss and row_lse may be null.
  * x and w are each held with 22 bits relative to every element down to 2^-29 of the tensor's largest
- * (of the kept rows for x), which a product needs to be as exact as one of fp32 operands; sums are fp32. */
+ * (of the kept rows for x), which a product needs to be as exact as one of fp32 operands; sums are fp32.
+ * (Up to 64 rows against a w of 2^22 elements or more: 24 bits of every element between 2^-110 and 3.38e38.)
+ * The library's scratch, which it keeps, grows to 4 bytes an element of x and of w, and for the
+ * gradients to as much again and 8 bytes a logit of a chunk of rows: 4 GiB, or 256 rows, at most. */
 int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,
                                 const int32_t* labels, int64_t rows, int64_t dim, int64_t classes);
 /* The gradients from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
