@@ -108,8 +108,9 @@ int hip_inject(const char* what) {
 }
 
 int hip_check(hipError_t e, const char* what) {
-    if (e != hipSuccess) return fail(MH_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    return MH_OK;
+    if (e == hipSuccess) return MH_OK;
+    (void)hipGetLastError();  // reported here: the next call's launch check does not meet it again
+    return fail(MH_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
 int require_init() {

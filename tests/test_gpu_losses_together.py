@@ -2,6 +2,8 @@
 hidden states also feed a router, a student's logits under distillation, gradients accumulated into the same
 tensors, Adam over all of them, several steps; against the same program in 64 bits. And the losses beside the
 library's other state: captured graphs, growing scratch, shut down and started again, calls that wait."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -151,3 +153,18 @@ def test_many_sizes_in_turn_share_the_scratch():
     for a, q in zip(alone, queued):
         for u, v in zip(a, q):
             assert np.array_equal(u, v.to_numpy())
+
+
+def test_a_refused_allocation_does_not_fail_the_next_call():
+    """An allocation that the device cannot hold returns an error, and the calls behind it go on."""
+    m = GpuEngine().m
+    d = data(3)
+    t, g, out = program(m, d)
+    step(m, t, g, out)
+    ref = {k: g[k].to_numpy() for k in "xws"}
+    with pytest.raises(m.MantleHipError) as e:
+        m._lib.call("mh_malloc", ctypes.byref(ctypes.c_void_p()), 1 << 46)
+    assert e.value.code == m._lib.ERR_HIP
+    step(m, t, g, out)
+    for k in "xws":
+        assert np.array_equal(g[k].to_numpy(), ref[k])
