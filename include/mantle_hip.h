@@ -292,7 +292,8 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
  * NaN; so does a kept row or a class that holds a NaN or an infinity. row_loss and row_lse may be null.
  * x and w are each held with 22 bits relative to every element down to 2^-29 of the tensor's largest
  * (of the kept rows for x), which a product needs to be as exact as one of fp32 operands; sums are fp32.
- * (Up to 64 rows against a w of 2^22 elements or more: 24 bits of every element between 2^-110 and 3.38e38.)
+ * (Up to 64 rows, or 128 forward, of 256 dims or more against 2^22 elements of w or more: 24 bits of
+ * every element between 2^-110 and 3.38e38.)
  * The library's scratch, which it keeps, grows to 4 bytes an element of x and of w, and for the
  * gradients to as much again and 8 bytes a logit of a chunk of rows: 4 GiB, or 256 rows, at most. */
 int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,

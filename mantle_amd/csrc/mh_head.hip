@@ -649,13 +649,15 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
 // ---------------------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------------------
-// Up to 64 rows against a large w, whose bytes bound both products that read it: w goes to the matrix unit from
-// memory, as it lies, split in registers. A power of two for all of it would take a pass of its own, so each
-// element becomes three bf16 (hi, mid, lo: 24 bits at fp32's own exponents), and a product six instructions:
-// all but mid lo, lo mid and lo lo, below 2^-24. [16, 4096] x [32000, 4096]: 433 -> 175 us forward,
-// 859 -> 497 with both gradients; torch's fp32 operations take 178 and 623.
+// Up to 64 rows, or 128 without gradients, against a large w, whose bytes bound both products that read it: w
+// goes to the matrix unit from memory, as it lies, split in registers. A power of two for all of it would take a
+// pass of its own, so each element becomes three bf16 (hi, mid, lo: 24 bits at fp32's own exponents), and a
+// product six instructions: all but mid lo, lo mid and lo lo, below 2^-24. [16, 4096] x [32000, 4096]: 433 ->
+// 175 us forward (3 TB/s of w), 859 -> 495 with both gradients; torch's fp32 operations take 178 and 626. Of 128
+// rows the forward gains, 429 -> 316 us, but k_few_dx would need 255 registers a thread: 1069 us a step, against
+// 895 by panels.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-constexpr int kFewRows = 64, kFewBlk = 3072;  // bytes of a block of x: three planes of 32 rows x 16
+constexpr int kFewRows = 64, kFewRowsForward = 128, kFewBlk = 3072;  // bytes of a block of x: three planes of 32 rows x 16
 
 struct Tri {
     bf16x8 h, m, l;
@@ -711,7 +713,7 @@ __global__ __launch_bounds__(64) void k_few_x(FewArg f) {
 // w under way a wavefront, and add up in LDS.
 template <int NT>
 __global__ __launch_bounds__(512) void k_few_logits(FewArg f) {
-    __shared__ float sums[8][NT][16 * 64];
+    __shared__ float sums[4][NT][16 * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int64_t v0 = (int64_t)blockIdx.x * 32, v = v0 + col;
     const int64_t per = (f.dkb + 7) / 8;
@@ -748,19 +750,28 @@ __global__ __launch_bounds__(512) void k_few_logits(FewArg f) {
             }
         }
     }
+    // the second four wavefronts' sums go to the first four, and theirs to one a row block
+    if (wave >= 4)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sums[wave][t][r * 64 + lane] = acc[t][r];
+            for (int r = 0; r < 16; ++r) sums[wave - 4][t][r * 64 + lane] = acc[t][r];
+    __syncthreads();
+    if (wave < 4)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                acc[t][r] += sums[wave][t][r * 64 + lane];
+                sums[wave][t][r * 64 + lane] = acc[t][r];
+            }
     __syncthreads();
     if (wave >= NT) return;
     float z[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        z[r] = sums[0][wave][r * 64 + lane];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) z[r] += sums[i][wave][r * 64 + lane];
-    }
+    for (int r = 0; r < 16; ++r)
+        z[r] = (sums[0][wave][r * 64 + lane] + sums[1][wave][r * 64 + lane]) +
+               (sums[2][wave][r * 64 + lane] + sums[3][wave][r * 64 + lane]);
     // register r: class v0 + 8 (r / 4) + 4 half + r % 4 of row n, as in k_gemm
     const int64_t n = wave * 32 + col;
     if (f.stat) {
@@ -984,8 +995,8 @@ int head_run(const HeadCall& h) {
     if (chunk > rowsP) chunk = rowsP;
     // w straight from memory where rows are few and w is large enough to bound the products, in rows long enough
     // for eight wavefronts each ([32, 64] x [100000, 64]: 178 us so, 146 by panels)
-    const bool few = rows <= kFewRows && dim >= 256 && classes * dim >= kFewElements;
-    const int nt = rows > 32 ? 2 : 1;
+    const bool few = rows <= (h.train ? kFewRows : kFewRowsForward) && dim >= 256 && classes * dim >= kFewElements;
+    const int nt = rows > 64 ? 4 : rows > 32 ? 2 : 1;
     const int64_t groups = few ? clsP / 32 : clsP / 64;
     const int64_t fdim = up(dim, 128), fkb = up(classes, 16) / 16;
     // splits of the classes that give every CU eight wavefronts or so, of 16 blocks at least
@@ -1060,7 +1071,8 @@ int head_run(const HeadCall& h) {
             hipLaunchKernelGGL(k_few_x, dim3((unsigned)(nt * dkb)), dim3(64), 0, st, fa);
             const dim3 grid((unsigned)(clsP / 32));
             if (nt == 1) hipLaunchKernelGGL((k_few_logits<1>), grid, dim3(512), 0, st, fa);
-            else hipLaunchKernelGGL((k_few_logits<2>), grid, dim3(512), 0, st, fa);
+            else if (nt == 2) hipLaunchKernelGGL((k_few_logits<2>), grid, dim3(512), 0, st, fa);
+            else hipLaunchKernelGGL((k_few_logits<4>), grid, dim3(512), 0, st, fa);
         } else {
             launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
         }

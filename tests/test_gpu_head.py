@@ -122,9 +122,9 @@ def test_larger_tiles_and_splits():
         check(run(m, x, w, labels), want, bound, str(size))
 
 
-@pytest.mark.parametrize("size", [(1, 513, 9001), (16, 4097, 1031), (32, 1024, 4100), (33, 700, 6007), (64, 2050, 2049), (9, 257, 16390), (9, 48, 100003)], ids=str)
+@pytest.mark.parametrize("size", [(1, 513, 9001), (16, 4097, 1031), (32, 1024, 4100), (33, 700, 6007), (64, 2050, 2049), (65, 1030, 4111), (128, 512, 8200), (9, 257, 16390), (9, 48, 100003)], ids=str)
 def test_few_rows_against_a_large_head(size):
-    """Up to 64 rows: w read as it lies, three bf16 an element, whose products are off by 2^-22 at most."""
+    """Up to 64 rows, 128 forward: w read as it lies, three bf16 an element, whose products are off by 2^-22 at most."""
     m = m_()
     x, w, labels = inputs(*size, seed=21)
     labels[0] = 3
