@@ -290,10 +290,13 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
  *   row_lse = log sum_v exp z_v,  row_loss = row_lse - z_label,  loss = sum row_loss / n
  * (0 without kept rows). A label of classes or more makes the row's loss, the loss and the gradients
  * NaN; so does a kept row or a class that holds a NaN or an infinity. row_loss and row_lse may be null.
- * x and w are each held with 22 bits relative to every element down to 2^-29 of the tensor's largest
- * (of the kept rows for x), which a product needs to be as exact as one of fp32 operands; sums are fp32.
- * (Up to 64 rows, or 128 forward, of 256 dims or more against 2^22 elements of w or more: 24 bits of
- * every element between 2^-110 and 3.38e38.)
+ * x and w are each held with 22 bits of every element down to 2^-17 of the largest, and to 2^-39 of the
+ * largest below: of the tensor's (for x: of the kept rows'), but in the logits of its row's for x, so that no
+ * row's loss depends on another row's size. Sums are fp32. A logit is off by at most
+ *   2^-21 sum |x w| + 2^-39 (max |x_row| sum |w_class| + max |w| sum |x_row|)
+ * and the roundings of its sum, grad_x and grad_w by as much with G in the place of the other operand.
+ * (Up to 64 rows, or 128 forward, of 256 dims or more against 2^22 elements of w or more, the logits and grad_x
+ * have 24 bits of every element between 2^-110 and 3.38e38.)
  * The library's scratch, which it keeps, grows to 4 bytes an element of x and of w, and for the
  * gradients to as much again and 8 bytes a logit of a chunk of rows: 4 GiB, or 256 rows, at most. */
 int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,

@@ -6,13 +6,18 @@
 //
 // Three products of 2 rows classes dim operations carry the time. The matrix instructions take fp32
 // operands at a sixteenth of the fp16 rate, so every fp32 operand is held as two halves (hi, lo):
-// v 2^e = hi + lo + r, |r| <= 2^-23 |v 2^e|, with one power of two e for the whole tensor that puts its
-// largest element into [2^14, 2^15). A product is hi hi + hi lo + lo hi, each exact in the fp32
+// v 2^e = hi + lo + r, |r| <= 2^-23 |v 2^e|, with a power of two e that puts the largest element into
+// [2^14, 2^15). A product is hi hi + hi lo + lo hi, each exact in the fp32
 // accumulator; what is dropped, lo lo, is below 2^-22 of |a b|. That is the error of fp32 operands within
 // a factor of 4 for one term and below the rounding of an fp32 sum from some tens of terms on, at three
-// fp16 instructions a product. Elements below 2^-29 of the tensor's largest lose bits to the halves' least
-// exponent: the absolute error stays below 2^-39 of the largest. G is held the same way with e = 15 (|G| <= 1
-// before the factor ug / n, which the store applies).
+// fp16 instructions a product. fp16's least step, 2^-24, is lo's: elements below 2^-17 of the largest lose bits to
+// it, and their absolute error stays below 2^-39 of the largest. For the logits e is a row's own in x, so that no
+// row's result depends on another's size; a power of two a class of w as well cost 2 % of a forward (a different
+// exponent for each sum at the product's end), and a logit's error, which is absolute, gains nothing from it while
+// |x| |w| stays below 2^17. Both gradients contract over rows or classes: there e is the tensor's. lo times 2^11
+// would hold 22 bits down to 2^-28, but its products need sums of their own, or a second pass over hi: 16.4 -> 18.4 ms
+// a step over [4096, 2048] x [131072, 2048]. G is held the same way with e = 15 (|G| <= 1 before the factor ug / n,
+// which the store applies).
 //
 // Operands lie in panels, the order the matrix instruction wants them: blocks of 32 rows x 16 of the
 // contracted axis, hi then lo, 1 KB each, lane l's 16 bytes being 8 elements of row l % 32 from
@@ -42,7 +47,7 @@ constexpr int kAmaxBlocks = 1024;  // workgroups of k_amax for each of x and w
 
 // What the kernels of one call share, in device memory.
 struct HeadInfo {
-    int32_t ex, ew;  // powers of two of x and w
+    int32_t ex, ew;  // powers of two of all of x and of w
     int32_t kept;    // rows with a label
     int32_t pad;
 };
@@ -69,13 +74,22 @@ __device__ __forceinline__ float finite_abs(float v) {
     return a <= 3.402823466e38f ? a : 0.0f;  // NaN and infinity do not set the scale
 }
 
-// The largest finite magnitude of x's kept rows and of w, and the kept rows' count, as partials.
+// The power of two that puts a into [2^14, 2^15).
+__device__ __forceinline__ int scale_exp(float a) {
+    if (!(a > 0.0f)) return 0;
+    int e;
+    __builtin_frexpf(a, &e);  // a = f 2^e, f in [1/2, 1)
+    return 15 - e;
+}
+
+// The largest finite magnitude of x's kept rows and of w, and the kept rows' count, as partials; each row's power of
+// two.
 __device__ __forceinline__ float amax4(float a, vf4 v) {
     return __builtin_fmaxf(__builtin_fmaxf(a, __builtin_fmaxf(finite_abs(v.x), finite_abs(v.y))),
                            __builtin_fmaxf(finite_abs(v.z), finite_abs(v.w)));
 }
-__global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, const float* w, const int32_t* labels,
-                                              int64_t rows, int64_t dim, int64_t nw) {
+__global__ __launch_bounds__(256) void k_amax(HeadPart* part, int32_t* row_exp, const float* x, const float* w,
+                                              const int32_t* labels, int64_t rows, int64_t dim, int64_t nw) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __shared__ float red[4];
     __shared__ int32_t cnt[4];
@@ -92,17 +106,25 @@ __global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, co
 #pragma unroll
             for (int u = 0; u < 4; ++u) kept += in[u];  // a row left out may hold anything
             const float* row = x + r0 * dim;
+            float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int64_t k = lane * 4; k + 3 < dim; k += 256) {
                 vf4 v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[u] = in[u] ? *reinterpret_cast<const vf4u*>(row + u * dim + k) : vf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int u = 0; u < 4; ++u) a = amax4(a, v[u]);
+                for (int u = 0; u < 4; ++u) m[u] = amax4(m[u], v[u]);
             }
             if (lane < (dim & 3))
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (in[u]) a = __builtin_fmaxf(a, finite_abs(row[u * dim + (dim & ~(int64_t)3) + lane]));
+                    if (in[u]) m[u] = __builtin_fmaxf(m[u], finite_abs(row[u * dim + (dim & ~(int64_t)3) + lane]));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                m[u] = wave_max(m[u]);
+                a = __builtin_fmaxf(a, m[u]);
+            }
+            const float mine = lane == 0 ? m[0] : lane == 1 ? m[1] : lane == 2 ? m[2] : m[3];
+            if (lane < 4 && r0 + lane < rows) row_exp[r0 + lane] = scale_exp(mine);
         }
     } else {
         const int64_t nq = nw >> 2, step = kAmaxBlocks * 256;
@@ -134,14 +156,6 @@ __global__ __launch_bounds__(256) void k_amax(HeadPart* part, const float* x, co
     }
 }
 
-// The power of two that puts a into [2^14, 2^15).
-__device__ __forceinline__ int scale_exp(float a) {
-    if (!(a > 0.0f)) return 0;
-    int e;
-    __builtin_frexpf(a, &e);  // a = f 2^e, f in [1/2, 1)
-    return 15 - e;
-}
-
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ void split8(f32x8 v, half8* hi, half8* lo) {
     *hi = __builtin_convertvector(v, half8);
@@ -155,6 +169,7 @@ constexpr int kSplitTile = 64;
 struct SplitOne {
     const float* src;
     int64_t nr, nc;      // the matrix
+    const int32_t* exps;  // its rows' powers of two, or null: one for all
     char* rowp;          // row blocks of rkb blocks, stride_of(rkb) apart; blocks at or past rkb are not stored
     char* colp;          // the same of ckb
     int64_t rkb, ckb;
@@ -178,6 +193,13 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
     if (lane == 0) red[wave] = a;
     // 16 threads a row, a quad each
     vf4 in[4];
+    int er[2];
+    if (s.exps)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t r = r0 + i * 32 + (lane & 31);
+            er[i] = r < s.nr ? s.exps[r] : 0;
+        }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t r = r0 + i * 16 + (tid >> 4), c = c0 + (tid & 15) * 4;
@@ -197,6 +219,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
     for (int i = 0; i < 4; ++i) *reinterpret_cast<vf4*>(&t[i * 16 + (tid >> 4)][(tid & 15) * 4]) = in[i];
     __syncthreads();
     const int e = scale_exp(__builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3])));
+    if (!s.exps) er[0] = er[1] = e;
     const int r = lane & 31, k8 = (lane >> 5) * 8;
     // 2 row blocks x 4 blocks of the contracted axis each way: 8 blocks, two a wavefront
 #pragma unroll
@@ -206,7 +229,7 @@ __global__ __launch_bounds__(256) void k_split(SplitOne sx, SplitOne sw, const H
         half8 hi, lo;
         if (r0 / 32 + rb < s.rb_end && c0 / 16 + kb < s.rkb) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[rb * 32 + r][kb * 16 + k8 + j], e);
+            for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(t[rb * 32 + r][kb * 16 + k8 + j], er[rb]);
             split8(v, &hi, &lo);
             half8* p = reinterpret_cast<half8*>(s.rowp + ((r0 / 32 + rb) * stride_of(s.rkb) + c0 / 16 + kb) * kBlk);
             p[lane] = hi;
@@ -255,6 +278,7 @@ struct GemmArg {
     // EPI_LOGITS: M is classes, N rows
     const int32_t* labels;   // at the first row of the panel; EPI_GRAD: rows to leave alone, or null
     int64_t rows, classes;   // of the operands; rows counted from the panel's first
+    const int32_t* row_exp;  // the rows' powers of two, of all that the tiles hold
     float* stat;             // [64-class groups][2][stat_ld]: maximum, sum of exponentials
     int64_t stat_ld;
     float* target;           // [rows] the label's logit
@@ -381,7 +405,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmPair pair) {
     // acc[i][j][r]: row (of M) 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4, column (of N) 32 j + lane % 32
     const int half = lane >> 5, col = lane & 31;
     if constexpr (EPI == EPI_LOGITS) {
-        const int e = -(g.info->ex + g.info->ew);
+        int e[NI];
+#pragma unroll
+        for (int j = 0; j < NI; ++j) e[j] = -(g.row_exp[tn * TN + (wn * NI + j) * 32 + col] + g.info->ew);
         const int64_t v0 = tm * TM + wm * MI * 32;  // the wavefront's first class
         // register r of tile i holds class v0 + 4 half + cls_of(i, r): compared with the label and the
         // last class relative to the first two terms
@@ -394,7 +420,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmPair pair) {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], e);
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], e[j]);
             if (g.stat) {
                 const int64_t want = (n < g.rows ? (int64_t)g.labels[n] : -1) - v0 - 4 * half;
                 if (want >= 0 && want < MI * 32) {
@@ -1006,6 +1032,7 @@ int head_run(const HeadCall& h) {
 
     Carve cv;
     const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
+    const size_t o_ex = cv.take(rowsP * 4);
     const size_t o_xr = cv.take(rowsP / 32 * stride_of(dkb) * kBlk),
                  o_wr = few ? 0 : cv.take(clsP / 32 * stride_of(dkb) * kBlk);
     const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
@@ -1034,11 +1061,12 @@ int head_run(const HeadCall& h) {
     double* block_loss = reinterpret_cast<double*>(base + o_rl);
     float* target = reinterpret_cast<float*>(base + o_tgt);
 
-    hipLaunchKernelGGL(k_amax, dim3(few ? kAmaxBlocks : 2 * kAmaxBlocks), dim3(256), 0, st, part, h.x, h.w, h.labels, rows, dim,
-                       classes * dim);
-    SplitOne sx = {h.x, rows, dim, base + o_xr, h.train && h.gw ? base + o_xt : nullptr, dkb, rowsP / 16,
+    int32_t* row_exp = reinterpret_cast<int32_t*>(base + o_ex);
+    hipLaunchKernelGGL(k_amax, dim3(few ? kAmaxBlocks : 2 * kAmaxBlocks), dim3(256), 0, st, part, row_exp, h.x, h.w, h.labels,
+                       rows, dim, classes * dim);
+    SplitOne sx = {h.x, rows, dim, row_exp, base + o_xr, h.train && h.gw ? base + o_xt : nullptr, dkb, rowsP / 16,
                    rowsP / 64, up(dim, 64) / 64, rowsP / 32, dimP / 32};
-    SplitOne sw = {h.w, classes, dim, base + o_wr, h.train && h.gx ? base + o_wt : nullptr, dkb, clsP / 16,
+    SplitOne sw = {h.w, classes, dim, nullptr, base + o_wr, h.train && h.gx ? base + o_wt : nullptr, dkb, clsP / 16,
                    clsP / 64, up(dim, 64) / 64, clsP / 32, dimP / 32};
     if (sx.colp) sx.tiles_c = dimP / 64;
     if (sw.colp) sw.tiles_c = dimP / 64;
@@ -1058,6 +1086,7 @@ int head_run(const HeadCall& h) {
         g.labels = h.labels + r0;
         g.rows = nr;
         g.classes = classes;
+        g.row_exp = row_exp + r0;
         g.stat = h.row_lse_in ? nullptr : reinterpret_cast<float*>(base + o_stat);
         g.stat_ld = chunk;
         g.target = target;
