@@ -302,8 +302,10 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
 int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,
                                 const int32_t* labels, int64_t rows, int64_t dim, int64_t classes);
 /* The gradients from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
- *   G = (exp(z - row_lse) - onehot(label)) ug / n,  grad_x = G w,  grad_w = G^T x.
- * Either gradient may be null. An element of G is exact to 2^-22 of itself or 2^-40 ug / n. */
+ *   G = (softmax(z) - onehot(label)) ug / n,  grad_x = G w,  grad_w = G^T x.
+ * Either gradient may be null. An element of G is held to 2^-22 of itself or 2^-40 ug / n; a probability is off by
+ * what its logit is and by 2^-20 of itself beside, whatever the size of row_lse: the rows' sums are taken again with
+ * the logits, and row_lse says only which rows are NaN. */
 int mh_linear_cross_entropy_bwd(float* grad_x, float* grad_w, const float* x, const float* w, const int32_t* labels,
                                 const float* row_lse, const float* ug, int64_t rows, int64_t dim, int64_t classes,
                                 int accumulate);

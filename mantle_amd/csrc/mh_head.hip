@@ -421,7 +421,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_gemm(GemmPair pair) {
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], e[j]);
-            if (g.stat) {
+            {
                 const int64_t want = (n < g.rows ? (int64_t)g.labels[n] : -1) - v0 - 4 * half;
                 if (want >= 0 && want < MI * 32) {
 #pragma unroll
@@ -533,12 +533,18 @@ __global__ __launch_bounds__(256) void k_join(GemmPair pair, int32_t tile) {
 // ---------------------------------------------------------------------------------------
 // rows' statistics, the loss, and G's panels
 // ---------------------------------------------------------------------------------------
-// Each row's log-sum-exp from its class groups' statistics, and the workgroup's sum of losses: 16 rows x 4 W
+// Each row's maximum and sum of exponentials from its class groups', its log-sum-exp, and the workgroup's sum of
+// losses: 16 rows x 4 W
 // threads, whose loads of a group's statistics are 64 bytes each. W = 16 wavefronts a workgroup, or 4 where the
 // groups are few ([32768, 512] x [1000, 512]'s 16 groups: 17 and 9 us).
 constexpr int kLseRows = 16;
 struct Lse {
     float top, sum;
+};
+// What makes a row's probabilities of its logits: e^(z - top) inv. The log-sum-exp would not do: rounded to fp32
+// it is off by up to 2^-24 of itself, and all of the row's probabilities with it, so that G's rows did not add up to 0.
+struct RowScale {
+    float top, inv;
 };
 // A sum that is not a number stays so; a group of logits at minus infinity adds nothing.
 __device__ __forceinline__ void lse_join(Lse& a, float m, float s) {
@@ -554,7 +560,8 @@ __device__ __forceinline__ void lse_join(Lse& a, float m, float s) {
 template <int W>
 __global__ __launch_bounds__(W * 64) void k_rows_lse(const float* stat, int64_t groups, int64_t stat_ld,
                                                    const float* target, const int32_t* labels, int64_t rows,
-                                                   int64_t classes, float* row_lse, float* row_loss, double* block_loss) {
+                                                   int64_t classes, const float* row_lse_in, float* row_lse,
+                                                   float* row_loss, double* block_loss, RowScale* row_scale) {
     __shared__ float sm[W][kLseRows], ss[W][kLseRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, p = wave * 4 + (lane >> 4);
     const int64_t n = (int64_t)blockIdx.x * kLseRows + r;
@@ -590,9 +597,14 @@ __global__ __launch_bounds__(W * 64) void k_rows_lse(const float* stat, int64_t 
         float lse = a.top + mlog(a.sum);
         if (label >= classes) lse = __builtin_nanf("");  // no such class: shown in the loss and the gradients
         if (label < 0) lse = 0.0f;
-        loss = label < 0 ? 0.0f : (label >= classes ? lse : lse - target[n]);
-        row_lse[n] = lse;
+        // the logits' common offset goes first
+        loss = label < 0 ? 0.0f : label >= classes ? lse : (a.top - target[n]) + mlog(a.sum);
+        if (row_lse) row_lse[n] = lse;
         if (row_loss) row_loss[n] = loss;
+        if (row_scale) {
+            const bool bad = label >= classes || (row_lse_in && row_lse_in[n] != row_lse_in[n]);
+            row_scale[n] = {a.top, bad ? __builtin_nanf("") : 1.0f / a.sum};
+        }
     }
     double total = loss;
 #pragma unroll
@@ -617,7 +629,7 @@ __global__ __launch_bounds__(256) void k_rows_loss(const double* block_loss, int
 // Logits to G's panels: a wavefront takes 32 rows x 32 classes (two blocks of logits, which become two
 // blocks of the row panel in place) and writes the same elements to the column panel through LDS. With `loss`,
 // `tiles` workgroups do that and one more adds up the loss.
-__global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, int64_t gtkb, int64_t gt_blocks, const float* lse,
+__global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, int64_t gtkb, int64_t gt_blocks, const RowScale* scale,
                                               const int32_t* labels, int64_t rows, int64_t classes, int64_t tiles_v,
                                               int64_t tiles, const double* block_loss, int64_t loss_blocks,
                                               const HeadInfo* info, float* loss) {
@@ -632,7 +644,7 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
     const int64_t nb = id / tiles_v, vt = id % tiles_v;  // the grid covers whole workgroups of tiles
     const int64_t n = nb * 32 + (lane & 31);
     const int32_t label = n < rows ? labels[n] : -1;
-    const float l = n < rows ? lse[n] : 0.0f;
+    const RowScale sc = n < rows ? scale[n] : RowScale{0.0f, 0.0f};
     const int k8 = (lane >> 5) * 8;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -642,9 +654,7 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int64_t cls = vt * 32 + b * 16 + k8 + j;
-            // above 0 only by the log-sum-exp's own rounding, which counts where logits are very large
-            const float d = v[j] - l;
-            const float p = exp_neg(d > 0.0f ? 0.0f : d) - (cls == label ? 1.0f : 0.0f);
+            const float p = exp_neg(v[j] - sc.top) * sc.inv - (cls == label ? 1.0f : 0.0f);
             v[j] = label < 0 || cls >= classes ? 0.0f : p * (float)(1 << kGExp);
         }
         half8 hi, lo;
@@ -800,7 +810,7 @@ __global__ __launch_bounds__(512) void k_few_logits(FewArg f) {
                (sums[2][wave][r * 64 + lane] + sums[3][wave][r * 64 + lane]);
     // register r: class v0 + 8 (r / 4) + 4 half + r % 4 of row n, as in k_gemm
     const int64_t n = wave * 32 + col;
-    if (f.stat) {
+    {
         const int64_t left = f.classes - v0 - 4 * half;
         const int64_t want = (n < f.rows ? (int64_t)f.labels[n] : -1) - v0 - 4 * half;
         float top = -__builtin_inff(), sum = 0.0f;
@@ -1037,8 +1047,8 @@ int head_run(const HeadCall& h) {
                  o_wr = few ? 0 : cv.take(clsP / 32 * stride_of(dkb) * kBlk);
     const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
     const size_t o_wt = h.train && h.gx && !few ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
-    const size_t o_stat = h.row_lse_in ? 0 : cv.take(groups * 2 * chunk * 4);
-    const size_t o_tgt = cv.take(chunk * 4), o_lse = cv.take(rowsP * 4), o_rl = cv.take(rowsP / kLseRows * 8);
+    const size_t o_stat = cv.take(groups * 2 * chunk * 4);
+    const size_t o_tgt = cv.take(chunk * 4), o_scale = cv.take(h.train ? chunk * sizeof(RowScale) : 0), o_rl = cv.take(rowsP / kLseRows * 8);
     size_t o_z = 0, o_gt = 0, o_sp = 0;
     if (h.train) {
         o_z = cv.take(chunk / 32 * stride_of(clsP / 16) * kBlk);
@@ -1057,7 +1067,7 @@ int head_run(const HeadCall& h) {
     hipStream_t st = ctx().stream;
     HeadInfo* info = reinterpret_cast<HeadInfo*>(base + o_info);
     HeadPart* part = reinterpret_cast<HeadPart*>(base + o_part);
-    float* lse = h.row_lse_out ? h.row_lse_out : reinterpret_cast<float*>(base + o_lse);
+    RowScale* scale = h.train ? reinterpret_cast<RowScale*>(base + o_scale) : nullptr;
     double* block_loss = reinterpret_cast<double*>(base + o_rl);
     float* target = reinterpret_cast<float*>(base + o_tgt);
 
@@ -1087,7 +1097,7 @@ int head_run(const HeadCall& h) {
         g.rows = nr;
         g.classes = classes;
         g.row_exp = row_exp + r0;
-        g.stat = h.row_lse_in ? nullptr : reinterpret_cast<float*>(base + o_stat);
+        g.stat = reinterpret_cast<float*>(base + o_stat);
         g.stat_ld = chunk;
         g.target = target;
         g.z = h.train ? base + o_z : nullptr;
@@ -1105,22 +1115,21 @@ int head_run(const HeadCall& h) {
         } else {
             launch_gemm<EPI_LOGITS>(&g, 1, f.logits.tile);
         }
-        if (!h.row_lse_in) {
-            const dim3 grid((unsigned)((nr + kLseRows - 1) / kLseRows));
-            float* rl = h.row_loss ? h.row_loss + r0 : nullptr;
-            double* bl = block_loss + r0 / kLseRows;
-            if (groups <= 32)
-                hipLaunchKernelGGL((k_rows_lse<4>), grid, dim3(256), 0, st, g.stat, groups, g.stat_ld, target,
-                                   h.labels + r0, nr, classes, lse + r0, rl, bl);
-            else
-                hipLaunchKernelGGL((k_rows_lse<16>), grid, dim3(1024), 0, st, g.stat, groups, g.stat_ld, target,
-                                   h.labels + r0, nr, classes, lse + r0, rl, bl);
-        }
+        const dim3 lse_grid((unsigned)((nr + kLseRows - 1) / kLseRows));
+        float *lse = h.row_lse_out ? h.row_lse_out + r0 : nullptr, *rl = h.row_loss ? h.row_loss + r0 : nullptr;
+        const float* lse_in = h.row_lse_in ? h.row_lse_in + r0 : nullptr;
+        double* bl = block_loss + r0 / kLseRows;
+        if (groups <= 32)
+            hipLaunchKernelGGL((k_rows_lse<4>), lse_grid, dim3(256), 0, st, g.stat, groups, g.stat_ld, target,
+                               h.labels + r0, nr, classes, lse_in, lse, rl, bl, scale);
+        else
+            hipLaunchKernelGGL((k_rows_lse<16>), lse_grid, dim3(1024), 0, st, g.stat, groups, g.stat_ld, target,
+                               h.labels + r0, nr, classes, lse_in, lse, rl, bl, scale);
         if (!h.train) continue;
         const int64_t tiles_v = clsP / 32, tiles = nrP / 32 * tiles_v / 4;
-        const bool with_loss = !h.row_lse_in && r0 + chunk >= rows;
+        const bool with_loss = h.loss && r0 + chunk >= rows;
         hipLaunchKernelGGL(k_to_g, dim3((unsigned)(tiles + with_loss)), dim3(256), 0, st, base + o_z, zkb,
-                           base + o_gt, gtkb, up(nr, 32) / 32, (h.row_lse_in ? h.row_lse_in : lse) + r0, h.labels + r0, nr,
+                           base + o_gt, gtkb, up(nr, 32) / 32, scale, h.labels + r0, nr,
                            classes, tiles_v, tiles, block_loss, (rows + kLseRows - 1) / kLseRows, info, h.loss);
         GemmArg d[2] = {};
         Form df[2];

@@ -109,3 +109,52 @@ def test_single_outliers(where):
         bound.update(gradient_bounds(want, parts, 2.0 ** -21 + 8 * U * (np.abs(want["z"]) + np.abs(want["row_lse"])[:, None])))
         for how in ("step", "two calls"):
             check(run(m_(), x, w, labels, how=how), want, bound, what=f"{size} {how}")
+
+
+OFFSETS = [((5, 40, 300), 30000.0), ((200, 70, 3000), -1000.0), ((7, 260, 17000), 30000.0), ((70, 300, 14100), 4000.0)]
+
+
+def with_offset(size, offset, seed):
+    """Inputs whose logits all lie near `offset`: a column of ones in x, of the offset in w."""
+    x, w, labels = inputs(*size, seed=seed, left_out=0)
+    x[:, 0], w[:, 0] = 1.0, offset
+    return x, w, labels
+
+
+@pytest.mark.parametrize("size, offset", OFFSETS, ids=str)
+def test_gradient_rows_add_up_to_zero(size, offset):
+    """sum_v G_nv = 0, whatever the log-sum-exp's size: column 0 of grad_x is offset times it. An element of G is off by
+    2^-22 of itself or 2^-40; a row of probabilities by its sums' roundings, those of 1 / sum and the product with it
+    (4 U in all), and by an exponential's, which the sum takes with another instruction: (3 |z - top| + 8) U each. The
+    product has its own bound."""
+    x, w, labels = with_offset(size, offset, 35)
+    want, _, parts = reference(x, w, labels)
+    ag, aw, product = parts[2], parts[4], parts[6]
+    away = want["z"].max(1)[:, None] - want["z"]
+    rows = (want["p"] * (3 * away + 8)).sum(1) * U + (128 + size[2] / 512 + 44) * U
+    tol = 2.0 ** -22 * ag.sum(1) + size[2] * 2.0 ** -40 + rows + ag.sum(1) * product(size[2] + 256)
+    for how in ("step", "two calls"):
+        g = run(m_(), x, w, labels, how=how)["grad_x"][:, 0].astype(np.float64) * size[0] / offset
+        assert (np.abs(g) <= tol).all(), f"{how}: {np.max(np.abs(g) / tol)} of the bound"
+        if size[2] < 1000:  # below what a log-sum-exp rounded to fp32 does; a long product's bound is above that
+            assert (tol < 2.0 ** -24 * abs(offset) / 4).all()
+
+
+@pytest.mark.parametrize("size, offset", OFFSETS, ids=str)
+def test_loss_of_logits_with_an_offset(size, offset):
+    """A row's loss is the difference of two logits, each rounded to U of itself beside its product's error, and a
+    logarithm; nothing of it is rounded at the size of the log-sum-exp. A logit near the offset is a sum of one large
+    product, exact but for its operands' (a power of two times a whole number holds in a half), and small ones."""
+    x, w, labels = with_offset(size, offset, 36)
+    w[:, 0] = np.ldexp(1.0, int(np.log2(abs(offset))))  # exact in one half
+    want, _, parts = reference(x, w, labels)
+    at = np.arange(size[0]), labels
+    small = np.abs(x[:, 1:].astype(np.float64)) @ np.abs(w[:, 1:].astype(np.float64)).T
+    k = size[1]
+    # small products' halves, floors, and the sum's additions at the size of the offset (truncating: 2 U each)
+    bz = small * 2.0 ** -21 + FLOOR * (np.abs(x).max(1)[:, None] * np.abs(w.astype(np.float64)).sum(1)[None]
+                                       + np.abs(w).max() * np.abs(x.astype(np.float64)).sum(1)[:, None]) \
+        + (3 * k / 16 + 2) * 2 * U * np.abs(want["z"])
+    tol = 2 * bz.max(1) + (128 + size[2] / 512 + 48) * U + 4 * U * want["row_loss"]
+    got = run(m_(), x, w, labels, how="two calls")
+    assert (np.abs(got["row_loss"] - want["row_loss"]) <= tol).all()
