@@ -85,8 +85,8 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
             any = any || in;
             bad = bad || (in && c >= a.classes);
             id[i] = in ? c : -1;
-            q[i] = in ? t * a.inv_t : ninf;
-            if (in) best = __builtin_fmaxf(best, t * a.inv_t);
+            q[i] = t;
+            if (in) best = __builtin_fmaxf(best, t);
         }
         any = __any(any);
         bad = __any(bad);
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
             many[s] = 0;
         }
         float mass = 0.0f;
-        for (int i = lane; i < a.k; i += 64) mass += id[i] >= 0 ? exp_neg(q[i] - best) : 0.0f;
+        for (int i = lane; i < a.k; i += 64) mass += id[i] >= 0 ? exp_neg((q[i] - best) * a.inv_t) : 0.0f;
         mass = wave_sum(mass);
         const float lm = mlog(mass), inv = 1.0f / mass;
         wave_sync();
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
                 q[i] = 0.0f;
                 continue;
             }
-            const float x = a.x[r * a.classes + c], u = q[i] - best;
+            const float x = a.x[r * a.classes + c], u = (q[i] - best) * a.inv_t;
             const float v = exp_neg(u) * inv;
             a.ent_x[at + i] = x;
             q[i] = v;
