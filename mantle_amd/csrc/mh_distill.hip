@@ -36,7 +36,8 @@ struct DistillArg {
     int32_t* kept;    // rows with an entry
     uint32_t* tickets;  // their sum so far and the workgroups' arrivals: zero before and after
     int32_t* flag;    // [rows] 0: no entry, 1, 2: an id past the classes
-    float* term;      // [rows] sum of q (log q - x / T)
+    float* term;      // [rows] sum of q (log q - (x - base) / T)
+    float* base;      // [rows] the largest of the entries' logits
     int32_t* ent_id;  // [rows][k] the class of its first entry, -1 at the others
     float* ent_q;     // the class's q
     float* ent_x;     // its logit
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
         if (lane == 0) a.flag[r] = bad ? 2 : any ? 1 : 0;
         if (!any || bad) {
             for (int i = lane; i < a.k; i += 64) a.ent_id[at + i] = -1;
-            if (lane == 0) a.term[r] = 0.0f;
+            if (lane == 0) a.term[r] = a.base[r] = 0.0f;
             continue;
         }
 #pragma unroll
@@ -109,7 +110,9 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
         mass = wave_sum(mass);
         const float lm = mlog(mass), inv = 1.0f / mass;
         wave_sync();
-        float term = 0.0f;
+        // sum q log q, and sum q (x - base) from the lane's own largest logit so far: the logits' common offset stays
+        // out of the sums, where it would be rounded at its own size
+        float term = 0.0f, part = 0.0f, weight = 0.0f, base = ninf;
         for (int i = lane; i < a.k; i += 64) {
             const int32_t c = id[i];
             if (c < 0) {
@@ -120,7 +123,15 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
             const float v = exp_neg(u) * inv;
             a.ent_x[at + i] = x;
             q[i] = v;
-            if (v != 0.0f) term += v * (u - lm - x * a.inv_t);  // 0 log 0 = 0
+            if (v != 0.0f) {  // 0 log 0 = 0
+                term += v * (u - lm);
+                if (x > base) {
+                    part += weight > 0.0f ? weight * (base - x) : 0.0f;
+                    base = x;
+                }
+                weight += v;
+                part += v * (x == ninf ? ninf : x - base);
+            }
             uint32_t s = ((uint32_t)c * 2654435761u) & (uint32_t)(a.slots - 1);
             for (;;) {  // ends: slots are more than entries
                 const int32_t old = atomicCAS(&key[s], -1, c);
@@ -145,8 +156,16 @@ __global__ __launch_bounds__(1024) void k_distill_entries(DistillArg a) {
             a.ent_id[at + i] = mine ? c : -1;
             a.ent_q[at + i] = v;
         }
-        term = wave_sum(term);
-        if (lane == 0) a.term[r] = term;
+        float top = base;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+        if (base > ninf && base < top) part += weight * (base - top);
+        part = wave_sum(part);
+        term = wave_sum(term) - part * a.inv_t;
+        if (lane == 0) {
+            a.term[r] = term;
+            a.base[r] = top > ninf ? top : 0.0f;
+        }
     }
     if (lane == 0) red[wave] = kept;
     __syncthreads();
@@ -252,11 +271,15 @@ __device__ void row_zero(const DistillArg& a, int64_t r, int64_t c0, int64_t c1)
     if ((int64_t)threadIdx.x < c1 - q1) g[q1 + threadIdx.x] = 0.0f;
 }
 
-// A row's loss before T^2 / n, its log-sum-exp, and the marks of a row without entries or with a bad id.
-__device__ __forceinline__ void row_out(const DistillArg& a, int64_t r, int flag, float lse) {
+// A row's loss before T^2 / n, its log-sum-exp, and the marks of a row without entries or with a bad id, from the
+// largest logit and the sum of exponentials below it.
+__device__ __forceinline__ void row_out(const DistillArg& a, int64_t r, int flag, float top, float sum) {
     if (threadIdx.x != 0) return;
-    a.row_loss[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : a.term[r] + lse;  // the q sum to 1
-    if (a.row_lse) a.row_lse[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : lse;
+    const float log_sum = mlog(sum);
+    // the q sum to 1, so what the entries' sum left out comes in whole
+    const float loss = a.term[r] + ((top - a.base[r]) * a.inv_t + log_sum);
+    a.row_loss[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : loss;
+    if (a.row_lse) a.row_lse[r] = flag == 0 ? 0.0f : flag == 2 ? __builtin_nanf("") : top * a.inv_t + log_sum;
 }
 
 // A thread's entries of classes c0..c1: with ACC what the gradient held there is read before the dense part
@@ -338,7 +361,7 @@ __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
     const int tid = threadIdx.x;
     const int flag = a.flag[r];
     if (flag == 0) {
-        row_out(a, r, 0, 0.0f);
+        row_out(a, r, 0, 0.0f, 1.0f);
         if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
         return;
     }
@@ -362,7 +385,7 @@ __global__ __launch_bounds__(W * 64) void k_distill_row(DistillArg a) {
         }
     }
     run = run_join<W>(run, kf, red);
-    row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
+    row_out(a, r, flag, run.top, run.sum);
     if (GRAD) {  // an id past the classes: NaN all over the row
         const Scale<false> s = {kf, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
         const float c = factor_of(a);
@@ -396,7 +419,7 @@ __global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(Distill
     const float ninf = -__builtin_inff();
     const int flag = a.flag[r];
     if (flag == 0) {
-        row_out(a, r, 0, 0.0f);
+        row_out(a, r, 0, 0.0f, 1.0f);
         if (GRAD) row_zero<W, ACC>(a, r, 0, a.classes);
         return;
     }
@@ -434,7 +457,7 @@ __global__ __launch_bounds__(W * 64, NQ > 8 ? 4 : 8) void k_distill_regs(Distill
     }
     last = prob(raw, last);
     sum = block_sum<W>(sum + last, red);
-    row_out(a, r, flag, top * a.inv_t + mlog(sum));
+    row_out(a, r, flag, top, sum);
     if (GRAD) {
         const float c = factor_of(a);
         const Scale<false> s = {kf, base, flag == 2 ? __builtin_nanf("") : 1.0f / sum};
@@ -498,13 +521,13 @@ __global__ __launch_bounds__(W * 64) void k_distill_split(DistillArg a) {
     const int64_t c0 = sp * a.span, c1 = c0 + a.span < a.classes ? c0 + a.span : a.classes;
     const int flag = a.flag[r];
     if (flag == 0) {
-        if (LOSS && sp == 0) row_out(a, r, 0, 0.0f);
+        if (LOSS && sp == 0) row_out(a, r, 0, 0.0f, 1.0f);
         if (GRAD) row_zero<W, ACC>(a, r, c0, c1);
         return;
     }
     if (LOSS) {
         const Run run = join_splits(a, r);
-        if (sp == 0) row_out(a, r, flag, run.top * a.inv_t + mlog(run.sum));
+        if (sp == 0) row_out(a, r, flag, run.top, run.sum);
         if (GRAD) {
             const Scale<false> s = {a.inv_t * kLog2e, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
             row_grad<W, ACC>(a, r, c0, c1, s, factor_of(a));
@@ -590,7 +613,7 @@ int distill_run(const DistillCall& d) {
     const size_t rows_b = ((size_t)d.rows * 4 + 255) & ~(size_t)255, ent_b = ((size_t)d.rows * a.k * 4 + 255) & ~(size_t)255;
     char* base = nullptr;
     MH_TRY(tickets(2 * kTicketStride, &a.tickets));
-    MH_TRY(scratch(256 + 3 * rows_b + 3 * ent_b + (size_t)d.rows * a.splits * 8, reinterpret_cast<void**>(&base)));
+    MH_TRY(scratch(256 + 4 * rows_b + 3 * ent_b + (size_t)d.rows * a.splits * 8, reinterpret_cast<void**>(&base)));
     auto take = [&base](size_t bytes) {
         char* p = base;
         base += bytes;
@@ -599,6 +622,7 @@ int distill_run(const DistillCall& d) {
     a.kept = reinterpret_cast<int32_t*>(take(256));
     a.flag = reinterpret_cast<int32_t*>(take(rows_b));
     a.term = reinterpret_cast<float*>(take(rows_b));
+    a.base = reinterpret_cast<float*>(take(rows_b));
     a.row_loss = reinterpret_cast<float*>(take(rows_b));
     a.ent_id = reinterpret_cast<int32_t*>(take(ent_b));
     a.ent_q = reinterpret_cast<float*>(take(ent_b));

@@ -23,3 +23,30 @@ def test_teacher_rows_of_the_lowest_value(T):
     want, bound = reference(x, ids, alike, T=T)
     for how in ("step", "two calls"):
         check(run(m_(), x, ids, teacher, T=T, how=how), want, bound, how)
+
+
+def with_offset(size, seed, offset=4096.0):
+    """Logits on a grid of 2^-10, and the same with the offset, which fp32 holds exactly."""
+    x, ids, teacher = inputs(*size, seed=seed, left_out=0.0 if size[0] < 4 else 0.1)
+    x = (np.round(x * 1024) / 1024).astype(np.float32)
+    moved = (x + np.float32(offset)).astype(np.float32)
+    assert np.array_equal(moved.astype(np.float64) - offset, x)
+    return x, moved, ids, teacher
+
+
+@pytest.mark.parametrize("offset", [4096.0, -4096.0])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_loss_of_logits_with_an_offset(size, offset):
+    """The loss does not change, nor does its bound: one row at a time, a mean would hide a row's rounding."""
+    x, moved, ids, teacher = with_offset(size, 42, offset)
+    rows = np.flatnonzero((ids >= 0).any(1))[:3]
+    for T in (1.0, 2.5):
+        for r in rows:
+            one = slice(r, r + 1)
+            want, bound = reference(x[one], ids[one], teacher[one], T=T)
+            got = run(m_(), moved[one], ids[one], teacher[one], T=T)
+            off = abs(float(got["loss"]) - want["loss"])
+            assert off <= bound["loss"], (r, T, off, bound["loss"])
+        want, bound = reference(x, ids, teacher, T=T)
+        off = abs(float(run(m_(), moved, ids, teacher, T=T)["loss"]) - want["loss"])
+        assert off <= bound["loss"], (T, off, bound["loss"])
