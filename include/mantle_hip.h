@@ -327,7 +327,8 @@ int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, flo
 int mh_distill_fwd(float* loss, float* row_lse, const float* x, const int32_t* ids, const float* teacher, int64_t rows,
                    int64_t classes, int64_t k, float temperature);
 /* The gradient from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
- * grad_x = ug T / n (p - q at the entries' classes). */
+ * grad_x = ug T / n (p - q at the entries' classes). p carries row_lse's rounding to fp32, 2^-19 of itself at most:
+ * a row whose row_lse lies beyond +-64 is read twice, for its sums and for its gradient. */
 int mh_distill_bwd(float* grad_x, const float* x, const int32_t* ids, const float* teacher, const float* row_lse,
                    const float* ug, int64_t rows, int64_t classes, int64_t k, float temperature, int accumulate);
 /* Both at once, for a training step whose ug is known before: the logits are read once, or while the

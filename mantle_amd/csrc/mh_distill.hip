@@ -234,8 +234,7 @@ __device__ __forceinline__ Run run_join(Run r, float kf, float* red) {
 }
 
 // A logit's probability from the row's maximum and sum, p = e^((x - top) / T) / sum, or from its log-sum-exp,
-// p = e^(x / T - lse) with x / T - lse rounded once: where the logits are so large that the log-sum-exp's own
-// rounding counts, the difference is held at 0, so that p stays below 1.
+// p = e^(x / T - lse) with x / T - lse rounded once, above 0 only by the log-sum-exp's rounding.
 template <bool LSE>
 struct Scale {
     float f, from, inv;  // 1 / T, lse; or log2(e) / T, top, 1 / sum
@@ -512,6 +511,10 @@ __device__ __forceinline__ Run join_splits(const DistillArg& a, int64_t r) {
     return {top, sum};
 }
 
+// The forward's log-sum-exp, rounded to fp32, scales a row's probabilities by its rounding: 2^-19 up to 64. Above,
+// where an offset common to a row's logits is most of it, the backward alone takes the row's statistics again.
+constexpr float kTrustedLse = 64.0f;
+
 // A split of a row's gradient, from the forward's log-sum-exp (LOSS off) or the splits' statistics, of which the
 // first split also writes the row's loss. GRAD off: the loss alone, a workgroup a row.
 template <int W, bool LOSS, bool GRAD, bool ACC>
@@ -532,8 +535,15 @@ __global__ __launch_bounds__(W * 64) void k_distill_split(DistillArg a) {
             const Scale<false> s = {a.inv_t * kLog2e, run.top, flag == 2 ? __builtin_nanf("") : 1.0f / run.sum};
             row_grad<W, ACC>(a, r, c0, c1, s, factor_of(a));
         }
+    } else if (const float lse = a.lse_in[r]; __builtin_fabsf(lse) > kTrustedLse && flag != 2) {
+        __shared__ float red[W];
+        const float kf = a.inv_t * kLog2e;
+        Run run = {-__builtin_inff(), 0.0f};
+        run_row<W>(run, a.x + r * a.classes, 0, a.classes, kf);
+        run = run_join<W>(run, kf, red);
+        row_grad<W, ACC>(a, r, c0, c1, Scale<false>{kf, run.top, 1.0f / run.sum}, factor_of(a));
     } else {
-        const Scale<true> s = {a.inv_t, flag == 2 ? __builtin_nanf("") : a.lse_in[r], 1.0f};
+        const Scale<true> s = {a.inv_t, flag == 2 ? __builtin_nanf("") : lse, 1.0f};
         row_grad<W, ACC>(a, r, c0, c1, s, factor_of(a));
     }
 }

@@ -50,3 +50,30 @@ def test_loss_of_logits_with_an_offset(size, offset):
         want, bound = reference(x, ids, teacher, T=T)
         off = abs(float(run(m_(), moved, ids, teacher, T=T)["loss"]) - want["loss"])
         assert off <= bound["loss"], (T, off, bound["loss"])
+
+
+@pytest.mark.parametrize("how", ["step", "two calls"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_gradient_of_logits_with_an_offset(size, how):
+    """Neither the gradient nor its bound changes, in the backward alone as in the step, accumulated too."""
+    for offset in (4096.0, -4096.0):
+        x, moved, ids, teacher = with_offset(size, 43, offset)
+        g = np.random.RandomState(0).standard_normal(x.shape).astype(np.float32)
+        for T in (1.0, 2.5):
+            want, bound = reference(x, ids, teacher, T=T)
+            got = run(m_(), moved, ids, teacher, T=T, how=how)["grad_x"]
+            check({"grad_x": got}, want, bound, f"{how} {offset} {T}")
+            assert np.array_equal(run(m_(), moved, ids, teacher, T=T, how=how, grad=g)["grad_x"], g + got)
+
+
+@pytest.mark.parametrize("T", [0.5, 1.0])
+@pytest.mark.parametrize("size", [(3, 500, 4), (2, 40001, 9), (3, 131072, 5), (300, 70001, 6)], ids=str)
+def test_rows_all_at_the_lowest_value(size, T):
+    """A student whose logits are all the type's lowest value has every class at 1 / classes."""
+    x, ids, teacher = inputs(*size, seed=44, left_out=0)
+    x[1] = 0.0
+    want, bound = reference(x, ids, teacher, T=T)
+    x[1] = LOWEST
+    for how in ("step", "two calls"):
+        got = run(m_(), x, ids, teacher, T=T, how=how)
+        check({"grad_x": got["grad_x"], "loss": got["loss"]}, want, bound, how)
