@@ -45,7 +45,7 @@ class Collection:
         if isinstance(value, Tensor):
             if value.num_elements() != n:
                 raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{value.num_elements()} elements for a slot of {n}")
-            _lib.call("mh_memcpy_d2d", dst, value.ptr, n * 4)
+            _lib.call("mh_memcpy_d2d", dst, value.f32, n * 4)
         else:
             a = np.ascontiguousarray(value, dtype=np.float32)
             if a.size != n:
@@ -115,7 +115,7 @@ class Model:
             n = t.num_elements() if isinstance(t, Tensor) else t.size
             if n != s.shape.num_elements():
                 raise _lib.MantleHipError(_lib.ERR_SHAPE, f"{n} elements for {s}")
-        ptrs = [t.ptr if isinstance(t, Tensor) else t.ctypes.data for t in keep]
+        ptrs = [t.f32 if isinstance(t, Tensor) else t.ctypes.data for t in keep]
         tab = (ctypes.c_void_p * len(ptrs))(*ptrs)
         return tab, (_lib.FROM_DEVICE if all(on_dev) else _lib.FROM_HOST), keep
 

@@ -83,12 +83,12 @@ def get_reduce_shape(t, axis: int) -> TensorShape:
 
 
 def fill(t: Tensor, val: float) -> None:
-    _lib.call("mh_fill", t.ptr, float(val), t.num_elements())
+    _lib.call("mh_fill", t.f32, float(val), t.num_elements())
 
 
 def elwise_transform(op: int, res: Tensor, t: Tensor) -> None:
     """elwise_transform, tensorutils.mojo:181-200, with op in EXP/LOG/SIGMOID/RELU/TANH."""
-    _lib.call("mh_unary_fwd", int(op), res.ptr, t.ptr, t.num_elements())
+    _lib.call("mh_unary_fwd", int(op), res.f32, t.f32, t.num_elements())
 
 
 def elwise_pow(res: Tensor, t: Tensor, n: int) -> None:
@@ -97,24 +97,24 @@ def elwise_pow(res: Tensor, t: Tensor, n: int) -> None:
     n = int(n)
     if not -(1 << 31) <= n < (1 << 31):
         raise ValueError(f"elwise_pow: exponent {n} outside int32")
-    _lib.call("mh_powi_fwd", res.ptr, t.ptr, n, t.num_elements())
+    _lib.call("mh_powi_fwd", res.f32, t.f32, n, t.num_elements())
 
 
 def elwise_op(op: int, res: Tensor, t1: Tensor, t2: Tensor) -> None:
     """elwise_op dispatcher, tensorutils.mojo:242-357."""
-    _lib.call("mh_binary_fwd", int(op), res.ptr, res.shape().c(), t1.ptr, t1.shape().c(), t2.ptr,
+    _lib.call("mh_binary_fwd", int(op), res.f32, res.shape().c(), t1.f32, t1.shape().c(), t2.f32,
               t2.shape().c())
 
 
 def accumulate_grad(grad: Tensor, res_grad: Tensor) -> None:
     """accumulate_grad, tensorutils.mojo:442-487 (same shape, scalar or un-broadcast)."""
-    _lib.call("mh_accumulate_grad", grad.ptr, grad.shape().c(), res_grad.ptr, res_grad.shape().c())
+    _lib.call("mh_accumulate_grad", grad.f32, grad.shape().c(), res_grad.f32, res_grad.shape().c())
 
 
 def _reduce(op: int, t: Tensor, axis: int, res: Optional[Tensor]) -> Tensor:
     if res is None:
         res = Tensor(TensorShape(1) if axis < 0 else get_reduce_shape(t.shape(), axis))
-    _lib.call("mh_reduce_fwd", int(op), res.ptr, t.ptr, t.shape().c(), int(axis))
+    _lib.call("mh_reduce_fwd", int(op), res.f32, t.f32, t.shape().c(), int(axis))
     return res
 
 
@@ -135,7 +135,7 @@ def tstd(t: Tensor, axis: int = -1, res: Optional[Tensor] = None) -> Tensor:
     population standard deviation. Each output reads the line tmean reads."""
     if res is None:
         res = Tensor(TensorShape(1) if axis < 0 else get_reduce_shape(t.shape(), axis))
-    _lib.call("mh_tstd", res.ptr, t.ptr, t.shape().c(), int(axis))
+    _lib.call("mh_tstd", res.f32, t.f32, t.shape().c(), int(axis))
     return res
 
 
@@ -212,7 +212,7 @@ class POW:
 
     @staticmethod
     def forward(res: Tensor, t1: Tensor, t2: Tensor) -> None:
-        _lib.call("mh_pow_fwd", res.ptr, t1.ptr, t1.num_elements(), t2.ptr)
+        _lib.call("mh_pow_fwd", res.f32, t1.f32, t1.num_elements(), t2.f32)
 
 
 class _Reduce:
@@ -252,7 +252,7 @@ class FMA:
     def forward(res: Tensor, t1: Tensor, t2: Tensor, t3: Tensor) -> None:
         if not (t1.shape() == t2.shape() == t3.shape() == res.shape()):
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "FMA needs four equal shapes")
-        _lib.call("mh_fma_fwd", res.ptr, t1.ptr, t2.ptr, t3.ptr, t1.num_elements())
+        _lib.call("mh_fma_fwd", res.f32, t1.f32, t2.f32, t3.f32, t1.num_elements())
 
 
 class LEAKYRELU:
@@ -272,7 +272,7 @@ class LEAKYRELU:
 
     @classmethod
     def forward(cls, res: Tensor, t1: Tensor, attributes=None) -> None:
-        _lib.call("mh_leakyrelu_fwd", res.ptr, t1.ptr, t1.num_elements(), cls.slope(attributes))
+        _lib.call("mh_leakyrelu_fwd", res.f32, t1.f32, t1.num_elements(), cls.slope(attributes))
 
 
 class CLIP:
@@ -292,7 +292,7 @@ class CLIP:
     @classmethod
     def forward(cls, res: Tensor, t1: Tensor, attributes=None) -> None:
         lo, hi = cls.bounds(attributes)
-        _lib.call("mh_clip_fwd", res.ptr, t1.ptr, t1.num_elements(), lo, hi)
+        _lib.call("mh_clip_fwd", res.f32, t1.f32, t1.num_elements(), lo, hi)
 
 
 STRUCTS = {OP.ADD: ADD, OP.SUB: SUB, OP.MUL: MUL, OP.DIV: DIV, OP.EXP: EXP, OP.LOG: LOG,
@@ -346,32 +346,32 @@ def backward_op(tensor_id: int, op: int, ug: Tensor, t1: Tensor, t2: Optional[Te
     if op == OP.FMA:
         if t2 is None or not (ug.shape() == t1.shape() == t2.shape() == grad.shape()):
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "FMA backward needs equal shapes")
-        _lib.call("mh_fma_bwd_accum", int(tensor_id), grad.ptr, ug.ptr, t1.ptr, t2.ptr, t1.num_elements())
+        _lib.call("mh_fma_bwd_accum", int(tensor_id), grad.f32, ug.f32, t1.f32, t2.f32, t1.num_elements())
     elif op in ATTR_UNARY:
         if ug.shape() != t1.shape() or grad.shape() != t1.shape():
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "ug / grad shape differs from the operand shape")
         if op == OP.LEAKYRELU:
-            _lib.call("mh_leakyrelu_bwd_accum", grad.ptr, t1.ptr, ug.ptr, t1.num_elements(),
+            _lib.call("mh_leakyrelu_bwd_accum", grad.f32, t1.f32, ug.f32, t1.num_elements(),
                       LEAKYRELU.slope(attributes))
         else:
             lo, hi = CLIP.bounds(attributes)
-            _lib.call("mh_clip_bwd_accum", grad.ptr, t1.ptr, ug.ptr, t1.num_elements(), lo, hi)
+            _lib.call("mh_clip_bwd_accum", grad.f32, t1.f32, ug.f32, t1.num_elements(), lo, hi)
     elif op in BINARY:
-        _lib.call("mh_binary_bwd_accum", int(op), int(tensor_id), grad.ptr, grad.shape().c(), ug.ptr,
-                  ug.shape().c(), t1.ptr, t1.shape().c(), t2.ptr, t2.shape().c())
+        _lib.call("mh_binary_bwd_accum", int(op), int(tensor_id), grad.f32, grad.shape().c(), ug.f32,
+                  ug.shape().c(), t1.f32, t1.shape().c(), t2.f32, t2.shape().c())
     elif op == OP.POW:
         if t2.num_elements() != 1 or t2.shape() != TensorShape(1):
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "POW exponent must be a shape-(1) graph scalar")
-        _lib.call("mh_pow_bwd_accum", int(tensor_id), grad.ptr, t1.ptr, t2.ptr, ug.ptr, t1.num_elements())
+        _lib.call("mh_pow_bwd_accum", int(tensor_id), grad.f32, t1.f32, t2.f32, ug.f32, t1.num_elements())
     elif op in UNARY:
         if ug.shape() != t1.shape():
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "ug shape differs from the operand shape")
-        _lib.call("mh_unary_bwd_accum", int(op), grad.ptr, t1.ptr, ug.ptr, t1.num_elements())
+        _lib.call("mh_unary_bwd_accum", int(op), grad.f32, t1.f32, ug.f32, t1.num_elements())
     elif op in REDUCE:
         ax = _axis(attributes)
         if ug.shape() != _Reduce.result_shape(t1.shape(), attributes):
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "ug shape is not the reduced shape")
-        _lib.call("mh_reduce_bwd_accum", int(op), grad.ptr, t1.ptr, t1.shape().c(), ug.ptr, ax)
+        _lib.call("mh_reduce_bwd_accum", int(op), grad.f32, t1.f32, t1.shape().c(), ug.f32, ax)
     else:
         raise _lib.MantleHipError(_lib.ERR_OP, f"Operator {op} not found.")
 
@@ -386,8 +386,8 @@ def backward_op_both(op: int, ug: Tensor, t1: Tensor, t2: Tensor, grad1: Optiona
     if op == OP.POW:
         if t2.shape() != TensorShape(1) or ug.shape() != t1.shape():
             raise _lib.MantleHipError(_lib.ERR_SHAPE, "POW exponent must be a shape-(1) graph scalar")
-        _lib.call("mh_pow_bwd_accum2", grad1.ptr if grad1 is not None else None,
-                  grad2.ptr if grad2 is not None else None, t1.ptr, t2.ptr, ug.ptr, t1.num_elements())
+        _lib.call("mh_pow_bwd_accum2", grad1.f32 if grad1 is not None else None,
+                  grad2.f32 if grad2 is not None else None, t1.f32, t2.f32, ug.f32, t1.num_elements())
         return
     if t1.shape() != t2.shape() or ug.shape() != t1.shape():
         if grad1 is not None:
@@ -395,8 +395,8 @@ def backward_op_both(op: int, ug: Tensor, t1: Tensor, t2: Tensor, grad1: Optiona
         if grad2 is not None:
             backward_op(1, op, ug, t1, t2, grad2)
         return
-    _lib.call("mh_binary_bwd_accum2", int(op), grad1.ptr if grad1 is not None else None,
-              grad2.ptr if grad2 is not None else None, ug.ptr, t1.ptr, t2.ptr, t1.shape().c())
+    _lib.call("mh_binary_bwd_accum2", int(op), grad1.f32 if grad1 is not None else None,
+              grad2.f32 if grad2 is not None else None, ug.f32, t1.f32, t2.f32, t1.shape().c())
 
 
 # ---------------------------------------------------------------------------------------
@@ -404,16 +404,16 @@ def backward_op_both(op: int, ug: Tensor, t1: Tensor, t2: Tensor, grad1: Optiona
 # ---------------------------------------------------------------------------------------
 def bias_relu_forward(y: Tensor, r: Tensor, x: Tensor, bias: Tensor) -> None:
     """The graph ADD(x, bias) -> RELU in one pass: y = x + bias (broadcast), r = relu(y)."""
-    _lib.call("mh_bias_relu_fwd", y.ptr, r.ptr, x.ptr, x.shape().c(), bias.ptr, bias.shape().c())
+    _lib.call("mh_bias_relu_fwd", y.f32, r.f32, x.f32, x.shape().c(), bias.f32, bias.shape().c())
 
 
 def bias_relu_backward(ug: Tensor, y: Tensor, bias_shape, grad_x: Optional[Tensor], grad_bias: Optional[Tensor],
                        grad_y: Optional[Tensor] = None) -> None:
     """Backward of ADD(x, bias) -> RELU from the grad ug of r: grad_y (if kept) += relu'(y) * ug,
     then grad_x += grad_y and grad_bias += its sum over the broadcast axes of bias_shape."""
-    _lib.call("mh_bias_relu_bwd_accum", grad_y.ptr if grad_y is not None else None,
-              grad_x.ptr if grad_x is not None else None, grad_bias.ptr if grad_bias is not None else None,
-              y.ptr, ug.ptr, y.shape().c(), as_shape(bias_shape).c())
+    _lib.call("mh_bias_relu_bwd_accum", grad_y.f32 if grad_y is not None else None,
+              grad_x.f32 if grad_x is not None else None, grad_bias.f32 if grad_bias is not None else None,
+              y.f32, ug.f32, y.shape().c(), as_shape(bias_shape).c())
 
 
 def softmax_log_mul_mean_forward(loss: Tensor, x: Tensor, target: Tensor) -> None:
@@ -421,13 +421,13 @@ def softmax_log_mul_mean_forward(loss: Tensor, x: Tensor, target: Tensor) -> Non
     x [rows, classes] in one pass (Softmax, mantle/nn/activations.mojo:74-87, then LOG, MUL,
     MEAN): loss[0] = mean(log(softmax(x)) * target)."""
     rows, classes = _row_operands(x, same=(("target", target),), scalar=(("loss", loss),))
-    _lib.call("mh_softmax_log_mul_mean_fwd", loss.ptr, x.ptr, target.ptr, rows, classes)
+    _lib.call("mh_softmax_log_mul_mean_fwd", loss.f32, x.f32, target.f32, rows, classes)
 
 
 def softmax_log_mul_mean_backward(grad_x: Tensor, x: Tensor, target: Tensor, ug: Tensor) -> None:
     """Backward of the same graph from the loss grad ug (shape (1)): grad_x += d loss / dx."""
     rows, classes = _row_operands(x, same=(("grad_x", grad_x), ("target", target)), scalar=(("ug", ug),))
-    _lib.call("mh_softmax_log_mul_mean_bwd_accum", grad_x.ptr, x.ptr, target.ptr, ug.ptr, rows, classes)
+    _lib.call("mh_softmax_log_mul_mean_bwd_accum", grad_x.f32, x.f32, target.f32, ug.f32, rows, classes)
 
 
 def _rows_classes(t: Tensor):
@@ -455,37 +455,37 @@ def _row_operands(x: Tensor, same=(), scalar=()):
 def softmax_forward(out: Tensor, x: Tensor) -> None:
     """Softmax over the last axis (activations.mojo:74-87), one fused pass."""
     r, k = _row_operands(x, same=(("out", out),))
-    _lib.call("mh_softmax_fwd", out.ptr, x.ptr, r, k)
+    _lib.call("mh_softmax_fwd", out.f32, x.f32, r, k)
 
 
 def softmax_backward(grad_x: Tensor, x: Tensor, grad_out: Tensor) -> None:
     """grad_x += the five Softmax backward nodes' contribution from grad_out."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("grad_out", grad_out)))
-    _lib.call("mh_softmax_bwd_accum", grad_x.ptr, x.ptr, grad_out.ptr, r, k)
+    _lib.call("mh_softmax_bwd_accum", grad_x.f32, x.f32, grad_out.f32, r, k)
 
 
 def logsoftmax_forward(out: Tensor, x: Tensor) -> None:
     """LogSoftmax over the last axis (activations.mojo:94-108), one fused pass."""
     r, k = _row_operands(x, same=(("out", out),))
-    _lib.call("mh_logsoftmax_fwd", out.ptr, x.ptr, r, k)
+    _lib.call("mh_logsoftmax_fwd", out.f32, x.f32, r, k)
 
 
 def logsoftmax_backward(grad_x: Tensor, x: Tensor, grad_out: Tensor) -> None:
     """grad_x += the six LogSoftmax backward nodes' contribution from grad_out."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("grad_out", grad_out)))
-    _lib.call("mh_logsoftmax_bwd_accum", grad_x.ptr, x.ptr, grad_out.ptr, r, k)
+    _lib.call("mh_logsoftmax_bwd_accum", grad_x.f32, x.f32, grad_out.f32, r, k)
 
 
 def cross_entropy_forward(loss: Tensor, x: Tensor, target: Tensor) -> None:
     """CrossEntropyLoss (loss.mojo:45-61) of x [rows, classes] against target, one fused pass."""
     r, k = _row_operands(x, same=(("target", target),), scalar=(("loss", loss),))
-    _lib.call("mh_cross_entropy_fwd", loss.ptr, x.ptr, target.ptr, r, k)
+    _lib.call("mh_cross_entropy_fwd", loss.f32, x.f32, target.f32, r, k)
 
 
 def cross_entropy_backward(grad_x: Tensor, x: Tensor, target: Tensor, ug: Tensor) -> None:
     """grad_x += d loss / dx of CrossEntropyLoss from the loss grad ug (one element)."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("target", target)), scalar=(("ug", ug),))
-    _lib.call("mh_cross_entropy_bwd_accum", grad_x.ptr, x.ptr, target.ptr, ug.ptr, r, k)
+    _lib.call("mh_cross_entropy_bwd_accum", grad_x.f32, x.f32, target.f32, ug.f32, r, k)
 
 
 # ---------------------------------------------------------------------------------------

@@ -50,6 +50,7 @@ class Adam:
         for p, g in self.params:
             if p.shape() != g.shape():
                 raise _lib.MantleHipError(_lib.ERR_SHAPE, "a parameter and its gradient differ in shape")
+            p.f32, g.f32  # neither holds whole numbers
         self.lr, self.beta1, self.beta2, self.epsilon = float(lr), float(beta1), float(beta2), float(epsilon)
         self.iter = 0
         # allocate_rms_and_momentum (optim.mojo:142-149): zero-initialised, one per parameter;
@@ -93,9 +94,9 @@ class Adam:
         made = (self.params, list(self.momentum_grads), list(self.rms_grads))
         if self._tables is None or self._tables[0] != made:
             VP = ctypes.c_void_p * n
-            self._tables = ((list(made[0]), made[1], made[2]), VP(*[p.ptr for p, _ in self.params]),
-                            VP(*[g.ptr for _, g in self.params]), VP(*[t.ptr for t in self.momentum_grads]),
-                            VP(*[t.ptr for t in self.rms_grads]),
+            self._tables = ((list(made[0]), made[1], made[2]), VP(*[p.f32 for p, _ in self.params]),
+                            VP(*[g.f32 for _, g in self.params]), VP(*[t.f32 for t in self.momentum_grads]),
+                            VP(*[t.f32 for t in self.rms_grads]),
                             (ctypes.c_int64 * n)(*[p.num_elements() for p, _ in self.params]))
         _, ps, gs, ms, vs, sizes = self._tables
         _lib.call("mh_adam_step_multi", n, ps, gs, ms, vs, sizes, self.lr, self.beta1, self.beta2, self.epsilon,

@@ -166,6 +166,11 @@ class Tensor:
     def ptr(self) -> int:
         return self._ptr
 
+    @property
+    def f32(self) -> int:
+        """The address, for a call that takes floats there."""
+        return self._ptr
+
     # ---- host transfer ----
     @staticmethod
     def from_numpy(a) -> "Tensor":
@@ -208,9 +213,14 @@ class Tensor:
 
 class IndexTensor(Tensor):
     """int32 tensor in device memory: class labels, chosen ids and counts. The reference holds these
-    as one-hot float tensors (loss.mojo:45-61), which a large vocabulary rules out."""
+    as one-hot float tensors (loss.mojo:45-61), which a large vocabulary rules out. The calls that take floats
+    refuse it."""
 
     __slots__ = ()
+
+    @property
+    def f32(self) -> int:
+        raise _lib.MantleHipError(_lib.ERR_INVALID, f"{self} holds whole numbers where the call takes floats")
 
     @staticmethod
     def from_numpy(a) -> "IndexTensor":
