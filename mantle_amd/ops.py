@@ -421,13 +421,13 @@ def softmax_log_mul_mean_forward(loss: Tensor, x: Tensor, target: Tensor) -> Non
     x [rows, classes] in one pass (Softmax, mantle/nn/activations.mojo:74-87, then LOG, MUL,
     MEAN): loss[0] = mean(log(softmax(x)) * target)."""
     rows, classes = _row_operands(x, same=(("target", target),), scalar=(("loss", loss),))
-    _lib.call("mh_softmax_log_mul_mean_fwd", loss.f32, x.f32, target.f32, rows, classes)
+    _lib.call("mh_softmax_log_mul_mean_fwd", loss.ptr, x.ptr, target.ptr, rows, classes)
 
 
 def softmax_log_mul_mean_backward(grad_x: Tensor, x: Tensor, target: Tensor, ug: Tensor) -> None:
     """Backward of the same graph from the loss grad ug (shape (1)): grad_x += d loss / dx."""
     rows, classes = _row_operands(x, same=(("grad_x", grad_x), ("target", target)), scalar=(("ug", ug),))
-    _lib.call("mh_softmax_log_mul_mean_bwd_accum", grad_x.f32, x.f32, target.f32, ug.f32, rows, classes)
+    _lib.call("mh_softmax_log_mul_mean_bwd_accum", grad_x.ptr, x.ptr, target.ptr, ug.ptr, rows, classes)
 
 
 def _rows_classes(t: Tensor):
@@ -441,6 +441,9 @@ def _row_operands(x: Tensor, same=(), scalar=()):
     one element. The C entry points take bare pointers and sizes, so a smaller tensor would
     reach the kernel as an out-of-bounds access; the check runs before any launch."""
     xs = x.shape()
+    for t in (x, *(t for _, t in same), *(t for _, t in scalar)):
+        if isinstance(t, IndexTensor):
+            t.f32  # refuses
     for name, t in same:
         if t is None or t.shape() != xs:
             got = None if t is None else t.shape()
@@ -455,37 +458,37 @@ def _row_operands(x: Tensor, same=(), scalar=()):
 def softmax_forward(out: Tensor, x: Tensor) -> None:
     """Softmax over the last axis (activations.mojo:74-87), one fused pass."""
     r, k = _row_operands(x, same=(("out", out),))
-    _lib.call("mh_softmax_fwd", out.f32, x.f32, r, k)
+    _lib.call("mh_softmax_fwd", out.ptr, x.ptr, r, k)
 
 
 def softmax_backward(grad_x: Tensor, x: Tensor, grad_out: Tensor) -> None:
     """grad_x += the five Softmax backward nodes' contribution from grad_out."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("grad_out", grad_out)))
-    _lib.call("mh_softmax_bwd_accum", grad_x.f32, x.f32, grad_out.f32, r, k)
+    _lib.call("mh_softmax_bwd_accum", grad_x.ptr, x.ptr, grad_out.ptr, r, k)
 
 
 def logsoftmax_forward(out: Tensor, x: Tensor) -> None:
     """LogSoftmax over the last axis (activations.mojo:94-108), one fused pass."""
     r, k = _row_operands(x, same=(("out", out),))
-    _lib.call("mh_logsoftmax_fwd", out.f32, x.f32, r, k)
+    _lib.call("mh_logsoftmax_fwd", out.ptr, x.ptr, r, k)
 
 
 def logsoftmax_backward(grad_x: Tensor, x: Tensor, grad_out: Tensor) -> None:
     """grad_x += the six LogSoftmax backward nodes' contribution from grad_out."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("grad_out", grad_out)))
-    _lib.call("mh_logsoftmax_bwd_accum", grad_x.f32, x.f32, grad_out.f32, r, k)
+    _lib.call("mh_logsoftmax_bwd_accum", grad_x.ptr, x.ptr, grad_out.ptr, r, k)
 
 
 def cross_entropy_forward(loss: Tensor, x: Tensor, target: Tensor) -> None:
     """CrossEntropyLoss (loss.mojo:45-61) of x [rows, classes] against target, one fused pass."""
     r, k = _row_operands(x, same=(("target", target),), scalar=(("loss", loss),))
-    _lib.call("mh_cross_entropy_fwd", loss.f32, x.f32, target.f32, r, k)
+    _lib.call("mh_cross_entropy_fwd", loss.ptr, x.ptr, target.ptr, r, k)
 
 
 def cross_entropy_backward(grad_x: Tensor, x: Tensor, target: Tensor, ug: Tensor) -> None:
     """grad_x += d loss / dx of CrossEntropyLoss from the loss grad ug (one element)."""
     r, k = _row_operands(x, same=(("grad_x", grad_x), ("target", target)), scalar=(("ug", ug),))
-    _lib.call("mh_cross_entropy_bwd_accum", grad_x.f32, x.f32, target.f32, ug.f32, r, k)
+    _lib.call("mh_cross_entropy_bwd_accum", grad_x.ptr, x.ptr, target.ptr, ug.ptr, r, k)
 
 
 # ---------------------------------------------------------------------------------------
