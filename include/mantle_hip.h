@@ -492,6 +492,8 @@ int mh_event_create(void** ev);
 int mh_event_destroy(void* ev);
 int mh_event_record(void* ev);
 int mh_event_elapsed_ms(float* ms, void* start, void* stop);
+/* *done: whether what was queued before the event's record has ended; with wait != 0 it waits for that. */
+int mh_event_done(void* ev, int wait, int* done);
 
 /* ---- diagnostics ---- */
 

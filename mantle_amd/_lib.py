@@ -148,6 +148,7 @@ SIGNATURES = {
     "mh_event_destroy": [_VP],
     "mh_event_record": [_VP],
     "mh_event_elapsed_ms": [ctypes.POINTER(_F), _VP, _VP],
+    "mh_event_done": [_VP, _I, ctypes.POINTER(ctypes.c_int)],
     "mh_graph_create": [ctypes.POINTER(_VP)],
     "mh_graph_destroy": [_VP],
     "mh_graph_input": [_VP, _S, _I, ctypes.POINTER(ctypes.c_int32)],

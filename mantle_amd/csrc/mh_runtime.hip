@@ -680,6 +680,23 @@ int mh_event_elapsed_ms(float* ms, void* start, void* stop) {
     return MH_OK;
 }
 
+int mh_event_done(void* ev, int wait, int* done) {
+    if (!ev || !done) return fail(MH_ERR_NULL, "mh_event_done: null");
+    *done = 0;
+    if (wait) {
+        MH_HIP(hipEventSynchronize((hipEvent_t)ev));
+    } else {
+        const hipError_t e = hipEventQuery((hipEvent_t)ev);
+        if (e == hipErrorNotReady) {
+            (void)hipGetLastError();  // no error, and none for the next call's launch check
+            return MH_OK;
+        }
+        MH_TRY(hip_check(e, "hipEventQuery"));
+    }
+    *done = 1;
+    return MH_OK;
+}
+
 int mh_plan_binary(const mh_shape* psres, const mh_shape* psa, const mh_shape* psb, mh_plan_info* out) {
     MH_SHAPE_ARG(sres);
     MH_SHAPE_ARG(sa);

@@ -8,7 +8,9 @@ tensor.mojo:250-302). Here the storage is HBM on the initialised gfx950 device
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+from collections import deque
 from typing import Iterable, Optional, Tuple, Union
 
 import numpy as np
@@ -18,13 +20,17 @@ from . import _lib
 MAX_RANK = _lib.MAX_RANK
 
 _initialized = False
+_queued = False  # calls return before their work is done
 
 
 def init(device: int = 0, asynchronous: bool = False) -> None:
     """Initialise the library on `device` (idempotent)."""
-    global _initialized
+    global _initialized, _queued
     _lib.call("mh_init", int(device), _lib.INIT_ASYNC if asynchronous else 0)
     _initialized = True
+    if _queued and not asynchronous:
+        sync()
+    _queued = bool(asynchronous)
 
 
 def ensure_init() -> None:
@@ -34,6 +40,65 @@ def ensure_init() -> None:
 
 def sync() -> None:
     _lib.call("mh_sync")
+    _held.clear()
+
+
+class _Held:
+    """Owners of other allocators' memory whose tensors are gone while queued calls may still use it. They are let go
+    when an event behind those calls has passed: one for _BATCH owners, or for _BATCH_BYTES of larger ones, so that a
+    loop that makes its tensors anew on each pass pays for an event every thirty passes or so (one every 256 MB made a
+    pass of 62 us over 246 MB one of 65), and waits for none unless _MOST batches or _MOST_BYTES are still held."""
+    _BATCH, _LARGE, _BATCH_BYTES = 256, 1 << 20, 4 << 30
+    _MOST, _MOST_BYTES = 64, 16 << 30
+
+    def __init__(self):
+        self.owners, self.bytes = [], 0  # bytes: of the large ones
+        self.batches, self.total = deque(), 0  # (event, owners, bytes); the bytes of all of them
+        self.events = []
+
+    def large(self, nbytes: int) -> None:
+        self.bytes += nbytes
+        if self.bytes >= self._BATCH_BYTES:
+            self.close()
+
+    def close(self) -> None:
+        try:
+            if not self.events:
+                p = ctypes.c_void_p()
+                _lib.call("mh_event_create", ctypes.byref(p))
+                self.events.append(p.value)
+            _lib.call("mh_event_record", self.events[-1])
+        except _lib.MantleHipError as e:
+            if e.code != _lib.ERR_NOT_INIT:
+                raise
+            self.clear()  # shut down, which has waited for every call
+            return
+        ev, owners, nbytes = self.events.pop(), self.owners[:], self.bytes
+        del self.owners[:len(owners)]
+        self.bytes = 0
+        self.batches.append((ev, owners, nbytes))
+        self.total += nbytes
+        done = ctypes.c_int()
+        while self.batches:
+            ev, _, nbytes = self.batches[0]
+            wait = len(self.batches) > 1 and (len(self.batches) > self._MOST or self.total > self._MOST_BYTES)
+            _lib.call("mh_event_done", ev, int(wait), ctypes.byref(done))
+            if not done.value:
+                break
+            self.batches.popleft()
+            self.total -= nbytes
+            self.events.append(ev)
+
+    def clear(self) -> None:
+        """Everything queued is done."""
+        self.owners.clear()
+        self.bytes = 0
+        while self.batches:
+            self.events.append(self.batches.popleft()[0])
+        self.total = 0
+
+
+_held = _Held()
 
 
 class TensorShape:
@@ -110,14 +175,20 @@ def as_shape(s) -> TensorShape:
     return s if isinstance(s, TensorShape) else TensorShape(s)
 
 
+# A shape is the same object every time its dims come from a tuple: a loop over tensors of other allocators' makes
+# eight of them on each pass of a few calls, and half of its time.
+_shape_of = functools.lru_cache(maxsize=1024)(TensorShape)
+
+
 class Tensor:
     """fp32 tensor in device memory. ``share()`` aliases, ``copy()`` deep-copies
     (tensor.mojo:345-393)."""
 
-    __slots__ = ("_shape", "_ptr", "_owner", "__weakref__")
+    __slots__ = ("_shape", "_ptr", "_owner", "_foreign", "__weakref__")
 
     def __init__(self, *shape, _ptr: Optional[int] = None, _owner=None):
         ensure_init()
+        self._foreign = 0  # 1 + the bytes of another allocator's memory with an owner
         self._shape = as_shape(shape[0]) if len(shape) == 1 and not isinstance(shape[0], (int, np.integer)) \
             else TensorShape(*shape)
         if _ptr is not None:
@@ -130,23 +201,44 @@ class Tensor:
         _lib.call("mh_zero", self._ptr, n)  # zero-initialised, tensor.mojo:266, 284
 
     def __del__(self):
-        if getattr(self, "_owner", 1) is None and getattr(self, "_ptr", None):
-            try:
+        try:
+            if self._foreign:
+                if _queued:
+                    _held.owners.append(self._owner)
+                    if self._foreign > _Held._LARGE:
+                        _held.large(self._foreign)
+            elif self._owner is None and self._ptr:
                 _lib.lib().mh_free(self._ptr)
-            except Exception:
-                pass
-            self._ptr = None
+                self._ptr = None
+        except Exception:
+            pass  # not made whole, or the library is shut down and has waited for every call
 
     @classmethod
     def over(cls, ptr: int, shape, owner=None) -> "Tensor":
-        """A tensor over device memory that another allocator holds, `owner` kept alive with it. What
-        wrote that memory has to be done: the library works on a stream of its own."""
+        """A tensor over device memory that another allocator holds: row-major, 4 bytes an element and aligned
+        to them. What wrote that memory has to be done: the library works on a stream of its own. `owner` is kept
+        alive with the tensor and, where calls are queued, until those that were queued while the tensor lived are
+        done; that shows at a sync(), or when tensors like this one come and go. Without an owner the memory has
+        to outlast those calls (sync() waits for them)."""
         if not _initialized:
             init(0)
+        if len(_held.owners) >= _Held._BATCH:
+            _held.close()
         t = cls.__new__(cls)
-        t._shape = shape if isinstance(shape, TensorShape) else TensorShape(shape)
-        t._ptr = int(ptr)
-        t._owner = t._ptr if owner is None else owner  # anything but None: not freed here
+        t._foreign = 0
+        t._owner = 0  # anything but None: not freed here
+        t._shape = _shape_of(shape) if type(shape) is tuple else as_shape(shape)
+        t._ptr = ptr = int(ptr)
+        if ptr & 3:
+            raise _lib.MantleHipError(_lib.ERR_INVALID, f"address {ptr:#x} is not aligned to 4 bytes")
+        if owner is not None:
+            try:
+                whole = owner.is_contiguous()
+            except AttributeError:  # not an array that could be strided
+                whole = True
+            if not whole and owner.data_ptr() == ptr and tuple(owner.shape) == t._shape._dims:
+                raise _lib.MantleHipError(_lib.ERR_INVALID, "the owner's elements do not lie one after another")
+            t._owner, t._foreign = owner, 4 * t._shape._n + 1
         return t
 
     # ---- properties ----
