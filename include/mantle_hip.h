@@ -297,8 +297,12 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
  * and the roundings of its sum, grad_x and grad_w by as much with G in the place of the other operand.
  * (Up to 64 rows, or 128 forward, of 256 dims or more against 2^22 elements of w or more, the logits and grad_x
  * have 24 bits of every element between 2^-110 and 3.38e38.)
- * The library's scratch, which it keeps, grows to 4 bytes an element of x and of w, and for the
- * gradients to as much again and 8 bytes a logit of a chunk of rows: 4 GiB, or 256 rows, at most. */
+ * The library's scratch, which it keeps, grows to what mh_plan_head reports: 4 bytes an element of x and of w, rows
+ * and classes rounded up to 256 and dims to 32, and 64 a row beside; for the gradients as much again, dims rounded up
+ * to 128 or 256, 8 bytes a logit of the rows at once, of which 4 GiB or 256 rows are taken at most, and a gradient's
+ * partial sums where its product is split; 8 bytes for 64 logits of the rows at once, 32768 rows at most, and 4 GiB
+ * or 256 rows (up to 128 rows: 8 bytes for 32, and 768 a dim). x and w hold 2^36 elements at most, dims rounded up to
+ * 256. */
 int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, const float* x, const float* w,
                                 const int32_t* labels, int64_t rows, int64_t dim, int64_t classes);
 /* The gradients from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
@@ -558,6 +562,14 @@ int mh_plan_launch(int32_t what, int64_t n, mh_launch_info* out);
  *   MH_PLAN_TSTD          tstd over B with C > 1: 2 column quads, 3 single columns */
 enum { MH_PLAN_COLUMNS = 0, MH_PLAN_MAX_BACKWARD = 1, MH_PLAN_CHANNELS = 2, MH_PLAN_TSTD = 3 };
 int mh_plan_reduction(int32_t what, int64_t A, int64_t B, int64_t C, int32_t variant, mh_launch_info* out);
+
+/* What mh_linear_cross_entropy_* take for x [rows, dim] and w [classes, dim] with the gradients asked for (host-only):
+ * the rows whose logits are at hand at once, the scratch, and the work-items of the largest launch that grows with
+ * the sizes. */
+typedef struct {
+    int64_t rows_at_once, scratch_bytes, largest_launch;
+} mh_head_info;
+int mh_plan_head(int64_t rows, int64_t dim, int64_t classes, int grad_x, int grad_w, mh_head_info* out);
 
 #ifdef __cplusplus
 }

@@ -41,6 +41,10 @@ class mh_reduce_plan_info(ctypes.Structure):
                 ("b", ctypes.c_int64 * MAX_RANK), ("c", ctypes.c_int64 * MAX_RANK)]
 
 
+class mh_head_info(ctypes.Structure):
+    _fields_ = [("rows_at_once", ctypes.c_int64), ("scratch_bytes", ctypes.c_int64), ("largest_launch", ctypes.c_int64)]
+
+
 class mh_launch_info(ctypes.Structure):
     _fields_ = [("kernel", ctypes.c_int32), ("threads", ctypes.c_int32), ("blocks", ctypes.c_int64),
                 ("launches", ctypes.c_int64)]
@@ -174,6 +178,7 @@ SIGNATURES = {
     "mh_plan_binary": [_S, _S, _S, ctypes.POINTER(mh_plan_info)],
     "mh_plan_unbroadcast": [_S, _S, ctypes.POINTER(mh_reduce_plan_info)],
     "mh_plan_launch": [ctypes.c_int32, _I64, ctypes.POINTER(mh_launch_info)],
+    "mh_plan_head": [_I64, _I64, _I64, _I, _I, ctypes.POINTER(mh_head_info)],
     "mh_plan_reduction": [ctypes.c_int32, _I64, _I64, _I64, ctypes.c_int32, ctypes.POINTER(mh_launch_info)],
 }
 _RESTYPE = {"mh_last_error": ctypes.c_char_p, "mh_status_string": ctypes.c_char_p}

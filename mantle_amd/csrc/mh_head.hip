@@ -884,8 +884,8 @@ __global__ __launch_bounds__(256) void k_few_dx(FewArg f) {
 // ---------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------
-// The logits of one chunk of rows and G's column panel take 8 bytes an element; a chunk's rows keep them
-// within this, 256 rows at least.
+// The logits of one chunk of rows and G's column panel take 8 bytes an element, a forward's statistics 8 bytes for 64;
+// a chunk's rows keep them within this, 256 rows at least.
 constexpr int64_t kChunkBytes = (int64_t)4 << 30;
 constexpr int64_t kMaxChunk = 32768;
 constexpr int64_t kFewElements = (int64_t)1 << 22;  // of w, from which its bytes and not launches count
@@ -948,9 +948,8 @@ void set_form(GemmArg& g, int64_t m, int64_t n, const Form& f) {
     g.splits = f.splits;
     g.kb = up((g.kb_all + f.splits - 1) / f.splits, 2);
 }
-uint32_t gemm_blocks(const GemmArg& g) {
-    return (uint32_t)(8 * (((int64_t)g.tiles_m * g.tiles_n * g.splits + 7) / 8));
-}
+int64_t gemm_blocks(int64_t tiles, int64_t splits) { return 8 * ((tiles * splits + 7) / 8); }
+uint32_t gemm_blocks(const GemmArg& g) { return (uint32_t)gemm_blocks((int64_t)g.tiles_m * g.tiles_n, g.splits); }
 // `n` products of one tile in a launch.
 template <int EPI>
 void launch_gemm(const GemmArg* g, int n, int tile) {
@@ -1005,91 +1004,136 @@ struct Forms {
     int64_t rows;          // padded to the tiles that read them
     size_t part[2];
 };
-Forms forms_of(const HeadCall& h, int64_t nr, int64_t dkb) {
+
+// How a call's work is cut and where its workspace lies: known before anything is launched.
+struct HeadPlan {
+    int64_t rowsP, clsP, dkb;  // padded
+    int64_t dim_x, dim_w;      // dims padded to the tiles that read x's and w's column panels
+    int64_t chunk, groups;
+    bool few;
+    int nt;
+    int64_t fdim, fkb, fsplits;
+    Forms whole, last;  // of a chunk, of the last one
+    size_t o_info, o_part, o_ex, o_xr, o_wr, o_xt, o_wt, o_stat, o_tgt, o_scale, o_rl, o_z, o_gt, o_sp, o_fx, bytes;
+    int64_t items;  // work-items of the largest launch that grows with the sizes
+};
+
+Forms forms_of(HeadPlan& p, int64_t nr, int64_t dim, int64_t classes, bool gx, bool gw) {
     Forms f = {};
-    f.logits = form_of(h.classes, nr, dkb, false);
+    auto launch = [](int64_t m, int64_t n, const Form& form) {
+        const int64_t blocks = gemm_blocks(up(m, form.tile) / form.tile * (up(n, form.tile) / form.tile), form.splits);
+        return blocks * (form.tile == 256 ? 512 : 256);
+    };
+    auto count = [&p](int64_t items) { p.items = items > p.items ? items : p.items; };
+    f.logits = form_of(classes, nr, p.dkb, false);
     f.rows = up(nr, f.logits.tile);
-    if (h.train) {
-        f.grad[0] = form_of(nr, h.dim, up(h.classes, 32) / 16, true);
-        f.grad[1] = form_of(h.classes, h.dim, up(nr, 32) / 16, true);
-        if (h.gx && up(nr, f.grad[0].tile) > f.rows) f.rows = up(nr, f.grad[0].tile);
-        f.part[0] = h.gx ? part_bytes(nr, h.dim, f.grad[0]) : 0;
-        f.part[1] = h.gw ? part_bytes(h.classes, h.dim, f.grad[1]) : 0;
+    int64_t grads = 0;
+    if (gx) {
+        f.grad[0] = form_of(nr, dim, up(classes, 32) / 16, true);
+        if (up(nr, f.grad[0].tile) > f.rows) f.rows = up(nr, f.grad[0].tile);
+        f.part[0] = part_bytes(nr, dim, f.grad[0]);
+        if (up(dim, f.grad[0].tile) > p.dim_w) p.dim_w = up(dim, f.grad[0].tile);
+        if (!p.few) grads += launch(nr, dim, f.grad[0]);
     }
+    if (gw) {
+        f.grad[1] = form_of(classes, dim, up(nr, 32) / 16, true);
+        f.part[1] = part_bytes(classes, dim, f.grad[1]);
+        if (up(dim, f.grad[1].tile) > p.dim_x) p.dim_x = up(dim, f.grad[1].tile);
+        grads += launch(classes, dim, f.grad[1]);
+    }
+    count(grads);
+    if (!p.few) count(launch(p.clsP, f.rows, f.logits));
+    if (gx || gw) count((f.rows / 32 * (p.clsP / 32) / 4 + 1) * 256);  // k_to_g
     return f;
 }
 
-int head_run(const HeadCall& h) {
-    const int64_t rows = h.rows, dim = h.dim, classes = h.classes;
-    const int64_t rowsP = up(rows, 256), dimP = up(dim, 256), clsP = up(classes, 256);
-    const int64_t dkb = up(dim, 32) / 16;
-    int64_t chunk = kMaxChunk;
-    if (h.train) {
-        chunk = kChunkBytes / (clsP * 8) / 256 * 256;
-        chunk = chunk < 256 ? 256 : chunk > kMaxChunk ? kMaxChunk : chunk;
-    }
-    if (chunk > rowsP) chunk = rowsP;
+HeadPlan plan_of(int64_t rows, int64_t dim, int64_t classes, bool gx, bool gw) {
+    HeadPlan p = {};
+    const bool train = gx || gw;
+    p.rowsP = up(rows, 256);
+    p.clsP = up(classes, 256);
+    p.dkb = up(dim, 32) / 16;
     // w straight from memory where rows are few and w is large enough to bound the products, in rows long enough
     // for eight wavefronts each ([32, 64] x [100000, 64]: 178 us so, 146 by panels)
-    const bool few = rows <= (h.train ? kFewRows : kFewRowsForward) && dim >= 256 && classes * dim >= kFewElements;
-    const int nt = rows > 64 ? 4 : rows > 32 ? 2 : 1;
-    const int64_t groups = few ? clsP / 32 : clsP / 64;
-    const int64_t fdim = up(dim, 128), fkb = up(classes, 16) / 16;
+    p.few = rows <= (train ? kFewRows : kFewRowsForward) && dim >= 256 && classes * dim >= kFewElements;
+    p.nt = rows > 64 ? 4 : rows > 32 ? 2 : 1;
+    p.groups = p.few ? p.clsP / 32 : p.clsP / 64;
+    p.chunk = (train ? kChunkBytes / (p.clsP * 8) : kChunkBytes / (p.groups * 8)) / 256 * 256;
+    p.chunk = p.chunk < 256 ? 256 : p.chunk > kMaxChunk ? kMaxChunk : p.chunk;
+    if (p.chunk > p.rowsP) p.chunk = p.rowsP;
+    p.fdim = up(dim, 128);
+    p.fkb = up(classes, 16) / 16;
     // splits of the classes that give every CU eight wavefronts or so, of 16 blocks at least
-    int64_t fsplits = few ? (2 * ctx().num_cus + fdim / 128 - 1) / (fdim / 128) : 1;
-    if (fsplits > fkb / 16) fsplits = fkb / 16;
-    fsplits = fsplits < 1 ? 1 : fsplits > kMaxSplit ? kMaxSplit : fsplits;
+    p.fsplits = p.few ? (2 * ctx().num_cus + p.fdim / 128 - 1) / (p.fdim / 128) : 1;
+    if (p.fsplits > p.fkb / 16) p.fsplits = p.fkb / 16;
+    p.fsplits = p.fsplits < 1 ? 1 : p.fsplits > kMaxSplit ? kMaxSplit : p.fsplits;
+    const int64_t behind = rows - (rows - 1) / p.chunk * p.chunk;  // rows of the last chunk
+    p.whole = forms_of(p, rows < p.chunk ? rows : p.chunk, dim, classes, gx, gw);
+    p.last = behind == p.chunk || rows < p.chunk ? p.whole : forms_of(p, behind, dim, classes, gx, gw);
+    const int64_t most = p.dim_x > p.dim_w ? p.dim_x : p.dim_w, wide = most > up(dim, 64) ? most : up(dim, 64);
+    const int64_t split = (p.rowsP / 64 + (p.few ? 0 : p.clsP / 64)) * (wide / 64) * 256, logits = p.few ? p.clsP / 32 * 512 : 0;
+    p.items = split > p.items ? split : p.items;
+    p.items = logits > p.items ? logits : p.items;
 
     Carve cv;
-    const size_t o_info = cv.take(sizeof(HeadInfo)), o_part = cv.take(sizeof(HeadPart));
-    const size_t o_ex = cv.take(rowsP * 4);
-    const size_t o_xr = cv.take(rowsP / 32 * stride_of(dkb) * kBlk),
-                 o_wr = few ? 0 : cv.take(clsP / 32 * stride_of(dkb) * kBlk);
-    const size_t o_xt = h.train && h.gw ? cv.take(dimP / 32 * stride_of(rowsP / 16) * kBlk) : 0;
-    const size_t o_wt = h.train && h.gx && !few ? cv.take(dimP / 32 * stride_of(clsP / 16) * kBlk) : 0;
-    const size_t o_stat = cv.take(groups * 2 * chunk * 4);
-    const size_t o_tgt = cv.take(chunk * 4), o_scale = cv.take(h.train ? chunk * sizeof(RowScale) : 0), o_rl = cv.take(rowsP / kLseRows * 8);
-    size_t o_z = 0, o_gt = 0, o_sp = 0;
-    if (h.train) {
-        o_z = cv.take(chunk / 32 * stride_of(clsP / 16) * kBlk);
-        o_gt = cv.take(clsP / 32 * stride_of(chunk / 16) * kBlk);
-        // every chunk has this many rows but the last
-        size_t sp = few ? (size_t)(fsplits * nt * 32 * fdim) * sizeof(float) : 0;
-        for (const int64_t nr : {rows < chunk ? rows : chunk, rows - (rows - 1) / chunk * chunk}) {
-            const Forms f = forms_of(h, nr, dkb);
-            if (f.part[0] + f.part[1] > sp) sp = f.part[0] + f.part[1];
-        }
-        o_sp = cv.take((int64_t)sp);
+    p.o_info = cv.take(sizeof(HeadInfo));
+    p.o_part = cv.take(sizeof(HeadPart));
+    p.o_ex = cv.take(p.rowsP * 4);
+    p.o_xr = cv.take(p.rowsP / 32 * stride_of(p.dkb) * kBlk);
+    p.o_wr = p.few ? 0 : cv.take(p.clsP / 32 * stride_of(p.dkb) * kBlk);
+    p.o_xt = gw ? cv.take(p.dim_x / 32 * stride_of(p.rowsP / 16) * kBlk) : 0;
+    p.o_wt = gx && !p.few ? cv.take(p.dim_w / 32 * stride_of(p.clsP / 16) * kBlk) : 0;
+    p.o_stat = cv.take(p.groups * 2 * p.chunk * 4);
+    p.o_tgt = cv.take(p.chunk * 4);
+    p.o_scale = cv.take(train ? p.chunk * (int64_t)sizeof(RowScale) : 0);
+    p.o_rl = cv.take(p.rowsP / kLseRows * 8);
+    if (train) {
+        p.o_z = cv.take(p.chunk / 32 * stride_of(p.clsP / 16) * kBlk);
+        p.o_gt = cv.take(p.clsP / 32 * stride_of(p.chunk / 16) * kBlk);
+        size_t sp = p.few ? (size_t)(p.fsplits * p.nt * 32 * p.fdim) * sizeof(float) : 0;
+        for (const Forms* f : {&p.whole, &p.last})
+            if (f->part[0] + f->part[1] > sp) sp = f->part[0] + f->part[1];
+        p.o_sp = cv.take((int64_t)sp);
     }
-    const size_t o_fx = few ? cv.take(nt * dkb * kFewBlk) : 0;
-    char* base = nullptr;
-    MH_TRY(scratch(cv.at, reinterpret_cast<void**>(&base)));
-    hipStream_t st = ctx().stream;
-    HeadInfo* info = reinterpret_cast<HeadInfo*>(base + o_info);
-    HeadPart* part = reinterpret_cast<HeadPart*>(base + o_part);
-    RowScale* scale = h.train ? reinterpret_cast<RowScale*>(base + o_scale) : nullptr;
-    double* block_loss = reinterpret_cast<double*>(base + o_rl);
-    float* target = reinterpret_cast<float*>(base + o_tgt);
+    p.o_fx = p.few ? cv.take(p.nt * p.dkb * kFewBlk) : 0;
+    p.bytes = cv.at;
+    return p;
+}
 
-    int32_t* row_exp = reinterpret_cast<int32_t*>(base + o_ex);
+int head_run(const HeadCall& h, const HeadPlan& pl) {
+    const int64_t rows = h.rows, dim = h.dim, classes = h.classes;
+    const int64_t rowsP = pl.rowsP, clsP = pl.clsP, dkb = pl.dkb, chunk = pl.chunk, groups = pl.groups;
+    const int64_t fdim = pl.fdim, fkb = pl.fkb, fsplits = pl.fsplits;
+    const bool few = pl.few;
+    const int nt = pl.nt;
+    char* base = nullptr;
+    MH_TRY(scratch(pl.bytes, reinterpret_cast<void**>(&base)));
+    hipStream_t st = ctx().stream;
+    HeadInfo* info = reinterpret_cast<HeadInfo*>(base + pl.o_info);
+    HeadPart* part = reinterpret_cast<HeadPart*>(base + pl.o_part);
+    RowScale* scale = h.train ? reinterpret_cast<RowScale*>(base + pl.o_scale) : nullptr;
+    double* block_loss = reinterpret_cast<double*>(base + pl.o_rl);
+    float* target = reinterpret_cast<float*>(base + pl.o_tgt);
+
+    int32_t* row_exp = reinterpret_cast<int32_t*>(base + pl.o_ex);
     hipLaunchKernelGGL(k_amax, dim3(few ? kAmaxBlocks : 2 * kAmaxBlocks), dim3(256), 0, st, part, row_exp, h.x, h.w, h.labels,
                        rows, dim, classes * dim);
-    SplitOne sx = {h.x, rows, dim, row_exp, base + o_xr, h.train && h.gw ? base + o_xt : nullptr, dkb, rowsP / 16,
-                   rowsP / 64, up(dim, 64) / 64, rowsP / 32, dimP / 32};
-    SplitOne sw = {h.w, classes, dim, nullptr, base + o_wr, h.train && h.gx ? base + o_wt : nullptr, dkb, clsP / 16,
-                   clsP / 64, up(dim, 64) / 64, clsP / 32, dimP / 32};
-    if (sx.colp) sx.tiles_c = dimP / 64;
-    if (sw.colp) sw.tiles_c = dimP / 64;
+    SplitOne sx = {h.x, rows, dim, row_exp, base + pl.o_xr, h.train && h.gw ? base + pl.o_xt : nullptr, dkb, rowsP / 16,
+                   rowsP / 64, up(dim, 64) / 64, rowsP / 32, pl.dim_x / 32};
+    SplitOne sw = {h.w, classes, dim, nullptr, base + pl.o_wr, h.train && h.gx ? base + pl.o_wt : nullptr, dkb, clsP / 16,
+                   clsP / 64, up(dim, 64) / 64, clsP / 32, pl.dim_w / 32};
+    if (sx.colp) sx.tiles_c = pl.dim_x / 64;
+    if (sw.colp) sw.tiles_c = pl.dim_w / 64;
     const int64_t nsplit = sx.tiles_r * sx.tiles_c + (few ? 0 : sw.tiles_r * sw.tiles_c);
     hipLaunchKernelGGL(k_split, dim3((unsigned)nsplit), dim3(256), 0, st, sx, sw, part, info, h.labels);
 
     for (int64_t r0 = 0; r0 < rows; r0 += chunk) {
         const int64_t nr = rows - r0 < chunk ? rows - r0 : chunk;
-        const Forms f = forms_of(h, nr, dkb);
+        const Forms& f = nr < chunk && r0 > 0 ? pl.last : pl.whole;
         const int64_t nrP = f.rows, zkb = stride_of(clsP / 16), gtkb = stride_of(up(nr, 32) / 16);
         GemmArg g = {};
-        g.a = base + o_wr;
-        g.b = base + o_xr + r0 / 32 * stride_of(dkb) * kBlk;
+        g.a = base + pl.o_wr;
+        g.b = base + pl.o_xr + r0 / 32 * stride_of(dkb) * kBlk;
         g.akb = g.bkb = stride_of(dkb);
         g.kb_all = dkb;
         g.info = info;
@@ -1097,15 +1141,15 @@ int head_run(const HeadCall& h) {
         g.rows = nr;
         g.classes = classes;
         g.row_exp = row_exp + r0;
-        g.stat = reinterpret_cast<float*>(base + o_stat);
+        g.stat = reinterpret_cast<float*>(base + pl.o_stat);
         g.stat_ld = chunk;
         g.target = target;
-        g.z = h.train ? base + o_z : nullptr;
+        g.z = h.train ? base + pl.o_z : nullptr;
         g.zkb = zkb;
         // every row and class that a gradient's tiles read gets its logits: the panels behind have no gaps
         set_form(g, clsP, nrP, f.logits);
-        FewArg fa = {h.x, h.w, h.labels, rows, dim, classes, dkb, base + o_fx, g.stat, g.stat_ld, target, g.z, zkb,
-                     reinterpret_cast<float*>(base + o_sp), fdim, fkb, (fkb + fsplits - 1) / fsplits};
+        FewArg fa = {h.x, h.w, h.labels, rows, dim, classes, dkb, base + pl.o_fx, g.stat, g.stat_ld, target, g.z, zkb,
+                     reinterpret_cast<float*>(base + pl.o_sp), fdim, fkb, (fkb + fsplits - 1) / fsplits};
         if (few) {
             hipLaunchKernelGGL(k_few_x, dim3((unsigned)(nt * dkb)), dim3(64), 0, st, fa);
             const dim3 grid((unsigned)(clsP / 32));
@@ -1128,18 +1172,18 @@ int head_run(const HeadCall& h) {
         if (!h.train) continue;
         const int64_t tiles_v = clsP / 32, tiles = nrP / 32 * tiles_v / 4;
         const bool with_loss = h.loss && r0 + chunk >= rows;
-        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(tiles + with_loss)), dim3(256), 0, st, base + o_z, zkb,
-                           base + o_gt, gtkb, up(nr, 32) / 32, scale, h.labels + r0, nr,
+        hipLaunchKernelGGL(k_to_g, dim3((unsigned)(tiles + with_loss)), dim3(256), 0, st, base + pl.o_z, zkb,
+                           base + pl.o_gt, gtkb, up(nr, 32) / 32, scale, h.labels + r0, nr,
                            classes, tiles_v, tiles, block_loss, (rows + kLseRows - 1) / kLseRows, info, h.loss);
         GemmArg d[2] = {};
         Form df[2];
         int nd = 0;
-        float* sp = reinterpret_cast<float*>(base + o_sp);
+        float* sp = reinterpret_cast<float*>(base + pl.o_sp);
         if (h.gx) {
             GemmArg& p = d[nd];
-            p.a = base + o_z;
+            p.a = base + pl.o_z;
             p.akb = zkb;
-            p.b = base + o_wt;
+            p.b = base + pl.o_wt;
             p.bkb = stride_of(clsP / 16);
             p.kb_all = up(classes, 32) / 16;
             p.exp_b = 1;
@@ -1167,9 +1211,9 @@ int head_run(const HeadCall& h) {
         }
         if (h.gw) {
             GemmArg& p = d[nd];
-            p.a = base + o_gt;
+            p.a = base + pl.o_gt;
             p.akb = gtkb;
-            p.b = base + o_xt + r0 / 16 * kBlk;
+            p.b = base + pl.o_xt + r0 / 16 * kBlk;
             p.bkb = stride_of(rowsP / 16);
             p.kb_all = up(nr, 32) / 16;
             p.out = h.gw;
@@ -1190,16 +1234,23 @@ int head_run(const HeadCall& h) {
     return finish(h.what);
 }
 
-int head_check(const HeadCall& h) {
-    if (h.rows < 0 || h.dim < 1 || h.classes < 1)
-        return fail(MH_ERR_INVALID, "%s: needs rows >= 0, dim >= 1, classes >= 1 (%lld, %lld, %lld)", h.what,
-                    (long long)h.rows, (long long)h.dim, (long long)h.classes);
-    if (h.classes > 0x7fffffff || h.dim > (1 << 24) || h.rows > 0x7fffffff)
-        return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 rows or classes, or 2^24 dims", h.what);
+int head_check(const char* what, int64_t rows, int64_t dim, int64_t classes, bool gx, bool gw, HeadPlan* p) {
+    if (rows < 0 || dim < 1 || classes < 1)
+        return fail(MH_ERR_INVALID, "%s: needs rows >= 0, dim >= 1, classes >= 1 (%lld, %lld, %lld)", what, (long long)rows,
+                    (long long)dim, (long long)classes);
+    if (classes > 0x7fffffff || dim > (1 << 24) || rows > 0x7fffffff)
+        return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 rows or classes, or 2^24 dims", what);
     // one workgroup a 64 x 64 tile of x and of w
-    if ((up(h.rows, 256) / 64 + up(h.classes, 256) / 64) * (up(h.dim, 256) / 64) > max_grid_blocks(256))
-        return fail(MH_ERR_OVERFLOW, "%s: operands of more than 2^36 elements", h.what);
+    if ((up(rows, 256) / 64 + up(classes, 256) / 64) * (up(dim, 256) / 64) > max_grid_blocks(256))
+        return fail(MH_ERR_OVERFLOW, "%s: operands of more than 2^36 elements, dims rounded up to 256", what);
+    if (rows == 0) return MH_OK;
+    *p = plan_of(rows, dim, classes, gx, gw);
+    if (p->items > kMaxDispatchItems)
+        return fail(MH_ERR_OVERFLOW, "%s: a launch of more than 2^32 work-items", what);
     return MH_OK;
+}
+int head_check(const HeadCall& h, HeadPlan* p) {
+    return head_check(h.what, h.rows, h.dim, h.classes, h.gx != nullptr, h.gw != nullptr, p);
 }
 
 }  // namespace
@@ -1223,11 +1274,12 @@ int mh_linear_cross_entropy_fwd(float* loss, float* row_loss, float* row_lse, co
     h.rows = rows;
     h.dim = dim;
     h.classes = classes;
-    MH_TRY(head_check(h));
+    HeadPlan p;
+    MH_TRY(head_check(h, &p));
     if (!loss || !w || (rows > 0 && (!x || !labels))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
     MH_TRY(require_init());
     if (rows == 0) return mh_fill(loss, 0.0f, 1);
-    return head_run(h);
+    return head_run(h, p);
 }
 
 int mh_linear_cross_entropy_bwd(float* grad_x, float* grad_w, const float* x, const float* w, const int32_t* labels,
@@ -1248,12 +1300,13 @@ int mh_linear_cross_entropy_bwd(float* grad_x, float* grad_w, const float* x, co
     h.classes = classes;
     h.train = true;
     h.accumulate = accumulate != 0;
-    MH_TRY(head_check(h));
+    HeadPlan p;
+    MH_TRY(head_check(h, &p));
     if (!grad_x && !grad_w) return MH_OK;
     if (!w || !ug || (rows > 0 && (!x || !labels || !row_lse))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
     MH_TRY(require_init());
     if (rows == 0) return grad_w && !accumulate ? mh_zero(grad_w, classes * dim) : MH_OK;
-    return head_run(h);
+    return head_run(h, p);
 }
 
 int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, float* grad_w, const float* x,
@@ -1275,14 +1328,27 @@ int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, flo
     h.classes = classes;
     h.train = grad_x || grad_w;
     h.accumulate = accumulate != 0;
-    MH_TRY(head_check(h));
+    HeadPlan p;
+    MH_TRY(head_check(h, &p));
     if (!loss || !w || (h.train && !ug) || (rows > 0 && (!x || !labels))) return fail(MH_ERR_NULL, "%s: null tensor", h.what);
     MH_TRY(require_init());
     if (rows == 0) {
         if (grad_w && !accumulate) MH_TRY(mh_zero(grad_w, classes * dim));
         return mh_fill(loss, 0.0f, 1);
     }
-    return head_run(h);
+    return head_run(h, p);
+}
+
+int mh_plan_head(int64_t rows, int64_t dim, int64_t classes, int grad_x, int grad_w, mh_head_info* out) {
+    if (!out) return fail(MH_ERR_NULL, "mh_plan_head: null");
+    *out = mh_head_info{};
+    HeadPlan p;
+    MH_TRY(head_check("mh_plan_head", rows, dim, classes, grad_x != 0, grad_w != 0, &p));
+    if (rows == 0) return MH_OK;
+    out->rows_at_once = rows < p.chunk ? rows : p.chunk;
+    out->scratch_bytes = (int64_t)p.bytes;
+    out->largest_launch = p.items;
+    return MH_OK;
 }
 
 }  // extern "C"
