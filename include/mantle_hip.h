@@ -292,7 +292,8 @@ int mh_cross_entropy_bwd_accum(float* grad_x, const float* x, const float* targe
  * NaN; so does a kept row or a class that holds a NaN or an infinity. row_loss and row_lse may be null.
  * x and w are each held with 22 bits of every element down to 2^-17 of the largest, and to 2^-39 of the
  * largest below: of the tensor's (for x: of the kept rows'), but in the logits of its row's for x, so that no
- * row's loss depends on another row's size. Sums are fp32. A logit is off by at most
+ * row's loss depends on another row's size. Sums are fp32, over all dims for a logit, 65536 rows or classes at
+ * a time for a gradient. A logit is off by at most
  *   2^-21 sum |x w| + 2^-39 (max |x_row| sum |w_class| + max |w| sum |x_row|)
  * and the roundings of its sum, grad_x and grad_w by as much with G in the place of the other operand.
  * (Up to 64 rows, or 128 forward, of 256 dims or more against 2^22 elements of w or more, the logits and grad_x

@@ -909,9 +909,10 @@ struct Form {
 // ones up to three share a CU, which then works at 0.5, 0.78 or 0.82 of the large tile's rate, with 10 around
 // them. Measured on either side: [4096, 1024] x [32000, 1024]'s logits take 625 us in large tiles and 670 in
 // small ones; a step of [1023, 513] x [30011, 513] 491 us with its grad_x in 21 splits of large tiles or 12 of small
-// ones. A split writes and reads its sums and costs one more launch. Sums run over at most 65536 elements
-// each: the matrix unit's fp32 sums drift by 4e-11 of themselves an element (8e-5 over 2^21 of them unsplit).
-constexpr int64_t kMaxSplit = 64, kLongest = 4096;
+// ones. A split writes and reads its sums and costs one more launch. A gradient's sums run over at most 65536
+// elements each, whatever that takes in splits: the matrix unit's fp32 sums drift by 4e-11 of themselves an element
+// (8e-5 over 2^21 of them unsplit). A logit's sum is one, over all dims: 7e-4 of itself at 2^24 of them.
+constexpr int64_t kMaxSplit = 64, kLongest = 4096;  // splits taken for speed at most, blocks of 16 of a split
 Form form_of(int64_t m, int64_t n, int64_t kb, bool split) {
     static const double rate[4] = {1.0, 0.5, 0.78, 0.82};
     const int64_t cus = ctx().num_cus, least = split ? (kb + kLongest - 1) / kLongest : 1;
@@ -919,7 +920,7 @@ Form form_of(int64_t m, int64_t n, int64_t kb, bool split) {
     double time = 0.0;
     for (const int T : {256, 128}) {
         const int64_t tiles = up(m, T) / T * (up(n, T) / T);
-        for (int64_t s = least < kMaxSplit ? least : kMaxSplit; s <= kMaxSplit; ++s) {
+        for (int64_t s = least; s <= (least > kMaxSplit ? least : kMaxSplit); ++s) {
             const int64_t wg = tiles * s, steps = (kb + s - 1) / s;
             double t;
             if (T == 256) {
@@ -1067,6 +1068,7 @@ HeadPlan plan_of(int64_t rows, int64_t dim, int64_t classes, bool gx, bool gw) {
     p.fsplits = p.few ? (2 * ctx().num_cus + p.fdim / 128 - 1) / (p.fdim / 128) : 1;
     if (p.fsplits > p.fkb / 16) p.fsplits = p.fkb / 16;
     p.fsplits = p.fsplits < 1 ? 1 : p.fsplits > kMaxSplit ? kMaxSplit : p.fsplits;
+    if (p.fsplits * kLongest < p.fkb) p.fsplits = (p.fkb + kLongest - 1) / kLongest;
     const int64_t behind = rows - (rows - 1) / p.chunk * p.chunk;  // rows of the last chunk
     p.whole = forms_of(p, rows < p.chunk ? rows : p.chunk, dim, classes, gx, gw);
     p.last = behind == p.chunk || rows < p.chunk ? p.whole : forms_of(p, behind, dim, classes, gx, gw);

@@ -4,8 +4,18 @@ import numpy as np
 import pytest
 
 from test_gpu_head import check, inputs, m_, reference, run
+from util import TEST_ASYNC
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_the_scratch_back():
+    """These sizes grow the library's scratch to tens of GB, which it keeps until it is shut down."""
+    yield
+    m = m_()
+    m._lib.call("mh_shutdown")
+    m.init(0, asynchronous=TEST_ASYNC)
 
 
 def forward(m, x, w, labels):
@@ -45,3 +55,35 @@ def test_forward_cut_by_its_statistics():
             assert (same == same[0]).all(), (name, k)
     loss = (np.array([o["row_loss"][0] for o in one])[which] * keep).sum() / keep.sum()
     assert abs(got["loss"] - loss) <= max(b["row_loss"][0] for b in bound)
+
+
+def test_gradient_sums_over_millions_of_classes():
+    """2^25 classes: grad_x's sums run over at most 65536 of them at a time. All terms are positive, so that an adder's
+    drift, 4e-11 of the sum an element, shows: 2.6e-6 then, 2.1e-5 over the 2^19 of one split in 64. The halves'
+    roundings (2^-22 and, of an element of G near 2^-25, 2^-15 of itself) are as good as random over 2^25 terms."""
+    m = m_()
+    rows, dim, classes = 3, 4, 1 << 25
+    tw = m.Tensor(classes, dim)
+    m._lib.call("mh_rand_uniform", tw.ptr, classes * dim, 62, 0.5, 1.5)
+    w = tw.to_numpy()
+    labels = np.array([5, 6, 7], np.int32)
+    zero = np.zeros((8, dim), np.float32)  # the labels' classes: -w_label adds nothing
+    m._lib.call("mh_memcpy_h2d", tw.ptr, zero.ctypes.data, zero.nbytes)
+    w[:8] = 0.0
+    x = (0.01 * np.random.RandomState(63).standard_normal((rows, dim))).astype(np.float32)
+    print("\n[head] 2^25 classes", flush=True)
+    gx, loss = m.Tensor(rows, dim), m.Tensor(1)
+    m.linear_cross_entropy_step(loss, gx, None, m.Tensor.from_numpy(x), tw, m.IndexTensor.from_numpy(labels),
+                                m.Tensor.from_numpy(np.float32([rows])), accumulate=False)
+    got = gx.to_numpy().astype(np.float64)
+    want = np.zeros((rows, dim))
+    total = np.zeros(rows)
+    for v in range(0, classes, 1 << 21):
+        part = w[v:v + (1 << 21)].astype(np.float64)
+        e = np.exp(part @ x.T.astype(np.float64))
+        total += e.sum(0)
+        want += e.T @ part
+    want /= total[:, None]
+    off = np.abs(got / want - 1)
+    print("[head] off by", off.max(), flush=True)
+    assert off.max() <= 5e-6
