@@ -87,3 +87,31 @@ def test_gradient_sums_over_millions_of_classes():
     off = np.abs(got / want - 1)
     print("[head] off by", off.max(), flush=True)
     assert off.max() <= 5e-6
+
+
+def test_forward_of_more_rows_than_at_once():
+    """33000 rows: 32768 and the rest, through the same statistics and targets."""
+    x, w, labels = inputs(33000, 8, 70, seed=64)
+    want, bound = reference(x, w, labels)
+    check(forward(m_(), x, w, labels), want, bound, "rows")
+    for how in ("step", "two calls"):
+        check(run(m_(), x, w, labels, how=how), want, bound, how)
+
+
+@pytest.mark.parametrize("place", ["first", "last"])
+def test_a_wide_w_whose_largest_is_at_an_end(place):
+    """10M elements of w: eight loads a thread and the rest. The power of two follows the largest wherever it lies: with
+    another one's products would overflow their halves."""
+    rows, dim, classes = 70, 100, 104003
+    x, w, labels = inputs(rows, dim, classes, seed=65)
+    at = (0, 3) if place == "first" else (classes - 1, dim - 1)
+    w[at] = 3000.0
+    x[:, at[1]] *= np.float32(1e-3)  # keeps the logits' size
+    want, bound = reference(x, w, labels)
+    floor = 2.0 ** -39 * (3000.0 * np.abs(x).sum(1) + np.abs(x).max(1) * np.abs(w).sum(1).max())
+    bound["row_lse"], bound["row_loss"] = bound["row_lse"] + floor, bound["row_loss"] + 2 * floor
+    bound["loss"] += 2 * floor.max()
+    bound["grad_x"] = bound["grad_x"] + (2.0 ** -39 * 3000.0 * 2 + 3 * floor[:, None] * np.abs(w).max(0)[None]) / rows
+    bound["grad_w"] = bound["grad_w"] + 3 * floor.max() * np.abs(x).max() / rows
+    for how in ("step", "two calls"):
+        check(run(m_(), x, w, labels, how=how), want, bound, f"{place} {how}")
