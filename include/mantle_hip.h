@@ -328,7 +328,8 @@ int mh_linear_cross_entropy_step(float* loss, float* row_lse, float* grad_x, flo
  * A row without entries is left out whatever its logits hold: row_lse 0, its gradient left alone
  * (accumulate == 0: zero). A class that several entries name gets the sum of their q, in their order. An id of
  * classes or more makes the row's row_lse and gradient, and the loss, NaN. 1 <= k <= 1024; row_lse
- * may be null. */
+ * may be null; rows are fewer than 2^22. The library's scratch, which it keeps, grows to 12 bytes an entry, 16 a row
+ * and 8 for each workgroup of a row, up to 64 where rows are few. */
 int mh_distill_fwd(float* loss, float* row_lse, const float* x, const int32_t* ids, const float* teacher, int64_t rows,
                    int64_t classes, int64_t k, float temperature);
 /* The gradient from ug = the gradient of the loss (a device scalar) and the forward's row_lse:
@@ -348,7 +349,9 @@ int mh_distill_step(float* loss, float* row_lse, float* grad_x, const float* x, 
  * an expert; and the balance loss
  *   loss = experts sum_e f_e P_e,  f_e = counts_e / (n k),  P_e = the mean of p_e,
  * over the n kept rows: those with keep[row] != 0, or all where keep is null. A row that is not kept has
- * chosen -1 and weights 0 and counts nowhere. 1 <= experts <= 1024, 1 <= k <= min(64, experts). */
+ * chosen -1 and weights 0 and counts nowhere. A kept row that holds a NaN, or nothing but minus infinity, has NaN for
+ * weights and gradient, and so has the loss; its choices stay below experts. 1 <= experts <= 1024,
+ * 1 <= k <= min(64, experts). */
 int mh_router_fwd(float* weights, int32_t* chosen, int32_t* counts, float* loss, const float* x, const int32_t* keep,
                   int64_t rows, int64_t experts, int64_t k, int normalise);
 /* The gradient of the logits from grad_weights [rows, k], the gradient of the weights, and ug, that of the

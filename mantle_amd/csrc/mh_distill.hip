@@ -10,8 +10,9 @@
 // entries). Then a workgroup takes a row: of up to 65536 classes it holds it in registers and reads it
 // once; a longer one it reads twice, the second time from its end, where the caches still hold it. Where
 // rows are fewer than CUs, several workgroups share a row: their statistics, then the gradient.
-// An exponential is a difference, a product with log2(e) / T and one instruction; sums are fp32 over at
-// most C / 1024 elements a thread, then a tree.
+// An exponential is a difference, a product with log2(e) / T and one instruction; sums are fp32, of C / (64 W)
+// elements a thread of a workgroup of W wavefronts (at most 16 of a row held by one, 32 by 4 to 16, 64 of more than
+// 32768 classes; C / 1024 of rows that are not held), then a tree.
 #include "mh_internal.h"
 #include "mh_math.h"
 #include "mh_rows.h"
