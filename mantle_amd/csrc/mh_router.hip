@@ -566,7 +566,7 @@ int router_check(const char* what, int64_t rows, int64_t experts, int64_t k) {
     if (rows < 0 || experts < 1 || experts > kMaxExperts || k < 1 || k > kMaxChosen || k > experts)
         return fail(MH_ERR_INVALID, "%s: needs rows >= 0, 1 <= experts <= %d, 1 <= k <= min(%d, experts) (%lld, %lld, %lld)",
                     what, kMaxExperts, kMaxChosen, (long long)rows, (long long)experts, (long long)k);
-    if (rows * k > 0x7fffffff) return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 choices", what);
+    if (rows > 0x7fffffff / k) return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 choices", what);
     return MH_OK;
 }
 
