@@ -290,14 +290,21 @@ class Tensor:
     def zero(self) -> None:
         _lib.call("mh_zero", self._ptr, self.num_elements())
 
+    def _at(self, i: int) -> int:
+        """The address of element i, counted over all dims."""
+        i = int(i)
+        if not 0 <= i < self._shape._n:
+            raise IndexError(f"element {i} of {self}")
+        return self._ptr + 4 * i
+
     def __getitem__(self, i: int) -> float:
         v = np.empty(1, dtype=np.float32)
-        _lib.call("mh_memcpy_d2h", v.ctypes.data, self._ptr + 4 * int(i), 4)
+        _lib.call("mh_memcpy_d2h", v.ctypes.data, self._at(i), 4)
         return float(v[0])
 
     def __setitem__(self, i: int, val: float) -> None:
         v = np.array([val], dtype=np.float32)
-        _lib.call("mh_memcpy_h2d", self._ptr + 4 * int(i), v.ctypes.data, 4)
+        _lib.call("mh_memcpy_h2d", self._at(i), v.ctypes.data, 4)
 
     def __repr__(self) -> str:
         return f"Tensor({self._shape})"
@@ -341,12 +348,12 @@ class IndexTensor(Tensor):
 
     def __getitem__(self, i: int) -> int:
         v = np.empty(1, dtype=np.int32)
-        _lib.call("mh_memcpy_d2h", v.ctypes.data, self._ptr + 4 * int(i), 4)
+        _lib.call("mh_memcpy_d2h", v.ctypes.data, self._at(i), 4)
         return int(v[0])
 
     def __setitem__(self, i: int, val: int) -> None:
         v = np.array([val], dtype=np.int32)
-        _lib.call("mh_memcpy_h2d", self._ptr + 4 * int(i), v.ctypes.data, 4)
+        _lib.call("mh_memcpy_h2d", self._at(i), v.ctypes.data, 4)
 
     def __repr__(self) -> str:
         return f"IndexTensor({self._shape})"

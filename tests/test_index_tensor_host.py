@@ -87,3 +87,18 @@ def test_what_an_index_tensor_keeps(no_calls):
     with pytest.raises(AssertionError, match="mh_zero was called"):  # zero bits are the whole number 0
         t.zero()
     assert F(3).f32 == 4096
+
+
+@pytest.mark.parametrize("make", [F, X])
+def test_an_element_past_the_ends_is_refused(no_calls, make):
+    t = make(2, 3)
+    for i in (-1, 6, 1 << 40):
+        with pytest.raises(IndexError):
+            t[i]
+        with pytest.raises(IndexError):
+            t[i] = 1
+    for i in (0, 5):
+        with pytest.raises(AssertionError, match="mh_memcpy_d2h was called"):
+            t[i]
+        with pytest.raises(AssertionError, match="mh_memcpy_h2d was called"):
+            t[i] = 1
