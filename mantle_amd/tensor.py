@@ -324,7 +324,7 @@ class IndexTensor(Tensor):
     @staticmethod
     def from_numpy(a) -> "IndexTensor":
         a = np.asarray(a)
-        if a.dtype.kind not in "iub" or (a.size and (a.max() > 0x7fffffff or a.min() < -0x80000000)):
+        if a.size and (a.dtype.kind not in "iub" or a.max() > 0x7fffffff or a.min() < -0x80000000):
             raise ValueError(f"ids are whole numbers of 32 bits, not {a.dtype}")
         a = np.ascontiguousarray(a, dtype=np.int32)
         t = IndexTensor(TensorShape(a.shape if a.ndim else (1,)))

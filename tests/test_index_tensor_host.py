@@ -102,3 +102,13 @@ def test_an_element_past_the_ends_is_refused(no_calls, make):
             t[i]
         with pytest.raises(AssertionError, match="mh_memcpy_h2d was called"):
             t[i] = 1
+
+
+def test_no_ids_at_all(monkeypatch):
+    made = []
+    monkeypatch.setattr(m.tensor, "_initialized", True)
+    monkeypatch.setattr(_lib, "call", lambda name, *a: made.append(name))
+    for none in ([], [[]]):
+        t = m.IndexTensor.from_numpy(none)
+        assert isinstance(t, m.IndexTensor) and t.num_elements() == 0
+    assert "mh_memcpy_h2d" not in made
