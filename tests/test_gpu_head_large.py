@@ -115,3 +115,52 @@ def test_a_wide_w_whose_largest_is_at_an_end(place):
     bound["grad_w"] = bound["grad_w"] + 3 * floor.max() * np.abs(x).max() / rows
     for how in ("step", "two calls"):
         check(run(m_(), x, w, labels, how=how), want, bound, f"{place} {how}")
+
+
+def test_a_w_of_more_than_2_31_elements():
+    """[131072, 16400] = 8.6 GB: offsets that pass 32 bits, in elements and in bytes. w is 0 but for classes at the ends
+    and on either side of 2^31 and 2^32 bytes and 2^31 elements, so that the rest of the logits are 0."""
+    m = m_()
+    rows, dim, classes = 130, 16400, 131072
+    assert rows > 128 and dim * classes > 1 << 31
+    r = np.random.RandomState(66)
+    some = sorted({0, 1, classes - 1} | {b // dim + d for b in (1 << 29, 1 << 30, (1 << 31) - dim) for d in (0, 1) if b // dim + d < classes})
+    ws = (r.standard_normal((len(some), dim)) * 2 / np.sqrt(dim)).astype(np.float32)
+    x = r.standard_normal((rows, dim)).astype(np.float32)
+    labels = np.array(some, np.int32)[r.randint(0, len(some), rows)]
+    labels[3] = -1
+    w, gw, gx, loss, lse = m.Tensor(classes, dim), m.Tensor(classes, dim), m.Tensor(rows, dim), m.Tensor(1), m.Tensor(rows)
+    for v, row in zip(some, ws):
+        m._lib.call("mh_memcpy_h2d", w.ptr + 4 * v * dim, row.ctypes.data, 4 * dim)
+    print("\n[head] 2^31 elements", flush=True)
+    m.linear_cross_entropy_step(loss, gx, gw, m.Tensor.from_numpy(x), w, m.IndexTensor.from_numpy(labels),
+                                m.Tensor.from_numpy(np.float32([1])), row_lse=lse, accumulate=False)
+    keep = labels >= 0
+    n = int(keep.sum())
+    xd, wd = np.where(keep[:, None], x, 0.0).astype(np.float64), ws.astype(np.float64)
+    z = xd @ wd.T
+    total = np.exp(z).sum(1) + (classes - len(some))
+    want = np.where(keep, np.log(total), 0.0)
+    p = np.exp(z) / total[:, None]
+    hit = labels[:, None] == np.array(some)[None]
+    g = (p - hit) * keep[:, None] / n
+    # bounds of test_gpu_head.py: a product of 16400 terms, the sums of 131072 exponentials
+    U = 2.0 ** -24
+    bz = (np.abs(xd) @ np.abs(wd).T) * (2.0 ** -21 + (3 * dim / 16 + 8) * 2 * U)
+    bl = (p * bz).sum(1) + (128 + classes / 512 + 40) * U + 4 * U * want
+    assert (np.abs(lse.to_numpy() - want)[keep] <= bl[keep]).all()
+    row = want - (z * hit).sum(1)
+    assert abs(loss.to_numpy()[0] - row[keep].mean()) <= (bl + bz.max(1) + 8 * U * (want + np.abs(z).max(1))).max()
+    dg = (p * (bz + bl[:, None] + 2.0 ** -20) + 2.0 ** -22 * np.abs(g) * n + 2.0 ** -40) / n
+    off = np.abs(gx.to_numpy() - g @ wd)
+    assert (off <= dg @ np.abs(wd) + (np.abs(g) @ np.abs(wd)) * (2.0 ** -21 + 3 * 65536 / 16 * 2 * U) + 1e-12).all()
+    part = np.empty((len(some), dim), np.float32)
+    for i, v in enumerate(some):
+        m._lib.call("mh_memcpy_d2h", part[i].ctypes.data, gw.ptr + 4 * v * dim, 4 * dim)
+    off = np.abs(part - g.T @ xd)
+    assert (off <= dg.T @ np.abs(xd) + (np.abs(g).T @ np.abs(xd)) * (2.0 ** -21 + 200 * U) + 1e-12).all()
+    other = np.empty(dim, np.float32)  # a class of zeros: its probability times x
+    m._lib.call("mh_memcpy_d2h", other.ctypes.data, gw.ptr + 4 * (classes - 2) * dim, 4 * dim)
+    q = keep / total / n
+    tol = (q * (bl + 2.0 ** -20) + 2.0 ** -40 / n) @ np.abs(xd) + (q @ np.abs(xd)) * (2.0 ** -21 + 200 * U)
+    assert (np.abs(other - q @ xd) <= tol).all()
