@@ -2,7 +2,7 @@
 // without the logits as a tensor, and both gradients.
 //
 //   z = x w^T;  lse_n = log sum_v exp z_nv;  loss = mean over the kept rows of lse_n - z_n,label
-//   G = (exp(z - lse) - onehot) ug / n;  grad_x = G w;  grad_w = G^T x
+//   G = (softmax(z) - onehot) ug / n;  grad_x = G w;  grad_w = G^T x
 //
 // Three products of 2 rows classes dim operations carry the time. The matrix instructions take fp32
 // operands at a sixteenth of the fp16 rate, so every fp32 operand is held as two halves (hi, lo):
@@ -25,11 +25,11 @@
 // reads it from there without bank conflicts. Panels are padded with zeros to whole tiles, so the loop
 // over the contracted axis tests nothing.
 //
-// A step over [4096, 2048] x [131072, 2048] takes 16.3-17.0 ms: 14.2 in the three products (1350 TFLOP/s of fp16,
-// 450 of fp32-exact ones; torch's fp16 product of this shape reaches 1170-1220, its fp32 one 149), which run
-// at 1.6 GHz, where the card's power holds them: tiles of 256 x 128 two a CU, or four wavefronts of 128 x 128
-// with a third less LDS traffic, take the same time. The rest is memory: G's panels 1.2 ms at 5.3 TB/s, w's 0.6, the
-// scales 0.2.
+// A step over [4096, 2048] x [131072, 2048] takes 16.2-17.0 ms by card: 14.2-14.9 in the three products (440-465
+// TFLOP/s of fp32-exact products, three times that of fp16; torch's fp16 product of this shape reaches 1170-1220,
+// its fp32 one 149), which run at 1.57 GHz with the matrix units busy in 80 % of the cycles: the card's power holds
+// them. Tiles of 256 x 128 two a CU, or four wavefronts of 128 x 128 with a third less LDS traffic, take the same
+// time. The rest is memory: G's panels 1.2 ms at 5.3 TB/s, w's 0.6, the scales 0.2.
 #include "mh_internal.h"
 #include "mh_math.h"
 #include "mh_rows.h"
