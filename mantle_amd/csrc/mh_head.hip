@@ -693,7 +693,7 @@ __global__ __launch_bounds__(256) void k_to_g(char* z, int64_t zkb, char* gt, in
 // rows the forward gains, 429 -> 316 us, but k_few_dx would need 255 registers a thread: 1069 us a step, against
 // 895 by panels.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-constexpr int kFewRows = 64, kFewRowsForward = 128, kFewBlk = 3072;  // bytes of a block of x: three planes of 32 rows x 16
+constexpr int kFewRows = 64, kFewRowsForward = 128, kFewBlk = 3 * 1024;  // bytes of a block of x: three planes of 32 rows x 16
 
 struct Tri {
     bf16x8 h, m, l;

@@ -234,7 +234,7 @@ class Tensor:
         if owner is not None:
             try:
                 whole = owner.is_contiguous()
-            except AttributeError:  # not an array that could be strided
+            except (AttributeError, TypeError):  # not an array that could be strided
                 whole = True
             if not whole and owner.data_ptr() == ptr and tuple(owner.shape) == t._shape._dims:
                 raise _lib.MantleHipError(_lib.ERR_INVALID, "the owner's elements do not lie one after another")
