@@ -362,6 +362,62 @@ int mh_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int3
                   const float* grad_weights, const float* ug, int64_t rows, int64_t experts, int64_t k, int normalise,
                   int accumulate);
 
+/* Routing to experts by scores of a chosen kind, with a bias for balance and groups, over x [rows, experts]:
+ *   s = sigmoid(x) or softmax(x);  b = s + bias, which the choice alone reads (bias may be null);
+ *   a group is experts / groups neighbouring experts, its score the sum of its group_best (1 or 2) largest b, or of the one
+ *   it has; the keep_groups groups of the largest scores are open;
+ *   chosen [rows, k] are the k largest b in open groups, largest first;
+ *   weights [rows, k] are scale s of the chosen, divided by the sum of their s with normalise != 0;
+ *   counts [experts] is how many rows chose an expert.
+ * Everything that is compared is made in 64 bits; ties, of groups too, go to the lowest index, and a NaN comes after every
+ * number. A row with keep[row] == 0 (keep may be null) has chosen -1 and weights 0 and counts nowhere. A softmax row that
+ * holds a NaN, plus infinity or nothing but minus infinity has NaN for weights; so has a chosen sigmoid that is NaN, and
+ * with normalise its whole row, or one whose chosen scores add up to 0. Choices stay below experts.
+ * 1 <= experts <= 1024, 1 <= k <= 64, 1 <= groups <= 64, which divide experts, and k experts at least in keep_groups
+ * groups. */
+enum mh_router_scores { MH_SCORES_SOFTMAX = 0, MH_SCORES_SIGMOID = 1 };
+int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const float* x, const float* bias,
+                        const int32_t* keep, int64_t rows, int64_t experts, int64_t k, int64_t groups, int64_t keep_groups,
+                        int group_best, int scores, int normalise, float scale);
+/* The gradient of the logits from grad_weights [rows, k]; chosen is the forward's, and the choice carries no gradient; keep,
+ * scores, normalise and scale as given to it. A row that is not kept is left alone (accumulate == 0: zero). An entry of
+ * chosen outside the experts counts as none. */
+int mh_group_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int32_t* chosen, const float* grad_weights,
+                        int64_t rows, int64_t experts, int64_t k, int scores, int normalise, float scale, int accumulate);
+/* The bias' step towards balance: bias_e += rate for experts that were chosen less often than the mean of counts,
+ * -= rate for those that were chosen more often. Compared in whole numbers. */
+int mh_router_bias_update(float* bias, const int32_t* counts, int64_t experts, float rate);
+
+/* ---- norm and sampling of a language model (no reference counterpart) ---- */
+
+/* Root-mean-square norm of rows with the residual's addition: h = x + residual (residual may be null: h = x),
+ * out = h w / sqrt(mean h^2 + eps) over the dim elements of a row, sum = h (may be null). The mean is taken in 64 bits, so
+ * that no finite h is too large or too small for it. sum may be x or residual, out may be x; no others may overlap.
+ * A row with a NaN is NaN; one with infinities is NaN where they are and 0 elsewhere. dim <= 2^30. */
+int mh_rms_norm_fwd(float* out, float* sum, const float* x, const float* residual, const float* w, int64_t rows, int64_t dim,
+                    float eps);
+/* The gradient of x and of residual, which are one, and of w, from grad_out and grad_sum, the gradients of out and sum
+ * (grad_sum may be null), and h, the forward's sum: with r = 1 / sqrt(mean h^2 + eps), u = h r, g = grad_out
+ *   grad_x = grad_sum + r (w g - u mean(w g u)),  grad_w = sum over rows of g u
+ * added to grad_x and grad_w, or written over them with accumulate == 0. Either may be null. grad_x may be grad_sum or
+ * grad_out. The library's scratch grows to 4 bytes for each element of 1024 rows at most, and 8 a row of more than 16384
+ * elements. */
+int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const float* grad_sum, const float* h, const float* w,
+                    int64_t rows, int64_t dim, float eps, int accumulate);
+
+/* A token for each row of logits x [rows, classes] from u [rows], uniform numbers in [0, 1). A row's own settings, each a
+ * tensor [rows] or null for none: temperature (1 without; 0, less or NaN: the largest logit, ties to the lowest index);
+ * then of p = softmax(x / temperature), over the classes by falling logits, ties by index, those are kept that each keeps:
+ *   top_k   the first top_k (0 or less: all);
+ *   top_p   of those the fewest whose sum is at least top_p times theirs, and one at least (1, more or NaN: all);
+ *   min_p   those with p >= min_p max p (0, less or NaN: all; more than 1: those of the largest logit).
+ * tokens [rows] is the first class, by index, where the running sum of the kept p exceeds u times their sum; logprob [rows]
+ * (may be null) the logarithm of its share in that sum. A class at minus infinity is never drawn; classes at plus infinity
+ * share a row evenly. A row that holds a NaN, or nothing but minus infinity, has token -1 and logprob NaN. u is held to
+ * [0, 1); a NaN counts as 0. classes <= 2^24. */
+int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const float* u, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p, int64_t rows, int64_t classes);
+
 /* ---- graph and model: Graph (mantle/autograd/graph.mojo:33-217), Model
  * (mantle/nn/model.mojo:55-340) and its Collections (mantle/autograd/collection.mojo:24-224)
  * in device memory ---- */
@@ -488,6 +544,19 @@ int mh_adam_step(float* param, const float* grad, float* m, float* v, int64_t n,
 int mh_adam_step_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
                        float* const* v, const int64_t* sizes, float lr, float beta1, float beta2, float eps,
                        int64_t iter);
+
+/* The norm of all gradients of a model together, norm[0] = sqrt(sum g^2) over ntensors tensors, added in 64 bits; 0
+ * without any. No reference counterpart. */
+int mh_grad_norm(int64_t ntensors, const float* const* grads, const int64_t* sizes, float* norm);
+/* The same, and the gradients scaled in place by c = min(1, max_norm / norm), a float that is made from the 64-bit
+ * norm. Where one of them is infinite or NaN none is scaled; norm says so. norm may be null; max_norm is 0 or more, and
+ * infinity scales nothing. Tensors that share elements are refused. */
+int mh_clip_grad_norm(int64_t ntensors, float* const* grads, const int64_t* sizes, float max_norm, float* norm);
+/* mh_adam_step_multi with c g in the place of each gradient g, which stays as it is: 32 bytes an element instead of the
+ * 40 of the two calls, and the same bits. norm may be null. */
+int mh_adam_clip_step_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
+                            float* const* v, const int64_t* sizes, float lr, float beta1, float beta2, float eps,
+                            int64_t iter, float max_norm, float* norm);
 
 /* Seeded synthetic fill (the device counterpart of rand_uniform / rand_normal,
  * mantle/core/rand_utils.mojo:23-63): element i of stream `seed` comes from a counter-based

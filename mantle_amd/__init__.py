@@ -7,7 +7,7 @@ the CPU: if the library is missing or the device is absent, calls raise.
 """
 from ._lib import MantleHipError, lib  # noqa: F401
 from .tensor import IndexTensor, Tensor, TensorShape, init, sync  # noqa: F401
-from .optim import Adam  # noqa: F401
+from .optim import Adam, clip_grad_norm, grad_norm  # noqa: F401
 from .graph import Graph, Symbol  # noqa: F401
 from .model import Collection, Model, Parameters  # noqa: F401
 from .checkpoint import (  # noqa: F401
@@ -22,6 +22,7 @@ from .ops import (  # noqa: F401
     softmax_forward, softmax_backward, logsoftmax_forward, logsoftmax_backward, cross_entropy_forward,
     cross_entropy_backward, linear_cross_entropy_forward, linear_cross_entropy_backward, linear_cross_entropy_step,
     distill_forward, distill_backward, distill_step, router_forward, router_backward,
+    group_router_forward, group_router_backward, router_bias_update, rms_norm_forward, rms_norm_backward, sample_tokens,
 )
 
 __all__ = [
@@ -32,6 +33,7 @@ __all__ = [
     "softmax_backward", "logsoftmax_forward", "logsoftmax_backward", "cross_entropy_forward",
     "cross_entropy_backward", "IndexTensor", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
     "linear_cross_entropy_step", "distill_forward", "distill_backward", "distill_step", "router_forward",
-    "router_backward", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
+    "router_backward", "group_router_forward", "group_router_backward", "router_bias_update", "rms_norm_forward",
+    "rms_norm_backward", "sample_tokens", "clip_grad_norm", "grad_norm", "CheckpointError", "CheckpointInfo", "save_checkpoint", "save_checkpoint_with_optim",
     "load_checkpoint", "load_checkpoint_with_optim",
 ]

@@ -67,6 +67,7 @@ FROM_HOST, FROM_DEVICE = 0, 1
 MODEL_FUSE_BIAS_RELU = 1
 MODEL_FUSE_ROWS = 2
 PASS_FORWARD, PASS_BACKWARD, PASS_STEP = 0, 1, 2
+SCORES_SOFTMAX, SCORES_SIGMOID = 0, 1
 
 
 class MantleHipError(RuntimeError):
@@ -136,6 +137,12 @@ SIGNATURES = {
     "mh_distill_step": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _F, _I],
     "mh_router_fwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I],
     "mh_router_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I, _I],
+    "mh_group_router_fwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I, _I, _I, _F],
+    "mh_group_router_bwd": [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I, _I, _F, _I],
+    "mh_router_bias_update": [_VP, _VP, _I64, _F],
+    "mh_rms_norm_fwd": [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _F],
+    "mh_rms_norm_bwd": [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _F, _I],
+    "mh_sample_tokens": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64],
     "mh_fma_fwd": [_VP, _VP, _VP, _VP, _I64],
     "mh_fma_bwd_accum": [_I, _VP, _VP, _VP, _VP, _I64],
     "mh_leakyrelu_fwd": [_VP, _VP, _I64, _F],
@@ -146,6 +153,10 @@ SIGNATURES = {
     "mh_adam_step": [_VP, _VP, _VP, _VP, _I64, _F, _F, _F, _F, _I64],
     "mh_adam_step_multi": [_I64, ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.POINTER(_VP),
                            ctypes.POINTER(_I64), _F, _F, _F, _F, _I64],
+    "mh_grad_norm": [_I64, ctypes.POINTER(_VP), ctypes.POINTER(_I64), _VP],
+    "mh_clip_grad_norm": [_I64, ctypes.POINTER(_VP), ctypes.POINTER(_I64), _F, _VP],
+    "mh_adam_clip_step_multi": [_I64, ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.POINTER(_VP),
+                                ctypes.POINTER(_I64), _F, _F, _F, _F, _I64, _F, _VP],
     "mh_rand_uniform": [_VP, _I64, ctypes.c_uint64, _F, _F],
     "mh_rand_normal": [_VP, _I64, ctypes.c_uint64, _F, _F],
     "mh_event_create": [ctypes.POINTER(_VP)],

@@ -1,0 +1,527 @@
+// mh_group_router.hip -- routing to experts by sigmoid or softmax scores, with a bias for balance, groups of experts and
+// a scale; the gradient of the logits; and the bias' step towards balance.
+//
+//   s = sigmoid(x) | softmax(x);  b = s + bias;  a group's score = the sum of its one or two largest b;
+//   chosen = the k largest b in the keep_groups best groups;  weights = scale s_chosen, or scale q with q = s / sum s
+//   With g the weights' gradient (0 where not chosen):
+//     sigmoid:  grad_i = scale s_i (1 - s_i) g_i            normalised: scale q_i (1 - s_i) (g_i - sum g q)
+//     softmax:  grad_j = scale p_j (g_j - sum g p)          normalised: scale q_i (g_i - sum g q)
+//
+// Scores decide a choice after a bias was added to them, so logits do not: experts whose biased scores agree to fp32 are
+// not rare over a long batch, and which of them is chosen shows. Scores, biased scores and groups' sums are therefore made
+// in 64 bits (an exponential's Taylor series, 13 terms within half of ln 2); weights and gradients are fp32.
+// Bound by the logits' read and the gradient's write, and over many experts by the scores' arithmetic. L lanes hold a row
+// in registers, V elements a lane in quads (element 4 (i L + lane) + c).
+#include "mh_internal.h"
+#include "mh_rows.h"
+
+namespace mh {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChosen = 64;
+constexpr int kMaxGroups = 64;
+constexpr int kRThreads = 256;
+constexpr int kRBlocks = 1024;  // workgroups of a forward at most: rows of its partial counts
+
+struct GroupArg {
+    const float* x;
+    const float* bias;    // or null
+    const int32_t* keep;  // or null: every row
+    int64_t rows;
+    int32_t experts, k;
+    int32_t groups, each, open, best;  // each: experts of a group
+    int32_t sigmoid, normalise, accumulate;
+    float scale;
+    FastDiv by_each;
+    // forward
+    float* weights;
+    int32_t* chosen;
+    int32_t* part_c;  // [blocks][experts]
+    // backward
+    float* grad;
+    const float* gw;
+    const int32_t* sel;
+};
+
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+// The value of the lane STEP beside, within groups of neighbouring lanes.
+template <int STEP>
+__device__ __forceinline__ int other_lane(int v) {
+    return STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(v) : STEP == 8 ? dpp<0x140>(v)
+                                                                                                  : __shfl_xor(v, STEP);
+}
+template <int STEP>
+__device__ __forceinline__ double other_lane(double v) {
+    return __hiloint2double(other_lane<STEP>(__double2hiint(v)), other_lane<STEP>(__double2loint(v)));
+}
+template <int STEP>
+__device__ __forceinline__ int64_t other_lane(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)other_lane<STEP>((int)(v >> 32)) << 32 | (uint32_t)other_lane<STEP>((int)v));
+}
+template <int STEP>
+__device__ __forceinline__ float other_lane(float v) { return __int_as_float(other_lane<STEP>(__float_as_int(v))); }
+// Reductions over groups of L neighbouring lanes, the result in every lane.
+template <int L, int STEP = 1, typename T, typename Op>
+__device__ __forceinline__ T group_red(T v, Op op) {
+    if constexpr (STEP < L) return group_red<L, 2 * STEP>(op(v, other_lane<STEP>(v)), op);
+    return v;
+}
+template <int L, typename T>
+__device__ __forceinline__ T group_sum(T v) { return group_red<L>(v, [](T p, T q) { return p + q; }); }
+template <int L>
+__device__ __forceinline__ float group_max(float v) { return group_red<L>(v, [](float p, float q) { return __builtin_fmaxf(p, q); }); }
+
+// A wavefront's LDS accesses so far come before those that follow.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// e^x for x <= 0 (a NaN stays one), to about an ulp: 2^n e^r, |r| <= ln(2) / 2, by Taylor's series.
+__device__ __forceinline__ double exp64(double x) {
+    x = x < -1000.0 ? -1000.0 : x;
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(n, -0.69314718055994530942, x);
+    r = __builtin_fma(n, -2.3190468138462996e-17, r);  // the rest of ln 2
+    double p = 1.0 / 6227020800.0;
+    p = __builtin_fma(p, r, 1.0 / 479001600.0);
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+__device__ __forceinline__ double sigmoid64(float x) {
+    const double e = exp64(-__builtin_fabs((double)x));
+    return (x < 0.0f ? e : 1.0) / (1.0 + e);
+}
+
+// A double as an integer of the same order; NaN below every number, -0 as +0; below them what may not be chosen.
+constexpr int64_t kNever = INT64_MIN;
+__device__ __forceinline__ int64_t sort_key(double v) {
+    const int64_t b = __double_as_longlong(v + 0.0);
+    return v != v ? kNever + 1 : (b < 0 ? b ^ 0x7fffffffffffffffll : b);
+}
+
+// Loads lane l's elements of a row; past the experts `none`.
+template <int L, int V>
+__device__ __forceinline__ void load_row(const float* row, int E, int l, float* v, float none) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        const int c = 4 * (i * L + l);
+        if (c + 3 < E) {
+            const vf4 q = *reinterpret_cast<const vf4u*>(row + c);
+            v[4 * i] = q.x;
+            v[4 * i + 1] = q.y;
+            v[4 * i + 2] = q.z;
+            v[4 * i + 3] = q.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = c + j < E ? row[c + j] : none;
+        }
+    }
+}
+
+// The k largest of a row's biased scores b, by rounds of a maximum: exact for any b. pick_id and pick_s get the
+// experts and their scores s, largest b first.
+template <int L, int V>
+__device__ __forceinline__ void choose_rounds(const double* b, const float* s, const bool* open, int k, int l, int32_t* pick_id,
+                                              float* pick_s) {
+    int64_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = open[i] ? sort_key(b[i]) : kNever;
+    for (int t = 0; t < k; ++t) {
+        int64_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
+        best = group_red<L>(best, [](int64_t p, int64_t q) { return p > q ? p : q; });
+        int at = 0x7fffffff;  // the lowest index that holds it
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? 4 * (i / 4) * L + (i & 3) + 4 * l : at;
+        at = group_red<L>(at, [](int p, int q) { return p < q ? p : q; });
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at == 4 * (i / 4) * L + (i & 3) + 4 * l) {
+                key[i] = kNever;
+                pick_id[t] = at;
+                pick_s[t] = s[i];
+            }
+    }
+}
+
+template <int L, int V>
+__global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
+    constexpr int G = kRThreads / L;  // rows in flight in a workgroup
+    constexpr int K = L * V < kMaxChosen ? L * V : kMaxChosen;
+    constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
+    __shared__ int32_t cnt[L * V];
+    __shared__ float pick_s[G][K];
+    __shared__ int32_t pick_id[G][K];
+    __shared__ double row[G][L * V], of_group[G][N];
+    const int tid = threadIdx.x, l = tid % L, g = tid / L;
+    for (int e = tid; e < L * V; e += kRThreads) cnt[e] = 0;
+    __syncthreads();
+    float bias[V];
+    int gid[V];
+    if (a.bias) {
+        load_row<L, V>(a.bias, a.experts, l, bias, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) bias[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) gid[i] = (int)fdiv((uint32_t)(4 * ((i / 4) * L + l) + (i & 3)), a.by_each);
+    const int64_t stride = (int64_t)gridDim.x * G;
+    // every wavefront walks whole rounds, so that its lanes reduce together
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += stride) {
+        const int64_t r = r0 + g;
+        const bool in = r < a.rows;
+        const bool keep = in && (!a.keep || a.keep[r] != 0);
+        float x[V], s[V];
+        double b[V];
+        load_row<L, V>(a.x + (in ? r : r0) * a.experts, a.experts, l, x, -__builtin_inff());
+        if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) b[i] = sigmoid64(x[i]);
+        } else {
+            float m = x[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) m = __builtin_fmaxf(m, x[i]);
+            m = group_max<L>(m);
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                b[i] = exp64((double)x[i] - (double)m);
+                sum += b[i];
+            }
+            sum = group_sum<L>(sum);
+#pragma unroll
+            for (int i = 0; i < V; ++i) b[i] = b[i] / sum;
+        }
+        bool open[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = (float)b[i];
+            b[i] += (double)bias[i];
+            open[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts;
+        }
+        if (a.groups > 1) {
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < V; ++i) row[g][4 * ((i / 4) * L + l) + (i & 3)] = b[i];
+            wave_sync();
+            for (int j = l; j < a.groups; j += L) {
+                const double* v = row[g] + j * a.each;
+                double first = v[0], second = 0.0;
+                bool two = false;
+                for (int e = 1; e < a.each; ++e) {
+                    const double c = v[e];
+                    if (c > first || first != first) {  // a NaN gives way to a number
+                        second = first;
+                        first = c;
+                    } else if (!two || c > second || second != second) {
+                        second = c;
+                    }
+                    two = true;
+                }
+                of_group[g][j] = a.best == 2 && two ? first + second : first;
+            }
+            wave_sync();
+            uint64_t mask = 0;
+            for (int j = l; j < a.groups; j += L) {
+                const double c = of_group[g][j];
+                const bool none = c != c;
+                int before = 0;
+                for (int o = 0; o < a.groups; ++o) {
+                    const double d = of_group[g][o];
+                    before += d > c || (none && d == d) || (o < j && (d == c || (none && d != d)));
+                }
+                if (before < a.open) mask |= (uint64_t)1 << j;
+            }
+            mask = (uint64_t)group_red<L>((int64_t)mask, [](int64_t p, int64_t q) { return p | q; });
+#pragma unroll
+            for (int i = 0; i < V; ++i) open[i] = open[i] && ((mask >> (gid[i] & 63)) & 1) != 0;
+        }
+        wave_sync();
+        choose_rounds<L, V>(b, s, open, a.k, l, pick_id[g], pick_s[g]);
+        wave_sync();
+        float total = 1.0f;
+        if (a.normalise) {
+            total = 0.0f;
+            for (int t = l; t < a.k; t += L) total += pick_s[g][t];
+            total = group_sum<L>(total);
+        }
+        if (in)
+            for (int t = l; t < a.k; t += L) {
+                const int32_t id = pick_id[g][t];
+                a.chosen[r * a.k + t] = keep ? id : -1;
+                a.weights[r * a.k + t] = keep ? a.scale * (pick_s[g][t] / total) : 0.0f;
+                if (keep) atomicAdd(&cnt[id], 1);
+            }
+    }
+    __syncthreads();
+    for (int e = tid; e < a.experts; e += kRThreads) a.part_c[(int64_t)blockIdx.x * a.experts + e] = cnt[e];
+}
+
+// The counts from the workgroups' partials: 32 experts and 8 shares of the partials a workgroup.
+__global__ __launch_bounds__(kRThreads) void k_group_router_counts(const int32_t* part, int32_t blocks, int32_t experts,
+                                                                   int32_t* counts) {
+    __shared__ int32_t buf[kRThreads];
+    const int e = blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
+    int32_t s = 0;
+    if (e < experts) {
+#pragma unroll 8
+        for (int b = share; b < blocks; b += 8) s += part[(int64_t)b * experts + e];
+    }
+    buf[threadIdx.x] = s;
+    __syncthreads();
+    if (share != 0 || e >= experts) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += buf[32 * i + (threadIdx.x & 31)];
+    counts[e] = s;
+}
+
+// What the chosen get goes to a row of LDS at their experts; a softmax's every expert gets its own part.
+template <int L, int V>
+__global__ __launch_bounds__(kRThreads) void k_group_router_bwd(GroupArg a) {
+    constexpr int G = kRThreads / L;
+    __shared__ __attribute__((aligned(16))) float mark[G][L * V];
+    const int l = threadIdx.x % L, g = threadIdx.x / L;
+    const int64_t stride = (int64_t)gridDim.x * G;
+    const bool whole = !a.sigmoid && !a.normalise;  // every expert has a gradient
+    for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += stride) {
+        const int64_t r = r0 + g;
+        const bool in = r < a.rows;
+        const bool keep = in && (!a.keep || a.keep[r] != 0);
+        const int64_t at = (in ? r : r0) * a.experts;
+        float v[V], inv = 0.0f, top = 0.0f;
+        if (whole) {
+            load_row<L, V>(a.x + at, a.experts, l, v, -__builtin_inff());
+            top = v[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, v[i]);
+            top = group_max<L>(top);
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i] = exp_neg(v[i] - top);
+                sum += v[i];
+            }
+            inv = 1.0f / group_sum<L>(sum);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = 0.0f;
+            if (!a.sigmoid) {  // the chosen's maximum
+                top = -__builtin_inff();
+                if (keep)
+                    for (int c = l; c < a.k; c += L) {
+                        const int32_t id = a.sel[r * a.k + c];
+                        if (id >= 0 && id < a.experts) top = __builtin_fmaxf(top, a.x[at + id]);
+                    }
+                top = group_max<L>(top);
+            }
+        }
+        // score s of an entry, or its exponential, and what of a sigmoid its derivative leaves
+        auto score = [&](int32_t id, float& rest) {
+            const float x = a.x[at + id];
+            rest = 1.0f;
+            if (!a.sigmoid) return exp_neg(x - top) * (whole ? inv : 1.0f);
+            const float e = exp_neg(-__builtin_fabsf(x)), d = 1.0f / (1.0f + e);
+            rest = x < 0.0f ? d : e * d;
+            return x < 0.0f ? e * d : d;
+        };
+        float all = 0.0f, inner = 0.0f;
+        if (keep)
+            for (int c = l; c < a.k; c += L) {
+                const int32_t id = a.sel[r * a.k + c];
+                if (id < 0 || id >= a.experts) continue;
+                float rest;
+                const float s = score(id, rest);
+                all += s;
+                inner += s * a.gw[r * a.k + c];
+            }
+        all = group_sum<L>(all);
+        inner = group_sum<L>(inner);
+        const float by = a.normalise ? 1.0f / all : 1.0f;
+        inner *= by;
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            vf4 q = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            *reinterpret_cast<vf4*>(&mark[g][4 * (i * L + l)]) = whole ? q * (-inv * inner) : q;
+        }
+        wave_sync();
+        if (keep)
+            for (int c = l; c < a.k; c += L) {
+                const int32_t id = a.sel[r * a.k + c];
+                if (id < 0 || id >= a.experts) continue;
+                float rest;
+                const float s = score(id, rest), gr = a.gw[r * a.k + c];
+                mark[g][id] = s * by * rest * (a.normalise || whole ? gr - inner : gr);
+            }
+        wave_sync();
+        if (!in || (!keep && a.accumulate)) continue;  // a padding row: as it was, or zero
+        float* o = a.grad + at;
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const int c = 4 * (i * L + l);
+            vf4 q = *reinterpret_cast<const vf4*>(&mark[g][c]);
+            q = keep ? q * a.scale : vf4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (c + 3 < a.experts) {
+                if (a.accumulate) q = q + ld_ntu(o + c);
+                st_ntu(o + c, q);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < a.experts) o[c + j] = a.accumulate ? o[c + j] + q[j] : q[j];
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(kRThreads) void k_router_bias(float* bias, const int32_t* counts, int64_t experts, float rate) {
+    __shared__ int64_t red[kRThreads / 64];
+    int64_t total = 0;
+    for (int64_t e = threadIdx.x; e < experts; e += kRThreads) total += counts[e];
+    total = block_sum<kRThreads / 64>(total, red);
+    for (int64_t e = threadIdx.x; e < experts; e += kRThreads) {
+        const int64_t c = counts[e] * experts;
+        if (c < total) bias[e] += rate;
+        if (c > total) bias[e] -= rate;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------
+#define MH_ROUTER(CALL)                      \
+    do {                                     \
+        if (a.experts <= 8) CALL(2, 4);      \
+        else if (a.experts <= 16) CALL(4, 4);   \
+        else if (a.experts <= 32) CALL(4, 8);   \
+        else if (a.experts <= 64) CALL(8, 8);   \
+        else if (a.experts <= 128) CALL(16, 8); \
+        else if (a.experts <= 256) CALL(32, 8); \
+        else if (a.experts <= 512) CALL(64, 8); \
+        else CALL(64, 16);                   \
+    } while (0)
+
+int router_lanes(int experts) {
+    return experts <= 8 ? 2 : experts <= 32 ? 4 : experts <= 64 ? 8 : experts <= 128 ? 16 : experts <= 256 ? 32 : 64;
+}
+
+int router_check(const char* what, int64_t rows, int64_t experts, int64_t k, int scores, float scale) {
+    if (rows < 0 || experts < 1 || experts > kMaxExperts || k < 1 || k > kMaxChosen || k > experts)
+        return fail(MH_ERR_INVALID, "%s: needs rows >= 0, 1 <= experts <= %d, 1 <= k <= min(%d, experts) (%lld, %lld, %lld)",
+                    what, kMaxExperts, kMaxChosen, (long long)rows, (long long)experts, (long long)k);
+    if (scores != MH_SCORES_SOFTMAX && scores != MH_SCORES_SIGMOID) return fail(MH_ERR_INVALID, "%s: scores %d", what, scores);
+    if (!(scale >= -3.4028234663852886e38f && scale <= 3.4028234663852886e38f))
+        return fail(MH_ERR_INVALID, "%s: scale %g is not finite", what, (double)scale);
+    if (rows > 0x7fffffff / k) return fail(MH_ERR_OVERFLOW, "%s: more than 2^31 - 1 choices", what);
+    return MH_OK;
+}
+
+}  // namespace
+}  // namespace mh
+
+using namespace mh;
+
+extern "C" {
+
+int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const float* x, const float* bias,
+                        const int32_t* keep, int64_t rows, int64_t experts, int64_t k, int64_t groups, int64_t keep_groups,
+                        int group_best, int scores, int normalise, float scale) {
+    MH_TRACE("mh_group_router_fwd");
+    MH_TRY(router_check("mh_group_router_fwd", rows, experts, k, scores, scale));
+    if (groups < 1 || groups > kMaxGroups || experts % groups != 0 || keep_groups < 1 || keep_groups > groups ||
+        keep_groups * (experts / groups) < k || (group_best != 1 && group_best != 2))
+        return fail(MH_ERR_INVALID,
+                    "mh_group_router_fwd: needs 1 <= groups <= %d that divide %lld experts, 1 <= keep_groups <= groups with %lld "
+                    "experts at least, group_best 1 or 2 (%lld, %lld, %d)",
+                    kMaxGroups, (long long)experts, (long long)k, (long long)groups, (long long)keep_groups, group_best);
+    if (!counts || (rows > 0 && (!weights || !chosen || !x))) return fail(MH_ERR_NULL, "mh_group_router_fwd: null tensor");
+    MH_TRY(require_init());
+    if (rows == 0) return mh_zero(reinterpret_cast<float*>(counts), experts);  // zero bits are the whole number 0 too
+    GroupArg a = {};
+    a.x = x;
+    a.bias = bias;
+    a.keep = keep;
+    a.rows = rows;
+    a.experts = (int32_t)experts;
+    a.k = (int32_t)k;
+    // where every group stays open there is nothing to sort out
+    a.groups = keep_groups == groups ? 1 : (int32_t)groups;
+    a.each = (int32_t)(experts / groups);
+    a.open = (int32_t)keep_groups;
+    a.best = group_best;
+    a.by_each = make_fastdiv((uint32_t)a.each);
+    a.sigmoid = scores == MH_SCORES_SIGMOID;
+    a.normalise = normalise != 0;
+    a.scale = scale;
+    a.weights = weights;
+    a.chosen = chosen;
+    const int64_t group = kRThreads / router_lanes(a.experts);
+    int64_t blocks = (rows + group - 1) / group;
+    if (blocks > kRBlocks) blocks = kRBlocks;
+    MH_TRY(scratch((size_t)blocks * experts * 4, reinterpret_cast<void**>(&a.part_c)));
+    hipStream_t st = ctx().stream;
+#define MH_CALL(L, V) hipLaunchKernelGGL((k_group_router_fwd<L, V>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a)
+    MH_ROUTER(MH_CALL);
+#undef MH_CALL
+    hipLaunchKernelGGL(k_group_router_counts, dim3((unsigned)((experts + 31) / 32)), dim3(kRThreads), 0, st, a.part_c,
+                       (int32_t)blocks, a.experts, counts);
+    return finish("mh_group_router_fwd");
+}
+
+int mh_group_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int32_t* chosen, const float* grad_weights,
+                        int64_t rows, int64_t experts, int64_t k, int scores, int normalise, float scale, int accumulate) {
+    MH_TRACE("mh_group_router_bwd");
+    MH_TRY(router_check("mh_group_router_bwd", rows, experts, k, scores, scale));
+    if (rows == 0) return MH_OK;
+    if (!grad_x || !x || !chosen || !grad_weights) return fail(MH_ERR_NULL, "mh_group_router_bwd: null tensor");
+    MH_TRY(require_init());
+    GroupArg a = {};
+    a.x = x;
+    a.keep = keep;
+    a.rows = rows;
+    a.experts = (int32_t)experts;
+    a.k = (int32_t)k;
+    a.sigmoid = scores == MH_SCORES_SIGMOID;
+    a.normalise = normalise != 0;
+    a.accumulate = accumulate != 0;
+    a.scale = scale;
+    a.grad = grad_x;
+    a.gw = grad_weights;
+    a.sel = chosen;
+    const int64_t group = kRThreads / router_lanes(a.experts);
+    int64_t blocks = (rows + group - 1) / group;
+    if (blocks > 2048) blocks = 2048;
+    hipStream_t st = ctx().stream;
+#define MH_CALL(L, V) hipLaunchKernelGGL((k_group_router_bwd<L, V>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a)
+    MH_ROUTER(MH_CALL);
+#undef MH_CALL
+    return finish("mh_group_router_bwd");
+}
+
+int mh_router_bias_update(float* bias, const int32_t* counts, int64_t experts, float rate) {
+    MH_TRACE("mh_router_bias_update");
+    if (experts < 1 || experts > kMaxExperts) return fail(MH_ERR_INVALID, "mh_router_bias_update: 1 <= experts <= %d (%lld)", kMaxExperts, (long long)experts);
+    if (!(rate >= -3.4028234663852886e38f && rate <= 3.4028234663852886e38f))
+        return fail(MH_ERR_INVALID, "mh_router_bias_update: rate %g is not finite", (double)rate);
+    if (!bias || !counts) return fail(MH_ERR_NULL, "mh_router_bias_update: null tensor");
+    MH_TRY(require_init());
+    hipLaunchKernelGGL(k_router_bias, dim3(1), dim3(kRThreads), 0, ctx().stream, bias, counts, experts, rate);
+    return finish("mh_router_bias_update");
+}
+
+}  // extern "C"

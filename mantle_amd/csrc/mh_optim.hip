@@ -14,9 +14,19 @@
 // optim.mojo:140): threads walk the concatenated element quads of the launch's tensors and
 // find their tensor by a wave-uniform binary search in a table passed by value, so a model of
 // many small tensors costs a launch per 80 tensors, not one per tensor.
+//
+// mh_grad_norm, mh_clip_grad_norm, mh_adam_clip_step_multi: the norm of all gradients together,
+// N = sqrt(sum g^2), and c = min(1, max_norm / N) times them, in place or on their way into Adam
+// (which saves the 8 bytes an element of writing them and reading them again). Bound by memory: 4
+// bytes an element for the norm, 8 more to scale them, 28 for Adam. The squares are added in 64
+// bits, which any fp32 gradient's fit: per thread, per workgroup, and over the workgroups by one
+// workgroup, always in the same order.
+#include <algorithm>
 #include <cmath>
+#include <new>
 
 #include "mh_internal.h"
+#include "mh_rows.h"
 
 namespace mh {
 
@@ -60,12 +70,14 @@ __device__ __forceinline__ void adam1(float& p, float g, float& m, float& v, con
 }
 
 // Elements [e0, e0 + cnt) of one tensor, cnt <= 4; a full quad at a 16-byte aligned address
-// moves as float4.
+// moves as float4. CLIP: the gradients count c times.
+template <bool CLIP>
 __device__ __forceinline__ void adam_unit(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
-                                          float* __restrict__ v, int64_t e0, int cnt, bool vec, const AdamScal& s) {
+                                          float* __restrict__ v, int64_t e0, int cnt, bool vec, const AdamScal& s, float c) {
     if (cnt == 4 && vec) {
         float4 pp = ld_nt4(p + e0, 0);
-        const float4 gg = ld_nt4(g + e0, 0);
+        float4 gg = ld_nt4(g + e0, 0);
+        if (CLIP) gg = make_float4(gg.x * c, gg.y * c, gg.z * c, gg.w * c);
         float4 mm = ld_nt4(m + e0, 0);
         float4 vv = ld_nt4(v + e0, 0);
         adam1(pp.x, gg.x, mm.x, vv.x, s);
@@ -78,7 +90,7 @@ __device__ __forceinline__ void adam_unit(float* __restrict__ p, const float* __
     } else {
         for (int j = 0; j < cnt; ++j) {
             float pp = p[e0 + j], mm = m[e0 + j], vv = v[e0 + j];
-            adam1(pp, g[e0 + j], mm, vv, s);
+            adam1(pp, CLIP ? g[e0 + j] * c : g[e0 + j], mm, vv, s);
             p[e0 + j] = pp;
             m[e0 + j] = mm;
             v[e0 + j] = vv;
@@ -98,13 +110,14 @@ struct UnitMap {
 
 __host__ __device__ __forceinline__ int64_t adam_units(int64_t n, int sh) { return (n + sh + 3) >> 2; }
 
+template <bool CLIP>
 __device__ __forceinline__ void adam_unit_k(float* __restrict__ p, const float* __restrict__ g,
                                             float* __restrict__ m, float* __restrict__ v, int64_t n, int64_t k,
-                                            UnitMap um, const AdamScal& s) {
+                                            UnitMap um, const AdamScal& s, float c) {
     const int64_t lo = 4 * k - um.sh;
     const int64_t e0 = lo < 0 ? 0 : lo;
     const int64_t e1 = (lo + 4) < n ? (lo + 4) : n;
-    adam_unit(p, g, m, v, e0, (int)(e1 - e0), um.vec != 0, s);
+    adam_unit<CLIP>(p, g, m, v, e0, (int)(e1 - e0), um.vec != 0, s, c);
 }
 
 static inline UnitMap unit_map(const void* p, const void* g, const void* m, const void* v) {
@@ -124,20 +137,22 @@ __global__ void __launch_bounds__(kOThreads)
     const int64_t units = adam_units(n, um.sh);
     const int64_t stride = (int64_t)gridDim.x * kOThreads;
     for (int64_t u = (int64_t)blockIdx.x * kOThreads + threadIdx.x; u < units; u += stride)
-        adam_unit_k(p, g, m, v, n, u, um, s);
+        adam_unit_k<false>(p, g, m, v, n, u, um, s, 1.0f);
 }
 
 // The common case of k_adam (all four tensors 16-byte aligned, sh == 0): thread q takes quad q,
 // with no unit arithmetic; the last n % 4 elements go to the thread after the last quad.
+template <bool CLIP>
 __global__ void __launch_bounds__(kOThreads)
     k_adam_al(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
-              int64_t n, AdamScal s) {
+              int64_t n, AdamScal s, const float* __restrict__ coef) {
+    const float c = CLIP ? coef[0] : 1.0f;
     const int64_t q = (int64_t)blockIdx.x * kOThreads + threadIdx.x;
     const int64_t nq = n >> 2;
     if (q < nq) {
-        adam_unit(p, g, m, v, 4 * q, 4, true, s);
+        adam_unit<CLIP>(p, g, m, v, 4 * q, 4, true, s, c);
     } else if (q == nq && (n & 3) != 0) {
-        adam_unit(p, g, m, v, 4 * q, (int)(n & 3), false, s);
+        adam_unit<CLIP>(p, g, m, v, 4 * q, (int)(n & 3), false, s, c);
     }
 }
 
@@ -168,7 +183,9 @@ struct AdamTable {
 // Each tensor starts on a wave boundary of the concatenated quad space (unit0 a multiple of
 // 64), so a wave belongs to one tensor: the search runs once per wave on wave-uniform values
 // (scalar loads from the kernel arguments), and lanes past the tensor's end idle.
-__global__ void __launch_bounds__(kOThreads) k_adam_multi(AdamTable tab, int64_t units, AdamScal s) {
+template <bool CLIP>
+__global__ void __launch_bounds__(kOThreads) k_adam_multi(AdamTable tab, int64_t units, AdamScal s, const float* coef) {
+    const float c = CLIP ? coef[0] : 1.0f;
     const int64_t stride = (int64_t)gridDim.x * kOThreads;
     const int wid = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = (int)(threadIdx.x & 63);
@@ -182,7 +199,7 @@ __global__ void __launch_bounds__(kOThreads) k_adam_multi(AdamTable tab, int64_t
         const AdamTensor& t = tab.t[lo];
         const UnitMap um = t.um();
         const int64_t k = uw - t.unit0() + lane;
-        if (k < adam_units(t.n, um.sh)) adam_unit_k(t.p, t.g, t.m, t.v, t.n, k, um, s);
+        if (k < adam_units(t.n, um.sh)) adam_unit_k<CLIP>(t.p, t.g, t.m, t.v, t.n, k, um, s, c);
     }
 }
 
@@ -207,47 +224,21 @@ static int check_hyper(const char* what, float lr, float b1, float b2, float eps
     return MH_OK;
 }
 
-}  // namespace mh
-
-using namespace mh;
-
-extern "C" {
-
-int mh_adam_step(float* param, const float* grad, float* m, float* v, int64_t n, float lr, float beta1,
-                 float beta2, float eps, int64_t iter) {
-    MH_TRACE("mh_adam_step");
-    MH_TRY(check_hyper("mh_adam_step", lr, beta1, beta2, eps, iter));
-    if (n < 0) return fail(MH_ERR_INVALID, "mh_adam_step: negative count");
-    if (n == 0) return MH_OK;
-    if (!param || !grad || !m || !v) return fail(MH_ERR_NULL, "mh_adam_step: null tensor");
-    MH_TRY(require_init());
-    const AdamScal s = adam_scalars(lr, beta1, beta2, eps, iter);
-    const UnitMap um = unit_map(param, grad, m, v);
-    const LaunchShape ls = adam_shape(n, um);
-    if (ls.kernel == 0)
-        hipLaunchKernelGGL(k_adam_al, dim3((unsigned)ls.blocks), dim3(ls.threads), 0, ctx().stream, param, grad, m, v,
-                           n, s);
-    else
-        hipLaunchKernelGGL(k_adam, dim3((unsigned)ls.blocks), dim3(ls.threads), 0, ctx().stream, param, grad, m, v, n,
-                           um, s);
-    return finish("mh_adam_step");
+static int check_adam(const char* what, int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
+                      float* const* v, const int64_t* sizes) {
+    if (ntensors < 0) return fail(MH_ERR_INVALID, "%s: negative tensor count", what);
+    if (ntensors > 0 && (!params || !grads || !m || !v || !sizes)) return fail(MH_ERR_NULL, "%s: null table", what);
+    for (int64_t i = 0; i < ntensors; ++i) {  // validate everything before any launch
+        if (sizes[i] < 0) return fail(MH_ERR_INVALID, "%s: negative size of tensor %lld", what, (long long)i);
+        if (sizes[i] > 0 && (!params[i] || !grads[i] || !m[i] || !v[i]))
+            return fail(MH_ERR_NULL, "%s: null pointer in tensor %lld", what, (long long)i);
+    }
+    return MH_OK;
 }
 
-int mh_adam_step_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
-                       float* const* v, const int64_t* sizes, float lr, float beta1, float beta2, float eps,
-                       int64_t iter) {
-    MH_TRACE("mh_adam_step_multi");
-    MH_TRY(check_hyper("mh_adam_step_multi", lr, beta1, beta2, eps, iter));
-    if (ntensors < 0) return fail(MH_ERR_INVALID, "mh_adam_step_multi: negative tensor count");
-    if (ntensors == 0) return MH_OK;
-    if (!params || !grads || !m || !v || !sizes) return fail(MH_ERR_NULL, "mh_adam_step_multi: null table");
-    for (int64_t i = 0; i < ntensors; ++i) {  // validate everything before any launch
-        if (sizes[i] < 0) return fail(MH_ERR_INVALID, "mh_adam_step_multi: negative size of tensor %lld", (long long)i);
-        if (sizes[i] > 0 && (!params[i] || !grads[i] || !m[i] || !v[i]))
-            return fail(MH_ERR_NULL, "mh_adam_step_multi: null pointer in tensor %lld", (long long)i);
-    }
-    MH_TRY(require_init());
-    const AdamScal s = adam_scalars(lr, beta1, beta2, eps, iter);
+template <bool CLIP>
+static void adam_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m, float* const* v,
+                       const int64_t* sizes, const AdamScal& s, const float* coef) {
     AdamTable tab;
     int64_t i = 0;
     while (i < ntensors) {
@@ -266,9 +257,279 @@ int mh_adam_step_multi(int64_t ntensors, float* const* params, const float* cons
             units += (adam_units(t.n, um.sh) + 63) & ~int64_t(63);  // next tensor starts on a wave
         }
         if (tab.nt > 0)
-            hipLaunchKernelGGL(k_adam_multi, dim3(grid_units(units)), dim3(kOThreads), 0, ctx().stream, tab, units, s);
+            hipLaunchKernelGGL(k_adam_multi<CLIP>, dim3(grid_units(units)), dim3(kOThreads), 0, ctx().stream, tab, units, s,
+                               coef);
     }
+}
+
+// ---------------------------------------------------------------------------------------
+// the norm of many gradients
+// ---------------------------------------------------------------------------------------
+constexpr int kGradThreads = 256;
+constexpr int kGradQuads = 4;                                          // quads a thread and chunk
+constexpr int64_t kGradChunk = (int64_t)kGradThreads * kGradQuads;     // quads of a chunk
+constexpr int64_t kGradBlocks = 2048;                                  // workgroups of a launch at most
+constexpr int kGradPerLaunch = 160;                                    // 3.8 KB of the 4 KB that arguments may take
+
+// A tensor and the first chunk of it in the launch's chunks. Quad k of a tensor whose address is sh floats past a
+// 16-byte boundary holds the elements [4k - sh, 4k - sh + 4) that it has, so whole quads are aligned.
+struct GradTensor {
+    float* g;
+    int64_t n, chunk0;
+};
+struct GradTable {
+    GradTensor t[kGradPerLaunch];
+    int32_t nt;
+};
+
+__host__ __device__ __forceinline__ int grad_shift(const float* g) { return (int)((reinterpret_cast<uintptr_t>(g) >> 2) & 3); }
+
+// The tensors from *i on that a launch takes, and its chunks.
+static int64_t grad_table(int64_t ntensors, const float* const* grads, const int64_t* sizes, int64_t* i, GradTable* tab) {
+    int64_t chunks = 0;
+    for (tab->nt = 0; *i < ntensors && tab->nt < kGradPerLaunch; ++*i) {
+        if (sizes[*i] == 0) continue;
+        GradTensor& t = tab->t[tab->nt++];
+        t.g = const_cast<float*>(grads[*i]);
+        t.n = sizes[*i];
+        t.chunk0 = chunks;
+        chunks += ((t.n + grad_shift(t.g) + 3) / 4 + kGradChunk - 1) / kGradChunk;
+    }
+    return chunks;
+}
+
+__device__ __forceinline__ const GradTensor& grad_find(const GradTable& tab, int64_t chunk) {
+    int lo = 0, hi = tab.nt - 1;  // the last tensor whose chunk0 <= chunk
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.t[mid].chunk0 <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return tab.t[lo];
+}
+
+__device__ __forceinline__ double square_add(double s, float v) { return __builtin_fma((double)v, (double)v, s); }
+
+__global__ __launch_bounds__(kGradThreads) void k_grad_norm(GradTable tab, int64_t chunks, double* part) {
+    __shared__ double red[kGradThreads / 64];
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const GradTensor& t = grad_find(tab, c);
+        const int sh = grad_shift(t.g);
+        const int64_t k0 = (c - t.chunk0) * kGradChunk;
+        if (4 * k0 >= sh && 4 * (k0 + kGradChunk) - sh <= t.n) {  // whole quads
+            vf4 v[kGradQuads];
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) v[i] = *reinterpret_cast<const vf4*>(t.g + 4 * (k0 + i * kGradThreads + threadIdx.x) - sh);
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) {
+                s[0] = square_add(s[0], v[i].x);
+                s[1] = square_add(s[1], v[i].y);
+                s[2] = square_add(s[2], v[i].z);
+                s[3] = square_add(s[3], v[i].w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) {
+                const int64_t e = 4 * (k0 + i * kGradThreads + threadIdx.x) - sh;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (e + j >= 0 && e + j < t.n) s[j] = square_add(s[j], t.g[e + j]);
+            }
+        }
+    }
+    const double sum = block_sum<kGradThreads / 64>((s[0] + s[1]) + (s[2] + s[3]), red);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+
+// The norm from the workgroups' sums, and what the gradients are scaled by.
+__global__ __launch_bounds__(1024) void k_grad_total(const double* part, int64_t parts, float max_norm, float* norm, float* coef) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < parts; i += 1024) s += part[i];
+    s = block_sum<16>(s, red);
+    if (threadIdx.x != 0) return;
+    const double n = __builtin_sqrt(s);
+    if (norm) norm[0] = (float)n;
+    // an infinity or a NaN among the gradients scales nothing
+    coef[0] = n > (double)max_norm && n <= 1.7976931348623157e308 ? (float)((double)max_norm / n) : 1.0f;
+}
+
+__global__ __launch_bounds__(kGradThreads) void k_clip_scale(GradTable tab, int64_t chunks, const float* coef) {
+    const float m = coef[0];
+    if (m == 1.0f) return;
+    for (int64_t c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {  // from the end, which the caches hold
+        const GradTensor& t = grad_find(tab, c);
+        const int sh = grad_shift(t.g);
+        const int64_t k0 = (c - t.chunk0) * kGradChunk;
+        if (4 * k0 >= sh && 4 * (k0 + kGradChunk) - sh <= t.n) {
+            vf4 v[kGradQuads];
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) v[i] = ld_ntv(t.g + 4 * (k0 + i * kGradThreads + threadIdx.x) - sh, 0);
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) st_ntv(t.g + 4 * (k0 + i * kGradThreads + threadIdx.x) - sh, 0, v[i] * m);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kGradQuads; ++i) {
+                const int64_t e = 4 * (k0 + i * kGradThreads + threadIdx.x) - sh;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (e + j >= 0 && e + j < t.n) t.g[e + j] *= m;
+            }
+        }
+    }
+}
+
+static int check_grads(const char* what, int64_t ntensors, const float* const* grads, const int64_t* sizes, float max_norm) {
+    if (ntensors < 0) return fail(MH_ERR_INVALID, "%s: negative tensor count", what);
+    if (!(max_norm >= 0.0f)) return fail(MH_ERR_INVALID, "%s: a largest norm of %g", what, (double)max_norm);
+    if (ntensors > 0 && (!grads || !sizes)) return fail(MH_ERR_NULL, "%s: null table", what);
+    int64_t n = 0;
+    for (int64_t i = 0; i < ntensors; ++i) {
+        if (sizes[i] < 0) return fail(MH_ERR_INVALID, "%s: negative size of tensor %lld", what, (long long)i);
+        if (sizes[i] > 0 && !grads[i]) return fail(MH_ERR_NULL, "%s: null pointer in tensor %lld", what, (long long)i);
+        if (sizes[i] > 0 && (reinterpret_cast<uintptr_t>(grads[i]) & 3))
+            return fail(MH_ERR_INVALID, "%s: tensor %lld is not aligned to 4 bytes", what, (long long)i);
+        if (sizes[i] > ((int64_t)1 << 46) - n) return fail(MH_ERR_OVERFLOW, "%s: more than 2^46 elements", what);
+        n += sizes[i];
+    }
+    return MH_OK;
+}
+
+// Refuses tensors that share elements, which would be scaled twice. Tensors in the order of their addresses, as an
+// arena has them, take one look each.
+static int check_apart(const char* what, int64_t ntensors, const float* const* grads, const int64_t* sizes) {
+    const float* end = nullptr;
+    bool rising = true;
+    for (int64_t i = 0; i < ntensors && rising; ++i) {
+        if (sizes[i] == 0) continue;
+        rising = grads[i] >= end;
+        end = grads[i] + sizes[i];
+    }
+    if (rising) return MH_OK;
+    int64_t* order = new (std::nothrow) int64_t[ntensors];
+    if (!order) return fail(MH_ERR_INVALID, "%s: no host memory for %lld tensors", what, (long long)ntensors);
+    int64_t n = 0;
+    for (int64_t i = 0; i < ntensors; ++i)
+        if (sizes[i] > 0) order[n++] = i;
+    std::sort(order, order + n, [&](int64_t p, int64_t q) { return grads[p] < grads[q]; });
+    int64_t twice = -1;
+    for (int64_t i = 1; i < n && twice < 0; ++i)
+        if (grads[order[i - 1]] + sizes[order[i - 1]] > grads[order[i]]) twice = order[i];
+    delete[] order;
+    return twice < 0 ? MH_OK : fail(MH_ERR_INVALID, "%s: tensor %lld shares elements with another", what, (long long)twice);
+}
+
+// Queues the norm of all gradients; *coef is where what they are scaled by will lie.
+static int norm_of(int64_t ntensors, const float* const* grads, const int64_t* sizes, float max_norm, float* norm, float** coef) {
+    GradTable tab;
+    int64_t parts = 0;
+    for (int64_t i = 0; i < ntensors;) {
+        const int64_t chunks = grad_table(ntensors, grads, sizes, &i, &tab);
+        parts += chunks < kGradBlocks ? chunks : kGradBlocks;
+    }
+    double* part = nullptr;
+    MH_TRY(scratch(8 * (size_t)(parts + 1), reinterpret_cast<void**>(&part)));
+    *coef = reinterpret_cast<float*>(part + parts);
+    double* at = part;
+    for (int64_t i = 0; i < ntensors;) {
+        const int64_t chunks = grad_table(ntensors, grads, sizes, &i, &tab);
+        if (chunks == 0) continue;
+        const int64_t blocks = chunks < kGradBlocks ? chunks : kGradBlocks;
+        hipLaunchKernelGGL(k_grad_norm, dim3((unsigned)blocks), dim3(kGradThreads), 0, ctx().stream, tab, chunks, at);
+        at += blocks;
+    }
+    hipLaunchKernelGGL(k_grad_total, dim3(1), dim3(1024), 0, ctx().stream, part, parts, max_norm, norm, *coef);
+    return MH_OK;
+}
+
+}  // namespace mh
+
+using namespace mh;
+
+extern "C" {
+
+int mh_adam_step(float* param, const float* grad, float* m, float* v, int64_t n, float lr, float beta1,
+                 float beta2, float eps, int64_t iter) {
+    MH_TRACE("mh_adam_step");
+    MH_TRY(check_hyper("mh_adam_step", lr, beta1, beta2, eps, iter));
+    if (n < 0) return fail(MH_ERR_INVALID, "mh_adam_step: negative count");
+    if (n == 0) return MH_OK;
+    if (!param || !grad || !m || !v) return fail(MH_ERR_NULL, "mh_adam_step: null tensor");
+    MH_TRY(require_init());
+    const AdamScal s = adam_scalars(lr, beta1, beta2, eps, iter);
+    const UnitMap um = unit_map(param, grad, m, v);
+    const LaunchShape ls = adam_shape(n, um);
+    if (ls.kernel == 0)
+        hipLaunchKernelGGL(k_adam_al<false>, dim3((unsigned)ls.blocks), dim3(ls.threads), 0, ctx().stream, param, grad, m,
+                           v, n, s, (const float*)nullptr);
+    else
+        hipLaunchKernelGGL(k_adam, dim3((unsigned)ls.blocks), dim3(ls.threads), 0, ctx().stream, param, grad, m, v, n,
+                           um, s);
+    return finish("mh_adam_step");
+}
+
+int mh_adam_step_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
+                       float* const* v, const int64_t* sizes, float lr, float beta1, float beta2, float eps,
+                       int64_t iter) {
+    MH_TRACE("mh_adam_step_multi");
+    MH_TRY(check_hyper("mh_adam_step_multi", lr, beta1, beta2, eps, iter));
+    MH_TRY(check_adam("mh_adam_step_multi", ntensors, params, grads, m, v, sizes));
+    if (ntensors == 0) return MH_OK;
+    MH_TRY(require_init());
+    adam_multi<false>(ntensors, params, grads, m, v, sizes, adam_scalars(lr, beta1, beta2, eps, iter), nullptr);
     return finish("mh_adam_step_multi");
+}
+
+int mh_grad_norm(int64_t ntensors, const float* const* grads, const int64_t* sizes, float* norm) {
+    MH_TRACE("mh_grad_norm");
+    MH_TRY(check_grads("mh_grad_norm", ntensors, grads, sizes, 0.0f));
+    if (!norm) return fail(MH_ERR_NULL, "mh_grad_norm: null norm");
+    MH_TRY(require_init());
+    float* coef = nullptr;
+    MH_TRY(norm_of(ntensors, grads, sizes, 0.0f, norm, &coef));
+    return finish("mh_grad_norm");
+}
+
+int mh_clip_grad_norm(int64_t ntensors, float* const* grads, const int64_t* sizes, float max_norm, float* norm) {
+    MH_TRACE("mh_clip_grad_norm");
+    MH_TRY(check_grads("mh_clip_grad_norm", ntensors, grads, sizes, max_norm));
+    MH_TRY(check_apart("mh_clip_grad_norm", ntensors, grads, sizes));
+    MH_TRY(require_init());
+    float* coef = nullptr;
+    MH_TRY(norm_of(ntensors, grads, sizes, max_norm, norm, &coef));
+    GradTable tab;
+    for (int64_t i = 0; i < ntensors;) {
+        const int64_t chunks = grad_table(ntensors, grads, sizes, &i, &tab);
+        if (chunks > 0)
+            hipLaunchKernelGGL(k_clip_scale, dim3((unsigned)(chunks < kGradBlocks ? chunks : kGradBlocks)), dim3(kGradThreads), 0,
+                               ctx().stream, tab, chunks, coef);
+    }
+    return finish("mh_clip_grad_norm");
+}
+
+int mh_adam_clip_step_multi(int64_t ntensors, float* const* params, const float* const* grads, float* const* m,
+                            float* const* v, const int64_t* sizes, float lr, float beta1, float beta2, float eps,
+                            int64_t iter, float max_norm, float* norm) {
+    MH_TRACE("mh_adam_clip_step_multi");
+    MH_TRY(check_hyper("mh_adam_clip_step_multi", lr, beta1, beta2, eps, iter));
+    MH_TRY(check_adam("mh_adam_clip_step_multi", ntensors, params, grads, m, v, sizes));
+    MH_TRY(check_grads("mh_adam_clip_step_multi", ntensors, grads, sizes, max_norm));
+    MH_TRY(require_init());
+    const AdamScal s = adam_scalars(lr, beta1, beta2, eps, iter);
+    float* coef = nullptr;
+    MH_TRY(norm_of(ntensors, grads, sizes, max_norm, norm, &coef));
+    if (ntensors == 1 && sizes[0] > 0) {
+        const UnitMap um = unit_map(params[0], grads[0], m[0], v[0]);
+        const LaunchShape ls = adam_shape(sizes[0], um);
+        if (ls.kernel == 0) {
+            hipLaunchKernelGGL(k_adam_al<true>, dim3((unsigned)ls.blocks), dim3(ls.threads), 0, ctx().stream, params[0], grads[0],
+                               m[0], v[0], sizes[0], s, (const float*)coef);
+            return finish("mh_adam_clip_step_multi");
+        }
+    }
+    adam_multi<true>(ntensors, params, grads, m, v, sizes, s, coef);
+    return finish("mh_adam_clip_step_multi");
 }
 
 }  // extern "C"

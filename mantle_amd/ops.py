@@ -604,3 +604,89 @@ def router_backward(grad_x: Tensor, x: Tensor, chosen: IndexTensor, counts: Inde
               _want("keep", keep, (rows,), index=True, optional=True), _want("chosen", chosen, (rows, k), index=True),
               _want("counts", counts, (experts,), index=True), _want("grad_weights", grad_weights, (rows, k), optional=True),
               _want("ug", ug, (1,), optional=True), rows, experts, k, int(bool(normalise)), int(bool(accumulate)))
+
+
+_SCORES = {"softmax": _lib.SCORES_SOFTMAX, "sigmoid": _lib.SCORES_SIGMOID}
+
+
+def _scores(kind: str) -> int:
+    if kind not in _SCORES:
+        raise _lib.MantleHipError(_lib.ERR_INVALID, f"scores must be one of {sorted(_SCORES)}, not {kind!r}")
+    return _SCORES[kind]
+
+
+def group_router_forward(weights: Tensor, chosen: IndexTensor, counts: IndexTensor, x: Tensor, bias: Optional[Tensor] = None,
+                         keep: Optional[IndexTensor] = None, groups: int = 1, keep_groups: Optional[int] = None,
+                         group_best: int = 2, scores: str = "sigmoid", normalise: bool = True, scale: float = 1.0) -> None:
+    """Routing to experts by scores = "sigmoid" or "softmax" of x [rows, experts], balanced by a bias [experts] that is
+    added for the choice alone: of `groups` groups of neighbouring experts the keep_groups (None: all) with the largest sums
+    of their group_best best are open, and in them the k best chosen [rows, k], ties to the lowest index. weights [rows, k] are
+    their scores without the bias, normalised over the chosen or not, times scale; counts [experts] how often each was
+    chosen. Rows with keep 0 are padding: chosen -1, weights 0, counted nowhere."""
+    (rows, experts), (_, k) = _matrix("x", x), _matrix("chosen", chosen)
+    _lib.call("mh_group_router_fwd", _want("weights", weights, (rows, k)), _want("chosen", chosen, (rows, k), index=True),
+              _want("counts", counts, (experts,), index=True), _want("x", x, (rows, experts)),
+              _want("bias", bias, (experts,), optional=True), _want("keep", keep, (rows,), index=True, optional=True), rows,
+              experts, k, int(groups), int(groups if keep_groups is None else keep_groups), int(group_best), _scores(scores),
+              int(bool(normalise)), float(scale))
+
+
+def group_router_backward(grad_x: Tensor, x: Tensor, chosen: IndexTensor, grad_weights: Tensor,
+                          keep: Optional[IndexTensor] = None, scores: str = "sigmoid", normalise: bool = True,
+                          scale: float = 1.0, accumulate: bool = True) -> None:
+    """grad_x += (accumulate=False: =) the gradient of group_router_forward from grad_weights, the weights', with the
+    forward's chosen and its settings. Neither the choice nor the bias has one."""
+    (rows, experts), (_, k) = _matrix("x", x), _matrix("chosen", chosen)
+    _lib.call("mh_group_router_bwd", _want("grad_x", grad_x, (rows, experts)), _want("x", x, (rows, experts)),
+              _want("keep", keep, (rows,), index=True, optional=True), _want("chosen", chosen, (rows, k), index=True),
+              _want("grad_weights", grad_weights, (rows, k)), rows, experts, k, _scores(scores), int(bool(normalise)),
+              float(scale), int(bool(accumulate)))
+
+
+def router_bias_update(bias: Tensor, counts: IndexTensor, rate: float) -> None:
+    """A step of the bias [experts] towards balance: + rate for experts chosen less often than the mean of counts [experts],
+    - rate for those chosen more often."""
+    experts = bias.num_elements() if isinstance(bias, Tensor) else 0
+    _lib.call("mh_router_bias_update", _want("bias", bias, (experts,)), _want("counts", counts, (experts,), index=True),
+              experts, float(rate))
+
+
+# ---------------------------------------------------------------------------------------
+# norm and sampling of a language model (no reference counterpart)
+# ---------------------------------------------------------------------------------------
+def rms_norm_forward(out: Tensor, x: Tensor, w: Tensor, residual: Optional[Tensor] = None, sum: Optional[Tensor] = None,
+                     eps: float = 1e-6) -> None:
+    """Root-mean-square norm over the last axis, with the residual's addition: h = x + residual (without one h = x),
+    out = h / sqrt(mean h^2 + eps) * w, and sum = h where it is given, which the backward takes. w has the last axis' length.
+    sum may be x or residual, and out may be x."""
+    _row_operands(x, same=[("out", out), *((n, t) for n, t in (("residual", residual), ("sum", sum)) if t is not None)])
+    rows, dim = _rows_classes(x)
+    _lib.call("mh_rms_norm_fwd", out.f32, None if sum is None else sum.f32, x.f32, None if residual is None else residual.f32,
+              _want("w", w, (dim,)), rows, dim, float(eps))
+
+
+def rms_norm_backward(grad_x: Optional[Tensor], grad_w: Optional[Tensor], grad_out: Tensor, h: Tensor, w: Tensor,
+                      grad_sum: Optional[Tensor] = None, eps: float = 1e-6, accumulate: bool = True) -> None:
+    """grad_x and grad_w += (accumulate=False: =) the gradients of rms_norm_forward from grad_out and grad_sum, those of its
+    out and sum; h is its sum, or x where it had no residual. grad_x is the residual's gradient too. Either may be None;
+    grad_x may be grad_sum or grad_out."""
+    _row_operands(h, same=[("grad_out", grad_out), *((n, t) for n, t in (("grad_x", grad_x), ("grad_sum", grad_sum)) if t is not None)])
+    rows, dim = _rows_classes(h)
+    _lib.call("mh_rms_norm_bwd", None if grad_x is None else grad_x.f32, _want("grad_w", grad_w, (dim,), optional=True),
+              grad_out.f32, None if grad_sum is None else grad_sum.f32, h.f32, _want("w", w, (dim,)), rows, dim, float(eps),
+              int(bool(accumulate)))
+
+
+def sample_tokens(tokens: IndexTensor, x: Tensor, u: Tensor, temperature: Optional[Tensor] = None,
+                  top_k: Optional[IndexTensor] = None, top_p: Optional[Tensor] = None, min_p: Optional[Tensor] = None,
+                  logprob: Optional[Tensor] = None) -> None:
+    """A token for each row of logits x [rows, classes] from uniform numbers u [rows] in [0, 1). temperature, top_k, top_p and
+    min_p are tensors [rows], a setting for each row, or None: temperature 0 takes the largest logit; top_k, then top_p of what
+    it left, and min_p cut the classes, in the order of falling logits, ties by index. tokens [rows] is the first class, by
+    index, where the running sum of what is kept exceeds u of its total; logprob [rows] the logarithm of its share. A row
+    that holds a NaN, or nothing but minus infinity, has token -1 and logprob NaN."""
+    rows, classes = _matrix("x", x)
+    _lib.call("mh_sample_tokens", _want("tokens", tokens, (rows,), index=True), _want("logprob", logprob, (rows,), optional=True),
+              _want("x", x, (rows, classes)), _want("u", u, (rows,)), _want("temperature", temperature, (rows,), optional=True),
+              _want("top_k", top_k, (rows,), index=True, optional=True), _want("top_p", top_p, (rows,), optional=True),
+              _want("min_p", min_p, (rows,), optional=True), rows, classes)

@@ -6,11 +6,15 @@ pairs, and keeps
 the momentum and rms tensors, zero-initialised, beside them. ``step()`` increments ``iter``
 and updates every parameter with one ``mh_adam_step_multi`` launch per 80 tensors;
 ``zero_grad()`` zeroes the gradients (``Collection.set_zero``, collection.mojo:221-224).
+
+``grad_norm`` and ``clip_grad_norm`` take the norm of many gradients together and scale them to
+a largest one; an Adam with ``max_norm`` does so on their way into its step (no counterparts in
+the reference).
 """
 from __future__ import annotations
 
 import ctypes
-from typing import List, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 from . import _lib
 from .tensor import Tensor
@@ -31,11 +35,41 @@ class SymbolTensors(list):
         return super().__getitem__(key)
 
 
+def _grad_tables(grads: Sequence[Tensor]):
+    """The addresses and sizes of gradients, as the C ABI takes them."""
+    n = len(grads)
+    return n, (ctypes.c_void_p * n)(*[g.f32 for g in grads]), (ctypes.c_int64 * n)(*[g.num_elements() for g in grads])
+
+
+def _norm_address(norm: Optional[Tensor]):
+    if norm is None:
+        return None
+    if norm.num_elements() != 1:
+        raise _lib.MantleHipError(_lib.ERR_SHAPE, f"norm must hold one element (holds {norm.num_elements()})")
+    return norm.f32
+
+
+def grad_norm(norm: Tensor, grads: Sequence[Tensor]) -> None:
+    """norm (one element) = the square root of the sum of the squares of every element of `grads`."""
+    n, ptrs, sizes = _grad_tables(grads)
+    _lib.call("mh_grad_norm", n, ptrs, sizes, _norm_address(norm))
+
+
+def clip_grad_norm(norm: Optional[Tensor], grads: Sequence[Tensor], max_norm: float) -> None:
+    """grad_norm, and every gradient scaled in place by min(1, max_norm / norm); none where one of their elements is
+    infinite or NaN, as norm then shows. Tensors that share elements are refused."""
+    n, ptrs, sizes = _grad_tables(grads)
+    _lib.call("mh_clip_grad_norm", n, ptrs, sizes, float(max_norm), _norm_address(norm))
+
+
 class Adam:
     def __init__(self, params, lr: float = 0.001, beta1: float = 0.9, beta2: float = 0.999,
-                 epsilon: float = 1e-8):
+                 epsilon: float = 1e-8, max_norm: Optional[float] = None):
         """``params``: a model's ``Parameters`` (its graph's trainable parameters, as
-        ``Adam[g](model.parameters, ...)`` takes them), or (param, grad) Tensor pairs."""
+        ``Adam[g](model.parameters, ...)`` takes them), or (param, grad) Tensor pairs.
+        ``max_norm``: each step takes the gradients scaled to at most this norm of all of them
+        together, which ``self.grad_norm`` (one element, or None to go without) gets; the gradients
+        themselves stay as they are."""
         self._collection = None
         self._span = None  # (params, grads, n) of a model's contiguous trainable span
         self.symbols = None  # the trainable parameters' symbols, for a model's parameters
@@ -52,6 +86,8 @@ class Adam:
                 raise _lib.MantleHipError(_lib.ERR_SHAPE, "a parameter and its gradient differ in shape")
             p.f32, g.f32  # neither holds whole numbers
         self.lr, self.beta1, self.beta2, self.epsilon = float(lr), float(beta1), float(beta2), float(epsilon)
+        self.max_norm = None if max_norm is None else float(max_norm)
+        self.grad_norm = None if max_norm is None else Tensor(1)
         self.iter = 0
         # allocate_rms_and_momentum (optim.mojo:142-149): zero-initialised, one per parameter;
         # over a model's span, two span-sized buffers whose slices are the per-parameter tensors
@@ -82,11 +118,18 @@ class Adam:
         self.iter += 1
         if self._span is not None:  # every parameter of the model in one launch
             p, g, n = self._span
+            if self.max_norm is not None:
+                one = [(ctypes.c_void_p * 1)(a) for a in (p, g, self._m_span.ptr, self._v_span.ptr)]
+                _lib.call("mh_adam_clip_step_multi", 1, *one, (ctypes.c_int64 * 1)(n), self.lr, self.beta1, self.beta2,
+                          self.epsilon, self.iter, self.max_norm, _norm_address(self.grad_norm))
+                return
             _lib.call("mh_adam_step", p, g, self._m_span.ptr, self._v_span.ptr, n, self.lr, self.beta1, self.beta2,
                       self.epsilon, self.iter)
             return
         n = len(self.params)
         if n == 0:
+            if self.max_norm is not None and self.grad_norm is not None:
+                self.grad_norm.zero()
             return
         # A tensor's address never changes, so the tables are made again only where a tensor was
         # exchanged (made on every step, those of 400 parameters cost as much as the step: 337 us
@@ -99,5 +142,9 @@ class Adam:
                             VP(*[t.f32 for t in self.rms_grads]),
                             (ctypes.c_int64 * n)(*[p.num_elements() for p, _ in self.params]))
         _, ps, gs, ms, vs, sizes = self._tables
+        if self.max_norm is not None:
+            _lib.call("mh_adam_clip_step_multi", n, ps, gs, ms, vs, sizes, self.lr, self.beta1, self.beta2, self.epsilon,
+                      self.iter, self.max_norm, _norm_address(self.grad_norm))
+            return
         _lib.call("mh_adam_step_multi", n, ps, gs, ms, vs, sizes, self.lr, self.beta1, self.beta2, self.epsilon,
                   self.iter)

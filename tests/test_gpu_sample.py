@@ -1,0 +1,268 @@
+"""Tokens from logits (sample_tokens) against the definition in 64 bits.
+
+A mass is off by D = (|x - max| / T + 4) 2^-24 of itself (the difference's rounding, an exponential) and 2^-shift of the largest, so
+a row's shares by delta = the mean of D over what is kept, twice. A row whose u, or whose top_p or min_p, lies within that of a
+border may go either way: it is left out, and counted; no more than one row in fifty may be."""
+import numpy as np
+import pytest
+
+from util import GpuEngine
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def m_():
+    return GpuEngine().m
+
+
+def reference(x, u, T=1.0, k=0, p=1.0, mp=0.0):
+    """(token, logprob, its bound, whether the row is sure) of one row; kept as an array too."""
+    x = (x + np.float32(0)).astype(np.float64)
+    n = len(x)
+    none = (-1, np.nan, 0.0, True, np.zeros(n, bool))
+    if np.isnan(x).any() or x.max() == -np.inf:
+        return none
+    top = x.max()
+    only = np.zeros(n, bool)
+    only[int(np.argmax(x))] = True
+    if not T > 0:
+        return int(np.argmax(x)), 0.0, 0.0, True, only
+    T = float(np.float32(T))
+    with np.errstate(invalid="ignore", over="ignore", under="ignore"):
+        y = np.where(x == top, 0.0, (x - top) / T if np.isfinite(T) else np.where(x == -np.inf, -np.inf, 0.0))
+        e = np.exp(y)
+        rel = np.where(e > 0, np.minimum(np.abs(y), 1e3) + 4, 0) * U
+    order = np.argsort(-x, kind="stable")
+    sure = True
+    m = e[order].copy()
+    if 0 < k < n:
+        m[k:] = 0
+    count = n if not 0 < k < n else k
+    if p < 1:
+        p = max(float(np.float32(p)), 0.0)
+        total = m.sum()
+        share = np.cumsum(m) / total
+        delta = 2 * (m * rel[order]).sum() / total + 2 * n * 2.0 ** -46
+        if p > 0 and np.abs(share[:count] - p).min() < delta and not exactly(m, share, p):
+            sure = False
+        count = max(1, min(count, int((share < p - 1e-15).sum()) + 1))
+    if mp > 0:
+        mp = float(np.float32(mp))
+        edge = T * np.log(min(mp, 1.0))
+        count = max(1, min(count, int((x[order] - top >= edge).sum())))
+        if np.abs(x[order] - top - edge)[x[order] < top].min(initial=1) < 1e-12 * abs(edge):
+            sure = False
+    keep = np.zeros(n, bool)
+    keep[order[:count]] = True
+    q = np.where(keep, e, 0.0)
+    total = q.sum()
+    share = np.cumsum(q) / total
+    delta = 2 * (q * rel).sum() / total + 2 * n * 2.0 ** -46
+    u = min(max(float(u), 0.0), 1 - U) if u == u else 0.0
+    at = int((share <= u).sum())
+    if at >= n or not keep[at] or np.abs(np.r_[0.0, share] - u)[np.r_[False, keep]].min() < delta and u > 0:
+        sure = sure and exact_shares(q, total) and u * total == np.floor(u * total)
+    at = min(at, int(order[:count].max()))
+    lp = np.log(q[at] / total) if q[at] > 0 else -np.inf
+    return at, lp, delta + rel[at] + 2 * U * abs(lp) + 1e-44, sure, keep
+
+
+def exact_shares(q, total):
+    """Masses that are all equal or nothing: no rounding on either side."""
+    return len(set(q[q > 0])) == 1
+
+
+def exactly(m, share, p):
+    return exact_shares(m, None)
+
+
+def run(m, x, u, T=None, k=None, p=None, mp=None, logprob=True):
+    rows = len(x)
+    f = lambda a: None if a is None else m.Tensor.from_numpy(np.broadcast_to(np.float32(a), (rows,)))  # noqa: E731
+    tok, lp = m.IndexTensor.from_numpy(np.full(rows, 77)), m.Tensor.from_numpy(np.full(rows, 77.0))
+    m.sample_tokens(tok, m.Tensor.from_numpy(x), m.Tensor.from_numpy(np.float32(u)), temperature=f(T),
+                    top_k=None if k is None else m.IndexTensor.from_numpy(np.broadcast_to(np.int32(k), (rows,))), top_p=f(p),
+                    min_p=f(mp), logprob=lp if logprob else None)
+    return tok.to_numpy(), lp.to_numpy()
+
+
+def check(m, x, u, T=None, k=None, p=None, mp=None, unsure=None, what=""):
+    got, lp = run(m, x, u, T, k, p, mp)
+    rows = len(x)
+    left = 0
+    at = lambda a, d, r: d if a is None else np.broadcast_to(a, (rows,))[r]  # noqa: E731
+    for r in range(rows):
+        tok, l, off, sure, keep = reference(x[r], np.float32(u[r]), at(T, 1.0, r), int(at(k, 0, r)), at(p, 1.0, r), at(mp, 0.0, r))
+        if not sure:
+            left += 1
+            continue
+        assert got[r] == tok, f"{what} row {r}: {got[r]} and not {tok}"
+        if np.isnan(l):
+            assert np.isnan(lp[r])
+        else:
+            assert abs(lp[r] - l) <= off, f"{what} row {r}: {lp[r]} and not {l} +- {off}"
+    assert left <= (rows / 50 if unsure is None else unsure), f"{what}: {left} of {rows} rows are too near a border"
+
+
+def logits(rows, classes, seed, std=2.0):
+    r = np.random.RandomState(seed)
+    x = std * r.standard_normal((rows, classes))
+    for i in range(rows):
+        x[i, r.randint(0, classes, 8)] += r.uniform(2, 10, 8)
+    return x.astype(np.float32), r.uniform(size=rows).astype(np.float32)
+
+
+SIZES = [(1, 1), (3, 2), (50, 3), (40, 7), (30, 64), (30, 65), (20, 1000), (9, 1023), (9, 1025), (7, 4096), (33, 5001), (5, 30011),
+         (3, 32000), (4, 65536), (3, 70001), (2, 131072), (2, 200003)]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_sizes(size):
+    print(f"\n[sample] {size}", flush=True)
+    m = m_()
+    x, u = logits(*size, seed=sum(size))
+    r = np.random.RandomState(1)
+    rows = size[0]
+    check(m, x, u, unsure=0, what="as they are")
+    for k in (1, 2, 50, size[1] // 2, size[1], size[1] + 5):
+        check(m, x, u, T=0.7, k=k, unsure=0, what=f"top_k {k}")
+    for p in (0.0, 0.3, 0.9, 0.999):
+        check(m, x, u, T=1.3, p=p, unsure=1, what=f"top_p {p}")
+    for mp in (0.01, 0.5, 1.0, 2.0):
+        check(m, x, u, mp=mp, unsure=0, what=f"min_p {mp}")
+    check(m, x, u, T=r.choice([0.0, 0.5, 1.0, 2.0, 50.0], rows), k=r.choice([-1, 0, 3, 40], rows), p=r.choice([1.0, 0.8, 0.5], rows),
+          mp=r.choice([0.0, 0.05, -1.0], rows), unsure=1, what="mixed")
+
+
+def test_many_rows():
+    m = m_()
+    x, u = logits(6000, 40, seed=2)
+    r = np.random.RandomState(3)
+    check(m, x, u, T=r.choice([0.0, 0.5, 1.0, 2.0], 6000), k=r.choice([0, 1, 5, 30], 6000), p=r.choice([1.0, 0.9, 0.3], 6000),
+          mp=r.choice([0.0, 0.1], 6000), unsure=20, what="rows")
+
+
+@pytest.mark.parametrize("classes", [40, 3000, 40000])
+def test_ties(classes):
+    """Logits of a few values: the lowest indices stay where a cut falls among equals, and sums of equals are exact."""
+    m = m_()
+    r = np.random.RandomState(4)
+    rows = 24
+    x = r.randint(0, 3, (rows, classes)).astype(np.float32)
+    x[0] = 1.0
+    x[1] = -0.0
+    x[1, ::2] = 0.0
+    u = r.uniform(size=rows).astype(np.float32)
+    for k in (1, 2, 7, classes // 2, classes - 1):
+        check(m, x, u, k=k, unsure=1, what=f"top_k {k}")
+    check(m, x, u, T=0.5, p=0.61803, unsure=2, what="top_p")
+    check(m, x, u, T=0.5, k=classes // 3, p=0.61803, unsure=2, what="both")
+    # halves and quarters of equal classes
+    y = np.zeros((4, classes), np.float32)
+    for p, many in ((0.5, classes // 2), (0.25, classes // 4), (0.75, classes * 3 // 4)):
+        tok, lp = run(m, y, [0.0, 0.5, 0.99, 1 - U], p=p)
+        assert tok.max() < many and tok[0] == 0 and tok[1] == many // 2 and tok[3] == many - 1
+        assert np.allclose(lp, -np.log(many), rtol=1e-6)
+
+
+def test_borders_of_u():
+    """u of 0 draws the first class that is kept, u just below 1 the last; out of range it is held to them."""
+    m = m_()
+    x, _ = logits(6, 500, seed=5)
+    x[:, 0] = x[:, -1] = -np.inf
+    for u, last in ((0.0, False), (-3.0, False), (np.nan, False), (1 - U, True), (1.0, True), (9.0, True), (np.inf, True)):
+        for k in (0, 5):
+            tok, _ = run(m, x, np.full(6, u, np.float32), k=k)
+            for r in range(6):
+                keep = reference(x[r], 0.5, 1.0, k)[4] & (x[r] > -np.inf)
+                at = np.flatnonzero(keep)
+                if last and k == 0:  # what is beyond the last 2^-24 of the mass
+                    assert keep[tok[r]] and np.exp(x[r, tok[r] + 1:].astype(np.float64)).sum() <= 4 * U * np.exp(x[r].astype(np.float64)).sum()
+                else:
+                    assert tok[r] == (at[-1] if last else at[0])
+
+
+def test_uniform_over_a_grid_of_u():
+    """Every u of a grid draws its own share."""
+    m = m_()
+    x, _ = logits(1, 30, seed=6)
+    n = 5000
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    check(m, np.repeat(x, n, 0), u, T=1.5, unsure=3, what="grid")
+    check(m, np.repeat(x, n, 0), u, T=1.5, k=6, p=0.95, unsure=3, what="grid cut")
+
+
+@pytest.mark.parametrize("classes", [6, 100, 5000, 70000])
+def test_masks_and_no_numbers(classes):
+    m = m_()
+    x, u = logits(8, classes, seed=7)
+    x[0, 1:] = -np.inf
+    x[1, :] = -np.inf
+    x[2, classes // 2] = np.nan
+    x[3, :] = np.nan
+    x[4, 3] = np.inf
+    x[5, 2] = x[5, 5] = np.inf
+    x[6, :-1] = -3.4028234663852886e38
+    x[7, ::2] = -np.inf
+    for a in ({}, {"k": 3}, {"p": 0.7}, {"mp": 0.2}, {"T": 0.0}, {"T": 0.3, "k": 3, "p": 0.9, "mp": 0.1}, {"k": classes}):
+        check(m, x, u, **a, unsure=0, what=str(a))
+
+
+@pytest.mark.parametrize("T", [1e-45, 1e-30, 1e-3, 1e3, 1e30, np.inf, -1.0, np.nan, -np.inf, 0.0])
+def test_temperatures(T):
+    m = m_()
+    x, u = logits(12, 300, seed=8)
+    x[0, :3] = x[0].max()
+    x[1, 10] = -np.inf
+    check(m, x, u, T=T, unsure=0, what=str(T))
+    check(m, x, u, T=T, k=9, unsure=0, what=f"{T} top_k")
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf, -1.0, 0.0])
+def test_settings_out_of_range(value):
+    m = m_()
+    x, u = logits(12, 300, seed=9)
+    as_p = value if value <= 0 else 1.0
+    got = run(m, x, u, p=value, mp=0.0)
+    want = run(m, x, u, p=as_p, mp=0.0)
+    assert np.array_equal(got[0], want[0])
+    if value <= 0:
+        assert np.array_equal(got[0], x.argmax(1)) and (got[1] == 0).all()
+    as_mp = value if value > 0 else 0.0
+    assert np.array_equal(run(m, x, u, mp=value)[0], run(m, x, u, mp=as_mp)[0])
+    if value > 1:
+        assert np.array_equal(run(m, x, u, mp=value)[0], x.argmax(1))
+
+
+def test_logits_of_all_sizes():
+    m = m_()
+    x, u = logits(20, 200, seed=10)
+    for by in (1e-38, 1e-6, 1e6, 1e36):
+        check(m, (x * np.float32(by)).astype(np.float32), u, k=50, p=0.9, unsure=1, what=str(by))
+    check(m, x + np.float32(30000.0), u, p=0.9, unsure=1, what="offset")
+
+
+def test_without_a_logprob_and_in_one_call():
+    m = m_()
+    x, u = logits(30, 900, seed=11)
+    a = dict(T=0.8, k=40, p=0.9, mp=0.01)
+    tok, _ = run(m, x, u, **a)
+    assert np.array_equal(tok, run(m, x, u, **a, logprob=False)[0])
+    for r in (0, 13, 29):  # a row does not depend on its neighbours
+        one = run(m, x[r:r + 1], u[r:r + 1], **a)
+        assert one[0][0] == tok[r]
+
+
+def test_the_same_bits_on_every_call():
+    m = m_()
+    x, u = logits(40, 50000, seed=12)
+    a = run(m, x, u, T=1.4, p=0.97)
+    for _ in range(3):
+        b = run(m, x, u, T=1.4, p=0.97)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_no_rows():
+    m = m_()
+    m.sample_tokens(m.IndexTensor((0,)), m.Tensor((0, 5)), m.Tensor((0,)))
