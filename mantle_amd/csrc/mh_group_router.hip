@@ -79,28 +79,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// e^x for x <= 0 (a NaN stays one), to about an ulp: 2^n e^r, |r| <= ln(2) / 2, by Taylor's series.
-__device__ __forceinline__ double exp64(double x) {
-    x = x < -1000.0 ? -1000.0 : x;
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(n, -0.69314718055994530942, x);
-    r = __builtin_fma(n, -2.3190468138462996e-17, r);  // the rest of ln 2
-    double p = 1.0 / 6227020800.0;
-    p = __builtin_fma(p, r, 1.0 / 479001600.0);
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p, (int)n);
-}
 __device__ __forceinline__ double sigmoid64(float x) {
     const double e = exp64(-__builtin_fabs((double)x));
     return (x < 0.0f ? e : 1.0) / (1.0 + e);

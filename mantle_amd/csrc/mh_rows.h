@@ -21,6 +21,29 @@ __device__ __forceinline__ float exp_neg(float x) {
     return __builtin_fmaf(e, r * 0.693147180559945f, e);
 }
 
+// e^x in 64 bits to about an ulp, for x of less than 700 (from -1000 down it is 0; a NaN stays one): 2^n e^r,
+__device__ __forceinline__ double exp64(double x) {
+    x = x < -1000.0 ? -1000.0 : x;
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(n, -0.69314718055994530942, x);
+    r = __builtin_fma(n, -2.3190468138462996e-17, r);  // the rest of ln 2
+    double p = 1.0 / 6227020800.0;
+    p = __builtin_fma(p, r, 1.0 / 479001600.0);
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+
 // Sums and maxima over a workgroup of W wavefronts; every thread gets the result. `red` holds W values and may
 // be used again right after.
 template <int W, typename T>

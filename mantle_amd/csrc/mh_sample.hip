@@ -5,20 +5,21 @@
 // of their sum.
 //
 // A workgroup takes a row, a wavefront a run of its classes, of which each lane holds 4 Q logits in registers (the whole
-// row up to 4 Q T classes; of a longer one the rest is read twice, the second time mostly from the caches):
-//   1. the largest logit held, and bins of a power-of-two width below (and some above) it;
+// row up to 4 Q T classes; of a longer one the rest is read as it is needed):
+//   1. the largest logit held, the reference, and bins of a power-of-two width, T / 64 or 1 / 64 at least, around it;
 //   2. for top-k and top-p how many classes each bin has and their mass, both in one 64-bit LDS atomic: 20 bits of count above
-//      44 of mass, a class 24 bits of its bin's largest. Whole numbers: the atomics' order does not show. A sum over the bins
+//      44 of mass, a class 24 bits of its bin's largest. Whole numbers: the atomics' order does not show. A scan of the bins
 //      then says in which of them a cut falls;
-//   3. a second walk over the logits adds up what lies above those bins and lists what lies in them;
-//   4. the list, a few hundred classes, is sorted, and the cuts are found in it by 64-bit sums;
+//   3. a second walk, over the quads that reach those bins, adds up what lies above them and lists what lies in them. More
+//      than 2048 listed: from 2. on with narrower bins in the place of those;
+//   4. the list is sorted, and the cuts are found in it by 64-bit sums;
 //   5. the run of classes where the running sum passes u of the total is walked by the whole workgroup.
-// Sums of step 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
+// Sums of steps 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
 // sign, moves a border by some 2^-24 of the row.
 //
-// Rows for which bins do not work (a list of more than 2048 classes, as ties of thousands give, an infinite logit,
-// temperatures beyond 1e30 or whose bins would span more than 16 powers of two, more than 2^19 classes) go by whole-number masses and a
-// search over the logits' bits, 8 at a time: right for every row, and slower.
+// Rows for which bins do not work (more than 2048 classes of one value at a cut, a cut 48 T below the largest, an infinite
+// logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over the logits'
+// bits, 8 at a time: right for every row, and slower.
 #include "mh_internal.h"
 #include "mh_rows.h"
 
@@ -26,7 +27,7 @@ namespace mh {
 namespace {
 
 constexpr int kBins = 4096;
-constexpr int kAbove = 1024;  // of them above the largest logit that step 1 saw
+constexpr int kAbove = 1024;  // of them above the reference at first
 constexpr int kList = 2048;
 constexpr int kCountAt = 44;
 constexpr int64_t kMaxBinned = (int64_t)1 << 19;
@@ -62,14 +63,57 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 }
 __device__ __forceinline__ float of_order(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
+// Lanes' values moved within the wavefront; 0 where there is none to move (its bits are 0 in every type).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) { return (uint32_t)moved<CTRL, ROWS>((int)v); }
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T moved(T v) {
+    static_assert(sizeof(T) == 8, "");
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t m = (uint64_t)(uint32_t)moved<CTRL, ROWS>((int)(b >> 32)) << 32 | (uint32_t)moved<CTRL, ROWS>((int)b);
+    return __builtin_bit_cast(T, m);
+}
+// Sums up to and with each lane of a row of 16 lanes, and of the wavefront.
 template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {  // sums up to and with each lane
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T w = __shfl_up(v, o);
-        if ((int)(threadIdx.x & 63) >= o) v += w;
-    }
+__device__ __forceinline__ T row_scan(T v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
     return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
+    v += moved<0x142, 0xa>(v);  // each row's last lane to the row behind it
+    v += moved<0x143, 0xc>(v);  // the lower half's last lane to the upper half
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                         (uint32_t)__builtin_amdgcn_readlane((int)b, lane));
+    }
+}
+// The largest of a wavefront's numbers, in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_with(float v) {
+    return __builtin_fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = max_with<0x111, 0xf>(v);
+    v = max_with<0x112, 0xf>(v);
+    v = max_with<0x114, 0xf>(v);
+    v = max_with<0x118, 0xf>(v);
+    v = max_with<0x142, 0xa>(v);
+    v = max_with<0x143, 0xc>(v);
+    return lane_value(v, 63);
 }
 
 // log of the drawn class's share of the kept mass, `total` in units of the largest class's mass.
@@ -245,8 +289,8 @@ __device__ __attribute__((noinline)) void slow_row(const float* x, int classes, 
             }
             break;
         }
-        before += __shfl(upto, 63);
-        ties_before += __shfl(at_tie, 63);
+        before += lane_value(upto, 63);
+        ties_before += lane_value(at_tie, 63);
     }
 }
 
@@ -261,23 +305,22 @@ struct FastLds {
             double upto[kList];   // sums of masses
         } list;
     };
+    float quad_top[kMaxBinned / 256];  // the largest of 256 classes
     double wave_d[16], seg[16];
     uint32_t wave_n[16];
     float wave_f[16];
-    int wave_i[16];
     // what one thread found out for all
-    uint32_t listed, k_bin, k_above_n, k_here, p_lo, p_hi;
-    double k_above, k_in, p_above, all;
-    int over, bad, first, last;
-    uint64_t cut;
+    uint32_t listed, k_bin, k_above_n, k_here, p_lo, p_hi, p_above_n;
+    double k_above, k_in, p_above;
+    int bad, first;
 };
 
-// Exclusive sums over the workgroup's threads of a count and a mass, and the totals; `after` is what each thread's own
-// gives the next one, the same bits as its neighbour's.
+// Exclusive sums over the workgroup's threads of a count and a mass, and the totals; m1 is the sum with the thread's own, the
+// same bits as the next thread's m0.
 template <int W>
 __device__ __forceinline__ void block_scan(uint32_t n, double m, uint32_t& n0, double& m0, double& m1, uint32_t& n_all, double& m_all,
                                            FastLds& s) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ni = wave_scan(n);
     const double mi = wave_scan(m);
     __syncthreads();
@@ -286,23 +329,15 @@ __device__ __forceinline__ void block_scan(uint32_t n, double m, uint32_t& n0, d
         s.wave_d[wave] = mi;
     }
     __syncthreads();
-    uint32_t nb = 0;
-    double mb = 0.0;
-    n_all = 0;
-    m_all = 0.0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        if (i == wave) {
-            nb = n_all;
-            mb = m_all;
-        }
-        n_all += s.wave_n[i];
-        m_all += s.wave_d[i];
-    }
-    const uint32_t np = __shfl_up(ni, 1);
-    const double mp = __shfl_up(mi, 1);
-    n0 = nb + (lane ? np : 0);
-    m0 = lane ? mb + mp : mb;
+    const uint32_t nw = row_scan(lane < W ? s.wave_n[lane & 15] : 0u);
+    const double mw = row_scan(lane < W ? s.wave_d[lane & 15] : 0.0);
+    n_all = lane_value(nw, W - 1);
+    m_all = lane_value(mw, W - 1);
+    const uint32_t nb = wave ? lane_value(nw, wave - 1) : 0;
+    const double mb = wave ? lane_value(mw, wave - 1) : 0.0;
+    const double mp = moved<0x138, 0xf>(mi);  // the lane's before
+    n0 = nb + ni - n;
+    m0 = mb + mp;
     m1 = mb + mi;
 }
 
@@ -321,11 +356,29 @@ __device__ __forceinline__ void close_row(vf4& v, int c, int classes) {
     for (int j = 0; j < 4; ++j) v[j] = c + j < classes ? v[j] : -__builtin_inff();
 }
 
-// Where a logit falls: places of bin width below the reference, negative above it; past the last bin, and at minus
-// infinity, the last.
-__device__ __forceinline__ float place_of(float v, float ref, float per_bin) {
-    return __builtin_fminf((ref - v) * per_bin, (float)(kBins - 1 - kAbove));
-}
+// What one class's mass is made from, in units of the largest's.
+struct Mass {
+    float best, hi, lo;  // the largest logit; log2(e) / T in two parts
+    float least;         // the least logit that min_p keeps
+    __device__ __forceinline__ Mass(float top, const Ask& ask) : best(top) {
+        const double per = 1.4426950408889634074 / ask.T;
+        hi = (float)per;
+        lo = (float)(per - (double)hi);
+        const double edge = (double)top + ask.limit;
+        least = (float)edge;
+        if ((double)least < edge) {  // the next one up
+            const uint32_t b = __float_as_uint(least + 0.0f);
+            least = __uint_as_float(b >> 31 ? b - 1 : b + 1);
+        }
+    }
+    __device__ __forceinline__ double operator()(float v) const {
+        const float d = v - best;
+        const float t = d * hi;
+        if (!(v >= least) || !(t > -150.0f)) return 0.0;
+        const float e = __builtin_amdgcn_exp2f(t);
+        return (double)__builtin_fmaf(e, (__builtin_fmaf(d, hi, -t) + d * lo) * 0.693147180559945f, e);
+    }
+};
 
 template <int T, int Q>
 __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
@@ -334,7 +387,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     __shared__ union { FastLds f; SlowLds s; } lds;
     FastLds& s = lds.f;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // a wavefront's run of classes: whole rounds of 256
+    // a wavefront's run of classes: whole rounds of 256, of which the first Q are held
     const int run = (a.classes + 256 * W - 1) / (256 * W) * 256;
     const int w0 = wave * run, c0 = w0 + 4 * lane;
     const int quads = run / 256;
@@ -344,156 +397,151 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     vf4 h[Q];
 #pragma unroll
     for (int i = 0; i < Q; ++i) h[i] = logits(row, i < quads ? c0 + 256 * i : a.classes);
-#pragma unroll
-    for (int i = 0; i < Q; ++i)
-        if (w0 + 256 * (i + 1) > a.classes || i >= quads) close_row(h[i], i < quads ? c0 + 256 * i : a.classes, a.classes);
-    // every logit of the row: those held, then the others
-    auto held = [&](auto&& f) {
-        int at = c0;
-        asm volatile("" : "+v"(at));  // or every walk shares 64 registers of indices
-#pragma unroll
-        for (int i = 0; i < Q; ++i)
-            if (i < quads) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = h[i][j];
-                    asm volatile("" : "+v"(v));  // nothing made of it is kept from one walk to the next
-                    f(v, at + 256 * i + j);
-                }
-                __builtin_amdgcn_sched_barrier(0);  // a quad's work at a time: all of them need 700 registers
-            }
-    };
-    auto rest = [&](auto&& f) {
-        if (quads <= Q) return;
-        vf4 next = logits(row, c0 + 256 * Q);
-        for (int i = Q; i < quads; ++i) {
-            vf4 v = next;
-            next = logits(row, i + 1 < quads ? c0 + 256 * (i + 1) : a.classes);
-            if (w0 + 256 * (i + 1) > a.classes) close_row(v, c0 + 256 * i, a.classes);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f(v[j], c0 + 256 * i + j);
-        }
-    };
-    const float T_ = a.temperature ? a.temperature[r] : 1.0f;
+    // the settings: addresses that are there in any case, so that all are on their way at once
+    float T_ = (a.temperature ? a.temperature : a.u)[r], mp = (a.min_p ? a.min_p : a.u)[r];
     Ask ask;
+    ask.k = (a.top_k ? a.top_k : reinterpret_cast<const int32_t*>(a.u))[r];
+    ask.p = (a.top_p ? a.top_p : a.u)[r];
+    ask.u = a.u[r];
+    T_ = a.temperature ? T_ : 1.0f;
+    mp = a.min_p ? mp : 0.0f;
     ask.T = (double)T_;
-    ask.k = a.top_k ? a.top_k[r] : 0;
-    ask.p = a.top_p ? a.top_p[r] : 1.0f;
-    if (!(ask.p < 1.0f)) ask.p = 1.0f;
+    ask.k = a.top_k ? ask.k : 0;
+    ask.p = a.top_p && ask.p < 1.0f ? ask.p : 1.0f;
     if (ask.p <= 0.0f) ask.k = 1, ask.p = 1.0f;  // the likeliest alone
     if (ask.k < 0 || ask.k >= a.classes) ask.k = 0;
-    const float mp = a.min_p ? a.min_p[r] : 0.0f;
-    ask.limit = mp > 0.0f ? (mp >= 1.0f ? 0.0 : log((double)mp) * ask.T) : -__builtin_inf();
-    ask.u = a.u[r];
+    ask.limit = -__builtin_inf();
+    if (mp > 0.0f) ask.limit = mp >= 1.0f ? 0.0 : log((double)mp) * ask.T;
     ask.u = ask.u > 0.0f ? (ask.u < 1.0f ? ask.u : 0.999999940395355f) : 0.0f;
     const bool greedy = !(T_ > 0.0f);
     const bool cuts = !greedy && (ask.k > 0 || ask.p < 1.0f);
-    // the largest logit held, and the least
-    float top = -__builtin_inff(), low = __builtin_inff();
-    bool nan = false;
-    held([&](float v, int) {
-        nan |= v != v;
-        top = __builtin_fmaxf(top, v);
-        low = v > -__builtin_inff() ? __builtin_fminf(low, v) : low;
-    });
-    auto block_top = [&](float& hi, float* lo) {
+    // the logits held: four at a time, or all of them at once need more registers than there are
+    auto held = [&](auto&& f) {
+        int at = c0;
+        asm volatile("" : "+v"(at));  // or every walk shares the registers of all indices
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            hi = __builtin_fmaxf(hi, __shfl_xor(hi, o));
-            if (lo) *lo = __builtin_fminf(*lo, __shfl_xor(*lo, o));
-        }
-        __syncthreads();
-        if (lane == 0) {
-            s.wave_f[wave] = hi;
-            if (lo) s.wave_d[wave] = (double)*lo;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            hi = __builtin_fmaxf(hi, s.wave_f[i]);
-            if (lo) *lo = __builtin_fminf(*lo, (float)s.wave_d[i]);
+        for (int i = 0; i < Q; ++i)
+            if (i < quads) {
+                f(h[i], at + 256 * i, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    // quads of the run from memory: those of the 64 from `g` on that `which` has a bit for
+    auto walk = [&](auto&& which, auto&& f) {
+        for (int g = 0; g < quads; g += 64) {
+            uint64_t m = which(g);
+            m &= quads - g >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << (quads - g)) - 1;
+            auto take = [&](int& i) {
+                i = m ? g + __builtin_ctzll(m) : -1;
+                m &= m - 1;
+                return logits(row, i >= 0 ? c0 + 256 * i : a.classes);
+            };
+            int i0, i1, i2;
+            vf4 v0 = take(i0), v1 = take(i1);
+            while (i0 >= 0) {
+                vf4 v = v0;
+                const int i = i0;
+                v0 = v1;
+                i0 = i1;
+                v1 = take(i2);
+                i1 = i2;
+                if (w0 + 256 * (i + 1) > a.classes) close_row(v, c0 + 256 * i, a.classes);
+                f(v, c0 + 256 * i, i);
+            }
         }
     };
-    if (tid == 0) s.bad = 0;
-    block_top(top, &low);
-    float best = top;
-    // bins as narrow as the held logits' range allows, none wider than what e^-44 of the largest needs
-    float width = 0.0f, per_bin = 0.0f, ref = top;
-    bool binned = false;
-    if (cuts && a.classes <= kMaxBinned && top > -__builtin_inff() && top < __builtin_inff()) {
-        const float widest = __builtin_fmaxf(T_ * (1.0f / 64.0f), 1.0f / 128.0f);
-        const float wish = __builtin_fminf(widest, (top - low) * (1.25f / (kBins - kAbove)));
-        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(wish, T_ * 1e-6f));
-        width = __builtin_ldexpf(1.0f, e);
-        per_bin = __builtin_ldexpf(1.0f, -e);
-        binned = true;
-    }
-    double rate = 0.0;  // a bin's width over T, in powers of two
-    bool wide = false;
-    for (int turn = 0; binned; ++turn) {
-        rate = (double)width * 1.4426950408889634074 / ask.T;
-        if (turn == 3 || !(rate <= 16.0) || !(rate >= 1e-9)) {
-            binned = false;
-            break;
-        }
-        const float neg = -(float)rate;
+    auto all = [](int) { return ~(uint64_t)0; };
+    auto others = [](int g) { return g ? ~(uint64_t)0 : ~(uint64_t)0 << Q; };
+    float top = -__builtin_inff();  // of what the thread has seen
+    bool nan = false;
+    auto look = [&](const vf4& v) {
+        nan |= __builtin_isunordered(v.x, v.y) | __builtin_isunordered(v.z, v.w);
+        const float q = __builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w));
+        top = __builtin_fmaxf(top, q);
+        return q;
+    };
+    float own_top;  // of the wavefront's run
+    auto block_top = [&]() {
+        own_top = wave_max(top);
         __syncthreads();
+        if (lane == 0) s.wave_f[wave] = own_top;
+        __syncthreads();
+        return wave_max(s.wave_f[lane % W]);
+    };
+    // the largest logit held
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+        if (w0 + 256 * (i + 1) > a.classes || i >= quads) close_row(h[i], i < quads ? c0 + 256 * i : a.classes, a.classes);
+    held([&](const vf4& v, int, int) { look(v); });
+    if (tid == 0) {
+        s.bad = 0;
+        s.first = 0x7fffffff;
+    }
+    float best = block_top();
+    const float ref = best;
+    // masses are e^((x - ref) / T) until the largest is known
+    bool binned = cuts && a.classes <= kMaxBinned && ref > -__builtin_inff() && ref < __builtin_inff() && T_ >= 0.01f && T_ <= 1e30f;
+    // the bins: place_of counts widths below ref and `start`, and bin b holds the places from b - off on
+    int off = kAbove;
+    float per_bin, start = 0.0f;
+    double width;
+    {
+        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * (1.0f / 64.0f));
+        per_bin = __builtin_ldexpf(1.0f, -e);
+        width = __builtin_ldexp(1.0, e);
+    }
+    auto place_of = [&](float v) {  // exact near the bins, so that narrower ones divide those before them
+        return __builtin_fminf(__builtin_fmaf(ref - v, per_bin, -start), 1e6f);
+    };
+    uint32_t base_n = 0;  // what lies above the bins
+    double base_m = 0.0, all_m = 0.0;
+    auto clear = [&]() {
 #pragma unroll
         for (int i = 0; i < B; ++i) s.hist[i * T + tid] = 0;
-        if (tid == 0) s.over = 0;
-        __syncthreads();
-        int over = 0;
-        // what lies past the last bin has less than e^-44 of the largest's mass, or the bins are too narrow
-        const float far = ref - 44.0f * T_;
-        auto count = [&](float v, int c) {
-            const float q = place_of(v, ref, per_bin);
-            const float f = __builtin_floorf(q);
-            const int b = (int)f + kAbove;
-            uint32_t m = (uint32_t)__builtin_fmaf(__builtin_amdgcn_exp2f((q - f) * neg), 16777216.0f, 0.5f);
-            const bool last = b == kBins - 1;
-            over |= (b < 0) | (last && v > far ? 2 : 0);
-            m = last ? 0 : m;
-            if (c < a.classes) atomicAdd(&s.hist[b < 0 ? 0 : b], (unsigned long long)1 << kCountAt | m);
-        };
-        held(count);
-        rest([&](float v, int c) {
-            nan |= v != v;
-            best = __builtin_fmaxf(best, v);
-            count(v, c);
-        });
-        if (over) atomicOr(&s.over, over);
-        if (quads > Q) block_top(best, nullptr);
-        else __syncthreads();
-        over = s.over;
-        if (!over || best == __builtin_inff()) break;
-        // a larger logit was among the others, or one far below: once more, from the largest, with wider bins
-        ref = best;
-        if ((over & 2) || wide) {
-            const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_ * (1.0f / 64.0f), 1.0f / 128.0f));
-            width = __builtin_ldexpf(1.0f, e);
-            per_bin = __builtin_ldexpf(1.0f, -e);
-            wide = true;
+        if (tid == 0) {
+            s.listed = 0;
+            s.k_bin = s.p_lo = s.p_hi = kBins;
         }
-    }
-    if (!binned && quads > Q) {
-        rest([&](float v, int) {
-            nan |= v != v;
-            best = __builtin_fmaxf(best, v);
+    };
+    auto count = [&](const vf4& v) {
+        const float neg = -(float)(width / ask.T * 1.4426950408889634074);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float q = place_of(v[j]);
+            const float f = __builtin_floorf(q);
+            const int b = (int)f + off;
+            uint32_t m = 0;
+            if (ask.p < 1.0f) m = (uint32_t)__builtin_fmaf(__builtin_amdgcn_exp2f((q - f) * neg), 16777216.0f, 0.5f);
+            if ((uint32_t)b < (uint32_t)kBins) atomicAdd(&s.hist[b], (unsigned long long)1 << kCountAt | m);
+        }
+    };
+    if (binned) {
+        clear();
+        __syncthreads();
+        held([&](const vf4& v, int, int i) {
+            count(v);
+            const float q = wave_max(__builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w)));
+            if (lane == 0) s.quad_top[wave * quads + i] = q;
         });
-        block_top(best, nullptr);
+        walk(others, [&](const vf4& v, int, int i) {
+            const float q = wave_max(look(v));
+            if (lane == 0) s.quad_top[wave * quads + i] = q;
+            count(v);
+        });
+    } else if (quads > Q) {
+        walk(others, [&](const vf4& v, int, int) { look(v); });
     }
     if (nan) s.bad = 1;
-    __syncthreads();
+    if (quads > Q || binned) best = block_top();
+    else __syncthreads();
     const bool none = s.bad != 0 || best == -__builtin_inff();
     if (none || greedy) {  // the lowest index of the largest
-        if (tid == 0) s.first = 0x7fffffff;
-        __syncthreads();
         int at = 0x7fffffff;
-        auto look = [&](float v, int c) { at = v == best && c < at ? c : at; };
-        if (!none) {
-            held(look);
-            rest(look);
-        }
+        if (!none && own_top == best)
+            walk(all, [&](const vf4& v, int c, int) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) at = v[j] == best && c + j < at ? c + j : at;
+            });
         if (at != 0x7fffffff) atomicMin(&s.first, at);
         __syncthreads();
         if (tid == 0) {
@@ -502,198 +550,204 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         }
         return;
     }
+    const Mass mass(best, ask);
     bool slow = (cuts && !binned) || best == __builtin_inff() || !(T_ >= 1e-30f && T_ <= 1e30f);
-    if (!slow && cuts) {
-        // the bins' counts and masses, from the top down
-        double M[B];
-        uint32_t N[B], n = 0;
+    // a logit among the others that lies above the bins
+    slow = slow || (cuts && (best - ref) * per_bin >= (float)kAbove);
+    uint64_t cut = ~(uint64_t)0;  // the last class that is kept, as the list's keys
+    for (int turn = 0; !slow && cuts; ++turn) {
+        // the bins' counts and masses, from the top down: each thread's B, then all before it
+        const double rate = width / ask.T;
+        auto bin_mass = [&](uint64_t v, int b) {
+            return (double)(v & (((uint64_t)1 << kCountAt) - 1)) * exp64(-rate * ((double)start + (double)(b - off))) * (1.0 / 16777216.0);
+        };
+        uint32_t n = 0;
         double m = 0.0;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const int b = tid * B + i;
+#pragma nounroll
+        for (int b = tid * B; b < tid * B + B; ++b) {
             const uint64_t v = s.hist[b];
-            N[i] = (uint32_t)(v >> kCountAt);
-            M[i] = N[i] ? (double)(v & (((uint64_t)1 << kCountAt) - 1)) * exp2(-rate * (double)(b - kAbove)) * (1.0 / 16777216.0) : 0.0;
-            n += N[i];
-            m += M[i];
+            n += (uint32_t)(v >> kCountAt);
+            if (v) m += bin_mass(v, b);
         }
-        uint32_t n0, n_all;
-        double m0, m1, m_all;
-        block_scan<W>(n, m, n0, m0, m1, n_all, m_all, s);
-        if (tid == 0) {
-            s.listed = 0;
-            s.k_bin = s.p_lo = s.p_hi = kBins;
-        }
-        __syncthreads();
+        uint32_t n0, n_bins;
+        double m0, m1, m_bins;
+        block_scan<W>(n, m, n0, m0, m1, n_bins, m_bins, s);
+        n0 += base_n;
+        if (turn == 0) all_m = m_bins;
+        // a cut lies in the bin whose sums pass it; where rounding lets none the row goes the slow way
         if (ask.k > 0 && n0 < (uint32_t)ask.k && n0 + n >= (uint32_t)ask.k) {
             uint32_t cn = n0;
             double cm = m0;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                if (cn < (uint32_t)ask.k && cn + N[i] >= (uint32_t)ask.k) {
-                    s.k_bin = tid * B + i;
+#pragma nounroll
+            for (int b = tid * B; b < tid * B + B; ++b) {
+                const uint64_t v = s.hist[b];
+                const uint32_t here = (uint32_t)(v >> kCountAt);
+                const double in = v ? bin_mass(v, b) : 0.0;
+                if (cn + here >= (uint32_t)ask.k) {
+                    s.k_bin = b;
                     s.k_above_n = cn;
-                    s.k_here = N[i];
-                    s.k_above = cm;
-                    s.k_in = M[i];
+                    s.k_here = here;
+                    s.k_above = base_m + cm;
+                    s.k_in = in;
+                    break;
                 }
-                cn += N[i];
-                cm += M[i];
+                cn += here;
+                cm += in;
             }
         }
-        __syncthreads();
-        const uint32_t k_bin = ask.k > 0 ? s.k_bin : kBins;
         if (ask.p < 1.0f) {
+            if (ask.k > 0) __syncthreads();
             // what top_p is a share of is known to within the bin where top_k ends
-            const double lo = (double)ask.p * (ask.k > 0 ? s.k_above : m_all), hi = (double)ask.p * (ask.k > 0 ? s.k_above + s.k_in : m_all);
-            double cm = m0;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const double to = i + 1 < B ? cm + M[i] : m1;
-                if (N[i] > 0 && to >= lo) atomicMin(&s.p_lo, (uint32_t)(tid * B + i));
-                if (N[i] > 0 && to >= hi) atomicMin(&s.p_hi, (uint32_t)(tid * B + i));
-                cm += M[i];
-            }
-            __syncthreads();
-            const uint32_t p_lo = s.p_lo < k_bin ? s.p_lo : k_bin;
-            cm = m0;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                if ((uint32_t)(tid * B + i) == p_lo) s.p_above = cm;
-                cm += M[i];
+            const double hi = (double)ask.p * (ask.k > 0 ? s.k_above + s.k_in : all_m) - base_m;
+            double lo = ask.k > 0 ? (double)ask.p * s.k_above - base_m : hi;
+            lo = lo > 0.0 ? lo : 1e-300;
+            if ((m0 < lo && m1 >= lo) || (m0 < hi && m1 >= hi)) {
+                uint32_t cn = n0;
+                double cm = m0;
+#pragma nounroll
+                for (int b = tid * B; b < tid * B + B; ++b) {
+                    const uint64_t v = s.hist[b];
+                    const double to = b + 1 < tid * B + B ? cm + (v ? bin_mass(v, b) : 0.0) : m1;
+                    if (cm < lo && to >= lo) {
+                        s.p_lo = b;
+                        s.p_above = base_m + cm;
+                        s.p_above_n = cn;
+                    }
+                    if (cm < hi && to >= hi) s.p_hi = b;
+                    cn += (uint32_t)(v >> kCountAt);
+                    cm = to;
+                }
             }
         }
         __syncthreads();
-        const uint32_t p_hi = ask.p < 1.0f ? (s.p_hi < k_bin ? s.p_hi : k_bin) : k_bin;
-        const uint32_t p_lo = ask.p < 1.0f ? (s.p_lo < p_hi ? s.p_lo : p_hi) : k_bin;
-        // a cut among what has no mass in the bins
-        slow = p_hi >= kBins - 1 || k_bin == kBins - 1;
-        if (!slow) {
-            // what lies in the bins of a cut is listed, what lies above is added up, a run each
-            const float p_from = (float)((int)p_lo - kAbove), p_to = (float)((int)p_hi - kAbove), k_at = (float)((int)k_bin - kAbove);
-            double sum = 0.0;
-            const bool all_above = !(mp > 0.0f);
-            const float rate_hi = (float)(1.4426950408889634074 / ask.T), rate_lo = (float)(1.4426950408889634074 / ask.T - (double)rate_hi);
-            auto mass = [&](float v) {
-                const float d = v - best;
-                const float t = d * rate_hi;
-                const float e = __builtin_amdgcn_exp2f(t);
-                return __builtin_fmaf(e, (__builtin_fmaf(d, rate_hi, -t) + d * rate_lo) * 0.693147180559945f, e);
-            };
-            auto pick = [&](float v, int c) {
-                const float f = __builtin_floorf(place_of(v, ref, per_bin));
-                if (f < p_from) {
-                    if (all_above || (double)v - (double)best >= ask.limit) sum += (double)mass(v);
-                } else if ((f <= p_to || f == k_at) && c < a.classes) {
-                    const uint32_t at = atomicAdd(&s.listed, 1u);
-                    if (at < kList) s.list.key[at] = (uint64_t)(~order_of(v)) << 32 | (uint32_t)c;
-                }
-            };
-            __syncthreads();  // the bins make room for the list
-            held(pick);
-            rest(pick);
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-            if (lane == 0) s.seg[wave] = sum;
-            __syncthreads();
-            const int n_list = (int)s.listed;
-            slow = n_list > kList;
-            if (!slow) {
-                int n2 = 2;
-                while (n2 < n_list) n2 *= 2;
-                for (int i = n_list + tid; i < n2; i += T) s.list.key[i] = ~(uint64_t)0;
-                __syncthreads();
-                for (int size = 2; size <= n2; size *= 2)
-                    for (int step = size / 2; step > 0; step /= 2) {
-                        for (int i = tid; i < n2 / 2; i += T) {
-                            const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                            const bool up = (lo & size) == 0;
-                            const uint64_t p = s.list.key[lo], q = s.list.key[hi];
-                            if ((p > q) == up) {
-                                s.list.key[lo] = q;
-                                s.list.key[hi] = p;
-                            }
-                        }
-                        __syncthreads();
-                    }
-                // their masses' running sums
-                constexpr int E = kList / T;
-                double own[E], sum_e = 0.0;
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int at = tid * E + i;
-                    own[i] = 0.0;
-                    if (at < n_list) {
-                        const float v = of_order(~(uint32_t)(s.list.key[at] >> 32));
-                        own[i] = exp2(((double)v - (double)ref) * (1.4426950408889634074 / ask.T));
-                    }
-                    sum_e += own[i];
-                }
-                uint32_t unused0, unused1;
-                double e0, e1, e_all;
-                block_scan<W>(0, sum_e, unused0, e0, e1, unused1, e_all, s);
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    e0 += own[i];
-                    if (tid * E + i < n_list) s.list.upto[tid * E + i] = e0;
-                }
-                if (tid == 0) s.first = n_list - 1;
-                __syncthreads();
-                int last = n_list - 1;  // the last that is kept
-                double need = 0.0;
-                if (ask.k > 0) {
-                    const int before = n_list - (int)s.k_here;  // above the bin where top_k ends
-                    const int k_last = before + (ask.k - (int)s.k_above_n) - 1;
-                    need = (double)ask.p * (s.k_above + s.list.upto[k_last] - (before > 0 ? s.list.upto[before - 1] : 0.0));
-                    last = k_last;
-                } else {
-                    need = (double)ask.p * m_all;
-                }
-                if (ask.p < 1.0f) {
-                    const int end = ask.k > 0 && k_bin > p_hi ? n_list - (int)s.k_here - 1 : last;
-                    for (int i = tid; i <= end; i += T)
-                        if (s.p_above + s.list.upto[i] >= need) {
-                            atomicMin(&s.first, i);
-                            break;
-                        }
-                    __syncthreads();
-                    last = s.first < end ? s.first : end;
-                }
-                if (tid == 0) s.cut = s.list.key[last];
-                // the kept of the list join their runs
-                const int per = (n_list + 63) / 64;
-                double add = 0.0;
-                for (int i = lane * per; i < lane * per + per && i <= last; ++i) {
-                    const uint64_t k = s.list.key[i];
-                    const int c = (int)(uint32_t)k;
-                    if (c / run != wave) continue;
-                    const float v = of_order(~(uint32_t)(k >> 32));
-                    if (all_above || (double)v - (double)best >= ask.limit) add += (double)mass(v);
-                }
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) add += __shfl_xor(add, o);
-                if (lane == 0) s.seg[wave] += add;
-                __syncthreads();
-            }
+        const int k_bin = ask.k > 0 ? (int)s.k_bin : kBins;
+        int p_lo = k_bin, p_hi = k_bin;
+        if (ask.p < 1.0f) {
+            p_lo = (int)s.p_lo;
+            p_hi = (int)s.p_hi < k_bin ? (int)s.p_hi : k_bin;
         }
-    } else if (!slow) {
-        // nothing but min_p: every class counts
-        const float rate_hi = (float)(1.4426950408889634074 / ask.T), rate_lo = (float)(1.4426950408889634074 / ask.T - (double)rate_hi);
+        const int most = k_bin < kBins ? k_bin : p_hi;  // the last bin that is listed
+        slow = p_lo > p_hi || most >= kBins || (ask.k > 0 && k_bin == kBins);
+        if (slow) break;
+        // what lies in the bins of a cut is listed, what lies above is added up, a run each
         double sum = 0.0;
-        auto add = [&](float v, int) {
-            if (!((double)v - (double)best >= ask.limit)) return;
-            const float d = v - best;
-            const float t = d * rate_hi;
-            if (!(t > -150.0f)) return;
-            const float e = __builtin_amdgcn_exp2f(t);
-            sum += (double)__builtin_fmaf(e, (__builtin_fmaf(d, rate_hi, -t) + d * rate_lo) * 0.693147180559945f, e);
-        };
-        held(add);
-        rest(add);
+        __syncthreads();  // the bins make room for the list
+        walk(
+            [&](int g) {
+                const float v = s.quad_top[wave * quads + (g + lane < quads ? g + lane : 0)];
+                return __ballot((int)__builtin_floorf(place_of(v)) + off <= most);
+            },
+            [&](const vf4& v, int c, int) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = (int)__builtin_floorf(place_of(v[j])) + off;
+                    if (b < p_lo) {
+                        sum += mass(v[j]);
+                    } else if (b <= p_hi || b == k_bin) {
+                        const uint32_t at = atomicAdd(&s.listed, 1u);
+                        if (at < kList) s.list.key[at] = (uint64_t)(~order_of(v[j])) << 32 | (uint32_t)(c + j);
+                    }
+                }
+            });
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
         if (lane == 0) s.seg[wave] = sum;
-        if (tid == 0) s.cut = ~(uint64_t)0;
+        __syncthreads();
+        const int n_list = (int)s.listed;
+        if (n_list > kList) {
+            // the bins of the cuts alone, as narrow as that makes them
+            const int e = __builtin_amdgcn_frexp_expf((float)(most + 1 - p_lo) * (1.0f / kBins));
+            slow = turn == 2 || e >= 0;
+            if (slow) break;
+            if (ask.p < 1.0f) {
+                base_n = s.p_above_n;
+                base_m = s.p_above;
+            } else {
+                base_n = s.k_above_n;
+                base_m = s.k_above;
+            }
+            start = __builtin_ldexpf(start + (float)(p_lo - off), -e);
+            off = 0;
+            width = __builtin_ldexp(width, e);
+            per_bin = __builtin_ldexpf(per_bin, -e);
+            __syncthreads();
+            clear();
+            __syncthreads();
+            walk(all, [&](const vf4& v, int, int) { count(v); });
+            __syncthreads();
+            continue;
+        }
+        int n2 = 2;
+        while (n2 < n_list) n2 *= 2;
+        for (int i = n_list + tid; i < n2; i += T) s.list.key[i] = ~(uint64_t)0;
+        __syncthreads();
+        for (int size = 2; size <= n2; size *= 2)
+            for (int step = size / 2; step > 0; step /= 2) {
+                for (int i = tid; i < n2 / 2; i += T) {
+                    const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                    const bool up = (lo & size) == 0;
+                    const uint64_t p = s.list.key[lo], q = s.list.key[hi];
+                    if ((p > q) == up) {
+                        s.list.key[lo] = q;
+                        s.list.key[hi] = p;
+                    }
+                }
+                __syncthreads();
+            }
+        // their masses' running sums
+        const int per = (n_list + T - 1) / T, i0 = tid * per, i1 = i0 + per < n_list ? i0 + per : n_list;
+        auto in_bins = [&](int i) {  // as the bins have it
+            return exp64(((double)of_order(~(uint32_t)(s.list.key[i] >> 32)) - (double)ref) / ask.T);
+        };
+        double own = 0.0;
+#pragma nounroll
+        for (int i = i0; i < i1; ++i) own += in_bins(i);
+        uint32_t unused0, unused1;
+        double e0, e1, e_all;
+        block_scan<W>(0, own, unused0, e0, e1, unused1, e_all, s);
+#pragma nounroll
+        for (int i = i0; i < i1; ++i) s.list.upto[i] = e0 += in_bins(i);
+        __syncthreads();
+        int last = n_list - 1;  // the last that is kept
+        double share = all_m;   // what top_p is a share of
+        int end = last;         // of top_p's part of the list
+        if (ask.k > 0) {
+            const int before = n_list - (int)s.k_here;  // above the bin where top_k ends
+            last = before + (ask.k - (int)s.k_above_n) - 1;
+            share = s.k_above + s.list.upto[last] - (before > 0 ? s.list.upto[before - 1] : 0.0);
+            end = k_bin > p_hi ? before - 1 : last;
+        }
+        if (ask.p < 1.0f) {
+            const double least = (double)ask.p * share - s.p_above;
+            for (int i = tid; i < end; i += T)
+                if (s.list.upto[i] >= least && (i == 0 || s.list.upto[i - 1] < least)) s.first = i;
+            __syncthreads();
+            last = s.first < end ? s.first : end;
+        }
+        cut = s.list.key[last];
+        // the kept of the list join their runs
+        const int each = (n_list + 63) / 64;
+        double add = 0.0;
+        for (int i = lane * each; i < lane * each + each && i <= last; ++i) {
+            const uint64_t k = s.list.key[i];
+            const int c = (int)(uint32_t)k;
+            if (c >= w0 && c < w0 + run) add += mass(of_order(~(uint32_t)(k >> 32)));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) add += __shfl_xor(add, o);
+        if (lane == 0) s.seg[wave] += add;
+        __syncthreads();
+        break;
+    }
+    if (!slow && !cuts) {  // nothing but min_p: every class counts
+        double sum = 0.0;
+        walk(all, [&](const vf4& v, int, int) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += mass(v[j]);
+        });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) s.seg[wave] = sum;
         __syncthreads();
     }
     if (slow) {
@@ -702,27 +756,17 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         return;
     }
     // the run where the running sum passes u of the total, and in it the class
-    double total = 0.0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) total += s.seg[i];
-    const double goal = (double)ask.u * total;
-    double before = 0.0, from = 0.0;
-    int seg = -1;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const double to = before + s.seg[i];
-        if (s.seg[i] > 0.0 && (seg < 0 || from + s.seg[seg] <= goal)) {
-            seg = i;
-            from = before;
-        }
-        before = to;
+    const double segs = row_scan(lane < W ? s.seg[lane & 15] : 0.0);
+    const double total = lane_value(segs, W - 1), goal = (double)ask.u * total;
+    int seg;
+    double from = 0.0;
+    {
+        // the first whose sum passes the goal, or where rounding lets none the last with any mass
+        const uint64_t passed = __ballot(lane < W && segs > goal), some = __ballot(lane < W && s.seg[lane & 15] > 0.0);
+        seg = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
+        if (seg > 0) from = lane_value(segs, seg - 1);
     }
-    const uint64_t cut = s.cut;
-    if (tid == 0) {
-        s.first = 0x7fffffff;
-        s.last = -1;
-    }
-    const float rate_hi = (float)(1.4426950408889634074 / ask.T), rate_lo = (float)(1.4426950408889634074 / ask.T - (double)rate_hi);
+    if (tid == 0) s.first = -1;
     // parts of the run in turn, 4 classes a thread
     for (int p0 = seg * run; p0 < (seg + 1) * run; p0 += 4 * T) {
         const int c = p0 + 4 * tid;
@@ -731,35 +775,33 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint64_t k = (uint64_t)(~order_of(v[j])) << 32 | (uint32_t)(c + j);
-            const float d = v[j] - best;
-            const float t = d * rate_hi;
-            w[j] = 0.0;
-            if (c < (seg + 1) * run && c + j < a.classes && k <= cut && (double)v[j] - (double)best >= ask.limit && t > -150.0f) {
-                const float e = __builtin_amdgcn_exp2f(t);
-                w[j] = (double)__builtin_fmaf(e, (__builtin_fmaf(d, rate_hi, -t) + d * rate_lo) * 0.693147180559945f, e);
-            }
+            w[j] = c < (seg + 1) * run && c + j < a.classes && k <= cut ? mass(v[j]) : 0.0;
             own += w[j];
         }
         uint32_t unused0, unused1;
-        double w0, w1, w_all;
-        block_scan<W>(0, own, unused0, w0, w1, unused1, w_all, s);
-        double upto = from + w0;
+        double m0, m1, part;
+        block_scan<W>(0, own, unused0, m0, m1, unused1, part, s);
+        double upto = from + m0;
+        if (own > 0.0 && upto <= goal && goal < from + m1) {
+            int at = -1, end = -1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            upto += w[j];
-            if (w[j] > 0.0) {
-                if (upto > goal) atomicMin(&s.first, c + j);
-                atomicMax(&s.last, c + j);
+            for (int j = 0; j < 4; ++j) {
+                upto += w[j];
+                end = w[j] > 0.0 ? c + j : end;
+                at = w[j] > 0.0 && at < 0 && upto > goal ? c + j : at;
             }
+            s.first = at >= 0 ? at : end;
         }
         __syncthreads();
-        if (s.first != 0x7fffffff) break;
-        from += w_all;
+        if (s.first >= 0) break;
+        from += part;
     }
-    // a sum that rounding left short of the goal ends at the run's last
-    __syncthreads();
     if (tid == 0) {
-        const int at = s.first != 0x7fffffff ? s.first : s.last;
+        int at = s.first;
+        if (at < 0) {  // a sum that rounding left short of the goal ends at the run's last
+            at = (seg + 1) * run < a.classes ? (seg + 1) * run : a.classes;
+            for (--at; ((uint64_t)(~order_of(x[at])) << 32 | (uint32_t)at) > cut || mass(x[at]) == 0.0;) --at;
+        }
         a.tokens[r] = at;
         if (a.logprob) a.logprob[r] = share_log(x[at], best, ask.T, total);
     }
