@@ -6,7 +6,7 @@
 //
 // A workgroup takes a row, a wavefront a run of its classes, of which each lane holds 4 Q logits in registers (the whole
 // row up to 4 Q T classes; of a longer one the rest is read as it is needed):
-//   1. the largest logit held, the reference, and bins of a power-of-two width, T / 64 or 1 / 64 at least, around it;
+//   1. the largest logit held, the reference, and bins of a power-of-two width, T / 112 or 1 / 112 at least, around it;
 //   2. for top-k and top-p how many classes each bin has and their mass, both in one 64-bit LDS atomic: 20 bits of count above
 //      44 of mass, a class 24 bits of its bin's largest. Whole numbers: the atomics' order does not show. A scan of the bins
 //      then says in which of them a cut falls;
@@ -17,7 +17,7 @@
 // Sums of steps 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
 // sign, moves a border by some 2^-24 of the row.
 //
-// Rows for which bins do not work (more than 2048 classes of one value at a cut, a cut 48 T below the largest, an infinite
+// Rows for which bins do not work (more than 2048 classes of one value at a cut, a cut 32 T below the largest, an infinite
 // logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over the logits'
 // bits, 8 at a time: right for every row, and slower.
 #include "mh_internal.h"
@@ -27,7 +27,7 @@ namespace mh {
 namespace {
 
 constexpr int kBins = 4096;
-constexpr int kAbove = 1024;  // of them above the reference at first
+constexpr int kAbove = 512;  // of them above the reference at first
 constexpr int kList = 2048;
 constexpr int kCountAt = 44;
 constexpr int64_t kMaxBinned = (int64_t)1 << 19;
@@ -297,6 +297,22 @@ __device__ __attribute__((noinline)) void slow_row(const float* x, int classes, 
 // ---------------------------------------------------------------------------------------
 // rows that bins sort out
 // ---------------------------------------------------------------------------------------
+// The least logit that `is` holds for; it holds for every larger one, infinity too. 64 at a time are looked at, 6 bits of
+// their order. By whole wavefronts.
+template <typename F>
+__device__ __forceinline__ float least_of(F&& is) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t key = 0;  // the largest known for which it does not hold: a NaN's
+#pragma unroll
+    for (int place = 26; place >= -4; place -= 6) {
+        const int p = place < 0 ? 0 : place;
+        const uint32_t k = key + ((place < 0 ? lane & 3 : lane) << p);
+        const bool no = k <= 0xff800000u && !is(of_order(k));
+        key += (uint32_t)(__builtin_popcountll(__ballot(no && (place >= 0 || lane < 4))) - 1) << p;
+    }
+    return of_order(key + 1);
+}
+
 struct FastLds {
     union {
         unsigned long long hist[kBins];
@@ -371,13 +387,13 @@ struct Mass {
             least = __uint_as_float(b >> 31 ? b - 1 : b + 1);
         }
     }
-    __device__ __forceinline__ double operator()(float v) const {
+    __device__ __forceinline__ float raw(float v) const {  // of a finite logit
         const float d = v - best;
         const float t = d * hi;
-        if (!(v >= least) || !(t > -150.0f)) return 0.0;
         const float e = __builtin_amdgcn_exp2f(t);
-        return (double)__builtin_fmaf(e, (__builtin_fmaf(d, hi, -t) + d * lo) * 0.693147180559945f, e);
+        return __builtin_fmaf(e, __builtin_fmaf(d, lo, __builtin_fmaf(d, hi, -t)) * 0.693147180559945f, e);
     }
+    __device__ __forceinline__ float operator()(float v) const { return v >= least && (v - best) * hi > -150.0f ? raw(v) : 0.0f; }
 };
 
 template <int T, int Q>
@@ -478,7 +494,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         s.first = 0x7fffffff;
     }
     float best = block_top();
-    const float ref = best;
+    float ref = best;
     // masses are e^((x - ref) / T) until the largest is known
     bool binned = cuts && a.classes <= kMaxBinned && ref > -__builtin_inff() && ref < __builtin_inff() && T_ >= 0.01f && T_ <= 1e30f;
     // the bins: place_of counts widths below ref and `start`, and bin b holds the places from b - off on
@@ -486,7 +502,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     float per_bin, start = 0.0f;
     double width;
     {
-        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * (1.0f / 64.0f));
+        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * (1.0f / 112.0f));
         per_bin = __builtin_ldexpf(1.0f, -e);
         width = __builtin_ldexp(1.0, e);
     }
@@ -552,8 +568,14 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     }
     const Mass mass(best, ask);
     bool slow = (cuts && !binned) || best == __builtin_inff() || !(T_ >= 1e-30f && T_ <= 1e30f);
-    // a logit among the others that lies above the bins
-    slow = slow || (cuts && (best - ref) * per_bin >= (float)kAbove);
+    if (!slow && cuts && (best - ref) * per_bin >= (float)kAbove) {  // one of the others lies above the bins
+        __syncthreads();
+        clear();
+        __syncthreads();
+        ref = best;
+        walk(all, [&](const vf4& v, int, int) { count(v); });
+        __syncthreads();
+    }
     uint64_t cut = ~(uint64_t)0;  // the last class that is kept, as the list's keys
     for (int turn = 0; !slow && cuts; ++turn) {
         // the bins' counts and masses, from the top down: each thread's B, then all before it
@@ -630,20 +652,30 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         slow = p_lo > p_hi || most >= kBins || (ask.k > 0 && k_bin == kBins);
         if (slow) break;
         // what lies in the bins of a cut is listed, what lies above is added up, a run each
+        auto bin_of = [&](float v) { return (int)__builtin_floorf(place_of(v)) + off; };
+        const float v_list = least_of([&](float v) { return bin_of(v) <= most; });
+        const float v_keep = least_of([&](float v) { return bin_of(v) < p_lo; });
+        // no mass below e^-100 of the largest's; what min_p drops has none
+        const float v_sum = __builtin_fmaxf(__builtin_fmaxf(v_keep, mass.least), (float)((double)best - 100.0 * ask.T));
         double sum = 0.0;
         __syncthreads();  // the bins make room for the list
         walk(
-            [&](int g) {
-                const float v = s.quad_top[wave * quads + (g + lane < quads ? g + lane : 0)];
-                return __ballot((int)__builtin_floorf(place_of(v)) + off <= most);
-            },
+            [&](int g) { return __ballot(s.quad_top[wave * quads + (g + lane < quads ? g + lane : 0)] >= v_list); },
             [&](const vf4& v, int c, int) {
+                float q = 0.0f;
+                bool some = false;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int b = (int)__builtin_floorf(place_of(v[j])) + off;
-                    if (b < p_lo) {
-                        sum += mass(v[j]);
-                    } else if (b <= p_hi || b == k_bin) {
+                    const float e = mass.raw(v[j]);
+                    q += v[j] >= v_sum ? e : 0.0f;
+                    some |= v[j] >= v_list && !(v[j] >= v_keep);
+                }
+                sum += (double)q;
+                if (some) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int b = bin_of(v[j]);
+                        if (b < p_lo || (b > p_hi && b != k_bin)) continue;
                         const uint32_t at = atomicAdd(&s.listed, 1u);
                         if (at < kList) s.list.key[at] = (uint64_t)(~order_of(v[j])) << 32 | (uint32_t)(c + j);
                     }
@@ -731,7 +763,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         for (int i = lane * each; i < lane * each + each && i <= last; ++i) {
             const uint64_t k = s.list.key[i];
             const int c = (int)(uint32_t)k;
-            if (c >= w0 && c < w0 + run) add += mass(of_order(~(uint32_t)(k >> 32)));
+            if (c >= w0 && c < w0 + run) add += (double)mass(of_order(~(uint32_t)(k >> 32)));
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) add += __shfl_xor(add, o);
@@ -742,8 +774,10 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     if (!slow && !cuts) {  // nothing but min_p: every class counts
         double sum = 0.0;
         walk(all, [&](const vf4& v, int, int) {
+            float q = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += mass(v[j]);
+            for (int j = 0; j < 4; ++j) q += mass(v[j]);
+            sum += (double)q;
         });
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -767,30 +801,57 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         if (seg > 0) from = lane_value(segs, seg - 1);
     }
     if (tid == 0) s.first = -1;
-    // parts of the run in turn, 4 classes a thread
-    for (int p0 = seg * run; p0 < (seg + 1) * run; p0 += 4 * T) {
-        const int c = p0 + 4 * tid;
-        const vf4 v = logits(row, c < (seg + 1) * run ? c : a.classes);
-        double w[4], own = 0.0;
+    // the run in parts, each thread its own neighbouring quads of a part
+    constexpr int P = Q < 8 ? Q : 8;
+    const int stop = (seg + 1) * run < a.classes ? (seg + 1) * run : a.classes;
+    for (int p0 = seg * run; p0 < stop; p0 += 4 * P * T) {
+        const int each = (stop - p0 + 4 * T - 1) / (4 * T) < P ? (stop - p0 + 4 * T - 1) / (4 * T) : P;
+        const int c = p0 + 4 * each * tid;
+        vf4 v[P];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint64_t k = (uint64_t)(~order_of(v[j])) << 32 | (uint32_t)(c + j);
-            w[j] = c < (seg + 1) * run && c + j < a.classes && k <= cut ? mass(v[j]) : 0.0;
-            own += w[j];
+        for (int i = 0; i < P; ++i) v[i] = logits(row, i < each ? c + 4 * i : a.classes);
+        double own[P], m = 0.0;
+        auto kept = [&](float x, int c) {
+            const uint64_t k = (uint64_t)(~order_of(x)) << 32 | (uint32_t)c;
+            return c < stop && k <= cut ? mass(x) : 0.0f;
+        };
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            own[i] = 0.0;
+            if (i < each) {
+                float q = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q += kept(v[i][j], c + 4 * i + j);
+                own[i] = (double)q;
+            }
+            m += own[i];
         }
         uint32_t unused0, unused1;
         double m0, m1, part;
-        block_scan<W>(0, own, unused0, m0, m1, unused1, part, s);
-        double upto = from + m0;
-        if (own > 0.0 && upto <= goal && goal < from + m1) {
-            int at = -1, end = -1;
+        block_scan<W>(0, m, unused0, m0, m1, unused1, part, s);
+        if (m > 0.0 && from + m0 <= goal && goal < from + m1) {
+            // the quad, the first that passes the goal or else the last with any mass, and in it the class
+            double upto = from + m0, to = upto;
+            int at = c;
+            vf4 quad = v[0];
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (own[i] > 0.0 && to <= goal) {
+                    upto = to;
+                    at = c + 4 * i;
+                    quad = v[i];
+                }
+                to += own[i];
+            }
+            int found = -1;
+            float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                upto += w[j];
-                end = w[j] > 0.0 ? c + j : end;
-                at = w[j] > 0.0 && at < 0 && upto > goal ? c + j : at;
+                const float e = kept(quad[j], at + j);
+                if (e > 0.0f && (found < 0 || upto + (double)sum <= goal)) found = at + j;
+                sum += e;
             }
-            s.first = at >= 0 ? at : end;
+            s.first = found;
         }
         __syncthreads();
         if (s.first >= 0) break;
@@ -799,8 +860,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     if (tid == 0) {
         int at = s.first;
         if (at < 0) {  // a sum that rounding left short of the goal ends at the run's last
-            at = (seg + 1) * run < a.classes ? (seg + 1) * run : a.classes;
-            for (--at; ((uint64_t)(~order_of(x[at])) << 32 | (uint32_t)at) > cut || mass(x[at]) == 0.0;) --at;
+            at = stop;
+            for (--at; at > 0 && (((uint64_t)(~order_of(x[at])) << 32 | (uint32_t)at) > cut || mass(x[at]) == 0.0f);) --at;
         }
         a.tokens[r] = at;
         if (a.logprob) a.logprob[r] = share_log(x[at], best, ask.T, total);
@@ -844,7 +905,8 @@ int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const floa
     a.classes = (int32_t)classes;
     a.shift = 62;
     while (((int64_t)1 << (62 - a.shift)) < classes) --a.shift;
-    launch_sample<1024, 16>(a, rows);
+    if (rows > 256) launch_sample<512, 16>(a, rows);
+    else launch_sample<1024, 16>(a, rows);
     return finish("mh_sample_tokens");
 }
 
