@@ -468,19 +468,22 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     };
     auto all = [](int) { return ~(uint64_t)0; };
     auto others = [](int g) { return g ? ~(uint64_t)0 : ~(uint64_t)0 << Q; };
-    float top = -__builtin_inff();  // of what the thread has seen
+    float top = -__builtin_inff();  // of what the wavefront has seen
     bool nan = false;
-    auto look = [&](const vf4& v) {
+    const bool tops = a.classes <= kMaxBinned;
+    auto look = [&](const vf4& v, int i) {
         nan |= __builtin_isunordered(v.x, v.y) | __builtin_isunordered(v.z, v.w);
-        const float q = __builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w));
+        const float q = wave_max(__builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w)));
         top = __builtin_fmaxf(top, q);
-        return q;
+        if (tops && lane == 0) s.quad_top[wave * quads + i] = q;
     };
-    float own_top;  // of the wavefront's run
+    // the quads that reach a logit
+    auto reach = [&](float v) {
+        return [=, &s](int g) { return tops ? __ballot(s.quad_top[wave * quads + (g + lane < quads ? g + lane : 0)] >= v) : ~(uint64_t)0; };
+    };
     auto block_top = [&]() {
-        own_top = wave_max(top);
         __syncthreads();
-        if (lane == 0) s.wave_f[wave] = own_top;
+        if (lane == 0) s.wave_f[wave] = top;
         __syncthreads();
         return wave_max(s.wave_f[lane % W]);
     };
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
 #pragma unroll
     for (int i = 0; i < Q; ++i)
         if (w0 + 256 * (i + 1) > a.classes || i >= quads) close_row(h[i], i < quads ? c0 + 256 * i : a.classes, a.classes);
-    held([&](const vf4& v, int, int) { look(v); });
+    held([&](const vf4& v, int, int i) { look(v, i); });
     if (tid == 0) {
         s.bad = 0;
         s.first = 0x7fffffff;
@@ -534,18 +537,13 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     if (binned) {
         clear();
         __syncthreads();
-        held([&](const vf4& v, int, int i) {
-            count(v);
-            const float q = wave_max(__builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w)));
-            if (lane == 0) s.quad_top[wave * quads + i] = q;
-        });
+        held([&](const vf4& v, int, int) { count(v); });
         walk(others, [&](const vf4& v, int, int i) {
-            const float q = wave_max(look(v));
-            if (lane == 0) s.quad_top[wave * quads + i] = q;
+            look(v, i);
             count(v);
         });
     } else if (quads > Q) {
-        walk(others, [&](const vf4& v, int, int) { look(v); });
+        walk(others, [&](const vf4& v, int, int i) { look(v, i); });
     }
     if (nan) s.bad = 1;
     if (quads > Q || binned) best = block_top();
@@ -553,8 +551,8 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     const bool none = s.bad != 0 || best == -__builtin_inff();
     if (none || greedy) {  // the lowest index of the largest
         int at = 0x7fffffff;
-        if (!none && own_top == best)
-            walk(all, [&](const vf4& v, int c, int) {
+        if (!none && top == best)
+            walk(reach(best), [&](const vf4& v, int c, int) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) at = v[j] == best && c + j < at ? c + j : at;
             });
@@ -660,7 +658,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         double sum = 0.0;
         __syncthreads();  // the bins make room for the list
         walk(
-            [&](int g) { return __ballot(s.quad_top[wave * quads + (g + lane < quads ? g + lane : 0)] >= v_list); },
+            reach(v_list),
             [&](const vf4& v, int c, int) {
                 float q = 0.0f;
                 bool some = false;
@@ -773,7 +771,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     }
     if (!slow && !cuts) {  // nothing but min_p: every class counts
         double sum = 0.0;
-        walk(all, [&](const vf4& v, int, int) {
+        walk(reach(mass.least), [&](const vf4& v, int, int) {
             float q = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) q += mass(v[j]);
