@@ -8,18 +8,20 @@
 //     softmax:  grad_j = scale p_j (g_j - sum g p)          normalised: scale q_i (g_i - sum g q)
 //
 // Scores decide a choice after a bias was added to them, so logits do not: experts whose biased scores agree to fp32 are
-// not rare over a long batch, and which of them is chosen shows. Scores, biased scores and groups' sums are therefore made
-// in 64 bits (an exponential's Taylor series, 13 terms within half of ln 2); weights and gradients are fp32.
-// Bound by the logits' read and the gradient's write, and over many experts by the scores' arithmetic. L lanes hold a row
-// in registers, V elements a lane in quads (element 4 (i L + lane) + c).
+// not rare over a long batch, and which of them is chosen shows. What is compared is therefore meant in 64 bits. Up to 8
+// choices are made in fp32 first, by sorted lists of the row, with a bound on its error: a row whose choice, or whose choice
+// of groups, turns on less than twice that (one in a few hundred) is chosen again in 64 bits by a whole wavefront, and so
+// is every row of more than 8. Weights are 64-bit scores rounded to fp32, whichever way the choice went; gradients fp32.
+//
+// Bound by the logits' read and the gradient's write, and over many experts by the sorting. L lanes hold a row in
+// registers, V elements a lane in quads (element 4 (i L + lane) + c).
 #include "mh_internal.h"
+#include "mh_lanes.h"
 #include "mh_rows.h"
 
 namespace mh {
 namespace {
 
-constexpr int kMaxExperts = 1024;
-constexpr int kMaxChosen = 64;
 constexpr int kMaxGroups = 64;
 constexpr int kRThreads = 256;
 constexpr int kRBlocks = 1024;  // workgroups of a forward at most: rows of its partial counts
@@ -44,40 +46,21 @@ struct GroupArg {
     const int32_t* sel;
 };
 
-template <int CTRL>
-__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
-// The value of the lane STEP beside, within groups of neighbouring lanes.
+// As group_red and others, of values of 64 bits.
 template <int STEP>
-__device__ __forceinline__ int other_lane(int v) {
-    return STEP == 1 ? dpp<0xB1>(v) : STEP == 2 ? dpp<0x4E>(v) : STEP == 4 ? dpp<0x141>(v) : STEP == 8 ? dpp<0x140>(v)
-                                                                                                  : __shfl_xor(v, STEP);
+__device__ __forceinline__ uint64_t other64(uint64_t v) {
+    return (uint64_t)(uint32_t)other_lane<STEP>((int)(v >> 32)) << 32 | (uint32_t)other_lane<STEP>((int)v);
 }
-template <int STEP>
-__device__ __forceinline__ double other_lane(double v) {
-    return __hiloint2double(other_lane<STEP>(__double2hiint(v)), other_lane<STEP>(__double2loint(v)));
-}
-template <int STEP>
-__device__ __forceinline__ int64_t other_lane(int64_t v) {
-    return (int64_t)((uint64_t)(uint32_t)other_lane<STEP>((int)(v >> 32)) << 32 | (uint32_t)other_lane<STEP>((int)v));
-}
-template <int STEP>
-__device__ __forceinline__ float other_lane(float v) { return __int_as_float(other_lane<STEP>(__float_as_int(v))); }
-// Reductions over groups of L neighbouring lanes, the result in every lane.
 template <int L, int STEP = 1, typename T, typename Op>
-__device__ __forceinline__ T group_red(T v, Op op) {
-    if constexpr (STEP < L) return group_red<L, 2 * STEP>(op(v, other_lane<STEP>(v)), op);
+__device__ __forceinline__ T group_red64(T v, Op op) {
+    if constexpr (STEP < L)
+        return group_red64<L, 2 * STEP>(op(v, __builtin_bit_cast(T, other64<STEP>(__builtin_bit_cast(uint64_t, v)))), op);
     return v;
 }
-template <int L, typename T>
-__device__ __forceinline__ T group_sum(T v) { return group_red<L>(v, [](T p, T q) { return p + q; }); }
 template <int L>
-__device__ __forceinline__ float group_max(float v) { return group_red<L>(v, [](float p, float q) { return __builtin_fmaxf(p, q); }); }
-
-// A wavefront's LDS accesses so far come before those that follow.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
+__device__ __forceinline__ double group_sum64(double v) { return group_red64<L>(v, [](double p, double q) { return p + q; }); }
+template <int L>
+__device__ __forceinline__ float group_min(float v) { return -group_max<L>(-v); }
 
 __device__ __forceinline__ double sigmoid64(float x) {
     const double e = exp64(-__builtin_fabs((double)x));
@@ -86,166 +69,268 @@ __device__ __forceinline__ double sigmoid64(float x) {
 
 // A double as an integer of the same order; NaN below every number, -0 as +0; below them what may not be chosen.
 constexpr int64_t kNever = INT64_MIN;
-__device__ __forceinline__ int64_t sort_key(double v) {
+__device__ __forceinline__ int64_t sort_key64(double v) {
     const int64_t b = __double_as_longlong(v + 0.0);
     return v != v ? kNever + 1 : (b < 0 ? b ^ 0x7fffffffffffffffll : b);
 }
 
-// Loads lane l's elements of a row; past the experts `none`.
-template <int L, int V>
-__device__ __forceinline__ void load_row(const float* row, int E, int l, float* v, float none) {
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-        const int c = 4 * (i * L + l);
-        if (c + 3 < E) {
-            const vf4 q = *reinterpret_cast<const vf4u*>(row + c);
-            v[4 * i] = q.x;
-            v[4 * i + 1] = q.y;
-            v[4 * i + 2] = q.z;
-            v[4 * i + 3] = q.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * i + j] = c + j < E ? row[c + j] : none;
-        }
-    }
+// Whether the group of score c at index j comes before that of d at o: the larger, ties to the lower index, a NaN last.
+template <typename T>
+__device__ __forceinline__ bool before(T c, int j, T d, int o) {
+    return c > d || (d != d && c == c) || (j < o && (c == d || (c != c && d != d)));
 }
 
-// The k largest of a row's biased scores b, by rounds of a maximum: exact for any b. pick_id and pick_s get the
-// experts and their scores s, largest b first.
-template <int L, int V>
-__device__ __forceinline__ void choose_rounds(const double* b, const float* s, const bool* open, int k, int l, int32_t* pick_id,
-                                              float* pick_s) {
-    int64_t key[V];
+// The choice of one row in 64 bits, by a wavefront: element 64 i + lane in the lane's i-th place. `row` holds C * 64
+// doubles, `score` one a group. The experts go to `ids`, best first.
+template <int C>
+__device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, double* row, double* score, int32_t* ids) {
+    const int lane = threadIdx.x & 63;
+    double b[C];
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = open[i] ? sort_key(b[i]) : kNever;
-    for (int t = 0; t < k; ++t) {
+    for (int i = 0; i < C; ++i) {
+        const int e = 64 * i + lane;
+        const float v = e < a.experts ? x[e] : -__builtin_inff();
+        top = __builtin_fmaxf(top, v);
+        b[i] = (double)v;
+    }
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) b[i] = sigmoid64((float)b[i]);
+    } else {
+        top = group_max<64>(top);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            b[i] = exp64(b[i] - (double)top);
+            sum += b[i];
+        }
+        sum = group_sum64<64>(sum);
+#pragma unroll
+        for (int i = 0; i < C; ++i) b[i] = b[i] / sum;
+    }
+    int64_t key[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int e = 64 * i + lane;
+        if (a.bias && e < a.experts) b[i] += (double)a.bias[e];
+        key[i] = e < a.experts ? sort_key64(b[i]) : kNever;
+    }
+    if (a.groups > 1) {
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < C; ++i) row[64 * i + lane] = b[i];
+        wave_sync();
+        if (lane < a.groups) {
+            const double* v = row + lane * a.each;
+            double first = v[0], second = __builtin_nan("");
+            for (int e = 1; e < a.each; ++e) {
+                const double c = v[e];
+                if (before(c, 1, first, 0)) {
+                    second = first;
+                    first = c;
+                } else if (before(c, 1, second, 0)) {
+                    second = c;
+                }
+            }
+            score[lane] = a.best == 2 && a.each > 1 ? first + second : first;
+        }
+        wave_sync();
+        bool open = false;
+        if (lane < a.groups) {
+            int n = 0;
+            for (int o = 0; o < a.groups; ++o) n += before(score[o], o, score[lane], lane);
+            open = n < a.open;
+        }
+        const uint64_t mask = __ballot(open);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (!(mask >> (fdiv((uint32_t)(64 * i + lane), a.by_each) & 63) & 1)) key[i] = kNever;
+    }
+    for (int t = 0; t < a.k; ++t) {
         int64_t best = key[0];
 #pragma unroll
-        for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
-        best = group_red<L>(best, [](int64_t p, int64_t q) { return p > q ? p : q; });
-        int at = 0x7fffffff;  // the lowest index that holds it
+        for (int i = 1; i < C; ++i) best = best > key[i] ? best : key[i];
+        best = group_red64<64>(best, [](int64_t p, int64_t q) { return p > q ? p : q; });
+        int at = 0;  // the lowest index that holds it
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? 4 * (i / 4) * L + (i & 3) + 4 * l : at;
-        at = group_red<L>(at, [](int p, int q) { return p < q ? p : q; });
+        for (int i = C - 1; i >= 0; --i) {
+            const uint64_t has = __ballot(key[i] == best);
+            at = has ? 64 * i + __builtin_ctzll(has) : at;
+        }
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (at == 4 * (i / 4) * L + (i & 3) + 4 * l) {
-                key[i] = kNever;
-                pick_id[t] = at;
-                pick_s[t] = s[i];
-            }
+        for (int i = 0; i < C; ++i)
+            if (at == 64 * i + lane) key[i] = kNever;
+        if (lane == 0) ids[t] = at;
     }
 }
 
 template <int L, int V>
 __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
     constexpr int G = kRThreads / L;  // rows in flight in a workgroup
-    constexpr int K = L * V < kMaxChosen ? L * V : kMaxChosen;
-    constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
+    constexpr int C = L * V < 64 ? 1 : L * V / 64;
     __shared__ int32_t cnt[L * V];
-    __shared__ float pick_s[G][K];
-    __shared__ int32_t pick_id[G][K];
-    __shared__ double row[G][L * V], of_group[G][N];
+    constexpr int K = L * V < kMaxChosen ? (L * V < kList ? kList : L * V) : kMaxChosen;
+    constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
+    __shared__ int32_t pick[G][K];
+    __shared__ __attribute__((aligned(16))) float row[G][L * V];
+    __shared__ float of_group[G][N];
+    __shared__ double wide[kRThreads / 64][C * 64 + kMaxGroups];
     const int tid = threadIdx.x, l = tid % L, g = tid / L;
+    const bool list = a.k <= kList;
     for (int e = tid; e < L * V; e += kRThreads) cnt[e] = 0;
     __syncthreads();
-    float bias[V];
-    int gid[V];
+    float bias[V], most = 0.0f;
     if (a.bias) {
-        load_row<L, V>(a.bias, a.experts, l, bias, 0.0f);
+        load_row<L, V>(a.bias, a.experts, l, bias);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float m = __builtin_fabsf(bias[i]);
+            most = m < __builtin_inff() ? __builtin_fmaxf(most, m) : most;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) bias[i] = 0.0f;
     }
+    most = group_max<L>(most);
+    uint32_t gid[V / 4];  // the elements' groups, a byte each
 #pragma unroll
-    for (int i = 0; i < V; ++i) gid[i] = (int)fdiv((uint32_t)(4 * ((i / 4) * L + l) + (i & 3)), a.by_each);
+    for (int i = 0; i < V / 4; ++i) {
+        gid[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) gid[i] |= (fdiv((uint32_t)(4 * (i * L + l) + j), a.by_each) & 63) << (8 * j);
+    }
     const int64_t stride = (int64_t)gridDim.x * G;
     // every wavefront walks whole rounds, so that its lanes reduce together
     for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += stride) {
         const int64_t r = r0 + g;
         const bool in = r < a.rows;
         const bool keep = in && (!a.keep || a.keep[r] != 0);
-        float x[V], s[V];
-        double b[V];
-        load_row<L, V>(a.x + (in ? r : r0) * a.experts, a.experts, l, x, -__builtin_inff());
-        if (a.sigmoid) {
+        const float* x = a.x + (in ? r : r0) * a.experts;
+        double sum = 0.0;
+        float top = 0.0f;
+        bool unsure = !list;
+        if (list || !a.sigmoid) {
+            float b[V];
+            load_row<L, V>(x, a.experts, l, b);
+            // scores to within 2^-22 (of the largest, where softmax)
+            float unit = 1.0f;
+            if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) b[i] = sigmoid64(x[i]);
-        } else {
-            float m = x[0];
+                for (int i = 0; i < V; ++i) b[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(b[i] * -kLog2e));
+            } else {
+                top = b[0];
 #pragma unroll
-            for (int i = 1; i < V; ++i) m = __builtin_fmaxf(m, x[i]);
-            m = group_max<L>(m);
-            double sum = 0.0;
+                for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, b[i]);
+                top = group_max<L>(top);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                b[i] = exp64((double)x[i] - (double)m);
-                sum += b[i];
+                for (int i = 0; i < V; ++i) {
+                    const double e = exp64((double)b[i] - (double)top);
+                    sum += e;
+                    b[i] = (float)e;
+                }
+                sum = group_sum64<L>(sum);
+                unit = (float)(1.0 / sum);
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[i] *= unit;
             }
-            sum = group_sum<L>(sum);
+            if (list) {
+                bool nan = false;
 #pragma unroll
-            for (int i = 0; i < V; ++i) b[i] = b[i] / sum;
-        }
-        bool open[V];
+                for (int i = 0; i < V; ++i) {
+                    const bool there = 4 * ((i / 4) * L + l) + (i & 3) < a.experts;
+                    b[i] = there ? b[i] + bias[i] : -__builtin_inff();
+                    nan |= b[i] != b[i];
+                }
+                // twice what two of them are off by together
+                const float tell = unit * 0x1p-20f + most * 0x1p-22f;
+                uint64_t mask = ~(uint64_t)0;
+                if (a.groups > 1) {
+                    wave_sync();
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            s[i] = (float)b[i];
-            b[i] += (double)bias[i];
-            open[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts;
-        }
-        if (a.groups > 1) {
-            wave_sync();
-#pragma unroll
-            for (int i = 0; i < V; ++i) row[g][4 * ((i / 4) * L + l) + (i & 3)] = b[i];
-            wave_sync();
-            for (int j = l; j < a.groups; j += L) {
-                const double* v = row[g] + j * a.each;
-                double first = v[0], second = 0.0;
-                bool two = false;
-                for (int e = 1; e < a.each; ++e) {
-                    const double c = v[e];
-                    if (c > first || first != first) {  // a NaN gives way to a number
-                        second = first;
-                        first = c;
-                    } else if (!two || c > second || second != second) {
-                        second = c;
+                    for (int i = 0; i < V / 4; ++i)
+                        *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = vf4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
+                    wave_sync();
+                    for (int j = l; j < a.groups; j += L) {
+                        const float* v = row[g] + j * a.each;
+                        float first = v[0], second = -__builtin_inff();
+#pragma unroll 4
+                        for (int e = 1; e < a.each; ++e) {
+                            second = __builtin_amdgcn_fmed3f(first, second, v[e]);
+                            first = __builtin_fmaxf(first, v[e]);
+                        }
+                        of_group[g][j] = a.best == 2 && a.each > 1 ? first + second : first;
                     }
-                    two = true;
+                    wave_sync();
+                    int lo = 0, hi = 0;  // halves of the open groups' bits
+                    float least = __builtin_inff(), best = -__builtin_inff();
+                    for (int j = l; j < a.groups; j += L) {
+                        const float c = of_group[g][j];
+                        int n = 0;
+                        for (int o = 0; o < a.groups; ++o) n += before(of_group[g][o], o, c, j);
+                        const bool open = n < a.open;
+                        least = open ? __builtin_fminf(least, c) : least;
+                        best = open ? best : __builtin_fmaxf(best, c);
+                        if (open) (j < 32 ? lo : hi) |= 1 << (j & 31);
+                    }
+                    lo = group_red<L>(lo, [](int p, int q) { return p | q; });
+                    hi = group_red<L>(hi, [](int p, int q) { return p | q; });
+                    mask = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+                    unsure |= !(group_min<L>(least) - group_max<L>(best) > 2.0f * tell);
                 }
-                of_group[g][j] = a.best == 2 && two ? first + second : first;
-            }
-            wave_sync();
-            uint64_t mask = 0;
-            for (int j = l; j < a.groups; j += L) {
-                const double c = of_group[g][j];
-                const bool none = c != c;
-                int before = 0;
-                for (int o = 0; o < a.groups; ++o) {
-                    const double d = of_group[g][o];
-                    before += d > c || (none && d == d) || (o < j && (d == c || (none && d != d)));
-                }
-                if (before < a.open) mask |= (uint64_t)1 << j;
-            }
-            mask = (uint64_t)group_red<L>((int64_t)mask, [](int64_t p, int64_t q) { return p | q; });
+                double d[V < 8 ? 8 : V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) open[i] = open[i] && ((mask >> (gid[i] & 63)) & 1) != 0;
+                for (int i = 0; i < (V < 8 ? 8 : V); ++i) {
+                    const int e = 4 * ((i / 4) * L + l) + (i & 3);
+                    const bool open = i < V && e < a.experts && (mask >> (gid[i < V ? i / 4 : 0] >> (8 * (i & 3)) & 255) & 1) != 0;
+                    if (i < V && !open) b[i < V ? i : 0] = -__builtin_inff();
+                    d[i] = open ? list_key(sort_key(b[i < V ? i : 0]), e) : 1.0;
+                }
+                list_rows<L, V>(d);
+                // those chosen have to differ by more than what they are off by, and the last of them from the rest
+                float last = 0.0f, gap = __builtin_inff(), was = __builtin_inff();
+#pragma unroll
+                for (int t = 0; t < kList; ++t) {
+                    const float v = key_value(list_value(d[t]));
+                    if (t < a.k) {
+                        if (t > 0) gap = __builtin_fminf(gap, was - v);
+                        last = was = v;
+                        if (l == 0) pick[g][t] = list_index(d[t]);
+                    }
+                }
+                int near = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) near += b[i] >= last - tell;
+                near = group_red<L>(near, [](int p, int q) { return p + q; });
+                nan = group_red<L>((int)nan, [](int p, int q) { return p | q; }) != 0;
+                unsure |= nan || !(gap > tell) || near != a.k || !(last > -__builtin_inff());
+            }
         }
         wave_sync();
-        choose_rounds<L, V>(b, s, open, a.k, l, pick_id[g], pick_s[g]);
-        wave_sync();
-        float total = 1.0f;
-        if (a.normalise) {
-            total = 0.0f;
-            for (int t = l; t < a.k; t += L) total += pick_s[g][t];
-            total = group_sum<L>(total);
+        // rows that fp32 does not decide
+        for (uint64_t todo = __ballot(unsure && in && l == 0); todo; todo &= todo - 1) {
+            const int at = (tid & ~63) + __builtin_ctzll(todo), gr = at / L;
+            choose_exact<C>(a, a.x + (r0 + gr) * a.experts, wide[tid / 64], wide[tid / 64] + C * 64, pick[gr]);
         }
+        wave_sync();
+        // weights from 64-bit scores
+        float total = 0.0f;
+        for (int t = l; in && t < a.k; t += L) {  // a row past the last has no choice
+            const float v = x[pick[g][t]];
+            const float s = a.sigmoid ? (float)sigmoid64(v) : (float)(exp64((double)v - (double)top) / sum);
+            total += s;
+        }
+        total = a.normalise ? group_sum<L>(total) : 1.0f;
         if (in)
             for (int t = l; t < a.k; t += L) {
-                const int32_t id = pick_id[g][t];
+                const int32_t id = pick[g][t];
+                const float v = x[id];
+                const float s = a.sigmoid ? (float)sigmoid64(v) : (float)(exp64((double)v - (double)top) / sum);
                 a.chosen[r * a.k + t] = keep ? id : -1;
-                a.weights[r * a.k + t] = keep ? a.scale * (pick_s[g][t] / total) : 0.0f;
+                a.weights[r * a.k + t] = keep ? a.scale * (s / total) : 0.0f;
                 if (keep) atomicAdd(&cnt[id], 1);
             }
+        wave_sync();
     }
     __syncthreads();
     for (int e = tid; e < a.experts; e += kRThreads) a.part_c[(int64_t)blockIdx.x * a.experts + e] = cnt[e];
@@ -284,7 +369,7 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_bwd(GroupArg a) {
         const int64_t at = (in ? r : r0) * a.experts;
         float v[V], inv = 0.0f, top = 0.0f;
         if (whole) {
-            load_row<L, V>(a.x + at, a.experts, l, v, -__builtin_inff());
+            load_row<L, V>(a.x + at, a.experts, l, v);
             top = v[0];
 #pragma unroll
             for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, v[i]);
@@ -388,14 +473,14 @@ __global__ __launch_bounds__(kRThreads) void k_router_bias(float* bias, const in
         else if (a.experts <= 16) CALL(4, 4);   \
         else if (a.experts <= 32) CALL(4, 8);   \
         else if (a.experts <= 64) CALL(8, 8);   \
-        else if (a.experts <= 128) CALL(16, 8); \
-        else if (a.experts <= 256) CALL(32, 8); \
-        else if (a.experts <= 512) CALL(64, 8); \
+        else if (a.experts <= 128) CALL(8, 16); \
+        else if (a.experts <= 256) CALL(16, 16); \
+        else if (a.experts <= 512) CALL(32, 16); \
         else CALL(64, 16);                   \
     } while (0)
 
 int router_lanes(int experts) {
-    return experts <= 8 ? 2 : experts <= 32 ? 4 : experts <= 64 ? 8 : experts <= 128 ? 16 : experts <= 256 ? 32 : 64;
+    return experts <= 8 ? 2 : experts <= 32 ? 4 : experts <= 128 ? 8 : experts <= 256 ? 16 : experts <= 512 ? 32 : 64;
 }
 
 int router_check(const char* what, int64_t rows, int64_t experts, int64_t k, int scores, float scale) {
