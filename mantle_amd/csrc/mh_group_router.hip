@@ -9,9 +9,10 @@
 //
 // Scores decide a choice after a bias was added to them, so logits do not: experts whose biased scores agree to fp32 are
 // not rare over a long batch, and which of them is chosen shows. What is compared is therefore meant in 64 bits. Up to 8
-// choices are made in fp32 first, by sorted lists of the row, with a bound on its error: a row whose choice, or whose choice
-// of groups, turns on less than twice that (one in a few hundred) is chosen again in 64 bits by a whole wavefront, and so
-// is every row of more than 8. Weights are 64-bit scores rounded to fp32, whichever way the choice went; gradients fp32.
+// choices are made in fp32 first, by sorted lists of the row, with a bound on its error; a row whose choice, or whose choice
+// of groups, turns on less than twice that (one in a few hundred) is listed, and a second kernel chooses for it in 64 bits, a
+// wavefront a row. That kernel alone takes short batches, whose rows it holds all at once, and more than 8 choices. Weights are
+// 64-bit scores rounded to fp32, by one formula in both; gradients are fp32.
 //
 // Bound by the logits' read and the gradient's write, and over many experts by the sorting. L lanes hold a row in
 // registers, V elements a lane in quads (element 4 (i L + lane) + c).
@@ -25,6 +26,7 @@ namespace {
 constexpr int kMaxGroups = 64;
 constexpr int kRThreads = 256;
 constexpr int kRBlocks = 1024;  // workgroups of a forward at most: rows of its partial counts
+constexpr int64_t kRExactRows = 2048;  // batches of up to this many rows go by wavefronts alone
 
 struct GroupArg {
     const float* x;
@@ -40,6 +42,8 @@ struct GroupArg {
     float* weights;
     int32_t* chosen;
     int32_t* part_c;  // [blocks][experts]
+    int64_t* todo;    // rows listed for the second kernel, or null: every row
+    uint32_t* ntodo;
     // backward
     float* grad;
     const float* gw;
@@ -67,6 +71,32 @@ __device__ __forceinline__ double sigmoid64(float x) {
     return (x < 0.0f ? e : 1.0) / (1.0 + e);
 }
 
+// e^x for x <= 0 to 2^-31 of itself: what a score that is rounded to fp32 needs of 64 bits.
+__device__ __forceinline__ double exp_short(double x) {
+    x = x < -1000.0 ? -1000.0 : x;
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    const double r = __builtin_fma(n, -0.69314718055994530942, x);
+    double p = 1.0 / 40320.0;
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+// 1 / x of a positive normal x, to 2^-48 or so: a step of Newton's on the unit's own.
+__device__ __forceinline__ double inverse(double x) {
+    const double y = __builtin_amdgcn_rcp(x);
+    return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
+// A weight's score; `top` and `by` are a softmax's largest logit and 1 / the sum of its exponentials.
+__device__ __forceinline__ float weight_score(bool sigmoid, float v, float top, double by) {
+    const double e = exp_short(sigmoid ? -__builtin_fabs((double)v) : (double)v - (double)top);
+    return (float)(sigmoid ? (v < 0.0f ? e : 1.0) * inverse(1.0 + e) : e * by);
+}
 // A double as an integer of the same order; NaN below every number, -0 as +0; below them what may not be chosen.
 constexpr int64_t kNever = INT64_MIN;
 __device__ __forceinline__ int64_t sort_key64(double v) {
@@ -83,10 +113,12 @@ __device__ __forceinline__ bool before(T c, int j, T d, int o) {
 // The choice of one row in 64 bits, by a wavefront: element 64 i + lane in the lane's i-th place. `row` holds C * 64
 // doubles, `score` one a group. The experts go to `ids`, best first.
 template <int C>
-__device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, double* row, double* score, int32_t* ids) {
+__device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, double* row, double* score, int32_t* ids, float& top,
+                                             double& by) {
     const int lane = threadIdx.x & 63;
     double b[C];
-    float top = -__builtin_inff();
+    top = -__builtin_inff();
+    by = 0.0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const int e = 64 * i + lane;
@@ -99,13 +131,15 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
         for (int i = 0; i < C; ++i) b[i] = sigmoid64((float)b[i]);
     } else {
         top = group_max<64>(top);
-        double sum = 0.0;
+        double sum = 0.0, rough = 0.0;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
+            rough += exp_short(b[i] - (double)top);
             b[i] = exp64(b[i] - (double)top);
             sum += b[i];
         }
         sum = group_sum64<64>(sum);
+        by = inverse(group_sum64<64>(rough));
 #pragma unroll
         for (int i = 0; i < C; ++i) b[i] = b[i] / sum;
     }
@@ -165,19 +199,34 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
     }
 }
 
-template <int L, int V>
+// A chosen row's results by L lanes, of which this is number l: its choices lie in `pick`.
+template <int L>
+__device__ __forceinline__ void put_choice(const GroupArg& a, const int32_t* pick, const float* x, int64_t r, int l, bool in, bool keep,
+                                           float top, double by, int32_t* cnt) {
+    float total = 0.0f, s = 0.0f;
+    for (int t = l; in && t < a.k; t += L) {
+        s = weight_score(a.sigmoid != 0, x[pick[t]], top, by);
+        total += s;
+    }
+    total = a.normalise ? group_sum<L>(total) : 1.0f;
+    for (int t = l; in && t < a.k; t += L) {
+        const int32_t id = pick[t];
+        if (a.k > L) s = weight_score(a.sigmoid != 0, x[id], top, by);
+        a.chosen[r * a.k + t] = keep ? id : -1;
+        a.weights[r * a.k + t] = keep ? a.scale * (s / total) : 0.0f;
+        if (keep) atomicAdd(&cnt[id], 1);
+    }
+}
+
+template <int L, int V, bool SIGMOID>
 __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
     constexpr int G = kRThreads / L;  // rows in flight in a workgroup
-    constexpr int C = L * V < 64 ? 1 : L * V / 64;
-    __shared__ int32_t cnt[L * V];
-    constexpr int K = L * V < kMaxChosen ? (L * V < kList ? kList : L * V) : kMaxChosen;
     constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
-    __shared__ int32_t pick[G][K];
+    __shared__ int32_t cnt[L * V];
+    __shared__ int32_t pick[G][kList];
     __shared__ __attribute__((aligned(16))) float row[G][L * V];
     __shared__ float of_group[G][N];
-    __shared__ double wide[kRThreads / 64][C * 64 + kMaxGroups];
     const int tid = threadIdx.x, l = tid % L, g = tid / L;
-    const bool list = a.k <= kList;
     for (int e = tid; e < L * V; e += kRThreads) cnt[e] = 0;
     __syncthreads();
     float bias[V], most = 0.0f;
@@ -190,7 +239,7 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) bias[i] = 0.0f;
+        for (int i = 0; i < V; ++i) bias[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts ? 0.0f : -__builtin_inff();
     }
     most = group_max<L>(most);
     uint32_t gid[V / 4];  // the elements' groups, a byte each
@@ -207,150 +256,153 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         const bool in = r < a.rows;
         const bool keep = in && (!a.keep || a.keep[r] != 0);
         const float* x = a.x + (in ? r : r0) * a.experts;
-        double sum = 0.0;
-        float top = 0.0f;
-        bool unsure = !list;
-        if (list || !a.sigmoid) {
-            float b[V];
-            load_row<L, V>(x, a.experts, l, b);
-            // scores to within 2^-22 (of the largest, where softmax)
-            float unit = 1.0f;
-            if (a.sigmoid) {
+        float b[V];
+        load_row<L, V>(x, a.experts, l, b);
+        // scores to within 2^-22 (of the largest, where softmax); past the experts the bias is minus infinity
+        float unit = 1.0f, top = 0.0f;
+        double by = 0.0;
+        if (SIGMOID) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) b[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(b[i] * -kLog2e));
-            } else {
-                top = b[0];
+            for (int i = 0; i < V; ++i) b[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(b[i] * -kLog2e));
+        } else {
+            top = b[0];
 #pragma unroll
-                for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, b[i]);
-                top = group_max<L>(top);
+            for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, b[i]);
+            top = group_max<L>(top);
+            double sum = 0.0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const double e = exp64((double)b[i] - (double)top);
-                    sum += e;
-                    b[i] = (float)e;
-                }
-                sum = group_sum64<L>(sum);
-                unit = (float)(1.0 / sum);
-#pragma unroll
-                for (int i = 0; i < V; ++i) b[i] *= unit;
+            for (int i = 0; i < V; ++i) {
+                const double e = exp_short((double)b[i] - (double)top);
+                sum += e;
+                b[i] = (float)e;
             }
-            if (list) {
-                bool nan = false;
+            by = inverse(group_sum64<L>(sum));
+            unit = (float)by;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const bool there = 4 * ((i / 4) * L + l) + (i & 3) < a.experts;
-                    b[i] = there ? b[i] + bias[i] : -__builtin_inff();
-                    nan |= b[i] != b[i];
-                }
-                // twice what two of them are off by together
-                const float tell = unit * 0x1p-20f + most * 0x1p-22f;
-                uint64_t mask = ~(uint64_t)0;
-                if (a.groups > 1) {
-                    wave_sync();
+            for (int i = 0; i < V; ++i) b[i] *= unit;
+        }
+        bool unsure = false;
 #pragma unroll
-                    for (int i = 0; i < V / 4; ++i)
-                        *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = vf4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
-                    wave_sync();
-                    for (int j = l; j < a.groups; j += L) {
-                        const float* v = row[g] + j * a.each;
-                        float first = v[0], second = -__builtin_inff();
+        for (int i = 0; i < V; ++i) {
+            b[i] += bias[i];
+            unsure |= b[i] != b[i];
+        }
+        // twice what two of them are off by together
+        const float tell = unit * 0x1p-20f + most * 0x1p-22f;
+        if (a.groups > 1) {
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i)
+                *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = vf4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
+            wave_sync();
+            for (int j = l; j < a.groups; j += L) {
+                const float* v = row[g] + j * a.each;
+                float first = v[0], second = -__builtin_inff();
 #pragma unroll 4
-                        for (int e = 1; e < a.each; ++e) {
-                            second = __builtin_amdgcn_fmed3f(first, second, v[e]);
-                            first = __builtin_fmaxf(first, v[e]);
-                        }
-                        of_group[g][j] = a.best == 2 && a.each > 1 ? first + second : first;
-                    }
-                    wave_sync();
-                    int lo = 0, hi = 0;  // halves of the open groups' bits
-                    float least = __builtin_inff(), best = -__builtin_inff();
-                    for (int j = l; j < a.groups; j += L) {
-                        const float c = of_group[g][j];
-                        int n = 0;
-                        for (int o = 0; o < a.groups; ++o) n += before(of_group[g][o], o, c, j);
-                        const bool open = n < a.open;
-                        least = open ? __builtin_fminf(least, c) : least;
-                        best = open ? best : __builtin_fmaxf(best, c);
-                        if (open) (j < 32 ? lo : hi) |= 1 << (j & 31);
-                    }
-                    lo = group_red<L>(lo, [](int p, int q) { return p | q; });
-                    hi = group_red<L>(hi, [](int p, int q) { return p | q; });
-                    mask = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
-                    unsure |= !(group_min<L>(least) - group_max<L>(best) > 2.0f * tell);
+                for (int e = 1; e < a.each; ++e) {
+                    second = __builtin_amdgcn_fmed3f(first, second, v[e]);
+                    first = __builtin_fmaxf(first, v[e]);
                 }
-                double d[V < 8 ? 8 : V];
+                of_group[g][j] = a.best == 2 && a.each > 1 ? first + second : first;
+            }
+            wave_sync();
+            int lo = 0, hi = 0;  // halves of the open groups' bits
+            float least = __builtin_inff(), best = -__builtin_inff();
+            for (int j = l; j < a.groups; j += L) {
+                const float c = of_group[g][j];
+                int n = 0;
+                for (int o = 0; o < a.groups; ++o) n += before(of_group[g][o], o, c, j);
+                const bool open = n < a.open;
+                least = open ? __builtin_fminf(least, c) : least;
+                best = open ? best : __builtin_fmaxf(best, c);
+                if (open) (j < 32 ? lo : hi) |= 1 << (j & 31);
+            }
+            lo = group_red<L>(lo, [](int p, int q) { return p | q; });
+            hi = group_red<L>(hi, [](int p, int q) { return p | q; });
+            const uint64_t mask = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+            unsure |= !(group_min<L>(least) - group_max<L>(best) > 2.0f * tell);
 #pragma unroll
-                for (int i = 0; i < (V < 8 ? 8 : V); ++i) {
-                    const int e = 4 * ((i / 4) * L + l) + (i & 3);
-                    const bool open = i < V && e < a.experts && (mask >> (gid[i < V ? i / 4 : 0] >> (8 * (i & 3)) & 255) & 1) != 0;
-                    if (i < V && !open) b[i < V ? i : 0] = -__builtin_inff();
-                    d[i] = open ? list_key(sort_key(b[i < V ? i : 0]), e) : 1.0;
-                }
-                list_rows<L, V>(d);
-                // those chosen have to differ by more than what they are off by, and the last of them from the rest
-                float last = 0.0f, gap = __builtin_inff(), was = __builtin_inff();
+            for (int i = 0; i < V; ++i)
+                b[i] = (mask >> (gid[i / 4] >> (8 * (i & 3)) & 255) & 1) != 0 ? b[i] : -__builtin_inff();
+        }
+        double d[V < 8 ? 8 : V];
 #pragma unroll
-                for (int t = 0; t < kList; ++t) {
-                    const float v = key_value(list_value(d[t]));
-                    if (t < a.k) {
-                        if (t > 0) gap = __builtin_fminf(gap, was - v);
-                        last = was = v;
-                        if (l == 0) pick[g][t] = list_index(d[t]);
-                    }
-                }
-                int near = 0;
+        for (int i = 0; i < (V < 8 ? 8 : V); ++i) d[i] = i < V ? list_key(sort_key(b[i < V ? i : 0]), 4 * ((i / 4) * L + l) + (i & 3)) : 1.0;
+        list_rows<L, V>(d);
+        // those chosen have to differ by more than what they are off by, and the last of them from the rest; what is closed or
+        // past the experts is minus infinity, which none of them may be
+        float last = 0.0f, gap = __builtin_inff(), was = __builtin_inff();
 #pragma unroll
-                for (int i = 0; i < V; ++i) near += b[i] >= last - tell;
-                near = group_red<L>(near, [](int p, int q) { return p + q; });
-                nan = group_red<L>((int)nan, [](int p, int q) { return p | q; }) != 0;
-                unsure |= nan || !(gap > tell) || near != a.k || !(last > -__builtin_inff());
+        for (int t = 0; t < kList; ++t) {
+            const float v = key_value(list_value(d[t]));
+            if (t < a.k) {
+                if (t > 0) gap = __builtin_fminf(gap, was - v);
+                last = was = v;
+            }
+        }
+        int near = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) near += b[i] >= last - tell;
+        near = group_red<L>(near, [](int p, int q) { return p + q; });
+        unsure = group_red<L>((int)unsure, [](int p, int q) { return p | q; }) != 0;
+        unsure |= !(gap > tell) || near != a.k || !(last > -__builtin_inff());
+        wave_sync();
+        if (l == 0) {
+#pragma unroll
+            for (int t = 0; t < kList; ++t) pick[g][t] = list_index(d[t]);
+            if (unsure && in) {
+                const uint32_t at = atomicAdd(a.ntodo, 1u);
+                if (at < (uint64_t)a.rows) a.todo[at] = r;
             }
         }
         wave_sync();
-        // rows that fp32 does not decide
-        for (uint64_t todo = __ballot(unsure && in && l == 0); todo; todo &= todo - 1) {
-            const int at = (tid & ~63) + __builtin_ctzll(todo), gr = at / L;
-            choose_exact<C>(a, a.x + (r0 + gr) * a.experts, wide[tid / 64], wide[tid / 64] + C * 64, pick[gr]);
-        }
-        wave_sync();
-        // weights from 64-bit scores
-        float total = 0.0f;
-        for (int t = l; in && t < a.k; t += L) {  // a row past the last has no choice
-            const float v = x[pick[g][t]];
-            const float s = a.sigmoid ? (float)sigmoid64(v) : (float)(exp64((double)v - (double)top) / sum);
-            total += s;
-        }
-        total = a.normalise ? group_sum<L>(total) : 1.0f;
-        if (in)
-            for (int t = l; t < a.k; t += L) {
-                const int32_t id = pick[g][t];
-                const float v = x[id];
-                const float s = a.sigmoid ? (float)sigmoid64(v) : (float)(exp64((double)v - (double)top) / sum);
-                a.chosen[r * a.k + t] = keep ? id : -1;
-                a.weights[r * a.k + t] = keep ? a.scale * (s / total) : 0.0f;
-                if (keep) atomicAdd(&cnt[id], 1);
-            }
-        wave_sync();
+        put_choice<L>(a, pick[g], x, r, l, in && !unsure, keep, top, by, cnt);
     }
     __syncthreads();
     for (int e = tid; e < a.experts; e += kRThreads) a.part_c[(int64_t)blockIdx.x * a.experts + e] = cnt[e];
 }
 
-// The counts from the workgroups' partials: 32 experts and 8 shares of the partials a workgroup.
-__global__ __launch_bounds__(kRThreads) void k_group_router_counts(const int32_t* part, int32_t blocks, int32_t experts,
-                                                                   int32_t* counts) {
-    __shared__ int32_t buf[kRThreads];
+// Rows in 64 bits, a wavefront each: all of them, or those listed.
+template <int C>
+__global__ __launch_bounds__(kRThreads) void k_group_router_exact(GroupArg a) {
+    __shared__ int32_t cnt[C * 64];
+    __shared__ int32_t pick[kRThreads / 64][kMaxChosen];
+    __shared__ double wide[kRThreads / 64][C * 64 + kMaxGroups];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    for (int e = tid; e < C * 64; e += kRThreads) cnt[e] = 0;
+    __syncthreads();
+    const int64_t listed = a.todo ? (int64_t)a.ntodo[0] : a.rows, rows = listed < a.rows ? listed : a.rows;
+    for (int64_t i = (int64_t)blockIdx.x * (kRThreads / 64) + wave; i < rows; i += (int64_t)gridDim.x * (kRThreads / 64)) {
+        const int64_t r = a.todo ? a.todo[i] : i;
+        const float* x = a.x + r * a.experts;
+        float top;
+        double by;
+        wave_sync();
+        choose_exact<C>(a, x, wide[wave], wide[wave] + C * 64, pick[wave], top, by);
+        wave_sync();
+        put_choice<64>(a, pick[wave], x, r, tid & 63, true, !a.keep || a.keep[r] != 0, top, by, cnt);
+    }
+    __syncthreads();
+    for (int e = tid; e < a.experts; e += kRThreads) a.part_c[(int64_t)blockIdx.x * a.experts + e] = cnt[e];
+}
+
+// The counts from the workgroups' partials: 32 experts and 32 shares of the partials a workgroup. The list of rows is
+// done with.
+__global__ __launch_bounds__(1024) void k_group_router_counts(const int32_t* part, int32_t blocks, int32_t experts, int32_t* counts,
+                                                              uint32_t* ntodo) {
+    __shared__ int32_t buf[1024];
     const int e = blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
     int32_t s = 0;
     if (e < experts) {
 #pragma unroll 8
-        for (int b = share; b < blocks; b += 8) s += part[(int64_t)b * experts + e];
+        for (int b = share; b < blocks; b += 32) s += part[(int64_t)b * experts + e];
     }
+    if (ntodo && blockIdx.x == 0 && threadIdx.x == 0) ntodo[0] = 0;
     buf[threadIdx.x] = s;
     __syncthreads();
     if (share != 0 || e >= experts) return;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += buf[32 * i + (threadIdx.x & 31)];
+    for (int i = 1; i < 32; ++i) s += buf[32 * i + (threadIdx.x & 31)];
     counts[e] = s;
 }
 
@@ -533,16 +585,35 @@ int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const 
     a.scale = scale;
     a.weights = weights;
     a.chosen = chosen;
-    const int64_t group = kRThreads / router_lanes(a.experts);
-    int64_t blocks = (rows + group - 1) / group;
-    if (blocks > kRBlocks) blocks = kRBlocks;
-    MH_TRY(scratch((size_t)blocks * experts * 4, reinterpret_cast<void**>(&a.part_c)));
     hipStream_t st = ctx().stream;
-#define MH_CALL(L, V) hipLaunchKernelGGL((k_group_router_fwd<L, V>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a)
-    MH_ROUTER(MH_CALL);
+    const int64_t waves = kRThreads / 64, group = kRThreads / router_lanes(a.experts);
+    const bool lists = a.k <= kList && rows > kRExactRows;
+    int64_t blocks = lists ? (rows + group - 1) / group : 0;
+    if (blocks > kRBlocks) blocks = kRBlocks;
+    int64_t exact = lists ? 128 : (rows + waves - 1) / waves;
+    if (exact > 2 * kRBlocks) exact = 2 * kRBlocks;
+    char* base = nullptr;
+    const size_t list_bytes = lists ? (size_t)rows * 8 : 0, part_bytes = (size_t)(blocks + exact) * experts * 4;
+    MH_TRY(scratch(list_bytes + part_bytes, reinterpret_cast<void**>(&base)));
+    int32_t* part = reinterpret_cast<int32_t*>(base + list_bytes);
+    a.part_c = part;
+    if (lists) {
+        MH_TRY(tickets(1, &a.ntodo));
+        a.todo = reinterpret_cast<int64_t*>(base);
+#define MH_CALL(L, V)                                                                                                             \
+    do {                                                                                                                         \
+        if (a.sigmoid) hipLaunchKernelGGL((k_group_router_fwd<L, V, true>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a);  \
+        else hipLaunchKernelGGL((k_group_router_fwd<L, V, false>), dim3((unsigned)blocks), dim3(kRThreads), 0, st, a);           \
+    } while (0)
+        MH_ROUTER(MH_CALL);
 #undef MH_CALL
-    hipLaunchKernelGGL(k_group_router_counts, dim3((unsigned)((experts + 31) / 32)), dim3(kRThreads), 0, st, a.part_c,
-                       (int32_t)blocks, a.experts, counts);
+        a.part_c += blocks * experts;
+    }
+    if (a.experts <= 64) hipLaunchKernelGGL(k_group_router_exact<1>, dim3((unsigned)exact), dim3(kRThreads), 0, st, a);
+    else if (a.experts <= 256) hipLaunchKernelGGL(k_group_router_exact<4>, dim3((unsigned)exact), dim3(kRThreads), 0, st, a);
+    else hipLaunchKernelGGL(k_group_router_exact<16>, dim3((unsigned)exact), dim3(kRThreads), 0, st, a);
+    hipLaunchKernelGGL(k_group_router_counts, dim3((unsigned)((experts + 31) / 32)), dim3(1024), 0, st, part,
+                       (int32_t)(blocks + exact), a.experts, counts, a.ntodo);
     return finish("mh_group_router_fwd");
 }
 
