@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kMaxGroups = 64;
 constexpr int kRThreads = 256;
-constexpr int kRBlocks = 1024;  // workgroups of a forward at most: rows of its partial counts
+constexpr int kRBlocks = 2048;  // workgroups of a forward at most: rows of its partial counts
 constexpr int64_t kRExactRows = 2048;  // batches of up to this many rows go by wavefronts alone
 
 struct GroupArg {
@@ -35,6 +35,7 @@ struct GroupArg {
     int64_t rows;
     int32_t experts, k;
     int32_t groups, each, open, best;  // each: experts of a group
+    int32_t parts;                     // lanes that share a group, a power of two
     int32_t sigmoid, normalise, accumulate;
     float scale;
     FastDiv by_each;
@@ -71,17 +72,21 @@ __device__ __forceinline__ double sigmoid64(float x) {
     return (x < 0.0f ? e : 1.0) / (1.0 + e);
 }
 
+// A constant in scalar registers, made where it stands: a loop's constants in vector registers cost a row's occupancy.
+__device__ __forceinline__ double scalar(double c) {
+    asm volatile("" : "+s"(c));
+    return c;
+}
 // e^x for x <= 0 to 2^-31 of itself: what a score that is rounded to fp32 needs of 64 bits.
 __device__ __forceinline__ double exp_short(double x) {
     x = x < -1000.0 ? -1000.0 : x;
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    const double r = __builtin_fma(n, -0.69314718055994530942, x);
-    double p = 1.0 / 40320.0;
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
+    const double n = __builtin_rint(x * scalar(1.4426950408889634074));
+    const double r = __builtin_fma(n, scalar(-0.69314718055994530942), x);
+    double p = __builtin_fma(scalar(1.0 / 40320.0), r, scalar(1.0 / 5040.0));
+    p = __builtin_fma(p, r, scalar(1.0 / 720.0));
+    p = __builtin_fma(p, r, scalar(1.0 / 120.0));
+    p = __builtin_fma(p, r, scalar(1.0 / 24.0));
+    p = __builtin_fma(p, r, scalar(1.0 / 6.0));
     p = __builtin_fma(p, r, 0.5);
     p = __builtin_fma(p, r, 1.0);
     p = __builtin_fma(p, r, 1.0);
@@ -108,6 +113,25 @@ __device__ __forceinline__ int64_t sort_key64(double v) {
 template <typename T>
 __device__ __forceinline__ bool before(T c, int j, T d, int o) {
     return c > d || (d != d && c == c) || (j < o && (c == d || (c != c && d != d)));
+}
+
+// The largest of a wavefront's, each lane's with the lanes' before it, then rows of 16 lanes and halves.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t larger(int64_t v) {
+    const int lo = (int)v, hi = (int)(v >> 32);
+    const int64_t w = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(hi, hi, CTRL, ROWS, 0xf, false) << 32 |
+                                (uint32_t)__builtin_amdgcn_update_dpp(lo, lo, CTRL, ROWS, 0xf, false));
+    return v > w ? v : w;
+}
+__device__ __forceinline__ int64_t wave_largest(int64_t v) {
+    v = larger<0x111, 0xf>(v);
+    v = larger<0x112, 0xf>(v);
+    v = larger<0x114, 0xf>(v);
+    v = larger<0x118, 0xf>(v);
+    v = larger<0x142, 0xa>(v);
+    v = larger<0x143, 0xc>(v);
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, 63));
 }
 
 // The choice of one row in 64 bits, by a wavefront: element 64 i + lane in the lane's i-th place. `row` holds C * 64
@@ -157,22 +181,24 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
         wave_sync();
         if (lane < a.groups) {
             const double* v = row + lane * a.each;
-            double first = v[0], second = __builtin_nan("");
-            for (int e = 1; e < a.each; ++e) {
+            double first = -__builtin_inf(), second = first;
+            int numbers = 0;  // a NaN comes behind them
+#pragma unroll 8
+            for (int e = 0; e < a.each; ++e) {
                 const double c = v[e];
-                if (before(c, 1, first, 0)) {
-                    second = first;
-                    first = c;
-                } else if (before(c, 1, second, 0)) {
-                    second = c;
-                }
+                numbers += c == c;
+                second = max_d(second, min_d(first, c == c ? c : -__builtin_inf()));
+                first = max_d(first, c == c ? c : -__builtin_inf());
             }
+            if (numbers < 2) second = __builtin_nan("");
+            if (numbers < 1) first = second;
             score[lane] = a.best == 2 && a.each > 1 ? first + second : first;
         }
         wave_sync();
         bool open = false;
         if (lane < a.groups) {
             int n = 0;
+#pragma unroll 8
             for (int o = 0; o < a.groups; ++o) n += before(score[o], o, score[lane], lane);
             open = n < a.open;
         }
@@ -185,7 +211,7 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
         int64_t best = key[0];
 #pragma unroll
         for (int i = 1; i < C; ++i) best = best > key[i] ? best : key[i];
-        best = group_red64<64>(best, [](int64_t p, int64_t q) { return p > q ? p : q; });
+        best = wave_largest(best);
         int at = 0;  // the lowest index that holds it
 #pragma unroll
         for (int i = C - 1; i >= 0; --i) {
@@ -218,28 +244,38 @@ __device__ __forceinline__ void put_choice(const GroupArg& a, const int32_t* pic
     }
 }
 
+// load_row, of rows that fill their lanes without a branch.
+template <int L, int V>
+__device__ __forceinline__ void load_next(const float* row, int E, int l, float* v) {
+    if (E == L * V) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const vf4 q = *reinterpret_cast<const vf4u*>(row + 4 * (i * L + l));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * i + j] = q[j];
+        }
+    } else {
+        load_row<L, V>(row, E, l, v);
+    }
+}
+
 template <int L, int V, bool SIGMOID>
 __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
     constexpr int G = kRThreads / L;  // rows in flight in a workgroup
     constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
     __shared__ int32_t cnt[L * V];
     __shared__ int32_t pick[G][kList];
-    __shared__ __attribute__((aligned(16))) float row[G][L * V];
+    __shared__ __attribute__((aligned(16))) float row[G][L * V], bias[L * V];
     __shared__ float of_group[G][N];
     const int tid = threadIdx.x, l = tid % L, g = tid / L;
     for (int e = tid; e < L * V; e += kRThreads) cnt[e] = 0;
+    // the bias; past the experts minus infinity
+    float most = 0.0f;
+    for (int e = tid; e < L * V; e += kRThreads) bias[e] = e < a.experts ? (a.bias ? a.bias[e] : 0.0f) : -__builtin_inff();
     __syncthreads();
-    float bias[V], most = 0.0f;
-    if (a.bias) {
-        load_row<L, V>(a.bias, a.experts, l, bias);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float m = __builtin_fabsf(bias[i]);
-            most = m < __builtin_inff() ? __builtin_fmaxf(most, m) : most;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) bias[i] = 4 * ((i / 4) * L + l) + (i & 3) < a.experts ? 0.0f : -__builtin_inff();
+    for (int e = l; e < a.experts; e += L) {
+        const float m = __builtin_fabsf(bias[e]);
+        most = m < __builtin_inff() ? __builtin_fmaxf(most, m) : most;
     }
     most = group_max<L>(most);
     uint32_t gid[V / 4];  // the elements' groups, a byte each
@@ -250,6 +286,11 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         for (int j = 0; j < 4; ++j) gid[i] |= (fdiv((uint32_t)(4 * (i * L + l) + j), a.by_each) & 63) << (8 * j);
     }
     const int64_t stride = (int64_t)gridDim.x * G;
+    float next[V];
+    {
+        const int64_t n = (int64_t)blockIdx.x * G + g;
+        load_next<L, V>(a.x + (n < a.rows ? n : 0) * a.experts, a.experts, l, next);
+    }
     // every wavefront walks whole rounds, so that its lanes reduce together
     for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.rows; r0 += stride) {
         const int64_t r = r0 + g;
@@ -257,7 +298,12 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         const bool keep = in && (!a.keep || a.keep[r] != 0);
         const float* x = a.x + (in ? r : r0) * a.experts;
         float b[V];
-        load_row<L, V>(x, a.experts, l, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = next[i];
+        {  // a round ahead
+            const int64_t n = r + stride < a.rows ? r + stride : r0;
+            load_next<L, V>(a.x + n * a.experts, a.experts, l, next);
+        }
         // scores to within 2^-22 (of the largest, where softmax); past the experts the bias is minus infinity
         float unit = 1.0f, top = 0.0f;
         double by = 0.0;
@@ -281,29 +327,52 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) b[i] *= unit;
         }
+        // with the bias, to LDS as well
         bool unsure = false;
+        wave_sync();
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            b[i] += bias[i];
-            unsure |= b[i] != b[i];
+        for (int i = 0; i < V / 4; ++i) {
+            const vf4 q = *reinterpret_cast<const vf4*>(&bias[4 * (i * L + l)]) + vf4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
+            *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = q;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                b[4 * i + j] = q[j];
+                unsure |= q[j] != q[j];
+            }
         }
+        wave_sync();
         // twice what two of them are off by together
         const float tell = unit * 0x1p-20f + most * 0x1p-22f;
+        uint64_t mask = ~(uint64_t)0;
         if (a.groups > 1) {
-            wave_sync();
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i)
-                *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = vf4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
-            wave_sync();
-            for (int j = l; j < a.groups; j += L) {
+            // a lane's share of a group, 4 experts at a time where they divide so
+            const int part = l & (a.parts - 1);
+            for (int j = l / a.parts; j < a.groups; j += L / a.parts) {
                 const float* v = row[g] + j * a.each;
-                float first = v[0], second = -__builtin_inff();
+                float first = -__builtin_inff(), second = first;
+                auto take = [&](float c) {
+                    second = __builtin_amdgcn_fmed3f(first, second, c);
+                    first = __builtin_fmaxf(first, c);
+                };
+                if ((a.each & 3) == 0) {
 #pragma unroll 4
-                for (int e = 1; e < a.each; ++e) {
-                    second = __builtin_amdgcn_fmed3f(first, second, v[e]);
-                    first = __builtin_fmaxf(first, v[e]);
+                    for (int e = 4 * part; e < a.each; e += 4 * a.parts) {
+                        const vf4 q = *reinterpret_cast<const vf4*>(v + e);
+                        take(q.x);
+                        take(q.y);
+                        take(q.z);
+                        take(q.w);
+                    }
+                } else {
+#pragma unroll 4
+                    for (int e = part; e < a.each; e += a.parts) take(v[e]);
                 }
-                of_group[g][j] = a.best == 2 && a.each > 1 ? first + second : first;
+                for (int o = 1; o < a.parts; o *= 2) {
+                    const float f = __shfl_xor(first, o), t = __shfl_xor(second, o);
+                    second = __builtin_fmaxf(__builtin_fminf(first, f), __builtin_fmaxf(second, t));
+                    first = __builtin_fmaxf(first, f);
+                }
+                if (part == 0) of_group[g][j] = a.best == 2 && a.each > 1 ? first + second : first;
             }
             wave_sync();
             int lo = 0, hi = 0;  // halves of the open groups' bits
@@ -311,6 +380,7 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
             for (int j = l; j < a.groups; j += L) {
                 const float c = of_group[g][j];
                 int n = 0;
+#pragma unroll 8
                 for (int o = 0; o < a.groups; ++o) n += before(of_group[g][o], o, c, j);
                 const bool open = n < a.open;
                 least = open ? __builtin_fminf(least, c) : least;
@@ -319,22 +389,46 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
             }
             lo = group_red<L>(lo, [](int p, int q) { return p | q; });
             hi = group_red<L>(hi, [](int p, int q) { return p | q; });
-            const uint64_t mask = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+            mask = (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
             unsure |= !(group_min<L>(least) - group_max<L>(best) > 2.0f * tell);
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                b[i] = (mask >> (gid[i / 4] >> (8 * (i & 3)) & 255) & 1) != 0 ? b[i] : -__builtin_inff();
         }
+        if (a.groups > 1) {
+            // a lane's elements in open groups, a bit each; a quad is of one group where they divide so
+            int bits = 0;
+            if ((a.each & 3) == 0) {
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i) bits |= (mask >> (gid[i] & 255) & 1) != 0 ? 15 << (4 * i) : 0;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) bits |= (int)(mask >> (gid[i / 4] >> (8 * (i & 3)) & 255) & 1) << i;
+            }
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                vf4 q;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int all = (bits << (31 - 4 * i - j)) >> 31, none = __float_as_int(-__builtin_inff());
+                    b[4 * i + j] = q[j] = __int_as_float((__float_as_int(b[4 * i + j]) & all) | (none & ~all));
+                }
+                *reinterpret_cast<vf4*>(&row[g][4 * (i * L + l)]) = q;
+            }
+            wave_sync();
+        }
+        // a double that begins with a float's bits has its order; the rest holds the expert, whose order does not matter: a row
+        // with two of a value among its choices is not decided here
         double d[V < 8 ? 8 : V];
 #pragma unroll
-        for (int i = 0; i < (V < 8 ? 8 : V); ++i) d[i] = i < V ? list_key(sort_key(b[i < V ? i : 0]), 4 * ((i / 4) * L + l) + (i & 3)) : 1.0;
+        for (int i = 0; i < (V < 8 ? 8 : V); ++i)
+            d[i] = i < V ? __hiloint2double(__float_as_int(b[i < V ? i : 0]), 4 * ((i / 4) * L + l) + (i & 3))
+                         : __hiloint2double(__float_as_int(-__builtin_inff()), 0);
         list_rows<L, V>(d);
         // those chosen have to differ by more than what they are off by, and the last of them from the rest; what is closed or
         // past the experts is minus infinity, which none of them may be
         float last = 0.0f, gap = __builtin_inff(), was = __builtin_inff();
 #pragma unroll
         for (int t = 0; t < kList; ++t) {
-            const float v = key_value(list_value(d[t]));
+            const float v = __int_as_float(__double2hiint(d[t]));
             if (t < a.k) {
                 if (t > 0) gap = __builtin_fminf(gap, was - v);
                 last = was = v;
@@ -342,14 +436,18 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         }
         int near = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) near += b[i] >= last - tell;
+        for (int i = 0; i < V / 4; ++i) {
+            const vf4 q = *reinterpret_cast<const vf4*>(&row[g][4 * (i * L + l)]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) near += q[j] >= last - tell;
+        }
         near = group_red<L>(near, [](int p, int q) { return p + q; });
         unsure = group_red<L>((int)unsure, [](int p, int q) { return p | q; }) != 0;
         unsure |= !(gap > tell) || near != a.k || !(last > -__builtin_inff());
         wave_sync();
         if (l == 0) {
 #pragma unroll
-            for (int t = 0; t < kList; ++t) pick[g][t] = list_index(d[t]);
+            for (int t = 0; t < kList; ++t) pick[g][t] = __double2loint(d[t]);
             if (unsure && in) {
                 const uint32_t at = atomicAdd(a.ntodo, 1u);
                 if (at < (uint64_t)a.rows) a.todo[at] = r;
@@ -588,10 +686,12 @@ int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const 
     hipStream_t st = ctx().stream;
     const int64_t waves = kRThreads / 64, group = kRThreads / router_lanes(a.experts);
     const bool lists = a.k <= kList && rows > kRExactRows;
+    a.parts = 1;
+    while (2 * a.parts * a.groups <= router_lanes(a.experts)) a.parts *= 2;
     int64_t blocks = lists ? (rows + group - 1) / group : 0;
-    if (blocks > kRBlocks) blocks = kRBlocks;
+    if (blocks > kRBlocks) blocks = (blocks + (blocks + kRBlocks - 1) / kRBlocks - 1) / ((blocks + kRBlocks - 1) / kRBlocks);  // equal rounds
     int64_t exact = lists ? 128 : (rows + waves - 1) / waves;
-    if (exact > 2 * kRBlocks) exact = 2 * kRBlocks;
+    if (exact > kRBlocks) exact = kRBlocks;
     char* base = nullptr;
     const size_t list_bytes = lists ? (size_t)rows * 8 : 0, part_bytes = (size_t)(blocks + exact) * experts * 4;
     MH_TRY(scratch(list_bytes + part_bytes, reinterpret_cast<void**>(&base)));

@@ -269,6 +269,7 @@ constexpr int kGradThreads = 256;
 constexpr int kGradQuads = 4;                                          // quads a thread and chunk
 constexpr int64_t kGradChunk = (int64_t)kGradThreads * kGradQuads;     // quads of a chunk
 constexpr int64_t kGradBlocks = 2048;                                  // workgroups of a launch at most
+constexpr int64_t kGradOne = 16;                                       // chunks that one workgroup takes alone
 constexpr int kGradPerLaunch = 160;                                    // 3.8 KB of the 4 KB that arguments may take
 
 // A tensor and the first chunk of it in the launch's chunks. Quad k of a tensor whose address is sh floats past a
@@ -284,6 +285,12 @@ struct GradTable {
 
 __host__ __device__ __forceinline__ int grad_shift(const float* g) { return (int)((reinterpret_cast<uintptr_t>(g) >> 2) & 3); }
 
+// The workgroups of a launch over chunks that each takes as many of, the last fewer.
+static int64_t grad_blocks(int64_t chunks) {
+    const int64_t each = (chunks + kGradBlocks - 1) / kGradBlocks;
+    return chunks ? (chunks + each - 1) / each : 0;
+}
+
 // The tensors from *i on that a launch takes, and its chunks.
 static int64_t grad_table(int64_t ntensors, const float* const* grads, const int64_t* sizes, int64_t* i, GradTable* tab) {
     int64_t chunks = 0;
@@ -298,29 +305,40 @@ static int64_t grad_table(int64_t ntensors, const float* const* grads, const int
     return chunks;
 }
 
-__device__ __forceinline__ const GradTensor& grad_find(const GradTable& tab, int64_t chunk) {
-    int lo = 0, hi = tab.nt - 1;  // the last tensor whose chunk0 <= chunk
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tab.t[mid].chunk0 <= chunk) lo = mid;
-        else hi = mid - 1;
+// The last tensor whose chunk0 <= chunk: each lane looks at three. (A binary search's eight reads wait for each other.)
+__device__ __forceinline__ int grad_find(const GradTable& tab, int64_t chunk) {
+    const int lane = threadIdx.x & 63;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < kGradPerLaunch; i += 64) {
+        const bool is = i + lane < tab.nt && tab.t[i + lane < kGradPerLaunch ? i + lane : 0].chunk0 <= chunk;
+        at += __builtin_popcountll(__ballot(is));
     }
-    return tab.t[lo];
+    return __builtin_amdgcn_readfirstlane(at);
 }
 
 __device__ __forceinline__ double square_add(double s, float v) { return __builtin_fma((double)v, (double)v, s); }
 
-__global__ __launch_bounds__(kGradThreads) void k_grad_norm(GradTable tab, int64_t chunks, double* part) {
-    __shared__ double red[kGradThreads / 64];
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const GradTensor& t = grad_find(tab, c);
-        const int sh = grad_shift(t.g);
-        const int64_t k0 = (c - t.chunk0) * kGradChunk;
-        if (4 * k0 >= sh && 4 * (k0 + kGradChunk) - sh <= t.n) {  // whole quads
+// The squares of the chunks from c on, `step` apart and below `end`, by 256 threads; s gets each thread's.
+__device__ __forceinline__ void chunk_squares(const GradTable& tab, int64_t c, int64_t end, int64_t step, int tid, double* s) {
+    const float* g = nullptr;
+    int64_t n = 0, chunk0 = 0, next = -1;  // of the tensor at hand, and the first chunk past it
+    int sh = 0;
+    for (; c < end; c += step) {
+        if (c >= next) {
+            const int at = grad_find(tab, c);
+            const GradTensor& t = tab.t[at];
+            g = t.g;
+            n = t.n;
+            chunk0 = t.chunk0;
+            sh = grad_shift(g);
+            next = at + 1 < tab.nt ? tab.t[at + 1].chunk0 : end;
+        }
+        const int64_t k0 = (c - chunk0) * kGradChunk;
+        if (4 * k0 >= sh && 4 * (k0 + kGradChunk) - sh <= n) {  // whole quads
             vf4 v[kGradQuads];
 #pragma unroll
-            for (int i = 0; i < kGradQuads; ++i) v[i] = *reinterpret_cast<const vf4*>(t.g + 4 * (k0 + i * kGradThreads + threadIdx.x) - sh);
+            for (int i = 0; i < kGradQuads; ++i) v[i] = *reinterpret_cast<const vf4*>(g + 4 * (k0 + i * kGradThreads + tid) - sh);
 #pragma unroll
             for (int i = 0; i < kGradQuads; ++i) {
                 s[0] = square_add(s[0], v[i].x);
@@ -331,15 +349,39 @@ __global__ __launch_bounds__(kGradThreads) void k_grad_norm(GradTable tab, int64
         } else {
 #pragma unroll
             for (int i = 0; i < kGradQuads; ++i) {
-                const int64_t e = 4 * (k0 + i * kGradThreads + threadIdx.x) - sh;
+                const int64_t e = 4 * (k0 + i * kGradThreads + tid) - sh;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (e + j >= 0 && e + j < t.n) s[j] = square_add(s[j], t.g[e + j]);
+                    if (e + j >= 0 && e + j < n) s[j] = square_add(s[j], g[e + j]);
             }
         }
     }
+}
+
+// A workgroup takes neighbouring chunks, nearly always of one tensor.
+__global__ __launch_bounds__(kGradThreads) void k_grad_norm(GradTable tab, int64_t chunks, int64_t each, double* part) {
+    __shared__ double red[kGradThreads / 64];
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    const int64_t c = blockIdx.x * each;
+    chunk_squares(tab, c, c + each < chunks ? c + each : chunks, 1, threadIdx.x, s);
     const double sum = block_sum<kGradThreads / 64>((s[0] + s[1]) + (s[2] + s[3]), red);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+
+__device__ __forceinline__ void put_norm(double squares, float max_norm, float* norm, float* coef) {
+    const double n = __builtin_sqrt(squares);
+    if (norm) norm[0] = (float)n;
+    // an infinity or a NaN among the gradients scales nothing
+    coef[0] = n > (double)max_norm && n <= 1.7976931348623157e308 ? (float)((double)max_norm / n) : 1.0f;
+}
+
+// Few chunks: one workgroup, and no second launch to add up.
+__global__ __launch_bounds__(1024) void k_grad_norm_one(GradTable tab, int64_t chunks, float max_norm, float* norm, float* coef) {
+    __shared__ double red[16];
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    chunk_squares(tab, threadIdx.x / kGradThreads, chunks, 1024 / kGradThreads, threadIdx.x % kGradThreads, s);
+    const double sum = block_sum<16>((s[0] + s[1]) + (s[2] + s[3]), red);
+    if (threadIdx.x == 0) put_norm(sum, max_norm, norm, coef);
 }
 
 // The norm from the workgroups' sums, and what the gradients are scaled by.
@@ -348,18 +390,14 @@ __global__ __launch_bounds__(1024) void k_grad_total(const double* part, int64_t
     double s = 0.0;
     for (int64_t i = threadIdx.x; i < parts; i += 1024) s += part[i];
     s = block_sum<16>(s, red);
-    if (threadIdx.x != 0) return;
-    const double n = __builtin_sqrt(s);
-    if (norm) norm[0] = (float)n;
-    // an infinity or a NaN among the gradients scales nothing
-    coef[0] = n > (double)max_norm && n <= 1.7976931348623157e308 ? (float)((double)max_norm / n) : 1.0f;
+    if (threadIdx.x == 0) put_norm(s, max_norm, norm, coef);
 }
 
 __global__ __launch_bounds__(kGradThreads) void k_clip_scale(GradTable tab, int64_t chunks, const float* coef) {
     const float m = coef[0];
     if (m == 1.0f) return;
     for (int64_t c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {  // from the end, which the caches hold
-        const GradTensor& t = grad_find(tab, c);
+        const GradTensor& t = tab.t[grad_find(tab, c)];
         const int sh = grad_shift(t.g);
         const int64_t k0 = (c - t.chunk0) * kGradChunk;
         if (4 * k0 >= sh && 4 * (k0 + kGradChunk) - sh <= t.n) {
@@ -423,20 +461,26 @@ static int check_apart(const char* what, int64_t ntensors, const float* const* g
 // Queues the norm of all gradients; *coef is where what they are scaled by will lie.
 static int norm_of(int64_t ntensors, const float* const* grads, const int64_t* sizes, float max_norm, float* norm, float** coef) {
     GradTable tab;
-    int64_t parts = 0;
+    int64_t parts = 0, first = 0;
     for (int64_t i = 0; i < ntensors;) {
         const int64_t chunks = grad_table(ntensors, grads, sizes, &i, &tab);
-        parts += chunks < kGradBlocks ? chunks : kGradBlocks;
+        if (first == 0) first = i == ntensors ? chunks : kGradOne + 1;  // all of them, if one launch takes them
+        parts += grad_blocks(chunks);
     }
     double* part = nullptr;
     MH_TRY(scratch(8 * (size_t)(parts + 1), reinterpret_cast<void**>(&part)));
     *coef = reinterpret_cast<float*>(part + parts);
+    if (first > 0 && first <= kGradOne) {
+        hipLaunchKernelGGL(k_grad_norm_one, dim3(1), dim3(1024), 0, ctx().stream, tab, first, max_norm, norm, *coef);
+        return MH_OK;
+    }
     double* at = part;
     for (int64_t i = 0; i < ntensors;) {
         const int64_t chunks = grad_table(ntensors, grads, sizes, &i, &tab);
         if (chunks == 0) continue;
-        const int64_t blocks = chunks < kGradBlocks ? chunks : kGradBlocks;
-        hipLaunchKernelGGL(k_grad_norm, dim3((unsigned)blocks), dim3(kGradThreads), 0, ctx().stream, tab, chunks, at);
+        const int64_t blocks = grad_blocks(chunks);
+        hipLaunchKernelGGL(k_grad_norm, dim3((unsigned)blocks), dim3(kGradThreads), 0, ctx().stream, tab, chunks,
+                           (chunks + kGradBlocks - 1) / kGradBlocks, at);
         at += blocks;
     }
     hipLaunchKernelGGL(k_grad_total, dim3(1), dim3(1024), 0, ctx().stream, part, parts, max_norm, norm, *coef);
