@@ -8,10 +8,10 @@
 //     softmax:  grad_j = scale p_j (g_j - sum g p)          normalised: scale q_i (g_i - sum g q)
 //
 // Scores decide a choice after a bias was added to them, so logits do not: experts whose biased scores agree to fp32 are
-// not rare over a long batch, and which of them is chosen shows. What is compared is therefore meant in 64 bits. Up to 8
-// choices are made in fp32 first, by sorted lists of the row, with a bound on its error; a row whose choice, or whose choice
+// not rare over a long batch, and which of them is chosen shows. What is compared is therefore meant in 64 bits.
+// Choices are made in fp32 first, 8 at a time by sorted lists of the row, with a bound on its error; a row whose choice, or whose choice
 // of groups, turns on less than twice that (one in a few hundred) is listed, and a second kernel chooses for it in 64 bits, a
-// wavefront a row. That kernel alone takes short batches, whose rows it holds all at once, and more than 8 choices. Weights are
+// wavefront a row. That kernel alone takes short batches, whose rows it holds all at once. Weights are
 // 64-bit scores rounded to fp32, by one formula in both; gradients are fp32.
 //
 // Bound by the logits' read and the gradient's write, and over many experts by the sorting. L lanes hold a row in
@@ -260,11 +260,12 @@ __device__ __forceinline__ void load_next(const float* row, int E, int l, float*
 }
 
 template <int L, int V, bool SIGMOID>
-__global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
+__global__ __launch_bounds__(kRThreads, V == 16 ? 3 : 4) void k_group_router_fwd(GroupArg a) {
     constexpr int G = kRThreads / L;  // rows in flight in a workgroup
     constexpr int N = L * V < kMaxGroups ? L * V : kMaxGroups;
     __shared__ int32_t cnt[L * V];
-    __shared__ int32_t pick[G][kList];
+    constexpr int K = L * V < kList ? kList : L * V < kMaxChosen ? L * V : kMaxChosen;
+    __shared__ int32_t pick[G][K];
     __shared__ __attribute__((aligned(16))) float row[G][L * V], bias[L * V];
     __shared__ float of_group[G][N];
     const int tid = threadIdx.x, l = tid % L, g = tid / L;
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 b[4 * i + j] = q[j];
-                unsure |= q[j] != q[j];
+                unsure |= !(q[j] < __builtin_inff());
             }
         }
         wave_sync();
@@ -415,23 +416,30 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
             }
             wave_sync();
         }
-        // a double that begins with a float's bits has its order; the rest holds the expert, whose order does not matter: a row
-        // with two of a value among its choices is not decided here
-        double d[V < 8 ? 8 : V];
+        // 8 choices at a time, of what lies below the last. A double that begins with a float's bits has its order; the rest
+        // holds the expert, whose order does not matter: a row with two of a value among its choices is not decided here.
+        // Those chosen have to differ by more than what they are off by, and the last of them from the rest; what is closed or
+        // past the experts is minus infinity, which none of them may be.
+        float last = __builtin_inff(), gap = __builtin_inff(), was = __builtin_inff();
+        for (int t0 = 0; t0 < a.k; t0 += kList) {
+            double d[V < 8 ? 8 : V];
 #pragma unroll
-        for (int i = 0; i < (V < 8 ? 8 : V); ++i)
-            d[i] = i < V ? __hiloint2double(__float_as_int(b[i < V ? i : 0]), 4 * ((i / 4) * L + l) + (i & 3))
-                         : __hiloint2double(__float_as_int(-__builtin_inff()), 0);
-        list_rows<L, V>(d);
-        // those chosen have to differ by more than what they are off by, and the last of them from the rest; what is closed or
-        // past the experts is minus infinity, which none of them may be
-        float last = 0.0f, gap = __builtin_inff(), was = __builtin_inff();
+            for (int i = 0; i < (V < 8 ? 2 : V / 4); ++i) {
+                vf4 q = vf4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (i < V / 4) q = *reinterpret_cast<const vf4*>(&row[g][4 * ((i < V / 4 ? i : 0) * L + l)]);
 #pragma unroll
-        for (int t = 0; t < kList; ++t) {
-            const float v = __int_as_float(__double2hiint(d[t]));
-            if (t < a.k) {
-                if (t > 0) gap = __builtin_fminf(gap, was - v);
-                last = was = v;
+                for (int j = 0; j < 4; ++j)
+                    d[4 * i + j] = __hiloint2double(__float_as_int(i < V / 4 && q[j] < last ? q[j] : -__builtin_inff()), 4 * (i * L + l) + j);
+            }
+            list_rows<L, V>(d);
+#pragma unroll
+            for (int t = 0; t < kList; ++t) {
+                const float v = __int_as_float(__double2hiint(d[t]));
+                if (t0 + t < a.k) {
+                    if (t0 + t > 0) gap = __builtin_fminf(gap, was - v);
+                    last = was = v;
+                    if (l == 0) pick[g][t0 + t] = __double2loint(d[t]);
+                }
             }
         }
         int near = 0;
@@ -444,14 +452,9 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_fwd(GroupArg a) {
         near = group_red<L>(near, [](int p, int q) { return p + q; });
         unsure = group_red<L>((int)unsure, [](int p, int q) { return p | q; }) != 0;
         unsure |= !(gap > tell) || near != a.k || !(last > -__builtin_inff());
-        wave_sync();
-        if (l == 0) {
-#pragma unroll
-            for (int t = 0; t < kList; ++t) pick[g][t] = __double2loint(d[t]);
-            if (unsure && in) {
-                const uint32_t at = atomicAdd(a.ntodo, 1u);
-                if (at < (uint64_t)a.rows) a.todo[at] = r;
-            }
+        if (l == 0 && unsure && in) {
+            const uint32_t at = atomicAdd(a.ntodo, 1u);
+            if (at < (uint64_t)a.rows) a.todo[at] = r;
         }
         wave_sync();
         put_choice<L>(a, pick[g], x, r, l, in && !unsure, keep, top, by, cnt);
@@ -685,7 +688,7 @@ int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const 
     a.chosen = chosen;
     hipStream_t st = ctx().stream;
     const int64_t waves = kRThreads / 64, group = kRThreads / router_lanes(a.experts);
-    const bool lists = a.k <= kList && rows > kRExactRows;
+    const bool lists = rows > kRExactRows;
     a.parts = 1;
     while (2 * a.parts * a.groups <= router_lanes(a.experts)) a.parts *= 2;
     int64_t blocks = lists ? (rows + group - 1) / group : 0;
