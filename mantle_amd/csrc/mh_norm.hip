@@ -264,8 +264,8 @@ __global__ __launch_bounds__(256) void k_norm_bwd_long(NormArg a, const vf2* sca
     vf4 acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int c0 = 4096 * blockIdx.y + 4 * threadIdx.x;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const int c0 = 4096 * blockIdx.x + 4 * threadIdx.x;
+    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         const int64_t at = r * a.dim;
         const vf2 s = scales[r];
 #pragma unroll
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void k_norm_bwd_long(NormArg a, const vf2* sca
         }
     }
     if (!a.part) return;
-    float* o = a.part + (int64_t)blockIdx.x * a.dim;
+    float* o = a.part + (int64_t)blockIdx.y * a.dim;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int c = c0 + 1024 * i;
@@ -418,7 +418,7 @@ int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const f
     if (lng) {
         vf2* sc = reinterpret_cast<vf2*>(base);
         hipLaunchKernelGGL(k_norm_scales_long, dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, a, sc);
-        hipLaunchKernelGGL(k_norm_bwd_long, dim3((unsigned)blocks, (unsigned)((dim + 4095) / 4096)), dim3(256), 0, st, a, sc);
+        hipLaunchKernelGGL(k_norm_bwd_long, dim3((unsigned)((dim + 4095) / 4096), (unsigned)blocks), dim3(256), 0, st, a, sc);
     } else {
 #define MH_CALL(L, Q, T) hipLaunchKernelGGL((k_norm_bwd<L, Q, T>), dim3((unsigned)blocks), dim3(T), 0, st, a)
         MH_NORM(MH_CALL);

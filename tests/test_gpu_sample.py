@@ -128,6 +128,57 @@ def test_sizes(size):
           mp=r.choice([0.0, 0.05, -1.0], rows), unsure=1, what="mixed")
 
 
+@pytest.mark.parametrize("size", [(257, 9000), (300, 40001)], ids=str)
+def test_many_rows_of_many_classes(size):
+    m = m_()
+    x, u = logits(*size, seed=sum(size))
+    r = np.random.RandomState(1)
+    rows = size[0]
+    check(m, x, u, T=r.choice([0.0, 0.5, 1.0, 1.4], rows), k=r.choice([0, 1, 40, 700], rows), p=r.choice([1.0, 0.95, 0.6], rows),
+          mp=r.choice([0.0, 0.03], rows), what="mixed")
+
+
+@pytest.mark.parametrize("classes", [(1 << 19) + 1, 700001])
+def test_more_classes_than_bins_count(classes):
+    m = m_()
+    x, u = logits(2, classes, seed=21)
+    for a in ({}, {"k": 50}, {"p": 0.9, "T": 0.7}, {"T": 0.0}, {"k": 1000, "p": 0.8, "mp": 0.01}):
+        check(m, x, u, **a, unsure=1, what=str(a))
+
+
+@pytest.mark.parametrize("rows, classes", [(3, 100000), (260, 40000)])
+def test_a_logit_far_above_those_before_it(rows, classes):
+    """One that lies beyond what a workgroup holds, by a little or by more than any bin."""
+    m = m_()
+    x, u = logits(rows, classes, seed=22)
+    for above in (5.0, 12.0, 40.0, 1e4):
+        x[:, classes - 7] = x.max() + above
+        x[:, classes - 300] = x.max() - 0.5
+        check(m, x, u, k=40, p=0.99, what=f"+{above}")
+        # shares of 1 / 20000 or so against borders of 2 delta, 1e-6: one row in thirty or so
+        check(m, x, u, T=3.0, p=0.5, unsure=rows / 20 + 1, what=f"+{above}, warm")
+
+
+@pytest.mark.parametrize("std", [1e-5, 0.01, 0.2])
+def test_logits_close_together(std):
+    """Thousands of classes in a bin: narrower ones, or where they are too close for any, the search over their bits."""
+    m = m_()
+    r = np.random.RandomState(23)
+    x = (std * r.standard_normal((4, 70000))).astype(np.float32)
+    u = r.uniform(size=4).astype(np.float32)
+    for a in ({"k": 30000}, {"p": 0.5}, {"k": 50000, "p": 0.4}, {"T": 0.05, "p": 0.9}, {"T": 20.0, "k": 100, "p": 0.3}):
+        check(m, x, u, **a, unsure=4, what=f"{std} {a}")
+
+
+@pytest.mark.parametrize("T", [0.005, 0.01, 0.02, 0.1])
+def test_cold(T):
+    """Cuts far below the largest, where masses are nothing."""
+    m = m_()
+    x, u = logits(6, 5000, seed=24)
+    for a in ({"k": 1}, {"k": 60}, {"k": 3000}, {"p": 0.9999}, {"k": 500, "p": 0.999999}):
+        check(m, x, u, T=T, **a, unsure=2, what=f"{T} {a}")
+
+
 def test_many_rows():
     m = m_()
     x, u = logits(6000, 40, seed=2)
