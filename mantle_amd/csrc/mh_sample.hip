@@ -4,20 +4,20 @@
 // class, the cut. The token is the first class, by index, where the running sum of the kept masses e^((x - max) / T) exceeds u
 // of their sum.
 //
-// A workgroup takes a row, a wavefront a run of its classes, of which each lane holds 4 Q logits in registers (the whole
+// A workgroup takes a row (64 threads of a short one where there are many, up to 1024), a wavefront a run of its classes, of which each lane holds 4 Q logits in registers (the whole
 // row up to 4 Q T classes; of a longer one the rest is read as it is needed):
 //   1. the largest logit held, the reference, and bins of a power-of-two width, T / 112 or 1 / 112 at least, around it;
 //   2. for top-k and top-p how many classes each bin has and their mass, both in one 64-bit LDS atomic: 20 bits of count above
 //      44 of mass, a class 24 bits of its bin's largest. Whole numbers: the atomics' order does not show. A scan of the bins
 //      then says in which of them a cut falls;
 //   3. a second walk, over the quads that reach those bins, adds up what lies above them and lists what lies in them. More
-//      than 2048 listed: from 2. on with narrower bins in the place of those;
+//      listed than there is room: from 2. on with narrower bins in the place of those;
 //   4. the list is sorted, and the cuts are found in it by 64-bit sums;
 //   5. the run of classes where the running sum passes u of the total is walked by the whole workgroup.
 // Sums of steps 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
 // sign, moves a border by some 2^-24 of the row.
 //
-// Rows for which bins do not work (more than 2048 classes of one value at a cut, a cut 32 T below the largest, an infinite
+// Rows for which bins do not work (more than 256 to 2048 classes of one value at a cut, a cut 32 T below the largest, an infinite
 // logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over the logits'
 // bits, 8 at a time: right for every row, and slower.
 #include "mh_internal.h"
@@ -26,9 +26,13 @@
 namespace mh {
 namespace {
 
-constexpr int kBins = 4096;
-constexpr int kAbove = 512;  // of them above the reference at first
-constexpr int kList = 2048;
+// By the threads T of a workgroup: the bins, those of them above the reference at first, the classes a list holds, and
+// those whose quads' largest logits are kept. Bins below the reference reach 32 T at least, whatever their power of two.
+template <int T>
+struct Sizes {
+    static constexpr int kBins = T >= 512 ? 4096 : 8 * T, kAbove = kBins / 8, kList = kBins / 2, kTops = T >= 512 ? 1 << 19 : 128 * T;
+    static constexpr float kWidth = 1.0f / (T >= 512 ? 112 : T / 5);  // of T, at least
+};
 constexpr int kCountAt = 44;
 constexpr int64_t kMaxBinned = (int64_t)1 << 19;
 constexpr int64_t kMaxSampled = (int64_t)1 << 24;
@@ -313,17 +317,22 @@ __device__ __forceinline__ float least_of(F&& is) {
     return of_order(key + 1);
 }
 
-struct FastLds {
+// What is known at once of a workgroup's sums.
+struct Sums {
+    double wave_d[16];
+    uint32_t wave_n[16];
+};
+template <int T>
+struct FastLds : Sums {
     union {
-        unsigned long long hist[kBins];
+        unsigned long long hist[Sizes<T>::kBins];
         struct {
-            uint64_t key[kList];  // order inverted, then the index: rising is the order that is kept
-            double upto[kList];   // sums of masses
+            uint64_t key[Sizes<T>::kList];  // order inverted, then the index: rising is the order that is kept
+            double upto[Sizes<T>::kList];   // sums of masses
         } list;
     };
-    float quad_top[kMaxBinned / 256];  // the largest of 256 classes
-    double wave_d[16], seg[16];
-    uint32_t wave_n[16];
+    float quad_top[Sizes<T>::kTops / 256];  // the largest of 256 classes
+    double seg[16];
     float wave_f[16];
     // what one thread found out for all
     uint32_t listed, k_bin, k_above_n, k_here, p_lo, p_hi, p_above_n;
@@ -335,7 +344,7 @@ struct FastLds {
 // same bits as the next thread's m0.
 template <int W>
 __device__ __forceinline__ void block_scan(uint32_t n, double m, uint32_t& n0, double& m0, double& m1, uint32_t& n_all, double& m_all,
-                                           FastLds& s) {
+                                           Sums& s) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ni = wave_scan(n);
     const double mi = wave_scan(m);
@@ -399,9 +408,14 @@ struct Mass {
 template <int T, int Q>
 __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     constexpr int W = T / 64;
+    constexpr int kBins = Sizes<T>::kBins, kAbove = Sizes<T>::kAbove, kList = Sizes<T>::kList;
     constexpr int B = kBins / T;  // bins of a thread
-    __shared__ union { FastLds f; SlowLds s; } lds;
-    FastLds& s = lds.f;
+    __shared__ union Lds {
+        FastLds<T> f;
+        SlowLds s;
+        __device__ Lds() {}
+    } lds;
+    FastLds<T>& s = lds.f;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // a wavefront's run of classes: whole rounds of 256, of which the first Q are held
     const int run = (a.classes + 256 * W - 1) / (256 * W) * 256;
@@ -470,7 +484,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     auto others = [](int g) { return g ? ~(uint64_t)0 : ~(uint64_t)0 << Q; };
     float top = -__builtin_inff();  // of what the wavefront has seen
     bool nan = false;
-    const bool tops = a.classes <= kMaxBinned;
+    const bool tops = a.classes <= Sizes<T>::kTops;
     auto look = [&](const vf4& v, int i) {
         nan |= __builtin_isunordered(v.x, v.y) | __builtin_isunordered(v.z, v.w);
         const float q = wave_max(__builtin_fmaxf(__builtin_fmaxf(v.x, v.y), __builtin_fmaxf(v.z, v.w)));
@@ -499,13 +513,13 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     float best = block_top();
     float ref = best;
     // masses are e^((x - ref) / T) until the largest is known
-    bool binned = cuts && a.classes <= kMaxBinned && ref > -__builtin_inff() && ref < __builtin_inff() && T_ >= 0.01f && T_ <= 1e30f;
+    bool binned = cuts && tops && ref > -__builtin_inff() && ref < __builtin_inff() && T_ >= 0.01f && T_ <= 1e30f;
     // the bins: place_of counts widths below ref and `start`, and bin b holds the places from b - off on
     int off = kAbove;
     float per_bin, start = 0.0f;
     double width;
     {
-        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * (1.0f / 112.0f));
+        const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * Sizes<T>::kWidth);
         per_bin = __builtin_ldexpf(1.0f, -e);
         width = __builtin_ldexp(1.0, e);
     }
@@ -875,6 +889,30 @@ void launch_sample(SampleArg a, int64_t rows) {
     }
 }
 
+// Threads a row: a CU holds 16, 4, 2 or 1 workgroups, and a row takes one so many microseconds and so many more for 1000
+// classes. [4096, 2000], settings of all kinds: 40, 62, 110 and 231 us with 64, 256, 512 and 1024 threads; [1024, 4000]: 40, 27,
+// 40, 68; [512, 16000]: 37, 32, 45 with 256 to 1024; [64, 4000]: 31, 18, 17, 19.
+int sample_threads(int64_t rows, int64_t classes) {
+    struct Form {
+        int threads, held;
+        double base, more;
+        int64_t most;
+    };
+    const Form forms[] = {{64, 16, 15.0, 5.0, Sizes<64>::kTops}, {256, 4, 15.0, 1.05, Sizes<256>::kTops}, {512, 2, 16.0, 0.55, kMaxSampled},
+                          {1024, 1, 18.0, 0.4, kMaxSampled}};
+    int best = 1024;
+    double least = 1e300;
+    for (const Form& f : forms) {
+        const double rounds = (double)((rows + 256 * f.held - 1) / (256 * f.held));
+        const double cost = rounds * (f.base + f.more * 1e-3 * (double)classes);
+        if (classes <= f.most && cost < least) {
+            least = cost;
+            best = f.threads;
+        }
+    }
+    return best;
+}
+
 }  // namespace
 }  // namespace mh
 
@@ -903,8 +941,12 @@ int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const floa
     a.classes = (int32_t)classes;
     a.shift = 62;
     while (((int64_t)1 << (62 - a.shift)) < classes) --a.shift;
-    if (rows > 256) launch_sample<512, 16>(a, rows);
-    else launch_sample<1024, 16>(a, rows);
+    switch (sample_threads(rows, classes)) {
+        case 64: launch_sample<64, 16>(a, rows); break;
+        case 256: launch_sample<256, 16>(a, rows); break;
+        case 512: launch_sample<512, 16>(a, rows); break;
+        default: launch_sample<1024, 16>(a, rows);
+    }
     return finish("mh_sample_tokens");
 }
 

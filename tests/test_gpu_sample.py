@@ -179,6 +179,33 @@ def test_cold(T):
         check(m, x, u, T=T, **a, unsure=2, what=f"{T} {a}")
 
 
+@pytest.mark.parametrize("rows", [12, 720, 3000])
+@pytest.mark.parametrize("kind", ["few", "ties", "close", "masked", "far"])
+def test_many_rows_take_other_workgroups(rows, kind):
+    """The same 12 rows over and over, which fewer threads a row take where there are many of them."""
+    m = m_()
+    x, u = logits(12, 3001, seed=25)
+    r = np.random.RandomState(26)
+    if kind == "ties":
+        x = np.round(x)
+    if kind == "close":
+        x = (1e-3 * r.standard_normal(x.shape)).astype(np.float32)
+    if kind == "masked":
+        x[:, 5:2900] = -np.inf
+        x[1], x[2, 7], x[3, 2950] = -np.inf, np.nan, np.inf
+    if kind == "far":
+        x[:, -2] = x.max() + np.float32([3, 9, 30] * 4)
+    for a in ({}, {"k": 7}, {"k": 1500}, {"p": 0.7}, {"k": 900, "p": 0.9, "mp": 1e-3, "T": 1.2}, {"T": 0.0}, {"T": 0.1, "p": 0.99}, {"T": 8.0, "k": 2000, "p": 0.8}):
+        check(m, x, u, **a, unsure=12, what=f"{kind} {a}")
+        tok, lp = run(m, x, u, **a)
+        many = run(m, np.tile(x, (rows // 12, 1)), np.tile(u, rows // 12), **a)
+        right = [reference(x[i], u[i], a.get("T", 1.0), a.get("k", 0), a.get("p", 1.0), a.get("mp", 0.0))[0] for i in range(12)]
+        for i in range(12):
+            assert len(set(many[0][i::12].tolist())) == 1
+            t, l = int(many[0][i]), many[1][i]
+            assert t in right[i] and any(np.isnan(l) and np.isnan(v) or abs(l - v) <= off for v, off in right[i][t]), f"{kind} {a} {i}"
+
+
 def test_many_rows():
     m = m_()
     x, u = logits(6000, 40, seed=2)
