@@ -374,14 +374,14 @@ int mh_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int3
  * holds a NaN, plus infinity or nothing but minus infinity has NaN for weights; so has a chosen sigmoid that is NaN, and
  * with normalise its whole row, or one whose chosen scores add up to 0. Choices stay below experts.
  * 1 <= experts <= 1024, 1 <= k <= 64, 1 <= groups <= 64, which divide experts, and k experts at least in keep_groups
- * groups. */
+ * groups. The library's scratch grows to 4 bytes a row, and 10 KB an expert at most. */
 enum mh_router_scores { MH_SCORES_SOFTMAX = 0, MH_SCORES_SIGMOID = 1 };
 int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const float* x, const float* bias,
                         const int32_t* keep, int64_t rows, int64_t experts, int64_t k, int64_t groups, int64_t keep_groups,
                         int group_best, int scores, int normalise, float scale);
 /* The gradient of the logits from grad_weights [rows, k]; chosen is the forward's, and the choice carries no gradient; keep,
  * scores, normalise and scale as given to it. A row that is not kept is left alone (accumulate == 0: zero). An entry of
- * chosen outside the experts counts as none. */
+ * chosen outside the experts counts as none; no expert may stand twice in a row, as none does in the forward's. */
 int mh_group_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int32_t* chosen, const float* grad_weights,
                         int64_t rows, int64_t experts, int64_t k, int scores, int normalise, float scale, int accumulate);
 /* The bias' step towards balance: bias_e += rate for experts that were chosen less often than the mean of counts,
@@ -392,15 +392,16 @@ int mh_router_bias_update(float* bias, const int32_t* counts, int64_t experts, f
 
 /* Root-mean-square norm of rows with the residual's addition: h = x + residual (residual may be null: h = x),
  * out = h w / sqrt(mean h^2 + eps) over the dim elements of a row, sum = h (may be null). The mean is taken in 64 bits, so
- * that no finite h is too large or too small for it. sum may be x or residual, out may be x; no others may overlap.
- * A row with a NaN is NaN; one with infinities is NaN where they are and 0 elsewhere. dim <= 2^30. */
+ * that no finite h is too large or too small for it, whatever 1 / sqrt() is in fp32. sum may be x or residual, out may be
+ * x; no others may overlap. A row with a NaN is NaN; one with infinities is NaN where they are and 0 elsewhere; with eps
+ * == 0 a row of zeros is NaN. dim <= 2^30. */
 int mh_rms_norm_fwd(float* out, float* sum, const float* x, const float* residual, const float* w, int64_t rows, int64_t dim,
                     float eps);
 /* The gradient of x and of residual, which are one, and of w, from grad_out and grad_sum, the gradients of out and sum
  * (grad_sum may be null), and h, the forward's sum: with r = 1 / sqrt(mean h^2 + eps), u = h r, g = grad_out
  *   grad_x = grad_sum + r (w g - u mean(w g u)),  grad_w = sum over rows of g u
  * added to grad_x and grad_w, or written over them with accumulate == 0. Either may be null. grad_x may be grad_sum or
- * grad_out. The library's scratch grows to 4 bytes for each element of 1024 rows at most, and 8 a row of more than 16384
+ * grad_out. The library's scratch grows to 4 bytes for each element of 1024 rows at most, and 12 a row of more than 16384
  * elements. */
 int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const float* grad_sum, const float* h, const float* w,
                     int64_t rows, int64_t dim, float eps, int accumulate);
@@ -414,7 +415,9 @@ int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const f
  * tokens [rows] is the first class, by index, where the running sum of the kept p exceeds u times their sum; logprob [rows]
  * (may be null) the logarithm of its share in that sum. A class at minus infinity is never drawn; classes at plus infinity
  * share a row evenly. A row that holds a NaN, or nothing but minus infinity, has token -1 and logprob NaN. u is held to
- * [0, 1); a NaN counts as 0. classes <= 2^24. */
+ * [0, 1); a NaN counts as 0. A class's p is made in 32 bits, to 2^-22 of itself, and all sums in 64: where u or top_p falls
+ * within some 2^-24 of a border between two classes either may be taken. The same call has the same tokens.
+ * classes <= 2^24. */
 int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const float* u, const float* temperature,
                      const int32_t* top_k, const float* top_p, const float* min_p, int64_t rows, int64_t classes);
 
@@ -550,7 +553,7 @@ int mh_adam_step_multi(int64_t ntensors, float* const* params, const float* cons
 int mh_grad_norm(int64_t ntensors, const float* const* grads, const int64_t* sizes, float* norm);
 /* The same, and the gradients scaled in place by c = min(1, max_norm / norm), a float that is made from the 64-bit
  * norm. Where one of them is infinite or NaN none is scaled; norm says so. norm may be null; max_norm is 0 or more, and
- * infinity scales nothing. Tensors that share elements are refused. */
+ * infinity scales nothing. Tensors that share elements are refused, and norm may be none of their elements. */
 int mh_clip_grad_norm(int64_t ntensors, float* const* grads, const int64_t* sizes, float max_norm, float* norm);
 /* mh_adam_step_multi with c g in the place of each gradient g, which stays as it is: 32 bytes an element instead of the
  * 40 of the two calls, and the same bits. norm may be null. */

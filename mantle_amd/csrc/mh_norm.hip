@@ -17,8 +17,6 @@
 namespace mh {
 namespace {
 
-typedef float vf2 __attribute__((ext_vector_type(2)));
-
 constexpr int64_t kMaxNormDim = (int64_t)1 << 30;
 
 struct NormArg {
@@ -94,6 +92,18 @@ __device__ __forceinline__ double dot4(vf4 a, vf4 b, double s) {
     return __builtin_fma((double)a.w, (double)b.w, s);
 }
 
+// s = q 2^e, for s itself may be past fp32's range either way: x s is x 2^e, exact, times q.
+struct Scale {
+    float q;
+    int32_t e;
+    __device__ __forceinline__ explicit Scale(double s) : q((float)__builtin_amdgcn_frexp_mant(s)), e(__builtin_amdgcn_frexp_exp(s)) {}
+    __device__ __forceinline__ Scale(float mant, int32_t exp) : q(mant), e(exp) {}
+    __device__ __forceinline__ vf4 up(vf4 v) const {
+        return vf4{__builtin_ldexpf(v.x, e), __builtin_ldexpf(v.y, e), __builtin_ldexpf(v.z, e), __builtin_ldexpf(v.w, e)};
+    }
+    __device__ __forceinline__ vf4 of(vf4 h) const { return up(h) * q; }
+};
+
 template <int L, int Q, int T>
 __global__ __launch_bounds__(T) void k_norm_fwd(NormArg a) {
     constexpr int G = T / L;  // rows in flight in a workgroup
@@ -121,13 +131,13 @@ __global__ __launch_bounds__(T) void k_norm_fwd(NormArg a) {
 #pragma unroll
         for (int i = 0; i < Q; ++i) s = dot4(h[i], h[i], s);
         row_sums<L>(s, none, red);
-        const float scale = (float)(1.0 / __builtin_sqrt(s / (double)a.dim + a.eps));
+        const Scale scale(1.0 / __builtin_sqrt(s / (double)a.dim + a.eps));
         if (!in) continue;
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
             const int c = 4 * (i * L + l);
             if (a.sum) store_quad(a.sum + at, c, a.dim, h[i]);
-            store_quad(a.out + at, c, a.dim, h[i] * scale * w[i]);
+            store_quad(a.out + at, c, a.dim, scale.of(h[i]) * w[i]);
         }
     }
 }
@@ -144,23 +154,23 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArg a) {
             s = dot4(h, h, s);
         }
         row_sums<1024>(s, none, red);
-        const float scale = (float)(1.0 / __builtin_sqrt(s / (double)a.dim + a.eps));
+        const Scale scale(1.0 / __builtin_sqrt(s / (double)a.dim + a.eps));
         for (int c = 4 * threadIdx.x; c < a.dim; c += 4096) {
             vf4 h = load_quad(a.x + at, c, a.dim);
             if (a.residual) h = h + load_quad(a.residual + at, c, a.dim);
             if (a.sum) store_quad(a.sum + at, c, a.dim, h);
-            store_quad(a.out + at, c, a.dim, h * scale * load_quad(a.w, c, a.dim));
+            store_quad(a.out + at, c, a.dim, scale.of(h) * load_quad(a.w, c, a.dim));
         }
     }
 }
 
 // s and mean(w g u) of a row from its sums of h^2 and w g h.
-__device__ __forceinline__ void row_scales(double hh, double wgh, int dim, double eps, float& scale, float& mean) {
+__device__ __forceinline__ Scale row_scales(double hh, double wgh, int dim, double eps, float& mean) {
     const double s = 1.0 / __builtin_sqrt(hh / (double)dim + eps);
-    scale = (float)s;
     mean = (float)(wgh * s / (double)dim);
+    return Scale(s);
 }
-__device__ __forceinline__ vf4 row_grad(vf4 wg, vf4 u, float scale, float mean) { return (wg - u * mean) * scale; }
+__device__ __forceinline__ vf4 row_grad(vf4 wg, vf4 u, Scale scale, float mean) { return scale.up((wg - u * mean) * scale.q); }
 
 template <int L, int Q, int T>
 __global__ __launch_bounds__(T) void k_norm_bwd(NormArg a) {
@@ -193,13 +203,13 @@ __global__ __launch_bounds__(T) void k_norm_bwd(NormArg a) {
             wgh = dot4(d[i] * w[i], h[i], wgh);
         }
         row_sums<L>(hh, wgh, red);
-        float scale, mean;
-        row_scales(hh, wgh, a.dim, a.eps, scale, mean);
+        float mean;
+        const Scale scale = row_scales(hh, wgh, a.dim, a.eps, mean);
         if (!in) continue;
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
             const int c = 4 * (i * L + l);
-            const vf4 u = h[i] * scale;
+            const vf4 u = scale.of(h[i]);
             acc[i] += d[i] * u;
             if (a.gx) {
                 vf4 o = row_grad(d[i] * w[i], u, scale, mean);
@@ -243,8 +253,13 @@ __global__ __launch_bounds__(T) void k_norm_bwd(NormArg a) {
     }
 }
 
+struct RowScale {
+    float q;
+    int32_t e;
+    float mean;
+};
 // Long rows: their scales first, then workgroups of 4096 columns over a share of the rows.
-__global__ __launch_bounds__(1024) void k_norm_scales_long(NormArg a, vf2* scales) {
+__global__ __launch_bounds__(1024) void k_norm_scales_long(NormArg a, RowScale* scales) {
     __shared__ double red[32];
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const int64_t at = r * a.dim;
@@ -255,27 +270,28 @@ __global__ __launch_bounds__(1024) void k_norm_scales_long(NormArg a, vf2* scale
             wgh = dot4(load_quad(a.g + at, c, a.dim) * load_quad(a.w, c, a.dim), h, wgh);
         }
         row_sums<1024>(hh, wgh, red);
-        float scale, mean;
-        row_scales(hh, wgh, a.dim, a.eps, scale, mean);
-        if (threadIdx.x == 0) scales[r] = vf2{scale, mean};
+        float mean;
+        const Scale scale = row_scales(hh, wgh, a.dim, a.eps, mean);
+        if (threadIdx.x == 0) scales[r] = RowScale{scale.q, scale.e, mean};
     }
 }
-__global__ __launch_bounds__(256) void k_norm_bwd_long(NormArg a, const vf2* scales) {
+__global__ __launch_bounds__(256) void k_norm_bwd_long(NormArg a, const RowScale* scales) {
     vf4 acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = vf4{0.0f, 0.0f, 0.0f, 0.0f};
     const int c0 = 4096 * blockIdx.x + 4 * threadIdx.x;
     for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         const int64_t at = r * a.dim;
-        const vf2 s = scales[r];
+        const float mean = scales[r].mean;
+        const Scale scale(scales[r].q, scales[r].e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = c0 + 1024 * i;
             if (c >= a.dim) continue;
-            const vf4 d = load_quad(a.g + at, c, a.dim), u = load_quad(a.x + at, c, a.dim) * s.x;
+            const vf4 d = load_quad(a.g + at, c, a.dim), u = scale.of(load_quad(a.x + at, c, a.dim));
             acc[i] += d * u;
             if (a.gx) {
-                vf4 o = row_grad(d * load_quad(a.w, c, a.dim), u, s.x, s.y);
+                vf4 o = row_grad(d * load_quad(a.w, c, a.dim), u, scale, mean);
                 if (a.gsum) o = o + load_quad(a.gsum + at, c, a.dim);
                 if (a.accumulate) o = o + load_quad(a.gx + at, c, a.dim);
                 store_quad(a.gx + at, c, a.dim, o);
@@ -299,18 +315,21 @@ __global__ __launch_bounds__(256) void k_norm_grad_w(const float* part, int32_t 
                                                      int accumulate) {
     __shared__ float buf[256];
     const int col = threadIdx.x & 31, share = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + col;
-    float s = 0.0f;
-    if (c < dim) {
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < dim; c0 += (int64_t)gridDim.x * 32) {
+        const int64_t c = c0 + col;
+        float s = 0.0f;
+        if (c < dim) {
 #pragma unroll 8
-        for (int b = share; b < blocks; b += 8) s += part[(int64_t)b * dim + c];
-    }
-    buf[threadIdx.x] = s;
-    __syncthreads();
-    if (share != 0 || c >= dim) return;
+            for (int b = share; b < blocks; b += 8) s += part[(int64_t)b * dim + c];
+        }
+        __syncthreads();
+        buf[threadIdx.x] = s;
+        __syncthreads();
+        if (share != 0 || c >= dim) continue;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += buf[32 * i + col];
-    grad_w[c] = accumulate ? grad_w[c] + s : s;
+        for (int i = 1; i < 8; ++i) s += buf[32 * i + col];
+        grad_w[c] = accumulate ? grad_w[c] + s : s;
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -412,11 +431,11 @@ int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const f
     const int64_t most = lng ? 64 : dim > 4096 ? 256 : dim > 1024 ? 512 : 1024;
     if (blocks > most) blocks = most;
     float* base = nullptr;
-    const size_t part = grad_w ? (size_t)blocks * dim * 4 : 0, scales = lng ? (size_t)rows * 8 : 0;
+    const size_t part = grad_w ? (size_t)blocks * dim * 4 : 0, scales = lng ? (size_t)rows * sizeof(RowScale) : 0;
     if (part + scales) MH_TRY(scratch(scales + part, reinterpret_cast<void**>(&base)));
     if (grad_w) a.part = base + scales / 4;
     if (lng) {
-        vf2* sc = reinterpret_cast<vf2*>(base);
+        RowScale* sc = reinterpret_cast<RowScale*>(base);
         hipLaunchKernelGGL(k_norm_scales_long, dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, a, sc);
         hipLaunchKernelGGL(k_norm_bwd_long, dim3((unsigned)((dim + 4095) / 4096), (unsigned)blocks), dim3(256), 0, st, a, sc);
     } else {
@@ -424,9 +443,11 @@ int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const f
         MH_NORM(MH_CALL);
 #undef MH_CALL
     }
-    if (grad_w)
-        hipLaunchKernelGGL(k_norm_grad_w, dim3((unsigned)((dim + 31) / 32)), dim3(256), 0, st, a.part, (int32_t)blocks, a.dim, grad_w,
-                           a.accumulate);
+    if (grad_w) {
+        const int64_t cols = (dim + 31) / 32, fit = max_grid_blocks(256);
+        hipLaunchKernelGGL(k_norm_grad_w, dim3((unsigned)(cols < fit ? cols : fit)), dim3(256), 0, st, a.part, (int32_t)blocks, a.dim,
+                           grad_w, a.accumulate);
+    }
     return finish("mh_rms_norm_bwd");
 }
 

@@ -154,6 +154,21 @@ def test_sizes_of_elements(size, std):
     check(got, want, bound, str(std))
 
 
+@pytest.mark.parametrize("size", [(20, 40), (5, 3000), (2, 9000), (3, 20000)], ids=str)
+def test_scales_past_the_range(size):
+    """1 / sqrt(mean h^2) above the largest float, and below the least normal one."""
+    r = np.random.RandomState(18)
+    d = inputs(size, seed=18, std=1e-41)
+    d["g"] = (1e-12 * d["g"]).astype(np.float32)
+    d["gsum"][:] = 0
+    large = dict(d, x=np.where(r.uniform(size=size) < 0.5, -3.3e38, 3.3e38).astype(np.float32), g=inputs(size, seed=19)["g"])
+    large["res"] = np.zeros(size, np.float32)
+    for what, e in (("small", d), ("large", large)):
+        got = run(m_(), e, eps=0.0)
+        want, bound = reference(e["x"] + e["res"], e["w"], 0.0, e["g"], e["gsum"])
+        check(got, want, bound, what)
+
+
 def test_rows_of_zeros_and_of_no_numbers():
     m = m_()
     for size in ((6, 50), (6, 1000), (6, 3000), (6, 20000)):
