@@ -231,6 +231,21 @@ def test_padding_rows_are_left_alone():
     assert (none["chosen"] == -1).all() and (none["counts"] == 0).all() and (none["grad_x"] == 0).all()
 
 
+@pytest.mark.parametrize("experts,k,groups,opened", [(30, 2, 5, 2), (60, 12, 1, 1), (250, 8, 5, 3)])
+def test_padding_rows_of_no_choice(experts, k, groups, opened):
+    """Many rows, of which padding ones hold ties, nothing or no numbers, up to the last."""
+    rows = 3000
+    d = inputs(rows, experts, k, seed=51)
+    d["keep"][-40:] = 0
+    shut = np.flatnonzero(d["keep"] == 0)
+    clean = d["x"].copy()
+    for i, v in enumerate((0.0, -np.inf, np.nan, np.inf)):
+        d["x"][shut[i::4]] = v
+    got = run(m_(), d["x"], k, d["bias"], d["keep"], groups, opened)
+    want, bound, whole = reference(clean, k, d["bias"], d["keep"], groups, opened)
+    check(got, want, bound, whole)
+
+
 def test_choices_past_the_experts_count_as_none():
     m = m_()
     d = inputs(5, 12, 3, seed=11)
