@@ -4,22 +4,30 @@
 // class, the cut. The token is the first class, by index, where the running sum of the kept masses e^((x - max) / T) exceeds u
 // of their sum.
 //
-// A workgroup takes a row (64 threads of a short one where there are many, up to 1024), a wavefront a run of its classes, of which each lane holds 4 Q logits in registers (the whole
-// row up to 4 Q T classes; of a longer one the rest is read as it is needed):
+// A workgroup takes a row (64 threads of a short one where there are many, up to 1024), a wavefront a run of its classes,
+// of which each lane holds 4 Q logits in registers (the whole row up to 4 Q T classes; of a longer one the rest is read
+// as it is needed):
 //   1. the largest logit held, the reference, and bins of a power-of-two width, T / 112 or 1 / 112 at least, around it;
 //   2. for top-k and top-p how many classes each bin has and their mass, both in one 64-bit LDS atomic: 20 bits of count above
 //      44 of mass, a class 24 bits of its bin's largest. Whole numbers: the atomics' order does not show. A scan of the bins
 //      then says in which of them a cut falls;
 //   3. a second walk, over the quads that reach those bins, adds up what lies above them and lists what lies in them. More
 //      listed than there is room: from 2. on with narrower bins in the place of those;
-//   4. the list is sorted, and the cuts are found in it by 64-bit sums;
+//   4. the list is sorted, up to 512 keys by counting what comes before each (128 keys by the 28 steps of a sorting network,
+//      each waiting for the last, take 11700 cycles; [33, 30011] takes 26.7 us instead of 29.9), and the cuts are found in
+//      it by 64-bit sums;
 //   5. the run of classes where the running sum passes u of the total is walked by the whole workgroup.
 // Sums of steps 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
 // sign, moves a border by some 2^-24 of the row.
 //
-// Rows for which bins do not work (more than 256 to 2048 classes of one value at a cut, a cut 32 T below the largest, an infinite
-// logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over the logits'
-// bits, 8 at a time: right for every row, and slower.
+// Rows for which bins do not work (more than 256 to 2048 classes of one value at a cut, a cut 32 T below the largest, an
+// infinite logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over
+// the logits' bits, 8 at a time: right for every row, and slower.
+//
+// The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 124 us, where reading takes 41: two
+// workgroups a CU, and of a row at a temperature of 1 or more, whose cut lies in the bulk, 80 thousand cycles of 280 are the
+// counting (one LDS atomic and 20 instructions a class) and 83 the second walk (20 instructions a class). A single row of
+// 32000 takes 20 us: 47 thousand cycles of short phases, a fetch or a barrier each.
 #include "mh_internal.h"
 #include "mh_rows.h"
 
@@ -34,6 +42,7 @@ struct Sizes {
     static constexpr float kWidth = 1.0f / (T >= 512 ? 112 : T / 5);  // of T, at least
 };
 constexpr int kCountAt = 44;
+constexpr int kRanked = 512;  // the longest list that is sorted by ranks
 constexpr int64_t kMaxBinned = (int64_t)1 << 19;
 constexpr int64_t kMaxSampled = (int64_t)1 << 24;
 
@@ -721,23 +730,40 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
             __syncthreads();
             continue;
         }
-        int n2 = 2;
-        while (n2 < n_list) n2 *= 2;
-        for (int i = n_list + tid; i < n2; i += T) s.list.key[i] = ~(uint64_t)0;
-        __syncthreads();
-        for (int size = 2; size <= n2; size *= 2)
-            for (int step = size / 2; step > 0; step /= 2) {
-                for (int i = tid; i < n2 / 2; i += T) {
-                    const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                    const bool up = (lo & size) == 0;
-                    const uint64_t p = s.list.key[lo], q = s.list.key[hi];
-                    if ((p > q) == up) {
-                        s.list.key[lo] = q;
-                        s.list.key[hi] = p;
-                    }
-                }
-                __syncthreads();
+        if (n_list <= kRanked) {
+            // each key's place is how many come before it: no step waits for another
+            const int n8 = (n_list + 7) & ~7;
+            for (int i = n_list + tid; i < n8; i += T) s.list.key[i] = ~(uint64_t)0;
+            __syncthreads();
+            for (int i = tid; i < n_list; i += T) {
+                const uint64_t k = s.list.key[i];
+                int at = 0;
+#pragma unroll 8
+                for (int o = 0; o < n8; ++o) at += s.list.key[o] < k;
+                s.list.upto[at] = __longlong_as_double((long long)k);
             }
+            __syncthreads();
+            for (int i = tid; i < n_list; i += T) s.list.key[i] = (uint64_t)__double_as_longlong(s.list.upto[i]);
+            __syncthreads();
+        } else {
+            int n2 = 2;
+            while (n2 < n_list) n2 *= 2;
+            for (int i = n_list + tid; i < n2; i += T) s.list.key[i] = ~(uint64_t)0;
+            __syncthreads();
+            for (int size = 2; size <= n2; size *= 2)
+                for (int step = size / 2; step > 0; step /= 2) {
+                    for (int i = tid; i < n2 / 2; i += T) {
+                        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                        const bool up = (lo & size) == 0;
+                        const uint64_t p = s.list.key[lo], q = s.list.key[hi];
+                        if ((p > q) == up) {
+                            s.list.key[lo] = q;
+                            s.list.key[hi] = p;
+                        }
+                    }
+                    __syncthreads();
+                }
+        }
         // their masses' running sums
         const int per = (n_list + T - 1) / T, i0 = tid * per, i1 = i0 + per < n_list ? i0 + per : n_list;
         auto in_bins = [&](int i) {  // as the bins have it
