@@ -27,7 +27,9 @@
 // The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 124 us, where reading takes 41: two
 // workgroups a CU, and of a row at a temperature of 1 or more, whose cut lies in the bulk, 80 thousand cycles of 280 are the
 // counting (one LDS atomic and 20 instructions a class) and 83 the second walk (20 instructions a class). A single row of
-// 32000 takes 20 us: 47 thousand cycles of short phases, a fetch or a barrier each.
+// 32000 takes 18 us: 42 thousand cycles, of which 13 count and 5 walk again, and the rest are short phases that each wait
+// for a fetch, a barrier or 64-bit exponentials. Of Q 4 was taken (8 of 512 threads): 16 hold more of a row, and cost the
+// short phases registers and code: [33, 30011] 26.8 us with 16, 24.8 with 4; [512, 131072] with 512 threads 124 with 8, 128 with 4.
 #include "mh_internal.h"
 #include "mh_rows.h"
 
@@ -415,7 +417,7 @@ struct Mass {
 };
 
 template <int T, int Q>
-__global__ __launch_bounds__(T) void k_sample(SampleArg a) {
+__global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
     constexpr int W = T / 64;
     constexpr int kBins = Sizes<T>::kBins, kAbove = Sizes<T>::kAbove, kList = Sizes<T>::kList;
     constexpr int B = kBins / T;  // bins of a thread
@@ -523,18 +525,16 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     float ref = best;
     // masses are e^((x - ref) / T) until the largest is known
     bool binned = cuts && tops && ref > -__builtin_inff() && ref < __builtin_inff() && T_ >= 0.01f && T_ <= 1e30f;
-    // the bins: place_of counts widths below ref and `start`, and bin b holds the places from b - off on
-    int off = kAbove;
-    float per_bin, start = 0.0f;
+    // the bins: bin b holds what lies from b + start widths below ref on, a whole number of them. Every step there is exact
+    // near the bins, so that narrower ones divide those before them, also where they begin above ref.
+    float per_bin, start = -(float)kAbove;
     double width;
     {
         const int e = __builtin_amdgcn_frexp_expf(__builtin_fmaxf(T_, 1.0f) * Sizes<T>::kWidth);
         per_bin = __builtin_ldexpf(1.0f, -e);
         width = __builtin_ldexp(1.0, e);
     }
-    auto place_of = [&](float v) {  // exact near the bins, so that narrower ones divide those before them
-        return __builtin_fminf(__builtin_fmaf(ref - v, per_bin, -start), 1e6f);
-    };
+    auto bin_at = [&](float below) { return (int)__builtin_fminf(below - start, 1e6f); };  // of whole widths below ref
     uint32_t base_n = 0;  // what lies above the bins
     double base_m = 0.0, all_m = 0.0;
     auto clear = [&]() {
@@ -549,9 +549,9 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         const float neg = -(float)(width / ask.T * 1.4426950408889634074);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float q = place_of(v[j]);
+            const float q = (ref - v[j]) * per_bin;
             const float f = __builtin_floorf(q);
-            const int b = (int)f + off;
+            const int b = bin_at(f);
             uint32_t m = 0;
             if (ask.p < 1.0f) m = (uint32_t)__builtin_fmaf(__builtin_amdgcn_exp2f((q - f) * neg), 16777216.0f, 0.5f);
             if ((uint32_t)b < (uint32_t)kBins) atomicAdd(&s.hist[b], (unsigned long long)1 << kCountAt | m);
@@ -601,16 +601,18 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
     for (int turn = 0; !slow && cuts; ++turn) {
         // the bins' counts and masses, from the top down: each thread's B, then all before it
         const double rate = width / ask.T;
-        auto bin_mass = [&](uint64_t v, int b) {
-            return (double)(v & (((uint64_t)1 << kCountAt) - 1)) * exp64(-rate * ((double)start + (double)(b - off))) * (1.0 / 16777216.0);
-        };
+        // of a count of 1 at the top of the thread's first bin the mass, and what the next bin has of it
+        double unit = 0.0, fall = 0.0;
+        auto bin_mass = [&](uint64_t v, double e) { return v ? (double)(v & (((uint64_t)1 << kCountAt) - 1)) * e : 0.0; };
         uint32_t n = 0;
-        double m = 0.0;
+        double m = 0.0, each_m;
+#pragma unroll
+        for (int b = 0; b < B; ++b) n += (uint32_t)(s.hist[tid * B + b] >> kCountAt);
+        if (n) {
+            each_m = unit = exp64(-rate * ((double)start + (double)(tid * B))) * (1.0 / 16777216.0);
+            fall = exp64(-rate);
 #pragma nounroll
-        for (int b = tid * B; b < tid * B + B; ++b) {
-            const uint64_t v = s.hist[b];
-            n += (uint32_t)(v >> kCountAt);
-            if (v) m += bin_mass(v, b);
+            for (int b = tid * B; b < tid * B + B; ++b, each_m *= fall) m += bin_mass(s.hist[b], each_m);
         }
         uint32_t n0, n_bins;
         double m0, m1, m_bins;
@@ -621,11 +623,12 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         if (ask.k > 0 && n0 < (uint32_t)ask.k && n0 + n >= (uint32_t)ask.k) {
             uint32_t cn = n0;
             double cm = m0;
+            each_m = unit;
 #pragma nounroll
-            for (int b = tid * B; b < tid * B + B; ++b) {
+            for (int b = tid * B; b < tid * B + B; ++b, each_m *= fall) {
                 const uint64_t v = s.hist[b];
                 const uint32_t here = (uint32_t)(v >> kCountAt);
-                const double in = v ? bin_mass(v, b) : 0.0;
+                const double in = bin_mass(v, each_m);
                 if (cn + here >= (uint32_t)ask.k) {
                     s.k_bin = b;
                     s.k_above_n = cn;
@@ -647,10 +650,11 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
             if ((m0 < lo && m1 >= lo) || (m0 < hi && m1 >= hi)) {
                 uint32_t cn = n0;
                 double cm = m0;
+                each_m = unit;
 #pragma nounroll
-                for (int b = tid * B; b < tid * B + B; ++b) {
+                for (int b = tid * B; b < tid * B + B; ++b, each_m *= fall) {
                     const uint64_t v = s.hist[b];
-                    const double to = b + 1 < tid * B + B ? cm + (v ? bin_mass(v, b) : 0.0) : m1;
+                    const double to = b + 1 < tid * B + B ? cm + bin_mass(v, each_m) : m1;
                     if (cm < lo && to >= lo) {
                         s.p_lo = b;
                         s.p_above = base_m + cm;
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
         slow = p_lo > p_hi || most >= kBins || (ask.k > 0 && k_bin == kBins);
         if (slow) break;
         // what lies in the bins of a cut is listed, what lies above is added up, a run each
-        auto bin_of = [&](float v) { return (int)__builtin_floorf(place_of(v)) + off; };
+        auto bin_of = [&](float v) { return bin_at(__builtin_floorf((ref - v) * per_bin)); };
         const float v_list = least_of([&](float v) { return bin_of(v) <= most; });
         const float v_keep = least_of([&](float v) { return bin_of(v) < p_lo; });
         // no mass below e^-100 of the largest's; what min_p drops has none
@@ -719,8 +723,7 @@ __global__ __launch_bounds__(T) void k_sample(SampleArg a) {
                 base_n = s.k_above_n;
                 base_m = s.k_above;
             }
-            start = __builtin_ldexpf(start + (float)(p_lo - off), -e);
-            off = 0;
+            start = __builtin_ldexpf(start + (float)p_lo, -e);
             width = __builtin_ldexp(width, e);
             per_bin = __builtin_ldexpf(per_bin, -e);
             __syncthreads();
@@ -915,22 +918,22 @@ void launch_sample(SampleArg a, int64_t rows) {
     }
 }
 
-// Threads a row: a CU holds 16, 4, 2 or 1 workgroups, and a row takes one so many microseconds and so many more for 1000
-// classes. [4096, 2000], settings of all kinds: 40, 62, 110 and 231 us with 64, 256, 512 and 1024 threads; [1024, 4000]: 40, 27,
-// 40, 68; [512, 16000]: 37, 32, 45 with 256 to 1024; [64, 4000]: 31, 18, 17, 19.
+// Threads a row, by the microseconds of a row alone and of each row more that a CU has to take, with c thousand classes,
+// as measured with settings of all kinds. [4096, 500]: 21, 45, 105, 190 us with 64 to 1024 threads; [1024, 8000]: 76, 31, 42,
+// 61; [512, 32000]: 57, 43, 50 with 256 to 1024; [1, 32000]: 28, 18, 16.
 int sample_threads(int64_t rows, int64_t classes) {
     struct Form {
-        int threads, held;
-        double base, more;
+        int threads;
+        double alone, alone_c, more, more_c;
         int64_t most;
     };
-    const Form forms[] = {{64, 16, 15.0, 5.0, Sizes<64>::kTops}, {256, 4, 15.0, 1.05, Sizes<256>::kTops}, {512, 2, 16.0, 0.55, kMaxSampled},
-                          {1024, 1, 18.0, 0.4, kMaxSampled}};
+    const Form forms[] = {{64, 10.0, 6.6, 0.63, 0.27, Sizes<64>::kTops}, {256, 13.0, 1.1, 2.2, 0.21, Sizes<256>::kTops},
+                          {512, 14.8, 0.5, 5.9, 0.21, kMaxSampled}, {1024, 15.4, 0.42, 11.2, 0.25, kMaxSampled}};
+    const double c = 1e-3 * (double)classes, others = rows > 256 ? (double)rows / 256 - 1 : 0.0;
     int best = 1024;
     double least = 1e300;
     for (const Form& f : forms) {
-        const double rounds = (double)((rows + 256 * f.held - 1) / (256 * f.held));
-        const double cost = rounds * (f.base + f.more * 1e-3 * (double)classes);
+        const double cost = f.alone + f.alone_c * c + others * (f.more + f.more_c * c);
         if (classes <= f.most && cost < least) {
             least = cost;
             best = f.threads;
@@ -968,10 +971,10 @@ int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const floa
     a.shift = 62;
     while (((int64_t)1 << (62 - a.shift)) < classes) --a.shift;
     switch (sample_threads(rows, classes)) {
-        case 64: launch_sample<64, 16>(a, rows); break;
-        case 256: launch_sample<256, 16>(a, rows); break;
-        case 512: launch_sample<512, 16>(a, rows); break;
-        default: launch_sample<1024, 16>(a, rows);
+        case 64: launch_sample<64, 4>(a, rows); break;
+        case 256: launch_sample<256, 4>(a, rows); break;
+        case 512: launch_sample<512, 8>(a, rows); break;
+        default: launch_sample<1024, 4>(a, rows);
     }
     return finish("mh_sample_tokens");
 }

@@ -159,6 +159,37 @@ def test_a_logit_far_above_those_before_it(rows, classes):
         check(m, x, u, T=3.0, p=0.5, unsure=rows / 20 + 1, what=f"+{above}, warm")
 
 
+@pytest.mark.parametrize("rows", [3, 300])
+def test_largest_logits_last(rows):
+    """Classes by rising logits, close together: the largest lie behind all that is looked at first, and bins begin among them."""
+    m = m_()
+    r = np.random.RandomState(31)
+    x = np.sort(1e-5 * r.standard_normal((rows, 120001)).astype(np.float32), axis=1)
+    x[3:] = -np.inf
+    x[3:, 7] = 1.0
+    u = r.uniform(size=rows).astype(np.float32)
+    for a in ({"k": 50000, "p": 0.4}, {"p": 0.02}, {"k": 900, "p": 0.6}, {"k": 70001}, {"p": 0.7, "T": 0.02}):
+        check(m, x, u, **a, unsure=3, what=str(a))
+
+
+def test_many_logits_at_the_edge_of_a_bin():
+    """Thousands within 2^-24 of a bin's edge, and more above the first look's largest: which bin is theirs may not turn on
+    how far from the edge the bins begin."""
+    m = m_()
+    r = np.random.RandomState(32)
+    n = 120001
+    # top_p ends among some 50000, top_k among as many behind them
+    x = (-2.0 ** -15 - 7e-6 * r.uniform(size=(2, n)) - np.where(r.uniform(size=(2, n)) < 0.5, 1.6e-5, 0.0)).astype(np.float32)
+    for row in x:
+        some = r.permutation(n)[:6000]
+        row[some] = (-2.0 ** -15 * (1 - np.arange(1, 6001) * 2.0 ** -24)).astype(np.float32)
+        row[0] = 0.0
+        for at in range(5000, n, 7680):
+            row[at:at + 100] = (1e-6 * r.uniform(1, 2, 100)).astype(np.float32)
+    for u in (0.2, 0.55, 0.91):
+        check(m, x, np.float32([u, u + 0.03]), k=90000, p=0.3, unsure=2, what=str(u))
+
+
 @pytest.mark.parametrize("std", [1e-5, 0.01, 0.2])
 def test_logits_close_together(std):
     """Thousands of classes in a bin: narrower ones, or where they are too close for any, the search over their bits."""
