@@ -512,6 +512,13 @@ def _matrix(name: str, t):
     return t._shape._dims
 
 
+def _last_axis(t: Tensor):
+    """The shape of t, its rows and their length."""
+    shape = t._shape._dims
+    dim = shape[-1] if shape else 1
+    return shape, t._shape._n // dim if dim else 0, dim
+
+
 def linear_cross_entropy_forward(loss: Tensor, row_lse: Optional[Tensor], x: Tensor, w: Tensor, labels: IndexTensor,
                                  row_loss: Optional[Tensor] = None) -> None:
     """Softmax cross entropy of a vocabulary head, CrossEntropyLoss (loss.mojo:45-61) of the logits
@@ -659,10 +666,9 @@ def rms_norm_forward(out: Tensor, x: Tensor, w: Tensor, residual: Optional[Tenso
     """Root-mean-square norm over the last axis, with the residual's addition: h = x + residual (without one h = x),
     out = h / sqrt(mean h^2 + eps) * w, and sum = h where it is given, which the backward takes. w has the last axis' length.
     sum may be x or residual, and out may be x."""
-    _row_operands(x, same=[("out", out), *((n, t) for n, t in (("residual", residual), ("sum", sum)) if t is not None)])
-    rows, dim = _rows_classes(x)
-    _lib.call("mh_rms_norm_fwd", out.f32, None if sum is None else sum.f32, x.f32, None if residual is None else residual.f32,
-              _want("w", w, (dim,)), rows, dim, float(eps))
+    shape, rows, dim = _last_axis(x)
+    _lib.call("mh_rms_norm_fwd", _want("out", out, shape), _want("sum", sum, shape, optional=True), _want("x", x, shape),
+              _want("residual", residual, shape, optional=True), _want("w", w, (dim,)), rows, dim, float(eps))
 
 
 def rms_norm_backward(grad_x: Optional[Tensor], grad_w: Optional[Tensor], grad_out: Tensor, h: Tensor, w: Tensor,
@@ -670,11 +676,10 @@ def rms_norm_backward(grad_x: Optional[Tensor], grad_w: Optional[Tensor], grad_o
     """grad_x and grad_w += (accumulate=False: =) the gradients of rms_norm_forward from grad_out and grad_sum, those of its
     out and sum; h is its sum, or x where it had no residual. grad_x is the residual's gradient too. Either may be None;
     grad_x may be grad_sum or grad_out."""
-    _row_operands(h, same=[("grad_out", grad_out), *((n, t) for n, t in (("grad_x", grad_x), ("grad_sum", grad_sum)) if t is not None)])
-    rows, dim = _rows_classes(h)
-    _lib.call("mh_rms_norm_bwd", None if grad_x is None else grad_x.f32, _want("grad_w", grad_w, (dim,), optional=True),
-              grad_out.f32, None if grad_sum is None else grad_sum.f32, h.f32, _want("w", w, (dim,)), rows, dim, float(eps),
-              int(bool(accumulate)))
+    shape, rows, dim = _last_axis(h)
+    _lib.call("mh_rms_norm_bwd", _want("grad_x", grad_x, shape, optional=True), _want("grad_w", grad_w, (dim,), optional=True),
+              _want("grad_out", grad_out, shape), _want("grad_sum", grad_sum, shape, optional=True), _want("h", h, shape),
+              _want("w", w, (dim,)), rows, dim, float(eps), int(bool(accumulate)))
 
 
 def sample_tokens(tokens: IndexTensor, x: Tensor, u: Tensor, temperature: Optional[Tensor] = None,

@@ -127,7 +127,7 @@ def test_shapes_and_kinds(tensor):
     refused(S, m.rms_norm_forward, *norm, residual=F(4))
     refused(I, m.rms_norm_forward, *norm, sum=X(3, 4))
     back = [F(3, 4), F(4), F(3, 4), F(3, 4), F(4)]
-    for at, t, code in [(0, F(3, 5), S), (1, F(3, 4), S), (1, X(4), I), (2, None, S), (2, F(4), S), (3, X(3, 4), I), (4, F(3), S)]:
+    for at, t, code in [(0, F(3, 5), S), (1, F(3, 4), S), (1, X(4), I), (2, None, I), (2, F(4), S), (3, X(3, 4), I), (4, F(3), S)]:
         refused(code, m.rms_norm_backward, *[t if i == at else a for i, a in enumerate(back)])
     refused(S, m.rms_norm_backward, *back, grad_sum=F(3))
     rf = [F(6, 2), X(6, 2), X(8), F(6, 8)]
