@@ -47,6 +47,7 @@ struct GroupArg {
     int32_t experts, k;
     int32_t groups, each, open, best;  // each: experts of a group
     int32_t parts;                     // lanes that share a group, a power of two
+    int32_t wave_parts;                // the same of a wavefront
     int32_t sigmoid, normalise, accumulate;
     float scale;
     FastDiv by_each;
@@ -154,15 +155,17 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
                                              double& by) {
     const int lane = threadIdx.x & 63;
     double b[C];
+    float plus[C];  // the bias, on its way with the logits
     top = -__builtin_inff();
     by = 0.0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const int e = 64 * i + lane;
-        const float v = e < a.experts ? x[e] : -__builtin_inff();
-        top = __builtin_fmaxf(top, v);
-        b[i] = (double)v;
+        b[i] = (double)(e < a.experts ? x[e] : -__builtin_inff());
+        plus[i] = a.bias && e < a.experts ? a.bias[e] : 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < C; ++i) top = __builtin_fmaxf(top, (float)b[i]);
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < C; ++i) b[i] = sigmoid64((float)b[i]);
@@ -184,7 +187,7 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const int e = 64 * i + lane;
-        if (a.bias && e < a.experts) b[i] += (double)a.bias[e];
+        if (a.bias) b[i] += (double)plus[i];
         key[i] = e < a.experts ? sort_key64(b[i]) : kNever;
     }
     if (a.groups > 1) {
@@ -192,21 +195,29 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
 #pragma unroll
         for (int i = 0; i < C; ++i) row[64 * i + lane] = b[i];
         wave_sync();
-        if (lane < a.groups) {
-            const double* v = row + lane * a.each;
-            double first = -__builtin_inf(), second = first;
-            int numbers = 0;  // a NaN comes behind them
-#pragma unroll 8
-            for (int e = 0; e < a.each; ++e) {
-                const double c = v[e];
+        // the wavefront's lanes in as many parts of a group as there are lanes for
+        const int parts = a.wave_parts, part = lane & (parts - 1), j = lane >> __builtin_ctz(parts);
+        double first = -__builtin_inf(), second = first;
+        int numbers = 0;  // a NaN comes behind them
+        if (j < a.groups) {
+            const double* v = row + j * a.each;
+#pragma unroll 4
+            for (int e = part; e < a.each; e += parts) {
+                const double c = v[e], d = c == c ? c : -__builtin_inf();
                 numbers += c == c;
-                second = max_d(second, min_d(first, c == c ? c : -__builtin_inf()));
-                first = max_d(first, c == c ? c : -__builtin_inf());
+                second = max_d(second, min_d(first, d));
+                first = max_d(first, d);
             }
-            if (numbers < 2) second = __builtin_nan("");
-            if (numbers < 1) first = second;
-            score[lane] = a.best == 2 && a.each > 1 ? first + second : first;
         }
+        for (int o = 1; o < parts; o *= 2) {
+            const double f = __shfl_xor(first, o), t = __shfl_xor(second, o);
+            second = max_d(min_d(first, f), max_d(second, t));
+            first = max_d(first, f);
+            numbers += __shfl_xor(numbers, o);
+        }
+        if (numbers < 2) second = __builtin_nan("");
+        if (numbers < 1) first = second;
+        if (part == 0 && j < a.groups) score[j] = a.best == 2 && a.each > 1 ? first + second : first;
         wave_sync();
         bool open = false;
         if (lane < a.groups) {
@@ -221,15 +232,20 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
             if (!(mask >> (fdiv((uint32_t)(64 * i + lane), a.by_each) & 63) & 1)) key[i] = kNever;
     }
     for (int t = 0; t < a.k; ++t) {
-        int64_t best = key[0];
+        int64_t own = key[0];
+        int in = 0;  // the lane's place of it, the first
 #pragma unroll
-        for (int i = 1; i < C; ++i) best = best > key[i] ? best : key[i];
-        best = wave_largest(best);
-        int at = 0;  // the lowest index that holds it
-#pragma unroll
-        for (int i = C - 1; i >= 0; --i) {
-            const uint64_t has = __ballot(key[i] == best);
-            at = has ? 64 * i + __builtin_ctzll(has) : at;
+        for (int i = 1; i < C; ++i) {
+            in = key[i] > own ? i : in;
+            own = key[i] > own ? key[i] : own;
+        }
+        const uint64_t has = __ballot(own == wave_largest(own));
+        int at = __builtin_ctzll(has);
+        at += 64 * __builtin_amdgcn_readlane(in, at);
+        if (has & (has - 1)) {  // ties: the lowest index is that of the lowest place
+            at = has >> lane & 1 ? 64 * in + lane : C * 64;
+            at = group_red<64>(at, [](int p, int q) { return p < q ? p : q; });
+            at = __builtin_amdgcn_readfirstlane(at);
         }
 #pragma unroll
         for (int i = 0; i < C; ++i)
@@ -727,6 +743,8 @@ int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const 
     const bool lists = rows > kRExactRows;
     a.parts = 1;
     while (2 * a.parts * a.groups <= router_lanes(a.experts)) a.parts *= 2;
+    a.wave_parts = 1;
+    while (2 * a.wave_parts * a.groups <= 64) a.wave_parts *= 2;
     int64_t blocks = lists ? (rows + group - 1) / group : 0;
     if (blocks > kRBlocks) blocks = (blocks + (blocks + kRBlocks - 1) / kRBlocks - 1) / ((blocks + kRBlocks - 1) / kRBlocks);  // equal rounds
     int64_t exact = lists ? kRExactBlocks : (rows + waves - 1) / waves;
