@@ -16,7 +16,7 @@
 //
 // L lanes hold a row in registers, V elements a lane in quads (element 4 (i L + lane) + c). Over [131072, 256], top 8 of 4 of
 // 8 groups, the forward takes 91 us, where its read alone takes 24: 1200 vector instructions for a wavefront's 4 rows
-// (scores, the groups' best, the sorted list, the check) fill three quarters of it. The listed rows take 13 us more, each k
+// (scores, the groups' best, the sorted list, the check) fill three quarters of it. The listed rows take 11 us more, each k
 // reductions that wait for each other, the counts 6, and the backward, which writes 134 MB and gathers the chosen's logits, 46.
 #include "mh_internal.h"
 #include "mh_lanes.h"
@@ -36,7 +36,7 @@ constexpr int64_t kRExactBlocks = 512;
 // Workgroups that add up their counts by themselves: over 16 experts 64 rows 10.7 us instead of 13.6, 500 rows (125) 13.0; over 256
 // experts 128 rows 19.9 and 19.4, 500 rows 23.7 and 20.0.
 constexpr int64_t kRArrivals = 32;
-// Batches of up to this many rows go by wavefronts alone: over 256 experts 2048 rows take 18 us, 2049 by lists first 24.5.
+// Batches of up to this many rows go by wavefronts alone: over 256 experts 2048 rows take 17 us, 2049 by lists first 25.
 constexpr int64_t kRExactRows = 2048;
 
 struct GroupArg {

@@ -24,7 +24,7 @@
 // infinite logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over
 // the logits' bits, 8 at a time: right for every row, and slower.
 //
-// The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 124 us, where reading takes 41: two
+// The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 125 us, where reading takes 41: two
 // workgroups a CU, and of a row at a temperature of 1 or more, whose cut lies in the bulk, 80 thousand cycles of 280 are the
 // counting (one LDS atomic and 20 instructions a class) and 83 the second walk (20 instructions a class). A single row of
 // 32000 takes 18 us: 42 thousand cycles, of which 13 count and 5 walk again, and the rest are short phases that each wait
