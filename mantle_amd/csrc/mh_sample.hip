@@ -589,7 +589,9 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
     }
     const Mass mass(best, ask);
     bool slow = (cuts && !binned) || best == __builtin_inff() || !(T_ >= 1e-30f && T_ <= 1e30f);
-    if (!slow && cuts && (best - ref) * per_bin >= (float)kAbove) {  // one of the others lies above the bins
+    // one of the others lies above the bins, or so far above ref that e^((best - ref) / T) is near a double's largest: at T =
+    // 0.01 the bins reach 800 T above it, and exp64 700, of which a thread's first bin may take 87
+    if (!slow && cuts && ((best - ref) * per_bin >= (float)kAbove || best - ref > 600.0f * T_)) {
         __syncthreads();
         clear();
         __syncthreads();
