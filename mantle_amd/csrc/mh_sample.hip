@@ -348,7 +348,7 @@ struct FastLds : Sums {
     // what one thread found out for all
     uint32_t listed, k_bin, k_above_n, k_here, p_lo, p_hi, p_above_n;
     double k_above, k_in, p_above;
-    int bad, first;
+    int bad, first, token;
 };
 
 // Exclusive sums over the workgroup's threads of a count and a mass, and the totals; m1 is the sum with the thread's own, the
@@ -832,22 +832,19 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
         slow_row<T>(x, a.classes, a.shift, a.tokens + r, a.logprob ? a.logprob + r : nullptr, best, ask, lds.s);
         return;
     }
-    // the run where the running sum passes u of the total, and in it the class
+    // The run where the running sum passes u of the total, and in it the class. Sums round, by the order that a scan adds them
+    // in: where one begins need not be where the one before it ends, and what passes the goal may hold nothing. So the last run with any
+    // mass that begins at the goal or before it is taken, of it the last such thread, and there is one of either.
     const double segs = row_scan(lane < W ? s.seg[lane & 15] : 0.0);
     const double total = lane_value(segs, W - 1), goal = (double)ask.u * total;
-    int seg;
-    double from = 0.0;
-    {
-        // the first whose sum passes the goal, or where rounding lets none the last with any mass
-        const uint64_t passed = __ballot(lane < W && segs > goal), some = __ballot(lane < W && s.seg[lane & 15] > 0.0);
-        seg = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
-        if (seg > 0) from = lane_value(segs, seg - 1);
-    }
+    const double ahead = moved<0x138, 0xf>(segs);
+    const int seg = 63 - __builtin_clzll(__ballot(lane < W && s.seg[lane & 15] > 0.0 && ahead <= goal));
+    double from = seg > 0 ? lane_value(segs, seg - 1) : 0.0;
     if (tid == 0) s.first = -1;
     // the run in parts, each thread its own neighbouring quads of a part
     constexpr int P = Q < 8 ? Q : 8;
     const int stop = (seg + 1) * run < a.classes ? (seg + 1) * run : a.classes;
-    for (int p0 = seg * run; p0 < stop; p0 += 4 * P * T) {
+    for (int p0 = seg * run, id = tid; p0 < stop; p0 += 4 * P * T, id += T) {
         const int each = (stop - p0 + 4 * T - 1) / (4 * T) < P ? (stop - p0 + 4 * T - 1) / (4 * T) : P;
         const int c = p0 + 4 * each * tid;
         vf4 v[P];
@@ -872,7 +869,10 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
         uint32_t unused0, unused1;
         double m0, m1, part;
         block_scan<W>(0, m, unused0, m0, m1, unused1, part, s);
-        if (m > 0.0 && from + m0 <= goal && goal < from + m1) {
+        const uint64_t begins = __ballot(m > 0.0 && from + m0 <= goal);
+        if (begins && lane == 63 - __builtin_clzll(begins)) atomicMax(&s.first, id);
+        __syncthreads();
+        if (s.first == id) {
             // the quad, the first that passes the goal or else the last with any mass, and in it the class
             double upto = from + m0, to = upto;
             int at = c;
@@ -894,18 +894,14 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
                 if (e > 0.0f && (found < 0 || upto + (double)sum <= goal)) found = at + j;
                 sum += e;
             }
-            s.first = found;
+            s.token = found;
         }
-        __syncthreads();
-        if (s.first >= 0) break;
         from += part;
+        if (goal < from) break;
     }
+    __syncthreads();
     if (tid == 0) {
-        int at = s.first;
-        if (at < 0) {  // a sum that rounding left short of the goal ends at the run's last
-            at = stop;
-            for (--at; at > 0 && (((uint64_t)(~order_of(x[at])) << 32 | (uint32_t)at) > cut || mass(x[at]) == 0.0f);) --at;
-        }
+        const int at = s.token;
         a.tokens[r] = at;
         if (a.logprob) a.logprob[r] = share_log(x[at], best, ask.T, total);
     }

@@ -9,10 +9,12 @@ pytestmark = pytest.mark.gpu
 
 
 def check(m, x, u, T=1.0, k=0, p=1.0, mp=0.0, rows=None, what=""):
-    """All rows in one call, of which those of `rows` are compared."""
+    """All rows in one call, of which those of `rows` are compared. A u of 0 lies at a border too, where the reference takes one side
+    alone: a first class of less than 2^-24 may be passed over. (Below 2^-126 of the largest a mass is 0 in 32 bits, and where whole
+    numbers stand for them below 2^-48 with 2^15 classes.) 2^-40 is off that border by less than any bound."""
     tok, lp = run(m, x, u, T, k, p, mp)
     for r in range(len(x)) if rows is None else rows:
-        may, _ = reference(x[r], u[r], T, k, p, mp)
+        may, _ = reference(x[r], max(u[r], np.float32(2.0 ** -40)), T, k, p, mp)
         assert tok[r] in may, f"{what} row {r}: {tok[r]} and not {may}"
         assert any(abs(lp[r] - v) <= off for v, off in may[tok[r]]), f"{what} row {r}: {lp[r]} and not {may[tok[r]]}"
 
@@ -35,3 +37,46 @@ def test_largest_logits_far_above_the_first_at_cold_temperatures(rows, classes, 
     for a in ({"p": 0.9}, {"p": 0.6}, {"k": 40, "p": 0.9}, {"k": 2, "p": 0.55}, {"k": 1}, {"k": 2}, {"p": 0.9, "mp": 0.5}):
         for v in {0.3, 0.7} if rows == 1 else {None}:
             check(m, x, u if v is None else np.float32([v]), T=T, **a, rows=range(min(rows, 24)), what=str(a))
+
+
+LOG2E = float(np.float32(1.4426950408889634))  # a temperature at which x of -n has a mass of 2^-n, but for 2^-26 n of it
+
+
+@pytest.mark.parametrize("classes, step", [(7000, 256), (32000, 256), (131072, 512)])
+def test_a_goal_where_sums_round_apart(classes, step):
+    """Masses of 1, 2^-53, 2^-53, a half and a half, `step` classes or a wavefront apart: the sum of the first three is 1 from the
+    left and 1 + 2^-52 from the right, and u = 1/2 of their total lies between. Far from it, behind it, is the last class."""
+    m = m_()
+    x = np.full((1, classes), -np.inf, np.float32)
+    x[0, 0], x[0, step], x[0, 2 * step] = 0, -53, -53
+    x[0, 3 * step] = x[0, 3 * step + 200] = -1
+    for a in ({}, {"mp": 2.0 ** -60}, {"k": 6}):
+        check(m, x, np.float32([0.5]), T=LOG2E, **a, what=str(a))
+
+
+@pytest.mark.parametrize("rows, classes", [(1, 900), (1, 7000), (1, 32000), (1, 131072), (300, 900), (720, 6000), (512, 32000), (2, 600001)])
+def test_masses_of_powers_of_two(rows, classes):
+    """A few classes of 1 to 2^-60 in a row of none, where a u of eighths meets the borders of their sums."""
+    m = m_()
+    r = np.random.RandomState(42)
+    for turn in range(20 if rows == 1 else 2):
+        x = np.full((rows, classes), -np.inf, np.float32)
+        for row in x:
+            some = np.unique(r.choice([1, 4, 64, 256, 512, 1024]) * r.randint(0, classes // 1024 + 1 if r.randint(2) else 1 + classes // 4, 12) % classes)
+            row[some] = -r.choice([0, 0, 1, 2, 52, 53, 54, 60], len(some))
+        x[0, 0] = 0
+        u = (r.randint(0, 9, rows) / 8).astype(np.float32)
+        for a in ({}, {"k": 900}, {"p": 0.75}):
+            check(m, x, u, T=LOG2E, **a, rows=range(min(rows, 30)), what=str(a))
+
+
+@pytest.mark.parametrize("classes", [900, 32000, 131072, 600001])
+def test_the_last_class_that_is_kept(classes):
+    """u just below 1 where nothing behind the first classes is kept."""
+    m = m_()
+    r = np.random.RandomState(43)
+    x = (0.1 * r.standard_normal((4, classes))).astype(np.float32)
+    x[:, :3] = [7.0, 7.1, 6.9]
+    for a in ({"k": 3}, {"mp": 0.5}, {"k": 3, "p": 0.9999}):
+        tok, _ = run(m, x, np.full(4, 1 - 2.0 ** -24, np.float32), **a)
+        assert (tok == 2).all(), (a, tok)
