@@ -352,7 +352,8 @@ struct FastLds : Sums {
 };
 
 // Exclusive sums over the workgroup's threads of a count and a mass, and the totals; m1 is the sum with the thread's own, the
-// same bits as the next thread's m0.
+// same bits as the next thread's m0. A sum over lanes is added in an order of its own for each, so the masses' need not
+// rise.
 template <int W>
 __device__ __forceinline__ void block_scan(uint32_t n, double m, uint32_t& n0, double& m0, double& m1, uint32_t& n_all, double& m_all,
                                            Sums& s) {
@@ -374,7 +375,7 @@ __device__ __forceinline__ void block_scan(uint32_t n, double m, uint32_t& n0, d
     const double mp = moved<0x138, 0xf>(mi);  // the lane's before
     n0 = nb + ni - n;
     m0 = mb + mp;
-    m1 = mb + mi;
+    m1 = lane < 63 ? mb + mi : lane_value(mw, wave);
 }
 
 // A row of logits as a buffer: reads past its end give 0 rather than branch.
@@ -643,12 +644,17 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
                 cm += in;
             }
         }
+        int p_bin = -1;  // where the thread finds top_p's border, and what lies above
+        double p_above = 0.0;
+        uint32_t p_above_n = 0;
         if (ask.p < 1.0f) {
             if (ask.k > 0) __syncthreads();
             // what top_p is a share of is known to within the bin where top_k ends
             const double hi = (double)ask.p * (ask.k > 0 ? s.k_above + s.k_in : all_m) - base_m;
             double lo = ask.k > 0 ? (double)ask.p * s.k_above - base_m : hi;
             lo = lo > 0.0 ? lo : 1e-300;
+            // Sums round: they need not rise from thread to thread, nor m1 be what the thread's bins add up to. Of several threads
+            // that find the border the first has it; a bin of none has none.
             if ((m0 < lo && m1 >= lo) || (m0 < hi && m1 >= hi)) {
                 uint32_t cn = n0;
                 double cm = m0;
@@ -657,23 +663,28 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
                 for (int b = tid * B; b < tid * B + B; ++b, each_m *= fall) {
                     const uint64_t v = s.hist[b];
                     const double to = b + 1 < tid * B + B ? cm + bin_mass(v, each_m) : m1;
-                    if (cm < lo && to >= lo) {
-                        s.p_lo = b;
-                        s.p_above = base_m + cm;
-                        s.p_above_n = cn;
+                    if (v && cm < lo && to >= lo) {
+                        p_bin = b;
+                        p_above = base_m + cm;
+                        p_above_n = cn;
+                        atomicMin(&s.p_lo, (uint32_t)b);
                     }
-                    if (cm < hi && to >= hi) s.p_hi = b;
+                    if (ask.k > 0 && v && cm < hi && to >= hi) atomicMin(&s.p_hi, (uint32_t)b);
                     cn += (uint32_t)(v >> kCountAt);
                     cm = to;
                 }
             }
         }
         __syncthreads();
+        if (p_bin == (int)s.p_lo) {  // read behind the next barrier
+            s.p_above = p_above;
+            s.p_above_n = p_above_n;
+        }
         const int k_bin = ask.k > 0 ? (int)s.k_bin : kBins;
         int p_lo = k_bin, p_hi = k_bin;
         if (ask.p < 1.0f) {
             p_lo = (int)s.p_lo;
-            p_hi = (int)s.p_hi < k_bin ? (int)s.p_hi : k_bin;
+            p_hi = ask.k == 0 ? p_lo : (int)s.p_hi < k_bin ? (int)s.p_hi : k_bin;
         }
         const int most = k_bin < kBins ? k_bin : p_hi;  // the last bin that is listed
         slow = p_lo > p_hi || most >= kBins || (ask.k > 0 && k_bin == kBins);
