@@ -59,7 +59,7 @@ struct SampleArg {
     float* logprob;  // or null
     int64_t row0;
     int32_t classes;
-    int32_t shift;  // of the whole-number masses: 2^shift for the largest, room for all classes
+    int32_t shift;  // of the whole-number masses: 2^shift for the largest, room for all of up to kMaxBinned classes
 };
 
 // A row's settings.
@@ -145,15 +145,16 @@ struct Heat {
     int shift;
 };
 // 2^shift e^((x - top) / T): the exponent in two parts, so that what rounds is the result.
-__device__ __forceinline__ uint64_t mass_of(float x, const Heat& h) {
-    if (x == h.top) return (uint64_t)1 << h.shift;
+__device__ __forceinline__ double scaled_mass(float x, const Heat& h) {
+    if (x == h.top) return __builtin_ldexp(1.0, h.shift);
     const float d = x - h.top;
     const float t = d * h.hi;
-    if (!(t > -63.0f)) return 0;
+    if (!(t > -63.0f)) return 0.0;
     const float n = __builtin_rintf(t);
     const float r = __builtin_fmaf(d, h.hi, -n) + d * h.lo;
-    return (uint64_t)(__builtin_ldexp((double)__builtin_amdgcn_exp2f(r), (int)n + h.shift) + 0.5);
+    return __builtin_ldexp((double)__builtin_amdgcn_exp2f(r), (int)n + h.shift);
 }
+__device__ __forceinline__ uint64_t mass_of(float x, const Heat& h) { return (uint64_t)(scaled_mass(x, h) + 0.5); }
 
 struct Threshold {
     uint32_t key;   // the value's order
@@ -163,6 +164,7 @@ struct Threshold {
 struct SlowLds {
     unsigned long long hist_m[256], said[4], seg_m[16];
     uint32_t hist_n[256], seg_n[16];
+    double sum_d[16];
 };
 
 // The first classes of a row, by falling logits, whose count reaches `count`, or whose mass reaches `mass` (whichever is not
@@ -227,6 +229,14 @@ __device__ __attribute__((noinline)) void slow_row(const float* x, int classes, 
     h.hi = (float)per;
     h.lo = (float)(per - (double)h.hi);
     h.shift = shift;
+    // Room for every class at the largest's mass rounds n of them by n^2 2^-63 of it at most, 2^-25 over 2^19; more have room for what
+    // they add up to, which they round by n 2^-63 of itself.
+    if (classes > kMaxBinned) {
+        h.shift = 0;
+        double m = 0.0;
+        for (int c = tid; c < classes; c += T) m += scaled_mass(x[c], h);
+        h.shift = 62 - __builtin_amdgcn_frexp_exp(block_sum<W>(m, s.sum_d));
+    }
     Threshold t = {0, 0};
     uint64_t sum = 0;
     bool cut = false;
@@ -300,7 +310,7 @@ __device__ __attribute__((noinline)) void slow_row(const float* x, int classes, 
         if (hit) {
             if (lane == __builtin_ctzll(hit)) {
                 *token = c;
-                if (logprob) *logprob = share_log(v, best, ask.T, __builtin_ldexp((double)total, -shift));
+                if (logprob) *logprob = share_log(v, best, ask.T, __builtin_ldexp((double)total, -h.shift));
             }
             break;
         }

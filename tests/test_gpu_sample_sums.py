@@ -100,3 +100,29 @@ def test_a_cut_where_sums_round_apart(classes, bins):
         for a in ({}, {"k": len(some) + 7}, {"mp": 1e-3}):
             for u in (0.0, 0.3, 0.77, 1 - 2.0 ** -24):
                 check(m, x, np.float32([u]), T=0.25, p=0.5, **a, what=f"{a} {u}")
+
+
+def test_a_bulk_of_classes_far_below_the_largest():
+    """2^24 classes of which all but the first have e^-26.9 = 2^-38.8 of its mass, 2^-14.8 together; u draws among them, and top_p's
+    border lies there. A class' mass is off by (26.9 + 4) 2^-24 of itself, and so the bulk's, a place by as much of what lies
+    behind it; u and top_p are exact."""
+    m = m_()
+    n = 1 << 24
+    x = np.full((1, n), -26.9, np.float32)
+    x[0, 0] = 0.0
+    each = np.exp(np.float64(x[0, 1]))
+    off = (26.9 + 4) * 2.0 ** -24
+    for behind in (2.0 ** -15.5, 2.0 ** -16, 2.0 ** -18):
+        u = np.float32(1 - behind)
+        for k in (n - 1, n - 12345):
+            total = 1 + (k - 1) * each
+            tok, lp = run(m, x, np.float32([u]), k=k)
+            left = (1 - np.float64(u)) * total / each  # classes behind the one that is drawn
+            assert abs(k - left - tok[0]) <= off * left + 2, (behind, k, tok)
+            assert abs(lp[0] + 26.9 + np.log(total)) <= 1e-5
+    p = np.float32(1 - 2.0 ** -16)
+    tok, lp = run(m, x, np.float32([1 - 2.0 ** -24]), p=p)
+    total = 1 + (n - 1) * each
+    kept = n - (1 - np.float64(p)) * total / each
+    left = 2.0 ** -24 * total / each
+    assert abs(kept - left - tok[0]) <= off * (n - kept + left) + 3, tok
