@@ -816,7 +816,7 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
         if (ask.p < 1.0f) {
             const double least = (double)ask.p * share - s.p_above;
             for (int i = tid; i < end; i += T)
-                if (s.list.upto[i] >= least && (i == 0 || s.list.upto[i - 1] < least)) s.first = i;
+                if (s.list.upto[i] >= least && (i == 0 || s.list.upto[i - 1] < least)) atomicMin(&s.first, i);  // where sums fall again, the first
             __syncthreads();
             last = s.first < end ? s.first : end;
         }

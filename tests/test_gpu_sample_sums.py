@@ -126,3 +126,20 @@ def test_a_bulk_of_classes_far_below_the_largest():
     kept = n - (1 - np.float64(p)) * total / each
     left = 2.0 ** -24 * total / each
     assert abs(kept - left - tok[0]) <= off * (n - kept + left) + 3, tok
+
+
+@pytest.mark.parametrize("rows, classes", [(300, 900), (720, 6000), (512, 32000), (1, 32000), (3, 600001)])
+@pytest.mark.parametrize("T", [0.01, 0.3, LOG2E])
+def test_the_same_tokens_on_every_call(rows, classes, T):
+    """Where sums round apart too: logits of 1 to 60 temperatures, the rows again and again."""
+    m = m_()
+    r = np.random.RandomState(44)
+    x = np.full((rows, classes), -np.inf, np.float32)
+    for row in x:
+        some = r.randint(0, classes, 700)
+        row[some] = -np.float32(T) * r.choice([0, 1, 2, 30, 36, 37, 38, 60], len(some))
+    x[:, 0] = 0
+    u = r.randint(0, 9, rows).astype(np.float32) / 8
+    for a in ({"p": 0.75}, {"k": 500, "p": 0.75}, {"k": 500}):
+        seen = [run(m, x, u, T=T, **a) for _ in range(4)]
+        assert all(np.array_equal(tok, seen[0][0]) and np.array_equal(lp, seen[0][1]) for tok, lp in seen)
