@@ -372,7 +372,8 @@ int mh_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int3
  * Everything that is compared is made in 64 bits; ties, of groups too, go to the lowest index, and a NaN comes after every
  * number. A row with keep[row] == 0 (keep may be null) has chosen -1 and weights 0 and counts nowhere. A softmax row that
  * holds a NaN, plus infinity or nothing but minus infinity has NaN for weights; so has a chosen sigmoid that is NaN, and
- * with normalise its whole row, or one whose chosen scores add up to 0. Choices stay below experts.
+ * with normalise its whole row, or one whose chosen scores add up to less than 2^-1022, the least of 64 bits. Choices stay
+ * below experts.
  * 1 <= experts <= 1024, 1 <= k <= 64, 1 <= groups <= 64, which divide experts, and k experts at least in keep_groups
  * groups. The library's scratch grows to 4 bytes a row, and 10 KB an expert at most. */
 enum mh_router_scores { MH_SCORES_SOFTMAX = 0, MH_SCORES_SIGMOID = 1 };

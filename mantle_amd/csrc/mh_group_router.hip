@@ -12,7 +12,8 @@
 // Choices are made in fp32 first, 8 at a time by sorted lists of the row, with a bound on its error; a row whose choice,
 // or whose choice of groups, turns on less than twice that (one in a few hundred) is listed, and a second kernel chooses
 // for it in 64 bits, a wavefront a row. That kernel alone takes short batches, whose rows it holds all at once. Weights
-// are 64-bit scores rounded to fp32, by one formula in both; gradients are fp32.
+// are made in 64 bits and rounded once, by one formula in both, for a bias may choose among scores that fp32 does not hold;
+// gradients are fp32.
 //
 // L lanes hold a row in registers, V elements a lane in quads (element 4 (i L + lane) + c). Over [131072, 256], top 8 of 4 of
 // 8 groups, the forward takes 91 us, where its read alone takes 24: 1200 vector instructions for a wavefront's 4 rows
@@ -112,9 +113,9 @@ __device__ __forceinline__ double inverse(double x) {
     return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
 }
 // A weight's score; `top` and `by` are a softmax's largest logit and 1 / the sum of its exponentials.
-__device__ __forceinline__ float weight_score(bool sigmoid, float v, float top, double by) {
+__device__ __forceinline__ double weight_score(bool sigmoid, float v, float top, double by) {
     const double e = exp_short(sigmoid ? -__builtin_fabs((double)v) : (double)v - (double)top);
-    return (float)(sigmoid ? (v < 0.0f ? e : 1.0) * inverse(1.0 + e) : e * by);
+    return sigmoid ? (v < 0.0f ? e : 1.0) * inverse(1.0 + e) : e * by;
 }
 // A double as an integer of the same order; NaN below every number, -0 as +0; below them what may not be chosen.
 constexpr int64_t kNever = INT64_MIN;
@@ -254,21 +255,22 @@ __device__ __forceinline__ void choose_exact(const GroupArg& a, const float* x, 
     }
 }
 
-// A chosen row's results by L lanes, of which this is number l: its choices lie in `pick`.
+// A chosen row's results by L lanes, of which this is number l: its choices lie in `pick`. Their scores are 64-bit until the weight
+// is rounded: a bias may choose among scores that fp32 does not hold.
 template <int L>
 __device__ __forceinline__ void put_choice(const GroupArg& a, const int32_t* pick, const float* x, int64_t r, int l, bool in, bool keep,
                                            float top, double by, int32_t* cnt) {
-    float total = 0.0f, s = 0.0f;
+    double total = 0.0, s = 0.0;
     for (int t = l; keep && in && t < a.k; t += L) {
         s = weight_score(a.sigmoid != 0, x[pick[t]], top, by);
         total += s;
     }
-    total = a.normalise ? group_sum<L>(total) : 1.0f;
+    const double times = (double)a.scale * (a.normalise ? inverse(group_sum64<L>(total)) : 1.0);
     for (int t = l; in && t < a.k; t += L) {
         const int32_t id = keep ? pick[t] : 0;  // nothing is known of a padding row's
-        if (a.k > L && keep) s = weight_score(a.sigmoid != 0, x[id], top, by);
+        if (L < kMaxChosen && a.k > L && keep) s = weight_score(a.sigmoid != 0, x[id], top, by);
         a.chosen[r * a.k + t] = keep ? id : -1;
-        a.weights[r * a.k + t] = keep ? a.scale * (s / total) : 0.0f;
+        a.weights[r * a.k + t] = keep ? (float)(s * times) : 0.0f;
         if (keep) atomicAdd(&cnt[id], 1);
     }
 }
