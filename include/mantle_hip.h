@@ -382,7 +382,8 @@ int mh_group_router_fwd(float* weights, int32_t* chosen, int32_t* counts, const 
                         int group_best, int scores, int normalise, float scale);
 /* The gradient of the logits from grad_weights [rows, k]; chosen is the forward's, and the choice carries no gradient; keep,
  * scores, normalise and scale as given to it. A row that is not kept is left alone (accumulate == 0: zero). An entry of
- * chosen outside the experts counts as none; no expert may stand twice in a row, as none does in the forward's. */
+ * chosen outside the experts counts as none; no expert may stand twice in a row, as none does in the forward's. With
+ * normalise a row whose chosen scores add up to less than 2^-1022 has NaN at the chosen. */
 int mh_group_router_bwd(float* grad_x, const float* x, const int32_t* keep, const int32_t* chosen, const float* grad_weights,
                         int64_t rows, int64_t experts, int64_t k, int scores, int normalise, float scale, int accumulate);
 /* The bias' step towards balance: bias_e += rate for experts that were chosen less often than the mean of counts,

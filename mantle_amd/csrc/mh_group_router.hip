@@ -12,8 +12,8 @@
 // Choices are made in fp32 first, 8 at a time by sorted lists of the row, with a bound on its error; a row whose choice,
 // or whose choice of groups, turns on less than twice that (one in a few hundred) is listed, and a second kernel chooses
 // for it in 64 bits, a wavefront a row. That kernel alone takes short batches, whose rows it holds all at once. Weights
-// are made in 64 bits and rounded once, by one formula in both, for a bias may choose among scores that fp32 does not hold;
-// gradients are fp32.
+// are made in 64 bits and rounded once, by one formula in both, for a bias may choose among scores that fp32 does not hold; so are the
+// gradients, but for the exponentials of a softmax of which every expert has one, to an ulp or so of fp32.
 //
 // L lanes hold a row in registers, V elements a lane in quads (element 4 (i L + lane) + c). Over [131072, 256], top 8 of 4 of
 // 8 groups, the forward takes 91 us, where its read alone takes 24: 1200 vector instructions for a wavefront's 4 rows
@@ -106,6 +106,13 @@ __device__ __forceinline__ double exp_short(double x) {
     p = __builtin_fma(p, r, 1.0);
     p = __builtin_fma(p, r, 1.0);
     return __builtin_ldexp(p, (int)n);
+}
+// e^x for x <= 0 to the exponential unit's own ulp and a quarter more of fp32: the exponent in 64 bits, its whole part taken off by a
+// sum that has room for no other.
+__device__ __forceinline__ float exp_rounded(double x) {
+    x = x < -1000.0 ? -1000.0 : x;  // a NaN stays one
+    const double t = x * scalar(1.4426950408889634074), whole = t + scalar(6755399441055744.0);
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(t - (whole - scalar(6755399441055744.0)))), __double2loint(whole));
 }
 // 1 / x of a positive normal x, to 2^-48 or so: a step of Newton's on the unit's own.
 __device__ __forceinline__ double inverse(double x) {
@@ -574,20 +581,23 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_bwd(GroupArg a) {
         const bool in = r < a.rows;
         const bool keep = in && (!a.keep || a.keep[r] != 0);
         const int64_t at = (in ? r : r0) * a.experts;
-        float v[V], inv = 0.0f, top = 0.0f;
+        // Scores and their sums are 64-bit, as the forward's: the chosen's may be less than fp32 holds, and a difference of gradients
+        // keeps the bits that it leaves.
+        float v[V], top = 0.0f;
+        double by = 1.0;
         if (whole) {
             load_row<L, V>(a.x + at, a.experts, l, v);
             top = v[0];
 #pragma unroll
             for (int i = 1; i < V; ++i) top = __builtin_fmaxf(top, v[i]);
             top = group_max<L>(top);
-            float sum = 0.0f;
+            double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] = exp_neg(v[i] - top);
-                sum += v[i];
+                v[i] = exp_rounded((double)v[i] - (double)top);
+                sum += (double)v[i];
             }
-            inv = 1.0f / group_sum<L>(sum);
+            by = inverse(group_sum64<L>(sum));
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = 0.0f;
@@ -601,43 +611,47 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_bwd(GroupArg a) {
                 top = group_max<L>(top);
             }
         }
-        // score s of an entry, or its exponential, and what of a sigmoid its derivative leaves
-        auto score = [&](int32_t id, float& rest) {
+        // an entry's expert, or -1; its score or exponential, what of a sigmoid its derivative leaves, and the weight's gradient
+        double score = 0.0, rest = 1.0, gr = 0.0;
+        auto entry = [&](int c) {
+            const int32_t id = a.sel[r * a.k + c];
+            if (id < 0 || id >= a.experts) return -1;
             const float x = a.x[at + id];
-            rest = 1.0f;
-            if (!a.sigmoid) return exp_neg(x - top) * (whole ? inv : 1.0f);
-            const float e = exp_neg(-__builtin_fabsf(x)), d = 1.0f / (1.0f + e);
-            rest = x < 0.0f ? d : e * d;
-            return x < 0.0f ? e * d : d;
+            gr = (double)a.gw[r * a.k + c];
+            const double e = exp_short(a.sigmoid ? -__builtin_fabs((double)x) : (double)x - (double)top);
+            score = e;
+            if (a.sigmoid) {
+                const double d = inverse(1.0 + e);
+                rest = x < 0.0f ? d : e * d;
+                score = x < 0.0f ? e * d : d;
+            }
+            return id;
         };
-        float all = 0.0f, inner = 0.0f;
+        int32_t id = -1;
+        double all = 0.0, inner = 0.0;
         if (keep)
             for (int c = l; c < a.k; c += L) {
-                const int32_t id = a.sel[r * a.k + c];
-                if (id < 0 || id >= a.experts) continue;
-                float rest;
-                const float s = score(id, rest);
-                all += s;
-                inner += s * a.gw[r * a.k + c];
+                id = entry(c);
+                if (id < 0) continue;
+                all += score;
+                inner += score * gr;
             }
-        all = group_sum<L>(all);
-        inner = group_sum<L>(inner);
-        const float by = a.normalise ? 1.0f / all : 1.0f;
+        all = group_sum64<L>(all);
+        inner = group_sum64<L>(inner);
+        if (a.normalise) by = inverse(all);
         inner *= by;
+        by *= (double)a.scale;
         wave_sync();
 #pragma unroll
         for (int i = 0; i < V / 4; ++i) {
             vf4 q = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-            *reinterpret_cast<vf4*>(&mark[g][4 * (i * L + l)]) = whole ? q * (-inv * inner) : q;
+            *reinterpret_cast<vf4*>(&mark[g][4 * (i * L + l)]) = whole ? q * (float)(by * -inner) : q;
         }
         wave_sync();
         if (keep)
             for (int c = l; c < a.k; c += L) {
-                const int32_t id = a.sel[r * a.k + c];
-                if (id < 0 || id >= a.experts) continue;
-                float rest;
-                const float s = score(id, rest), gr = a.gw[r * a.k + c];
-                mark[g][id] = s * by * rest * (a.normalise || whole ? gr - inner : gr);
+                if (L < kMaxChosen && a.k > L) id = entry(c);
+                if (id >= 0) mark[g][id] = (float)(score * by * rest * (a.normalise || whole ? gr - inner : gr));
             }
         wave_sync();
         if (!in || (!keep && a.accumulate)) continue;  // a padding row: as it was, or zero
@@ -646,7 +660,7 @@ __global__ __launch_bounds__(kRThreads) void k_group_router_bwd(GroupArg a) {
         for (int i = 0; i < V / 4; ++i) {
             const int c = 4 * (i * L + l);
             vf4 q = *reinterpret_cast<const vf4*>(&mark[g][c]);
-            q = keep ? q * a.scale : vf4{0.0f, 0.0f, 0.0f, 0.0f};
+            q = keep ? q : vf4{0.0f, 0.0f, 0.0f, 0.0f};
             if (c + 3 < a.experts) {
                 if (a.accumulate) q = q + ld_ntu(o + c);
                 st_ntu(o + c, q);
