@@ -92,7 +92,7 @@ class Adam:
                 raise _lib.MantleHipError(_lib.ERR_SHAPE, "a parameter and its gradient differ in shape")
             p.f32, g.f32  # neither holds whole numbers
         self.lr, self.beta1, self.beta2, self.epsilon = float(lr), float(beta1), float(beta2), float(epsilon)
-        self.max_norm = None if max_norm is None else float(max_norm)
+        self.max_norm = max_norm
         self.grad_norm = None if max_norm is None else Tensor(1)
         self.iter = 0
         # allocate_rms_and_momentum (optim.mojo:142-149): zero-initialised, one per parameter;
@@ -112,6 +112,18 @@ class Adam:
         self.rms_grads = SymbolTensors(rms, self.symbols)
         self._tables = None  # step()'s pointer tables, with the tensors they were made from
 
+    _max_norm: Optional[float] = None
+
+    @property
+    def max_norm(self) -> Optional[float]:
+        return self._max_norm
+
+    @max_norm.setter
+    def max_norm(self, value: Optional[float]) -> None:
+        if value is not None and not float(value) >= 0.0:
+            raise _lib.MantleHipError(_lib.ERR_INVALID, f"a largest norm of {value}")
+        self._max_norm = None if value is None else float(value)
+
     def zero_grad(self) -> None:
         """Adam.zero_grad (optim.mojo:90-92): parameters.grads.set_zero()."""
         if self._collection is not None:
@@ -121,13 +133,14 @@ class Adam:
             g.zero()
 
     def step(self) -> None:
+        norm = None if self.max_norm is None else _norm_address(self.grad_norm)
         self.iter += 1
         if self._span is not None:  # every parameter of the model in one launch
             p, g, n = self._span
             if self.max_norm is not None:
                 one = [(ctypes.c_void_p * 1)(a) for a in (p, g, self._m_span.ptr, self._v_span.ptr)]
                 _lib.call("mh_adam_clip_step_multi", 1, *one, (ctypes.c_int64 * 1)(n), self.lr, self.beta1, self.beta2,
-                          self.epsilon, self.iter, self.max_norm, _norm_address(self.grad_norm))
+                          self.epsilon, self.iter, self.max_norm, norm)
                 return
             _lib.call("mh_adam_step", p, g, self._m_span.ptr, self._v_span.ptr, n, self.lr, self.beta1, self.beta2,
                       self.epsilon, self.iter)
@@ -150,7 +163,7 @@ class Adam:
         _, ps, gs, ms, vs, sizes = self._tables
         if self.max_norm is not None:
             _lib.call("mh_adam_clip_step_multi", n, ps, gs, ms, vs, sizes, self.lr, self.beta1, self.beta2, self.epsilon,
-                      self.iter, self.max_norm, _norm_address(self.grad_norm))
+                      self.iter, self.max_norm, norm)
             return
         _lib.call("mh_adam_step_multi", n, ps, gs, ms, vs, sizes, self.lr, self.beta1, self.beta2, self.epsilon,
                   self.iter)
