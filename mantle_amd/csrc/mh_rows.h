@@ -21,7 +21,8 @@ __device__ __forceinline__ float exp_neg(float x) {
     return __builtin_fmaf(e, r * 0.693147180559945f, e);
 }
 
-// e^x in 64 bits to about an ulp, for x of less than 700 (from -1000 down it is 0; a NaN stays one): 2^n e^r,
+// e^x in 64 bits to about an ulp, for x of less than 700 (from -1000 down it is 0; a NaN stays one): 2^n e^r with n the whole
+// number next to x log2(e), r = x - n ln 2 from ln 2 in two parts, and e^r by its series to r^13.
 __device__ __forceinline__ double exp64(double x) {
     x = x < -1000.0 ? -1000.0 : x;
     const double n = __builtin_rint(x * 1.4426950408889634074);

@@ -36,16 +36,19 @@
 namespace mh {
 namespace {
 
+// The most classes that bins count: a bin's count and mass share 64 bits.
+constexpr int64_t kMaxBinned = (int64_t)1 << 19;
+constexpr int kCountAt = 44;  // the first bit of the count
+static_assert(kMaxBinned < (int64_t)1 << (64 - kCountAt) && kMaxBinned << 24 <= (int64_t)1 << (kCountAt - 1), "a bin holds every class");
 // By the threads T of a workgroup: the bins, those of them above the reference at first, the classes a list holds, and
 // those whose quads' largest logits are kept. Bins below the reference reach 32 T at least, whatever their power of two.
 template <int T>
 struct Sizes {
-    static constexpr int kBins = T >= 512 ? 4096 : 8 * T, kAbove = kBins / 8, kList = kBins / 2, kTops = T >= 512 ? 1 << 19 : 128 * T;
+    static constexpr int kBins = T >= 512 ? 4096 : 8 * T, kAbove = kBins / 8, kList = kBins / 2, kTops = T >= 512 ? (int)kMaxBinned : 128 * T;
     static constexpr float kWidth = 1.0f / (T >= 512 ? 112 : T / 5);  // of T, at least
+    static_assert(kTops <= kMaxBinned, "");
 };
-constexpr int kCountAt = 44;
 constexpr int kRanked = 512;  // the longest list that is sorted by ranks
-constexpr int64_t kMaxBinned = (int64_t)1 << 19;
 constexpr int64_t kMaxSampled = (int64_t)1 << 24;
 
 struct SampleArg {
