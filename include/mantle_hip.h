@@ -417,8 +417,9 @@ int mh_rms_norm_bwd(float* grad_x, float* grad_w, const float* grad_out, const f
  * tokens [rows] is the first class, by index, where the running sum of the kept p exceeds u times their sum; logprob [rows]
  * (may be null) the logarithm of its share in that sum. A class at minus infinity is never drawn; classes at plus infinity
  * share a row evenly. A row that holds a NaN, or nothing but minus infinity, has token -1 and logprob NaN. u is held to
- * [0, 1); a NaN counts as 0. A class's p is made in 32 bits, to 2^-22 of itself, and all sums in 64: where u or top_p falls
- * within some 2^-24 of a border between two classes either may be taken. The same call has the same tokens.
+ * [0, 1); a NaN counts as 0. A class's p is made in 32 bits, to (6 + |x - max x| / temperature) 2^-24 of itself with three
+ * neighbours added to it, and all other sums in 64: where u or top_p falls within as much of a border between two classes, as
+ * the mean of what is kept, either may be taken. The same call has the same tokens.
  * classes <= 2^24. */
 int mh_sample_tokens(int32_t* tokens, float* logprob, const float* x, const float* u, const float* temperature,
                      const int32_t* top_k, const float* top_p, const float* min_p, int64_t rows, int64_t classes);

@@ -16,9 +16,10 @@
 // gradients, but for the exponentials of a softmax of which every expert has one, to an ulp or so of fp32.
 //
 // L lanes hold a row in registers, V elements a lane in quads (element 4 (i L + lane) + c). Over [131072, 256], top 8 of 4 of
-// 8 groups, the forward takes 91 us, where its read alone takes 24: 1200 vector instructions for a wavefront's 4 rows
+// 8 groups, the forward takes 92 us, where its read alone takes 24: 1200 vector instructions for a wavefront's 4 rows
 // (scores, the groups' best, the sorted list, the check) fill three quarters of it. The listed rows take 11 us more, each k
-// reductions that wait for each other, the counts 6, and the backward, which writes 134 MB and gathers the chosen's logits, 46.
+// reductions that wait for each other, the counts 6, and the backward, which writes 134 MB and gathers the chosen's logits, 39 (with its
+// scores made twice, in fp32, 46).
 #include "mh_internal.h"
 #include "mh_lanes.h"
 #include "mh_rows.h"
@@ -28,16 +29,17 @@ namespace {
 
 constexpr int kMaxGroups = 64;
 constexpr int kRThreads = 256;
-// Workgroups of a forward at most, and rows of its partial counts: [131072, 256] 139 us, 768 139, 1024 147, 1536 145; [2^20, 16]
-// 114, 127, 114, 123.
+// Workgroups of a forward at most, and rows of its partial counts: its call over [131072, 256] 104 us, with 512 of them 116, 768 104,
+// 1024 111, 1536 110; over [2^20, 16] 62.5, 83.5, 70.5, 62, 67.
 constexpr int kRBlocks = 2048;
-// Workgroups for listed rows: where every row is tied, a router of zeros, [131072, 256] takes 0.93 ms with 512 and 2.29 with
-// 128; 1024 add 1 us to the counts of any call.
+// Workgroups for listed rows: where every row is tied, a router of zeros, [131072, 256] takes 0.94 ms with 512, 2.5 with 128 and 0.76
+// with 1024, which add 1 to 1.5 us to any call.
 constexpr int64_t kRExactBlocks = 512;
-// Workgroups that add up their counts by themselves: over 16 experts 64 rows 10.7 us instead of 13.6, 500 rows (125) 13.0; over 256
-// experts 128 rows 19.9 and 19.4, 500 rows 23.7 and 20.0.
+// Workgroups that add up their counts by themselves: over 16 experts 64 rows (16 workgroups) 6.8 us instead of 8.5, 500 rows (125) 12.0
+// instead of 8.6; over 256 experts 128 rows (32) 11.8 and 11.5, 500 rows 16.4 and 12.4.
 constexpr int64_t kRArrivals = 32;
-// Batches of up to this many rows go by wavefronts alone: over 256 experts 2048 rows take 17 us, 2049 by lists first 25.
+// Batches of up to this many rows go by wavefronts alone: over 256 experts 2048 rows take 13 us, by lists first 21; 4096 16.6 and 21,
+// 8192 27 and 23, 131072 299 and 104.
 constexpr int64_t kRExactRows = 2048;
 
 struct GroupArg {

@@ -17,19 +17,21 @@
 //      each waiting for the last, take 11700 cycles; [33, 30011] takes 26.7 us instead of 29.9), and the cuts are found in
 //      it by 64-bit sums;
 //   5. the run of classes where the running sum passes u of the total is walked by the whole workgroup.
-// Sums of steps 3 to 5 are 64-bit floats in a fixed order. Masses are fp32: their rounding, 2^-22 of each and without a common
-// sign, moves a border by some 2^-24 of the row.
+// Sums of steps 3 to 5 are 64-bit floats in a fixed order, of quads, which are added in fp32. Masses are fp32 too, for a walk is bound
+// by its instructions: a class' is off by 2^-24 of itself for each T below the largest (the difference's rounding), three for the
+// exponential and three for the quad's sum. That moves a border by as much as what is kept is off by together, where it has a common
+// sign.
 //
 // Rows for which bins do not work (more than 256 to 2048 classes of one value at a cut, a cut 32 T below the largest, an
 // infinite logit, temperatures outside 0.01 to 1e30, more than 2^19 classes) go by whole-number masses and a search over
 // the logits' bits, 8 at a time: right for every row, and slower.
 //
-// The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 125 us, where reading takes 41: two
+// The slowest row decides. Over [512, 131072] with settings of all kinds the call takes 124 us, where reading takes 41: two
 // workgroups a CU, and of a row at a temperature of 1 or more, whose cut lies in the bulk, 80 thousand cycles of 280 are the
 // counting (one LDS atomic and 20 instructions a class) and 83 the second walk (20 instructions a class). A single row of
-// 32000 takes 18 us: 42 thousand cycles, of which 13 count and 5 walk again, and the rest are short phases that each wait
+// 32000 takes 18.5 us: some 42 thousand cycles, of which 13 count and 5 walk again, and the rest are short phases that each wait
 // for a fetch, a barrier or 64-bit exponentials. Of Q 4 was taken (8 of 512 threads): 16 hold more of a row, and cost the
-// short phases registers and code: [33, 30011] 26.8 us with 16, 24.8 with 4; [512, 131072] with 512 threads 124 with 8, 128 with 4.
+// short phases registers and code: [33, 30011] 26.8 us with 16, 24.8 to 25.5 with 4; [512, 131072] with 512 threads 124 with 8, 128 with 4.
 #include "mh_internal.h"
 #include "mh_rows.h"
 
@@ -940,9 +942,10 @@ void launch_sample(SampleArg a, int64_t rows) {
     }
 }
 
-// Threads a row, by the microseconds of a row alone and of each row more that a CU has to take, with c thousand classes,
-// as measured with settings of all kinds. [4096, 500]: 21, 45, 105, 190 us with 64 to 1024 threads; [1024, 8000]: 76, 31, 42,
-// 61; [512, 32000]: 57, 43, 50 with 256 to 1024; [1, 32000]: 28, 18, 16.
+// Threads a row, by the microseconds of a row alone and of each row more that a CU has to take, with c thousand classes: of the
+// slowest of rows with settings of all kinds, which a batch waits for. [4096, 500]: 21, 46, 107, 195 us with 64 to 1024 threads;
+// [1024, 8000]: 79, 31, 43, 63; [512, 32000]: 58, 43, 50 with 256 to 1024; [128, 32000]: 51, 32, 28; [128, 500] 14.5, 14.5, 16, 16.
+// (Many a row alone is not that slow, and has the same order: [1, 32000] 28, 18, 16.)
 int sample_threads(int64_t rows, int64_t classes) {
     struct Form {
         int threads;
