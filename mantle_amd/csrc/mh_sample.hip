@@ -866,7 +866,10 @@ __global__ __launch_bounds__(T, T == 256 ? 5 : 4) void k_sample(SampleArg a) {
     const double ahead = moved<0x138, 0xf>(segs);
     const int seg = 63 - __builtin_clzll(__ballot(lane < W && s.seg[lane & 15] > 0.0 && ahead <= goal));
     double from = seg > 0 ? lane_value(segs, seg - 1) : 0.0;
-    if (tid == 0) s.first = -1;
+    if (tid == 0) {
+        s.first = -1;
+        s.token = 0;
+    }
     // the run in parts, each thread its own neighbouring quads of a part
     constexpr int P = Q < 8 ? Q : 8;
     const int stop = (seg + 1) * run < a.classes ? (seg + 1) * run : a.classes;
